@@ -79,6 +79,9 @@ class LinearDescF64(ctypes.Structure):
     ]
 
 
+# Element types of the node-wise operators (fc_dtype).
+NODE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 BASIS_CHEBYSHEV_AFFINE = 0
 BASIS_CHEBYSHEV_COSINE = 1
 BASIS_BESSEL = 2
@@ -145,6 +148,10 @@ _SIGNATURES = {
     "fc_rms_norm_bwd": (c_int, [c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "fc_rms_norm_dbwd": (c_int, [c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "fc_gate_dbwd": (c_int, [c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "fc_embedding_fwd": (c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_f32, c_vp, c_vp]),
+    "fc_embedding_bwd_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64]),
+    "fc_embedding_bwd": (c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_f32, c_i64, c_vp, c_vp, c_i64, c_vp]),
+    "fc_dropout_add": (c_int, [c_i32, c_i64, c_vp, c_vp, c_f64, c_vp, c_vp, c_vp]),
     "fc_neighbor_list": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp]),
     "fc_neighbor_list_device_workspace": (c_i64, [c_i64]),
     "fc_neighbor_list_device": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp, c_vp,

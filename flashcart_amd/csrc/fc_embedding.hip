@@ -1,0 +1,484 @@
+// Embedding lookup out[i] = scale table[ids[i]] and the table's gradient g[r] = scale sum_{i: ids[i] = r} grad[i].
+//
+// The gradient is formed without atomics on values, so that it is the same in every run: token numbers are sorted by
+// index (a stable radix sort, 8 bits a pass), the sorted list is cut into pieces of equal length, and each piece adds
+// the gradient rows of its runs of equal indices in float32, in token order. Runs inside one piece are written at once;
+// runs that cross pieces leave one partial sum per piece, which a second kernel joins in piece order. Rows without
+// tokens are zero: the table is filled while the sort counts, since most rows of a large table have no token.
+// Indices outside the table (a device-side check cannot raise) give rows of NaN and take no part in the gradient.
+#include "fc_node.h"
+
+namespace fc {
+
+constexpr int kEmbTile = 2048;  // keys of a workgroup in the sort
+
+// ---- forward: one 16-byte chunk of a row per thread ----
+template <class T, class I>
+__global__ void __launch_bounds__(256) embedding_fwd_kernel(I total, I chunks, int64_t rows, int64_t width,
+                                                            const int64_t* __restrict__ ids,
+                                                            const T* __restrict__ table, float scale,
+                                                            T* __restrict__ out) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (int64_t)total) return;
+  const I row = (I)t / chunks, chunk = (I)t - row * chunks;
+  const int64_t c0 = (int64_t)chunk * V;
+  const int64_t id = ids[row];
+  const bool ok = id >= 0 && id < rows;
+  const T* src = table + (ok ? id : 0) * width + c0;
+  T* dst = out + (int64_t)row * width + c0;
+  if (c0 + V <= width) {
+    const Pack<T, V> v = load_pack<T, V>(src);
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(ok ? to_f32(v.v[i]) * scale : __builtin_nanf(""));
+    store_pack<T, V>(dst, o);
+    return;
+  }
+  for (int i = 0; i < width - c0; ++i) dst[i] = from_f32<T>(ok ? to_f32(src[i]) * scale : __builtin_nanf(""));
+}
+
+// ---- sort ----
+struct EmbSort {
+  int64_t n, rows, padding;
+  int32_t tiles;
+  const int64_t* ids;  // first pass
+  const uint32_t* keys;
+  const int32_t* order;  // later passes
+  uint32_t* keys_out;
+  int32_t* order_out;
+  int32_t* hist;    // (256, tiles): counts, then the keys of the digit in earlier tiles
+  int32_t* total;   // (256)
+  int32_t shift;
+  // table to be filled with zeros by the workgroups behind the tiles
+  uint8_t* fill;
+  int64_t fill_bytes;
+  int32_t* counter;  // of the joins, cleared here
+};
+
+// Tokens that add to no row (index outside the table, or the padding row) get the key `rows`: they sort last.
+__device__ __forceinline__ uint32_t emb_key(const EmbSort& a, int64_t i) {
+  if (!a.ids) return a.keys[i];
+  const int64_t id = a.ids[i];
+  return (id < 0 || id >= a.rows || id == a.padding) ? (uint32_t)a.rows : (uint32_t)id;
+}
+
+constexpr int kEmbFillBytes = 64 << 10;  // of a filling workgroup
+
+__device__ void emb_fill(uint8_t* p, int64_t bytes) {
+  const int head = (int)min((int64_t)((16 - ((uintptr_t)p & 15)) & 15), bytes);
+  if ((int)threadIdx.x < head) p[threadIdx.x] = 0;
+  p += head;
+  bytes -= head;
+  for (int64_t o = threadIdx.x * 16; o + 16 <= bytes; o += blockDim.x * 16) *(uint4*)(p + o) = make_uint4(0, 0, 0, 0);
+  const int64_t done = bytes & ~(int64_t)15;
+  if (done + threadIdx.x < bytes) p[done + threadIdx.x] = 0;
+}
+
+__global__ void __launch_bounds__(256) emb_hist_kernel(EmbSort a) {
+  __shared__ int32_t cnt[256];
+  const int t = threadIdx.x;
+  if ((int)blockIdx.x >= a.tiles) {
+    const int64_t b0 = (int64_t)(blockIdx.x - a.tiles) * kEmbFillBytes;
+    emb_fill(a.fill + b0, min((int64_t)kEmbFillBytes, a.fill_bytes - b0));
+    return;
+  }
+  if (blockIdx.x == 0 && t == 0 && a.counter) *a.counter = 0;
+  cnt[t] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kEmbTile;
+  for (int k = 0; k < kEmbTile / 256; ++k) {
+    const int64_t i = i0 + k * 256 + t;
+    if (i < a.n) atomicAdd(&cnt[(emb_key(a, i) >> a.shift) & 255], 1);
+  }
+  __syncthreads();
+  a.hist[(int64_t)t * a.tiles + blockIdx.x] = cnt[t];
+}
+
+// Exclusive sum over a workgroup of 256; every thread gets the total too.
+__device__ __forceinline__ int block_scan(int v, int* wave_sums, int* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(s, o, 64);
+    if (lane >= o) s += u;
+  }
+  if (lane == 63) wave_sums[w] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int x = wave_sums[k];
+    if (k < w) before += x;
+    all += x;
+  }
+  __syncthreads();
+  *total = all;
+  return before + s - v;
+}
+
+// One workgroup per digit: its counts become the number of its keys in earlier tiles.
+__global__ void __launch_bounds__(256) emb_scan_kernel(EmbSort a) {
+  __shared__ int ws[4];
+  int32_t* h = a.hist + (int64_t)blockIdx.x * a.tiles;
+  int base = 0;
+  for (int k = 0; k < a.tiles; k += 256) {
+    const int i = k + threadIdx.x;
+    const int v = i < a.tiles ? h[i] : 0;
+    int all;
+    const int ex = block_scan(v, ws, &all);
+    if (i < a.tiles) h[i] = base + ex;
+    base += all;
+  }
+  if (threadIdx.x == 0) a.total[blockIdx.x] = base;
+}
+
+// Lanes of this wave whose 8-bit digit equals this lane's, among the active ones.
+__device__ __forceinline__ uint64_t match_digit(uint32_t d, bool active) {
+  uint64_t m = __ballot(active);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const bool bit = (d >> b) & 1;
+    const uint64_t v = __ballot(bit);
+    m &= bit ? v : ~v;
+  }
+  return m;
+}
+
+// Stable placement: each wave ranks 512 consecutive keys, 64 at a time.
+__global__ void __launch_bounds__(256) emb_scatter_kernel(EmbSort a) {
+  constexpr int ROUNDS = kEmbTile / 256;
+  __shared__ int32_t cnt[4][256];
+  __shared__ int32_t base[256];
+  __shared__ int ws[4];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) cnt[k][t] = 0;
+  int all;
+  const int ex = block_scan(a.total[t], ws, &all);
+  base[t] = ex + a.hist[(int64_t)t * a.tiles + blockIdx.x];
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kEmbTile + w * (kEmbTile / 4);
+  uint32_t key[ROUNDS];
+  int rank[ROUNDS];
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int64_t i = i0 + k * 64 + lane;
+    const bool ok = i < a.n;
+    key[k] = ok ? emb_key(a, i) : 0;
+    const uint32_t d = (key[k] >> a.shift) & 255;
+    const uint64_t m = match_digit(d, ok);
+    const int before = __popcll(m & ((1ull << lane) - 1));
+    rank[k] = ok ? cnt[w][d] + before : 0;
+    __builtin_amdgcn_wave_barrier();
+    if (ok && before == 0) cnt[w][d] += __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  {
+    int b = base[t];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = cnt[k][t];
+      cnt[k][t] = b;
+      b += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int64_t i = i0 + k * 64 + lane;
+    if (i >= a.n) continue;
+    const int to = cnt[w][(key[k] >> a.shift) & 255] + rank[k];
+    a.keys_out[to] = key[k];
+    a.order_out[to] = a.ids ? (int32_t)i : a.order[i];
+  }
+}
+
+// ---- sums of runs ----
+struct EmbSum {
+  int64_t n, rows, width;
+  int32_t pieces, len, col_threads;  // col_threads: a power of two, <= 256
+  const uint32_t* keys;
+  const int32_t* order;
+  const void* grad;
+  void* out;
+  float scale;
+  float* head;  // (pieces, width): sum of the run that began in an earlier piece
+  float* tail;  // (pieces, width): sum of the run that goes on in the next piece
+  int32_t* joins;  // pieces whose last run has to be joined
+  int32_t* counter;
+};
+
+template <class T, int V>
+__device__ __forceinline__ void load_f32(const T* p, int valid, float (&x)[V]) {
+  if (valid >= V) {
+    const Pack<T, V> v = load_pack<T, V>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = to_f32(v.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = i < valid ? to_f32(p[i]) : 0.f;
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_f32(T* p, int valid, const float (&x)[V]) {
+  if (valid >= V) {
+    Pack<T, V> v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.v[i] = from_f32<T>(x[i]);
+    store_pack<T, V>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < valid) p[i] = from_f32<T>(x[i]);
+  }
+}
+
+// A group of col_threads lanes sums one piece over V columns each; U gradient rows are loaded ahead.
+template <class T>
+__global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const int groups = 256 / a.col_threads;
+  const int64_t p = (int64_t)blockIdx.x * groups + threadIdx.x / a.col_threads;
+  const int64_t c0 = ((int64_t)blockIdx.y * a.col_threads + threadIdx.x % a.col_threads) * V;
+  if (p >= a.pieces || c0 >= a.width) return;
+  const int valid = (int)min((int64_t)V, a.width - c0);
+  const int64_t t0 = p * a.len, t1 = min(a.n, t0 + a.len);
+  const T* grad = (const T*)a.grad + c0;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  uint32_t run = a.keys[t0];
+  bool from_left = p > 0 && a.keys[t0 - 1] == run;
+  auto flush = [&](bool to_right) {
+    if (run < (uint32_t)a.rows) {
+      if (from_left || to_right) {
+        store_f32<float, V>((from_left ? a.head : a.tail) + p * a.width + c0, valid, acc);
+        if (!from_left && c0 == 0) a.joins[atomicAdd(a.counter, 1)] = (int32_t)p;
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+        store_f32<T, V>((T*)a.out + (int64_t)run * a.width + c0, valid, acc);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  };
+  for (int64_t t = t0; t < t1; t += U) {
+    uint32_t key[U];
+    float g[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = min(t + u, t1 - 1);
+      key[u] = a.keys[at];
+      load_f32<T, V>(grad + (int64_t)a.order[at] * a.width, valid, g[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) break;
+      if (key[u] != run) {
+        flush(false);
+        run = key[u];
+        from_left = false;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += g[u][i];
+    }
+  }
+  flush(t1 < a.n && a.keys[t1] == run);
+}
+
+// A run of several pieces: tail of the first, heads of the others. Groups of lanes add consecutive spans of pieces, the
+// groups' sums are added in order.
+template <class T>
+__global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float part[256 * V];
+  const int groups = 256 / a.col_threads, grp = threadIdx.x / a.col_threads, ct = threadIdx.x % a.col_threads;
+  const int64_t c0 = ((int64_t)blockIdx.y * a.col_threads + ct) * V;
+  const int valid = (int)max((int64_t)0, min((int64_t)V, a.width - c0));
+  const int count = *a.counter;
+  for (int j = blockIdx.x; j < count; j += gridDim.x) {
+    const int64_t p = a.joins[j];
+    const int64_t first = (p + 1) * a.len;  // of the second piece: the run goes on here
+    const uint32_t key = a.keys[first];
+    int64_t lo = first, hi = a.n;  // keys[lo] == key; the first larger key is in (lo, hi]
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.keys[mid] == key) lo = mid;
+      else hi = mid;
+    }
+    const int64_t last = lo / a.len, m = last - p + 1, span = (m + groups - 1) / groups;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    if (valid > 0)
+      for (int64_t q = p + grp * span; q < min(p + (grp + 1) * span, last + 1); ++q) {
+        float x[V];
+        load_f32<float, V>((q == p ? a.tail : a.head) + q * a.width + c0, valid, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += x[i];
+      }
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = acc[i];
+    __syncthreads();
+    if (grp == 0 && valid > 0) {
+      for (int k = 1; k < groups; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += part[(k * a.col_threads + ct) * V + i];
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+      store_f32<T, V>((T*)a.out + (int64_t)key * a.width + c0, valid, acc);
+    }
+    __syncthreads();
+  }
+}
+
+struct EmbPlan {
+  int64_t tiles, pieces, len;
+  int col_threads, col_blocks, passes;
+  int64_t keys[2], order[2], hist, total, head, tail, joins, counter, bytes;
+};
+
+static EmbPlan emb_plan(int32_t dtype, int64_t n, int64_t rows, int64_t width) {
+  EmbPlan p{};
+  const int64_t V = 16 / node_dtype_size(dtype), cols = (width + V - 1) / V;
+  p.tiles = (n + kEmbTile - 1) / kEmbTile;
+  int ct = 1;
+  while (ct < 256 && ct < cols) ct *= 2;
+  p.col_threads = ct;
+  p.col_blocks = (int)((cols + ct - 1) / ct);
+  p.len = 16;
+  while (p.len < 1024 && n / p.len * cols > (1 << 18)) p.len *= 2;
+  p.pieces = (n + p.len - 1) / p.len;
+  int bits = 1;
+  while ((rows >> bits) > 0) ++bits;
+  p.passes = (bits + 7) / 8;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  for (int k = 0; k < 2; ++k) {
+    p.keys[k] = take(4 * n);
+    p.order[k] = take(4 * n);
+  }
+  p.hist = take(1024 * p.tiles);
+  p.total = take(1024);
+  p.head = take(4 * p.pieces * width);
+  p.tail = take(4 * p.pieces * width);
+  p.joins = take(4 * p.pieces);
+  p.counter = take(4);
+  p.bytes = at;
+  return p;
+}
+
+static int emb_check(int32_t dtype, int64_t n, int64_t rows, int64_t width) {
+  if (!node_dtype_ok(dtype)) return FC_ERR_BAD_DESC;
+  if (n < 0 || rows < 1 || width < 1 || n > 0x7fff0000 || rows > 0x7fff0000 || width > 0x7fff0000) return FC_ERR_SHAPE;
+  return FC_OK;
+}
+
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" int fc_embedding_fwd(int32_t dtype, int64_t n, int64_t rows, int64_t width, const int64_t* ids,
+                                const void* table, float scale, void* out, void* stream) {
+  const int st = emb_check(dtype, n, rows, width);
+  if (st != FC_OK) return st;
+  if (n == 0) return FC_OK;
+  if (!ids || !table || !out) return FC_ERR_NULL;
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const int64_t chunks = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), total = n * chunks;
+    if ((total + 255) / 256 > 0x7fffffff) return FC_ERR_SHAPE;
+    const dim3 grid((unsigned)((total + 255) / 256)), block(256);
+    hipStream_t s = (hipStream_t)stream;
+    if (total <= 0xffffffffll)
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, uint32_t>), grid, block, 0, s, (uint32_t)total, (uint32_t)chunks,
+                         rows, width, ids, (const T*)table, scale, (T*)out);
+    else
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, uint64_t>), grid, block, 0, s, (uint64_t)total, (uint64_t)chunks,
+                         rows, width, ids, (const T*)table, scale, (T*)out);
+    FC_LAUNCH_CHECK();
+    return FC_OK;
+  });
+}
+
+extern "C" int64_t fc_embedding_bwd_workspace(int32_t dtype, int64_t n, int64_t rows, int64_t width) {
+  const int st = emb_check(dtype, n, rows, width);
+  if (st != FC_OK) return -st;
+  return emb_plan(dtype, n, rows, width).bytes;
+}
+
+extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t width, const int64_t* ids,
+                                const void* grad_out, float scale, int64_t padding, void* grad_table, void* ws,
+                                int64_t ws_bytes, void* stream) {
+  const int st = emb_check(dtype, n, rows, width);
+  if (st != FC_OK) return st;
+  if (!grad_table || (n > 0 && (!ids || !grad_out))) return FC_ERR_NULL;
+  const EmbPlan p = emb_plan(dtype, n, rows, width);
+  if (ws_bytes < p.bytes || !ws) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  char* w = (char*)ws;
+  EmbSort a{};
+  a.n = n;
+  a.rows = rows;
+  a.padding = padding;
+  a.tiles = (int32_t)p.tiles;
+  a.hist = (int32_t*)(w + p.hist);
+  a.total = (int32_t*)(w + p.total);
+  a.counter = (int32_t*)(w + p.counter);
+  const int64_t table_bytes = rows * width * node_dtype_size(dtype);
+  const int64_t fills = (table_bytes + kEmbFillBytes - 1) / kEmbFillBytes;
+  if (p.tiles + fills > 0x7fffffff || p.col_blocks > 65535) return FC_ERR_SHAPE;
+  for (int k = 0; k < p.passes; ++k) {
+    a.ids = k == 0 ? ids : nullptr;
+    a.keys = (uint32_t*)(w + p.keys[(k + 1) & 1]);
+    a.order = (int32_t*)(w + p.order[(k + 1) & 1]);
+    a.keys_out = (uint32_t*)(w + p.keys[k & 1]);
+    a.order_out = (int32_t*)(w + p.order[k & 1]);
+    a.shift = 8 * k;
+    a.fill = (uint8_t*)grad_table;
+    a.fill_bytes = table_bytes;
+    const int64_t blocks = p.tiles + (k == 0 ? fills : 0);
+    hipLaunchKernelGGL(emb_hist_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    FC_LAUNCH_CHECK();
+    if (n == 0) return FC_OK;
+    hipLaunchKernelGGL(emb_scan_kernel, dim3(256), dim3(256), 0, s, a);
+    FC_LAUNCH_CHECK();
+    hipLaunchKernelGGL(emb_scatter_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, a);
+    FC_LAUNCH_CHECK();
+  }
+  EmbSum b{};
+  b.n = n;
+  b.rows = rows;
+  b.width = width;
+  b.pieces = (int32_t)p.pieces;
+  b.len = (int32_t)p.len;
+  b.col_threads = p.col_threads;
+  b.keys = (uint32_t*)(w + p.keys[(p.passes - 1) & 1]);
+  b.order = (int32_t*)(w + p.order[(p.passes - 1) & 1]);
+  b.grad = grad_out;
+  b.out = grad_table;
+  b.scale = scale;
+  b.head = (float*)(w + p.head);
+  b.tail = (float*)(w + p.tail);
+  b.joins = (int32_t*)(w + p.joins);
+  b.counter = (int32_t*)(w + p.counter);
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const int groups = 256 / p.col_threads;
+    hipLaunchKernelGGL((emb_piece_kernel<T>), dim3((unsigned)((p.pieces + groups - 1) / groups), p.col_blocks),
+                       dim3(256), 0, s, b);
+    FC_LAUNCH_CHECK();
+    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 512 ? p.pieces : 512), p.col_blocks),
+                       dim3(256), 0, s, b);
+    FC_LAUNCH_CHECK();
+    return FC_OK;
+  });
+}

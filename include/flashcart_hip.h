@@ -488,6 +488,32 @@ int64_t fc_neighbor_list_device_noalloc(int64_t n, const double* pos, const doub
                                         double cutoff, int64_t capacity, int64_t* out_i, int64_t* out_j,
                                         int32_t* out_shift, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Node-wise operators of three element types (no counterpart in the reference,  */
+/* which composes them of torch calls on float32). Values are held in float32    */
+/* in the kernels and rounded once to the element type. Pointers need the        */
+/* alignment of one element.                                                     */
+/* ------------------------------------------------------------------------- */
+typedef enum fc_dtype { FC_F32 = 0, FC_BF16 = 1, FC_F16 = 2 } fc_dtype;
+
+/* Embedding: out (n, width) = scale * table[ids], table (rows, width), ids (n) int64. An index outside the
+ * table gives a row of NaN. */
+int fc_embedding_fwd(int32_t dtype, int64_t n, int64_t rows, int64_t width, const int64_t* ids, const void* table,
+                     float scale, void* out, void* stream);
+/* grad_table[r] = scale * sum of grad_out[i] over ids[i] == r, summed in a fixed order; the row `padding`
+ * (-1: none) and rows without tokens are zero, indices outside the table are left out. The workspace is in
+ * bytes, its base aligned to 16. n, rows and width are below 2^31 - 65536. */
+int64_t fc_embedding_bwd_workspace(int32_t dtype, int64_t n, int64_t rows, int64_t width);
+int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t width, const int64_t* ids, const void* grad_out,
+                     float scale, int64_t padding, void* grad_table, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/* Residual dropout over n elements: out = residual + keep * x / (1 - p) (residual may be NULL; out may be x or
+ * residual). keep[e] is word e % 4 >= floor(p 2^32) of the Philox4x32-10 block of counter (e / 4, rng[1]) and key
+ * rng[0]; rng: two int64 on the device. Its gradient by x is the same call on grad_out without residual. */
+int fc_dropout_add(int32_t dtype, int64_t n, const void* x, const void* residual, double p, const int64_t* rng,
+                   void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

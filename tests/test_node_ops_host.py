@@ -1,0 +1,65 @@
+"""Node-wise operators without a GPU: the generator's published answers, refusals, shapes of fake tensors."""
+
+import numpy as np
+import pytest
+import torch
+
+from flashcart_amd.nn import functional as F
+from oracle import node_ops as O
+
+
+@pytest.mark.parametrize("word,key,want", [
+    (0, 0, "6627e8d5 e169c58d bc57ac4c 9b00dbd8"),
+    (0xFFFFFFFF, 0xFFFFFFFF, "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+])
+def test_philox_known_answers(word, key, want):
+    got = O.philox4x32(np.full((1, 4), word, dtype=np.uint64), (key, key))[0]
+    assert " ".join(f"{int(v):08x}" for v in got) == want
+
+
+def test_cpu_tensors_are_refused():
+    table, rng = torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        F.embedding(torch.zeros(2, dtype=torch.int64), table)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        F.dropout_add(table, None, 0.5, rng)
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda: F.embedding(torch.zeros(2), torch.zeros(3, 4)), "int64 or int32"),
+    (lambda: F.embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4), padding_idx=3), "outside the table"),
+    (lambda: F.embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4), padding_idx=-4), "outside the table"),
+    (lambda: F.embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4, dtype=torch.float64)), "float32, bfloat16"),
+    (lambda: F.dropout_add(torch.zeros(3, dtype=torch.int32), None, 0.5, torch.zeros(2)), "float32, bfloat16"),
+])
+def test_arguments_are_refused(call, error):
+    with pytest.raises((TypeError, ValueError), match=error):
+        call()
+
+
+def test_fake_tensors_have_the_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        ids, table = torch.empty(2, 5, dtype=torch.int64), torch.empty(7, 3, dtype=torch.bfloat16)
+        assert F.embedding(ids, table).shape == (2, 5, 3)
+        x = torch.empty(4, 6, dtype=torch.float16)
+        assert F.dropout_add(x, x, 0.1, torch.empty(2, dtype=torch.int64)).shape == (4, 6)
+
+
+def test_library_refuses_bad_arguments():
+    """Status codes of the C entry points, decided before anything is launched."""
+    from flashcart_amd import _lib
+    lib = _lib.load()
+    bad_desc, shape, null, workspace = 1, 4, 5, 6
+    assert lib.fc_embedding_fwd(3, 1, 1, 1, 1, 1, 1.0, 1, None) == bad_desc
+    assert lib.fc_embedding_fwd(0, -1, 1, 1, None, None, 1.0, None, None) == shape
+    assert lib.fc_embedding_fwd(0, 1, 0, 1, None, None, 1.0, None, None) == shape
+    assert lib.fc_embedding_fwd(0, 1, 1, 1, None, None, 1.0, None, None) == null
+    assert lib.fc_embedding_bwd_workspace(0, 1 << 31, 4, 4) == -shape
+    need = lib.fc_embedding_bwd_workspace(1, 100, 7, 16)
+    assert need > 0
+    assert lib.fc_embedding_bwd(1, 100, 7, 16, 16, 16, 1.0, -1, 16, 16, need - 1, None) == workspace
+    for p in (-0.1, 1.1, float("nan")):
+        assert lib.fc_dropout_add(0, 1, 16, None, p, 16, 16, None) == bad_desc
+    assert lib.fc_dropout_add(0, 1, 16, None, 0.5, None, 16, None) == null
+    assert lib.fc_dropout_add(0, 0, None, None, 0.5, None, None, None) == 0
