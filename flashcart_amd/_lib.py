@@ -79,6 +79,11 @@ class LinearDescF64(ctypes.Structure):
     ]
 
 
+class FfnDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("act", c_i32), ("width", c_i32), ("hidden", c_i32), ("aligned", c_i32),
+                ("act_scale", c_f32), ("scale_in", c_f32), ("scale_out", c_f32)]
+
+
 # Element types of the node-wise operators (fc_dtype).
 NODE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -152,6 +157,11 @@ _SIGNATURES = {
     "fc_embedding_bwd_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64]),
     "fc_embedding_bwd": (c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_f32, c_i64, c_vp, c_vp, c_i64, c_vp]),
     "fc_dropout_add": (c_int, [c_i32, c_i64, c_vp, c_vp, c_f64, c_vp, c_vp, c_vp]),
+    "fc_ffn_saved": (c_i64, [ctypes.POINTER(FfnDesc), c_i64]),
+    "fc_ffn_fwd_workspace": (c_i64, [ctypes.POINTER(FfnDesc), c_i64, c_i32]),
+    "fc_ffn_fwd": (c_int, [ctypes.POINTER(FfnDesc), c_i64] + [c_vp] * 6 + [c_i64, c_vp]),
+    "fc_ffn_bwd_workspace": (c_i64, [ctypes.POINTER(FfnDesc), c_i64, c_i32, c_i32, c_i32]),
+    "fc_ffn_bwd": (c_int, [ctypes.POINTER(FfnDesc), c_i64] + [c_vp] * 9 + [c_i64, c_vp]),
     "fc_neighbor_list": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp]),
     "fc_neighbor_list_device_workspace": (c_i64, [c_i64]),
     "fc_neighbor_list_device": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp, c_vp,

@@ -1,0 +1,428 @@
+// Gated feed-forward block: [gate | up] = s_in x W_in^T, a = c act(gate), h = a up, y = s_out h W_out^T, and its gradients
+//   dh = s_out g W_out,  d up = dh a,  d gate = dh b  with b = c act'(gate) up,
+//   dx = s_in [d gate | d up] W_in,  dW_in = s_in [d gate | d up]^T x,  dW_out = s_out g^T h.
+// Two products forward (the first forms gate and up of the same hidden columns in one workgroup and applies the
+// activation and the product in its epilogue), four backward (the first applies the factors a and b, kept from the
+// forward pass, in its epilogue). h and [d gate | d up] are rounded to the operator's type between the products, as
+// operands of the 16-bit matrix instructions; everything else is float32 until an output is rounded.
+#include "fc_ffn_gemm.h"
+
+namespace fc {
+
+// ---- operands whose rows are not a multiple of 16 bytes, and float32 operands: a padded copy, split into planes ----
+struct PrepItem {
+  const void* src;
+  uint16_t* dst;
+  int64_t cols, ld, plane;  // of src; of dst
+  int32_t rows, rows_out, gap_at, gap;  // dst row r is src row r (r < gap_at) or r - gap (r >= gap_at + gap), else zeros
+  int32_t block_base;
+};
+struct PrepArgs {
+  PrepItem it[4];
+  int32_t count;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
+  int k = 0;
+#pragma unroll
+  for (int q = 1; q < 4; ++q)
+    if (q < a.count && (int)blockIdx.x >= a.it[q].block_base) k = q;
+  const PrepItem& it = a.it[k];
+  const int64_t chunks = it.ld / 8, t = (int64_t)(blockIdx.x - it.block_base) * 256 + threadIdx.x;
+  if (t >= it.rows_out * chunks) return;
+  const int64_t row = t / chunks, c0 = (t - row * chunks) * 8;
+  int64_t from = row < it.gap_at ? row : row < it.gap_at + it.gap ? -1 : row - it.gap;
+  if (from >= it.rows) from = -1;
+  float x[8];
+  const T* src = (const T*)it.src + from * it.cols + c0;
+  if (from >= 0 && c0 + 8 <= it.cols) {
+    const Pack<T, 8> v = load_pack<T, 8>(src);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = from >= 0 && c0 + i < it.cols ? to_f32(src[i]) : 0.f;
+  }
+  const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+  uint16_t* dst = it.dst + row * it.ld + c0;
+  using MT = std::conditional_t<std::is_same_v<T, float>, bf16_t, T>;
+  put4<MT, std::is_same_v<T, float>>(dst, it.plane, lo);
+  put4<MT, std::is_same_v<T, float>>(dst + 4, it.plane, hi);
+}
+
+// ---- sum over the parts of a split K loop ----
+template <class OT, bool F32, bool ATR, bool BTR>
+__global__ void __launch_bounds__(256) ffn_sum_kernel(FfnJob g) {
+  const int64_t chunks = g.N / 4, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= g.M * chunks) return;
+  int64_t row = t / chunks;
+  const int64_t col = (t - row * chunks) * 4, m = row;
+  f32x4v s{0.f, 0.f, 0.f, 0.f};
+  const float* p = g.partial + row * g.N + col;
+  for (int k = 0; k < g.splits; ++k) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+  if (row >= g.gap_at) {
+    if (row < g.gap_at + g.gap) return;
+    row -= g.gap;
+  }
+  if (row >= g.m_out) return;
+  OT* out = (OT*)g.out + row * g.ld_out;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    if (col + v >= g.n_out) break;
+    float x = s[v] * g.scale;
+    if constexpr (F32) {
+      if (!(fabsf(x) < __builtin_inff())) {  // again in plain float32, as where the sum is not split
+        x = 0.f;
+        const int k_end = max(g.A.k, g.B.k);
+        for (int k = 0; k < k_end; ++k) x = fmaf(g.scale * plane_sum<ATR>(g.A, m, k), plane_sum<BTR>(g.B, col + v, k), x);
+      }
+    }
+    out[col + v] = from_f32<OT>(x);
+  }
+}
+
+using TileL = Tile<256, 256, 2, 4>;
+using TileM = Tile<128, 128, 2, 2>;
+using TileS = Tile<64, 64, 2, 2>;
+
+template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI>
+__global__ void __launch_bounds__(T::NT) ffn_gemm_kernel(FfnJob g) {
+  __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
+  FfnTile<T, MT, F32, ATR, BTR, EPI>::run(g, blockIdx.x, (lds_char*)lds0, (lds_char*)lds1);
+}
+
+static int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <class T>
+static void count_tiles(FfnJob& g, bool gate) {
+  g.tiles_m = cdiv(g.M, T::BM);
+  g.tiles_n = cdiv(g.N, gate ? T::BN / 2 : T::BN);
+}
+
+// Tile size: the largest that still fills the device; splits of the K loop (plain outputs only) where even the smallest
+// does not.
+static int plan_job(FfnJob& g, bool f32, bool gate, bool can_split) {
+  const int cus = device_cu_count();
+  g.steps = cdiv(g.A.k > g.B.k ? g.A.k : g.B.k, 64) * (f32 ? 6 : 1);
+  g.splits = 1;
+  int kind = 2;
+  count_tiles<TileL>(g, gate);
+  if ((int64_t)g.tiles_m * g.tiles_n < cus / 2) {
+    kind = 1;
+    count_tiles<TileM>(g, gate);
+    if ((int64_t)g.tiles_m * g.tiles_n < cus / 2) {
+      kind = 0;
+      count_tiles<TileS>(g, gate);
+    }
+  }
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  if (can_split && tiles < cus && g.steps >= 8) {
+    g.splits = (int)(2 * cus / tiles);
+    if (g.splits > g.steps / 4) g.splits = g.steps / 4;
+    if (g.splits < 1) g.splits = 1;
+  }
+  return kind;
+}
+static int64_t partial_bytes(const FfnJob& g) { return g.splits > 1 ? 4ll * g.splits * g.M * g.N : 0; }
+
+template <class MT, bool F32, bool ATR, bool BTR, int EPI>
+static int launch(const FfnJob& g, int kind, hipStream_t s) {
+  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks);
+  if (kind == 2) hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR, BTR, EPI>), grid, dim3(TileL::NT), 0, s, g);
+  else if (kind == 1) hipLaunchKernelGGL((ffn_gemm_kernel<TileM, MT, F32, ATR, BTR, EPI>), grid, dim3(TileM::NT), 0, s, g);
+  else hipLaunchKernelGGL((ffn_gemm_kernel<TileS, MT, F32, ATR, BTR, EPI>), grid, dim3(TileS::NT), 0, s, g);
+  FC_LAUNCH_CHECK();
+  if constexpr (EPI == EPI_OUT) {
+    if (g.splits > 1) {
+      using OT = std::conditional_t<F32, float, MT>;
+      hipLaunchKernelGGL((ffn_sum_kernel<OT, F32, ATR, BTR>), dim3(cdiv((int64_t)g.M * (g.N / 4), 256)), dim3(256), 0, s, g);
+      FC_LAUNCH_CHECK();
+    }
+  }
+  return FC_OK;
+}
+
+static int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+
+// What is where, for one call; pointers are null where only sizes are asked for.
+struct Ffn {
+  const fc_ffn_desc& d;
+  int64_t n, w, hid, wp, hp, esize;
+  bool f32;
+  int planes;
+  char* ws;
+  int64_t at = 0;
+  PrepArgs prep{};
+  int64_t prep_blocks = 0;
+
+  Ffn(const fc_ffn_desc& desc, int64_t rows, void* workspace)
+      : d(desc), n(rows), w(desc.width), hid(desc.hidden), wp(up8(w)), hp(up8(hid)), esize(node_dtype_size(desc.dtype)),
+        f32(desc.dtype == FC_F32), planes(f32 ? 3 : 1), ws((char*)workspace) {}
+
+  char* take(int64_t bytes) {
+    char* p = ws + at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  // (rows, cols) of the caller as an operand: itself, or its padded copy of rows_out rows
+  Opnd operand(const void* src, int64_t rows, int64_t cols, int64_t rows_out, int64_t gap_at) {
+    const int64_t ld = up8(cols);
+    Opnd o{};
+    o.ld = ld;
+    if (!f32 && d.aligned && ld == cols && rows == rows_out) {
+      o.p = (const uint16_t*)src;
+      return o;
+    }
+    PrepItem& it = prep.it[prep.count++];
+    o.plane = rows_out * ld;
+    it.src = src;
+    it.dst = (uint16_t*)take(2 * planes * o.plane);
+    it.cols = cols;
+    it.ld = ld;
+    it.plane = o.plane;
+    it.rows = (int32_t)rows;
+    it.rows_out = (int32_t)rows_out;
+    it.gap_at = (int32_t)gap_at;
+    it.gap = (int32_t)(gap_at < rows_out ? (rows_out - rows) / 2 : 0);
+    it.block_base = (int32_t)prep_blocks;
+    prep_blocks += (o.plane / 8 + 255) / 256;
+    o.p = it.dst;
+    return o;
+  }
+  Opnd x(const void* p) { return operand(p, n, w, n, INT32_MAX); }
+  Opnd w_out(const void* p) { return operand(p, w, hid, w, INT32_MAX); }
+  Opnd w_in(const void* p) { return operand(p, 2 * hid, w, 2 * hp, hid); }
+  int run_prep(hipStream_t s) {
+    if (prep.count == 0) return FC_OK;
+    if (prep_blocks > 0x7fffffff) return FC_ERR_SHAPE;
+    const dim3 grid((unsigned)prep_blocks), block(256);
+    return with_dtype(d.dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      hipLaunchKernelGGL((ffn_prep_kernel<T>), grid, block, 0, s, prep);
+      FC_LAUNCH_CHECK();
+      return FC_OK;
+    });
+  }
+  int64_t h_bytes() const { return 2 * planes * n * hp; }
+  int64_t factor_bytes() const { return (f32 ? 8 : 6) * n * hp; }
+};
+
+static Opnd view(Opnd o, int64_t rows, int64_t k) {
+  o.rows = (int32_t)rows;
+  o.k = (int32_t)k;
+  return o;
+}
+
+static void set_out(FfnJob& g, void* out, int64_t m_out, int64_t n_out, float scale) {
+  g.out = out;
+  g.ld_out = n_out;
+  g.m_out = (int32_t)m_out;
+  g.n_out = (int32_t)n_out;
+  g.gap_at = INT32_MAX;
+  g.scale = scale;
+}
+
+static int ffn_check(const fc_ffn_desc* d, int64_t n) {
+  if (!d) return FC_ERR_NULL;
+  if (!node_dtype_ok(d->dtype) || d->act < 0 || d->act > 2) return FC_ERR_BAD_DESC;
+  if (d->width < 1 || d->hidden < 1 || d->width > (1 << 20) || d->hidden > (1 << 20) || n < 0 || n > 0x7ffffff)
+    return FC_ERR_SHAPE;
+  return FC_OK;
+}
+
+struct FfnFwd {
+  FfnJob gate{}, out{};
+  int gate_kind, out_kind;
+};
+static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_out, void* saved, void* y) {
+  FfnFwd p;
+  const Opnd ox = f.x(x), oi = f.w_in(w_in), oo = f.w_out(w_out);
+  char* keep = saved ? (char*)saved : f.take(f.h_bytes());
+  FfnJob& g = p.gate;
+  g.A = view(ox, f.n, f.wp);
+  g.B = view(oi, f.hp, f.wp);
+  g.M = (int32_t)f.n;
+  g.N = (int32_t)f.hp;
+  g.n_out = (int32_t)f.hid;
+  g.scale = f.d.scale_in;
+  g.h = (uint16_t*)keep;
+  g.h_plane = f.n * f.hp;
+  g.saved = saved ? keep + f.h_bytes() : nullptr;
+  g.act = f.d.act;
+  g.act_scale = f.d.act_scale;
+  p.gate_kind = plan_job(g, f.f32, true, false);
+  FfnJob& o = p.out;
+  Opnd h{};
+  h.p = (const uint16_t*)keep;
+  h.ld = f.hp;
+  h.plane = f.n * f.hp;
+  o.A = view(h, f.n, f.hp);
+  o.B = view(oo, f.w, f.hp);
+  o.M = (int32_t)f.n;
+  o.N = (int32_t)f.wp;
+  set_out(o, y, f.n, f.w, f.d.scale_out);
+  p.out_kind = plan_job(o, f.f32, false, true);
+  o.partial = (float*)f.take(partial_bytes(o));
+  return p;
+}
+
+struct FfnBwd {
+  FfnJob dh{}, dx{}, dwi{}, dwo{};
+  int dh_kind = 0, dx_kind = 0, dwi_kind = 0, dwo_kind = 0;
+};
+static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in, const void* w_out, const void* saved,
+                       int need, void* gx, void* gwi, void* gwo) {
+  FfnBwd p;
+  const bool nx = need & 1, ni = need & 2, no = need & 4;
+  const Opnd og = f.x(grad);
+  Opnd h{};
+  h.p = (const uint16_t*)saved;
+  h.ld = f.hp;
+  h.plane = f.n * f.hp;
+  Opnd dpre{};
+  if (nx || ni) {
+    const Opnd oo = f.w_out(w_out);
+    dpre.ld = 2 * f.hp;
+    dpre.plane = f.n * 2 * f.hp;
+    dpre.p = (const uint16_t*)f.take(2 * f.planes * dpre.plane);
+    FfnJob& g = p.dh;
+    g.A = view(og, f.n, f.wp);
+    g.B = view(oo, f.hp, f.w);
+    g.M = (int32_t)f.n;
+    g.N = (int32_t)f.hp;
+    g.n_out = (int32_t)f.hid;
+    g.scale = f.d.scale_out;
+    g.saved = saved ? (char*)saved + f.h_bytes() : nullptr;
+    g.dpre = (uint16_t*)dpre.p;
+    g.dpre_plane = dpre.plane;
+    p.dh_kind = plan_job(g, f.f32, false, false);
+  }
+  if (nx) {
+    const Opnd oi = f.w_in(w_in);
+    FfnJob& g = p.dx;
+    g.A = view(dpre, f.n, 2 * f.hp);
+    g.B = view(oi, f.wp, 2 * f.hp);
+    g.M = (int32_t)f.n;
+    g.N = (int32_t)f.wp;
+    set_out(g, gx, f.n, f.w, f.d.scale_in);
+    p.dx_kind = plan_job(g, f.f32, false, true);
+    g.partial = (float*)f.take(partial_bytes(g));
+  }
+  if (ni) {
+    const Opnd ox = f.x(x);
+    FfnJob& g = p.dwi;
+    g.A = view(dpre, 2 * f.hp, f.n);
+    g.B = view(ox, f.wp, f.n);
+    g.M = (int32_t)(2 * f.hp);
+    g.N = (int32_t)f.wp;
+    set_out(g, gwi, 2 * f.hid, f.w, f.d.scale_in);
+    g.gap_at = (int32_t)f.hid;
+    g.gap = (int32_t)(f.hp - f.hid);
+    p.dwi_kind = plan_job(g, f.f32, false, true);
+    g.partial = (float*)f.take(partial_bytes(g));
+  }
+  if (no) {
+    FfnJob& g = p.dwo;
+    g.A = view(og, f.wp, f.n);
+    g.B = view(h, f.hp, f.n);
+    g.M = (int32_t)f.wp;
+    g.N = (int32_t)f.hp;
+    set_out(g, gwo, f.w, f.hid, f.d.scale_out);
+    p.dwo_kind = plan_job(g, f.f32, false, true);
+    g.partial = (float*)f.take(partial_bytes(g));
+  }
+  return p;
+}
+
+// f(operand type, is it float32 in planes)
+template <class F>
+static int with_operand(int32_t dtype, F&& f) {
+  if (dtype == FC_F32) return f(bf16_t{}, std::true_type{});
+  if (dtype == FC_BF16) return f(bf16_t{}, std::false_type{});
+  return f(f16_t{}, std::false_type{});
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" int64_t fc_ffn_saved(const fc_ffn_desc* d, int64_t n) {
+  const int st = ffn_check(d, n);
+  if (st != FC_OK) return -st;
+  Ffn f(*d, n, nullptr);
+  return f.h_bytes() + f.factor_bytes();
+}
+
+extern "C" int64_t fc_ffn_fwd_workspace(const fc_ffn_desc* d, int64_t n, int32_t save) {
+  const int st = ffn_check(d, n);
+  if (st != FC_OK) return -st;
+  Ffn f(*d, n, nullptr);
+  plan_fwd(f, nullptr, nullptr, nullptr, save ? (void*)16 : nullptr, nullptr);
+  return f.at;
+}
+
+extern "C" int fc_ffn_fwd(const fc_ffn_desc* d, int64_t n, const void* x, const void* w_in, const void* w_out, void* y,
+                          void* saved, void* ws, int64_t ws_bytes, void* stream) {
+  int st = ffn_check(d, n);
+  if (st != FC_OK) return st;
+  if (n == 0) return FC_OK;
+  if (!x || !w_in || !w_out || !y) return FC_ERR_NULL;
+  if (d->aligned && !(aligned16(x) && aligned16(w_in) && aligned16(w_out))) return FC_ERR_BAD_DESC;
+  Ffn f(*d, n, ws);
+  FfnFwd p = plan_fwd(f, x, w_in, w_out, saved, y);
+  if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
+  if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  st = f.run_prep(s);
+  if (st != FC_OK) return st;
+  return with_operand(d->dtype, [&](auto m, auto is32) -> int {
+    using MT = decltype(m);
+    constexpr bool F32 = decltype(is32)::value;
+    const int r = launch<MT, F32, false, false, EPI_GATE>(p.gate, p.gate_kind, s);
+    return r != FC_OK ? r : launch<MT, F32, false, false, EPI_OUT>(p.out, p.out_kind, s);
+  });
+}
+
+extern "C" int64_t fc_ffn_bwd_workspace(const fc_ffn_desc* d, int64_t n, int32_t need_x, int32_t need_w_in,
+                                        int32_t need_w_out) {
+  const int st = ffn_check(d, n);
+  if (st != FC_OK) return -st;
+  Ffn f(*d, n, nullptr);
+  plan_bwd(f, nullptr, nullptr, nullptr, nullptr, nullptr, (need_x != 0) | 2 * (need_w_in != 0) | 4 * (need_w_out != 0),
+           nullptr, nullptr, nullptr);
+  return f.at;
+}
+
+extern "C" int fc_ffn_bwd(const fc_ffn_desc* d, int64_t n, const void* grad, const void* x, const void* w_in,
+                          const void* w_out, const void* saved, void* gx, void* gwi, void* gwo, void* ws,
+                          int64_t ws_bytes, void* stream) {
+  int st = ffn_check(d, n);
+  if (st != FC_OK) return st;
+  const int need = (gx != nullptr) | 2 * (gwi != nullptr) | 4 * (gwo != nullptr);
+  if (n == 0 || need == 0) return n == 0 && (gwi || gwo) ? FC_ERR_SHAPE : FC_OK;
+  if (!grad || !saved || (gx && !w_in) || (gwi && !x) || ((gx || gwi) && !w_out)) return FC_ERR_NULL;
+  if (d->aligned && !(aligned16(grad) && aligned16(x) && aligned16(w_in) && aligned16(w_out))) return FC_ERR_BAD_DESC;
+  Ffn f(*d, n, ws);
+  FfnBwd p = plan_bwd(f, grad, x, w_in, w_out, saved, need, gx, gwi, gwo);
+  if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
+  if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  st = f.run_prep(s);
+  if (st != FC_OK) return st;
+  return with_operand(d->dtype, [&](auto m, auto is32) -> int {
+    using MT = decltype(m);
+    constexpr bool F32 = decltype(is32)::value;
+    int r = FC_OK;
+    if (gx || gwi) r = launch<MT, F32, false, true, EPI_DH>(p.dh, p.dh_kind, s);
+    if (r == FC_OK && gwo) r = launch<MT, F32, true, true, EPI_OUT>(p.dwo, p.dwo_kind, s);
+    if (r == FC_OK && gwi) r = launch<MT, F32, true, true, EPI_OUT>(p.dwi, p.dwi_kind, s);
+    if (r == FC_OK && gx) r = launch<MT, F32, false, true, EPI_OUT>(p.dx, p.dx_kind, s);
+    return r;
+  });
+}

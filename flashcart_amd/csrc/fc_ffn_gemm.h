@@ -1,0 +1,477 @@
+// Matrix products of the gated feed-forward block (included by fc_ffn.hip): D[m, n] = sum_k A(m, k) B(n, k) on the 16-bit
+// matrix instructions with float32 accumulation, with the block's elementwise steps in the epilogues.
+//
+// Operands lie as (rows, K), or as (K, rows) ("TR"), so that no operand of the backward pass is transposed in memory.
+// float32 operands come as three bf16 planes (x = h + m + l, each the nearest bf16 of what the ones before it leave: the
+// split is exact); the K loop then runs over the six plane pairs of relative size 1, 2^-8, 2^-16, smallest first, and
+// what is left out is below 2^-24 of a product. A result that comes out infinite or NaN is formed again in plain float32.
+//
+// Tiles of BM x BN outputs and 64 k, by waves of 16x16x32 instructions. Both operand tiles go from memory to LDS without
+// passing through registers, one step ahead of the products. Chunks of 16 bytes are permuted on the way so that the
+// reads of the fragments spread over the banks: a (rows, 64) tile is read 16 bytes a lane, a (64, rows) tile by the
+// transposing LDS read, whose group of 16 lanes takes 4 k x 16 rows and returns 4 consecutive k of one row to each.
+#pragma once
+
+#include "fc_node.h"
+
+namespace fc {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+template <class MT>
+__device__ __forceinline__ f32x4v mfma16(const s16x8& a, const s16x8& b, const f32x4v& c) {
+  if constexpr (std::is_same_v<MT, f16_t>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// One operand: `rows` output rows (or columns), k valid up to `k`; element (r, k) at p[r * ld + k], or p[k * ld + r].
+// ld is a multiple of 8 and p is aligned to 16 bytes; in the TR form `rows` is a multiple of 8 too.
+struct Opnd {
+  const uint16_t* p;
+  int64_t ld, plane;  // elements; plane: from one bf16 plane to the next
+  int32_t rows, k;
+};
+
+enum { EPI_GATE = 0, EPI_OUT = 1, EPI_DH = 2 };
+
+struct FfnJob {
+  Opnd A, B;
+  int32_t M, N;          // outputs; for EPI_GATE N is the hidden size of one half, padded to 8
+  int32_t tiles_m, tiles_n, splits, steps;  // steps: of 64 k, over all planes; a split takes steps / splits of them
+  int32_t block_base;
+  float scale;
+  // EPI_OUT: out (., ld_out) of the operator's type; rows m >= gap_at are written gap rows earlier, rows in between not
+  void* out;
+  int64_t ld_out;
+  int32_t n_out, m_out, gap_at, gap;
+  float* partial;        // splits > 1: (splits, M, N)
+  // EPI_GATE: h (n, N) and, in training, the factors a = c act(gate), b = c act'(gate) up; EPI_DH: a, b and dpre
+  uint16_t* h;
+  int64_t h_plane;
+  void* saved;           // 16-bit types: (3, n, N) uint16; float32: (2, n, N) float
+  uint16_t* dpre;        // (n, 2 N)
+  int64_t dpre_plane;
+  int32_t act;
+  float act_scale;
+};
+
+constexpr uint32_t kOutOfRange = 0x7ffffff0u;  // byte offset that a buffer load answers with zeros
+
+__device__ __forceinline__ void plane_pair(int i, int& a, int& b) {  // smallest products first
+  a = i == 0 ? 0 : i == 1 ? 2 : i == 2 ? 1 : i == 3 ? 0 : i == 4 ? 1 : 0;
+  b = i == 0 ? 2 : i == 1 ? 0 : i == 2 ? 1 : i == 3 ? 1 : 0;
+}
+
+// act(g) and its derivative; 0 silu, 1 sigmoid, 2 gelu (erf form)
+__device__ __forceinline__ void ffn_act(int act, float g, float& f, float& d) {
+  if (act == 2) {
+    const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    f = g * cdf;
+    d = cdf + g * __expf(-0.5f * g * g) * 0.3989422804014327f;
+    return;
+  }
+  const float s = 1.f / (1.f + __expf(-g));
+  f = act == 0 ? g * s : s;
+  d = act == 0 ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
+}
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, NT = 64 * NW;
+  static constexpr int TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
+  static constexpr int STAGE = (BM + BN) * 128;  // bytes
+};
+
+// The part of a wave in bringing one (R rows, 64 k) operand tile to LDS: R / 8 segments of 1 KB, shared by the waves.
+template <int R, int NW, bool TR>
+struct Loader {
+  static constexpr int SEGS = R / 8 / NW;
+  static_assert(R % (8 * NW) == 0, "segments");
+  const char* base[SEGS];
+  uint32_t off[SEGS];
+  int kl[TR ? SEGS : 1];  // k of the lane's chunk, counted from the step's first
+
+  // HALF > 0: rows r with r % (2 HALF) >= HALF come from `up` rows further on (gate and up rows of one weight)
+  template <int HALF>
+  __device__ __forceinline__ void init(const Opnd& o, int r0, int wave, int lane, int up) {
+#pragma unroll
+    for (int j = 0; j < SEGS; ++j) {
+      const int seg = wave + NW * j;
+      if constexpr (!TR) {
+        int row = seg * 8 + (lane >> 3);
+        int64_t first = r0;
+        if constexpr (HALF > 0) {
+          const bool second = (seg * 8) % (2 * HALF) >= HALF;
+          row = row / (2 * HALF) * HALF + row % HALF;
+          if (second) first += up;
+        }
+        base[j] = (const char*)(o.p + first * o.ld);
+        row = min(row, o.rows - 1 - r0);
+        off[j] = (uint32_t)row * (uint32_t)(o.ld * 2) + 16 * ((lane & 7) ^ (lane >> 3));
+        kl[0] = 8 * ((lane & 7) ^ (lane >> 3));
+      } else {
+        constexpr int CPR = R / 8;  // chunks per row
+        const int k = seg * (64 / CPR) + lane / CPR, phys = lane % CPR;
+        const int f = R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+        const int col = min(r0 + 8 * ((((phys >> 1) ^ f) << 1) | (phys & 1)), o.rows - 8);
+        base[j] = (const char*)o.p;
+        off[j] = (uint32_t)k * (uint32_t)(o.ld * 2) + 2 * col;
+        kl[j] = k;
+      }
+    }
+  }
+  // the step at k0 of the plane that starts `plane` elements behind the first
+  __device__ __forceinline__ void load(const Opnd& o, int k0, int64_t plane, lds_char* dst, int wave) const {
+    const int64_t shift = 2 * (plane + (TR ? (int64_t)k0 * o.ld : k0));
+    const int left = o.k - k0;
+#pragma unroll
+    for (int j = 0; j < SEGS; ++j) {
+      __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base[j] + shift), 0, kOutOfRange, 0x00020000);
+      const uint32_t at = (left >= 64 || kl[TR ? j : 0] < left) ? off[j] : kOutOfRange;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (wave + NW * j) * 1024),
+                                               16, at, 0, 0, 0);
+    }
+  }
+};
+
+// Fragments of a wave: F blocks of 16 rows from row `r0` of an operand tile of R rows; s: which 32 k of the step.
+template <int R, int F, bool TR>
+struct Reader {
+  uint32_t at[TR ? F : 2];
+  __device__ __forceinline__ void init(int r0, int lane) {
+    const int g = lane >> 4, r = lane & 15;
+    if constexpr (!TR) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = (r0 + r) * 128 + 16 * ((4 * s + g) ^ (r & 7));
+    } else {
+      const int k = 8 * g + (r >> 2);
+      const int f = R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
+#pragma unroll
+      for (int j = 0; j < F; ++j) at[j] = k * (R * 2) + (((r0 >> 4) + j) ^ f) * 32 + (r & 3) * 8;
+    }
+  }
+  __device__ __forceinline__ void read(const lds_char* tile, int s, s16x8 (&x)[F]) const {
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      if constexpr (!TR) {
+        x[j] = *(const __attribute__((address_space(3))) s16x8*)(tile + at[s] + j * 16 * 128);
+      } else {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const lds_char* p = tile + at[j] + s * 32 * (R * 2);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+        // k + 4: for R = 64 bit 1 of k is as before, bit 2 is not part of the permutation
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * (R * 2)));
+        x[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ uint64_t pack4(const uint16_t (&x)[4]) {
+  return (uint64_t)(x[0] | (uint32_t)x[1] << 16) | (uint64_t)(x[2] | (uint32_t)x[3] << 16) << 32;
+}
+template <class T>
+__device__ __forceinline__ uint16_t bits16(float x) {
+  return from_f32<T>(x).v;
+}
+
+// Three bf16 numbers whose sum is x. What rounds to infinity is cut off instead, so that only an infinite or NaN x has
+// parts that are not finite, and its other parts are zero.
+__device__ __forceinline__ void split3(float x, uint16_t& h, uint16_t& m, uint16_t& l) {
+  h = bits16<bf16_t>(x);
+  if ((h & 0x7fff) == 0x7f80) h = (uint16_t)(__float_as_uint(x) >> 16);
+  const float r = (h & 0x7f80) == 0x7f80 ? 0.f : x - to_f32(bf16_t{h});
+  m = bits16<bf16_t>(r);
+  l = bits16<bf16_t>(r - to_f32(bf16_t{m}));
+}
+
+// Four consecutive values of a (n, ld) matrix of the operator's operand form.
+template <class MT, bool F32>
+__device__ __forceinline__ void put4(uint16_t* p, int64_t plane, const float (&x)[4]) {
+  uint16_t h[4], m[4], l[4];
+  if constexpr (F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split3(x[i], h[i], m[i], l[i]);
+    *(uint64_t*)(p + plane) = pack4(m);
+    *(uint64_t*)(p + 2 * plane) = pack4(l);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = bits16<MT>(x[i]);
+  }
+  *(uint64_t*)p = pack4(h);
+}
+
+// Factors kept for the backward pass. For 16-bit types they keep 24 bits (a bf16 number cut off and the next 8 bits of
+// each of the pair in one more uint16), so that their rounding does not add to those of dpre and of the gradients.
+__device__ __forceinline__ uint32_t round24(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x7f800000u) == 0x7f800000u ? u : u + 0x7f + ((u >> 8) & 1);
+}
+template <bool F32>
+__device__ __forceinline__ void put_factors(void* saved, int64_t at, int64_t count, const float (&a)[4],
+                                            const float (&b)[4]) {
+  if constexpr (F32) {
+    float* p = (float*)saved + at;
+    *(float4*)p = make_float4(a[0], a[1], a[2], a[3]);
+    *(float4*)(p + count) = make_float4(b[0], b[1], b[2], b[3]);
+  } else {
+    uint16_t ah[4], bh[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t ua = round24(a[i]), ub = round24(b[i]);
+      ah[i] = (uint16_t)(ua >> 16);
+      bh[i] = (uint16_t)(ub >> 16);
+      lo[i] = (uint16_t)(((ua >> 8) & 255) | (ub & 0xff00));
+    }
+    uint16_t* p = (uint16_t*)saved + at;
+    *(uint64_t*)p = pack4(ah);
+    *(uint64_t*)(p + count) = pack4(bh);
+    *(uint64_t*)(p + 2 * count) = pack4(lo);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void get_factors(const void* saved, int64_t at, int64_t count, float (&a)[4], float (&b)[4]) {
+  if constexpr (F32) {
+    const float4 u = *(const float4*)((const float*)saved + at), v = *(const float4*)((const float*)saved + count + at);
+    a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
+    b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+  } else {
+    const uint16_t* p = (const uint16_t*)saved + at;
+    const uint64_t ah = *(const uint64_t*)p, bh = *(const uint64_t*)(p + count), lo = *(const uint64_t*)(p + 2 * count);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = (uint32_t)(lo >> (16 * i)) & 0xffff;
+      a[i] = __uint_as_float(((uint32_t)(ah >> (16 * i)) << 16) | (x & 255) << 8);
+      b[i] = __uint_as_float(((uint32_t)(bh >> (16 * i)) << 16) | (x & 0xff00));
+    }
+  }
+}
+
+// A float32 operand's value from its planes.
+template <bool TR>
+__device__ __forceinline__ float plane_sum(const Opnd& o, int64_t r, int k) {
+  if (k >= o.k) return 0.f;
+  const uint16_t* p = o.p + (TR ? (int64_t)k * o.ld + r : r * o.ld + k);
+  return to_f32(bf16_t{p[0]}) + (to_f32(bf16_t{p[o.plane]}) + to_f32(bf16_t{p[2 * o.plane]}));
+}
+
+template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI>
+struct FfnTile {
+  using OT = std::conditional_t<F32, float, MT>;
+
+  __device__ static __forceinline__ void run(const FfnJob& g, int block, lds_char* lds0, lds_char* lds1) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / T::WN, wn = wave % T::WN;
+    // block -> split, tile. Consecutive blocks go to the 8 XCDs in turn: each XCD takes a run of tiles, in groups of 8
+    // tile rows, whose operands its L2 then serves.
+    const int tiles = g.tiles_m * g.tiles_n;
+    int split = 0, tile = block;
+    if (g.splits > 1) {
+      split = block / tiles;
+      tile = block - split * tiles;
+    }
+    if (tiles >= 64) {
+      const int per = tiles / 8, rest = tiles % 8, x = tile % 8;
+      tile = x * per + min(x, rest) + tile / 8;
+    }
+    const int group = tile / (8 * g.tiles_n), in = tile - group * 8 * g.tiles_n;
+    const int gm = min(8, g.tiles_m - group * 8);
+    const int mt = group * 8 + in % gm, nt = in / gm;
+    constexpr int BNO = EPI == EPI_GATE ? T::BN / 2 : T::BN;  // output columns of a tile
+    const int m0 = mt * T::BM, n0 = nt * BNO;
+
+    Loader<T::BM, T::NW, ATR> la;
+    Loader<T::BN, T::NW, BTR> lb;
+    la.template init<0>(g.A, m0, wave, lane, 0);
+    lb.template init<EPI == EPI_GATE ? T::TN / 2 : 0>(g.B, n0, wave, lane, g.N);
+    Reader<T::BM, T::MF, ATR> ra;
+    Reader<T::BN, T::NF, BTR> rb;
+    ra.init(wm * T::TM, lane);
+    rb.init(wn * T::TN, lane);
+
+    f32x4v acc[T::MF][T::NF];
+#pragma unroll
+    for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+      for (int j = 0; j < T::NF; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+
+    const int s0 = (int)((int64_t)g.steps * split / g.splits), s1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
+    const int per_pair = F32 ? g.steps / 6 : g.steps;
+    auto fetch = [&](int s, lds_char* at) {
+      int pa = 0, pb = 0, k = s;
+      if constexpr (F32) {
+        const int i = s / per_pair;
+        k = s - i * per_pair;
+        plane_pair(i, pa, pb);
+      }
+      la.load(g.A, 64 * k, pa * g.A.plane, at, wave);
+      lb.load(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
+    };
+    // One step from `at`, while the next one's tiles go to `next`. The two are separate arrays and every access names
+    // one of them, so that no read waits for the loads into the other.
+    auto step = [&](int s, const lds_char* at, lds_char* next) {
+      // this step's tiles have arrived, and everyone has read the other buffer
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (s + 1 < s1) fetch(s + 1, next);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        s16x8 a[T::MF], b[T::NF];
+        ra.read(at, ks, a);
+        rb.read(at + T::BM * 128, ks, b);
+#pragma unroll
+        for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+          for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(b[j], a[i], acc[i][j]);
+      }
+    };
+    if (s0 < s1) fetch(s0, lds0);
+    for (int s = s0; s < s1; s += 2) {
+      step(s, lds0, lds1);
+      if (s + 1 >= s1) break;
+      step(s + 1, lds1, lds0);
+    }
+    const int r = lane & 15, q4 = 4 * (lane >> 4);
+    const int row0 = m0 + wm * T::TM + r;
+    float scale = g.scale;
+    if constexpr (F32) {
+      float probe = 0.f;
+#pragma unroll
+      for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+        for (int j = 0; j < T::NF; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) probe = fmaf(acc[i][j][v], 0.f, probe);
+      // (a split K loop leaves this to the sum over its parts)
+      if (g.splits == 1 && __any(probe != probe)) {
+        again(g, m0, n0, wm, wn, lane, acc);
+        scale = 1.f;
+      }
+    }
+    epilogue(g, scale, split, row0, n0, wn, q4, acc);
+  }
+
+  // In plain float32, scaled before the sum, which may stay finite where the sum of the unscaled products does not: lane
+  // (r, q) of a 16x16x4 product takes k = 4 t + q of row r.
+  __device__ static __forceinline__ void again(const FfnJob& g, int m0, int n0, int wm, int wn, int lane,
+                                            f32x4v (&acc)[T::MF][T::NF]) {
+    const int r = lane & 15, q = lane >> 4, k_end = max(g.A.k, g.B.k);
+#pragma unroll
+    for (int j = 0; j < T::NF; ++j) {
+      int64_t col;
+      if constexpr (EPI == EPI_GATE) {
+        constexpr int H = T::TN / 2;
+        col = min(n0 + wn * H + (j * 16) % H + r, g.N - 1) + (j * 16 >= H ? g.N : 0);
+      } else {
+        col = min(n0 + wn * T::TN + j * 16 + r, g.B.rows - 1);
+      }
+#pragma unroll
+      for (int i = 0; i < T::MF; ++i) {
+        f32x4v c{0.f, 0.f, 0.f, 0.f};
+        const int row = min(m0 + wm * T::TM + i * 16 + r, g.A.rows - 1);
+#pragma unroll 1
+        for (int k = q; k < k_end + q; k += 4)
+          c = __builtin_amdgcn_mfma_f32_16x16x4f32(plane_sum<BTR>(g.B, col, k),
+                                                   g.scale * plane_sum<ATR>(g.A, row, k), c, 0, 0, 0);
+        acc[i][j] = c;
+      }
+    }
+  }
+
+  __device__ static __forceinline__ void epilogue(const FfnJob& g, float scale, int split, int row0, int n0, int wn, int q4,
+                                                  f32x4v (&acc)[T::MF][T::NF]) {
+    if constexpr (EPI == EPI_OUT) {
+#pragma unroll
+      for (int i = 0; i < T::MF; ++i) {
+        int64_t row = row0 + 16 * i;
+        if (row >= g.M) continue;
+        if (g.splits > 1) {
+          float* p = g.partial + ((int64_t)split * g.M + row) * g.N;
+#pragma unroll
+          for (int j = 0; j < T::NF; ++j) {
+            const int col = n0 + wn * T::TN + 16 * j + q4;  // N is a multiple of 4
+            if (col < g.N) *(f32x4v*)(p + col) = acc[i][j];
+          }
+          continue;
+        }
+        if (row >= g.gap_at) {
+          if (row < g.gap_at + g.gap) continue;
+          row -= g.gap;
+        }
+        if (row >= g.m_out) continue;
+        OT* p = (OT*)g.out + row * g.ld_out;
+#pragma unroll
+        for (int j = 0; j < T::NF; ++j) {
+          const int col = n0 + wn * T::TN + 16 * j + q4;
+          Pack<OT, 4> o;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o.v[v] = from_f32<OT>(acc[i][j][v] * scale);
+          if (col + 4 <= g.n_out) store_pack<OT, 4>(p + col, o);
+          else
+            for (int v = 0; v < 4; ++v)
+              if (col + v < g.n_out) p[col + v] = o.v[v];
+        }
+      }
+    } else if constexpr (EPI == EPI_GATE) {
+      constexpr int HF = T::NF / 2;
+      const int64_t count = (int64_t)g.M * g.N;
+#pragma unroll
+      for (int i = 0; i < T::MF; ++i) {
+        const int64_t row = row0 + 16 * i;
+        if (row >= g.M) continue;
+#pragma unroll
+        for (int j = 0; j < HF; ++j) {
+          const int col = n0 + wn * (T::TN / 2) + 16 * j + q4;
+          if (col >= g.N) continue;
+          float a[4], b[4], h[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float gate = acc[i][j][v] * scale, up = acc[i][j + HF][v] * scale;
+            float f, d;
+            ffn_act(g.act, gate, f, d);
+            a[v] = g.act_scale * f;
+            b[v] = g.act_scale * d * up;
+            h[v] = a[v] * up;
+            if (col + v >= g.n_out) h[v] = 0.f;  // pad columns take part in the next product
+          }
+          const int64_t at = row * g.N + col;
+          put4<MT, F32>(g.h + at, g.h_plane, h);
+          if (g.saved) put_factors<F32>(g.saved, at, count, a, b);
+        }
+      }
+    } else {
+      const int64_t count = (int64_t)g.M * g.N;
+#pragma unroll
+      for (int i = 0; i < T::MF; ++i) {
+        const int64_t row = row0 + 16 * i;
+        if (row >= g.M) continue;
+#pragma unroll
+        for (int j = 0; j < T::NF; ++j) {
+          const int col = n0 + wn * T::TN + 16 * j + q4;
+          if (col >= g.N) continue;
+          float a[4], b[4], dg[4], du[4];
+          get_factors<F32>(g.saved, row * g.N + col, count, a, b);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float dh = acc[i][j][v] * scale;
+            dg[v] = col + v < g.n_out ? dh * b[v] : 0.f;
+            du[v] = col + v < g.n_out ? dh * a[v] : 0.f;
+          }
+          uint16_t* p = g.dpre + row * 2 * g.N + col;
+          put4<MT, F32>(p, g.dpre_plane, dg);
+          put4<MT, F32>(p + g.N, g.dpre_plane, du);
+        }
+      }
+    }
+  }
+};
+
+}  // namespace fc

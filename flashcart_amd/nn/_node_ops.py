@@ -1,10 +1,10 @@
-"""Registered operators of the node-wise functions (``flashcart_amd.nn.functional``): embedding and residual dropout.
-float32, bfloat16 and float16 tensors on a ROCm device; every value is formed in float32 and rounded once.
+"""Registered operators of the node-wise functions (``flashcart_amd.nn.functional``): embedding, gated feed-forward
+block, residual dropout. float32, bfloat16 and float16 tensors on a ROCm device; values are formed in float32.
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -160,3 +160,128 @@ def _dropout_backward(ctx, grad):
 
 
 _register_autograd(dropout_add, _dropout_backward, _dropout_setup)
+
+
+# ---------------------------------------------------------------------------
+# Gated feed-forward block
+# ---------------------------------------------------------------------------
+
+ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2}
+
+
+def _ffn_desc(what: str, rows: Tensor, w_in: Tensor, w_out: Tensor, act: int, act_scale: float, scale_in: float,
+              scale_out: float):
+    """(descriptor without ``aligned``, rows of the block)."""
+    code = _code("x", rows)
+    if w_out.dim() != 2 or w_in.dim() != 2 or w_in.shape[0] != 2 * w_out.shape[1] or w_in.shape[1] != w_out.shape[0]:
+        raise ValueError(f"{what}: w_in {tuple(w_in.shape)} and w_out {tuple(w_out.shape)} are not (2 hidden, width) "
+                         "and (width, hidden).")
+    width, hidden = w_out.shape
+    if width < 1 or hidden < 1 or rows.dim() < 1 or rows.shape[-1] != width:
+        raise ValueError(f"{what}: rows {tuple(rows.shape)} do not match weights of width {width}, hidden {hidden}.")
+    if act not in (0, 1, 2):
+        raise ValueError(f"{what}: act must be 0 (silu), 1 (sigmoid) or 2 (gelu), got {act}.")
+    desc = _lib.FfnDesc(code, act, width, hidden, 0, float(act_scale), float(scale_in), float(scale_out))
+    return desc, rows.numel() // width
+
+
+def _aligned(*tensors: Tensor) -> int:
+    return int(all(t.data_ptr() % 16 == 0 for t in tensors))
+
+
+@operator("flashcart::gated_feed_forward")
+def gated_feed_forward(x: Tensor, w_in: Tensor, w_out: Tensor, act: int, act_scale: float, scale_in: float,
+                       scale_out: float, save: bool) -> Tuple[Tensor, Tensor]:
+    """(y, what the backward pass needs besides the inputs, empty unless ``save``)."""
+    desc, n = _ffn_desc("gated_feed_forward", x, w_in, w_out, act, act_scale, scale_in, scale_out)
+    x = _lib.contig("x", x, x.dtype)
+    w_in, w_out = _lib.contig("w_in", w_in, x.dtype), _lib.contig("w_out", w_out, x.dtype)
+    _same_device(x, w_in=w_in, w_out=w_out)
+    desc.aligned = _aligned(x, w_in, w_out)
+    lib = _lib.load()
+    y = torch.empty_like(x)
+    saved = _workspace(x, lib.fc_ffn_saved(desc, n) if save else 0)
+    size = lib.fc_ffn_fwd_workspace(desc, n, int(save))
+    ws = _workspace(x, size)
+    _lib_call("fc_ffn_fwd", desc, n, x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), y.data_ptr(),
+              saved.data_ptr() if save and n else None, ws.data_ptr(), size, _lib.stream_of(x))
+    return y, saved
+
+
+@gated_feed_forward.register_fake
+def _(x, w_in, w_out, act, act_scale, scale_in, scale_out, save):
+    desc, n = _ffn_desc("gated_feed_forward", x, w_in, w_out, act, act_scale, scale_in, scale_out)
+    planes, factors = (3, 8) if x.dtype == torch.float32 else (1, 6)
+    size = n * -(-w_out.shape[1] // 8) * 8 * (2 * planes + factors) if save else 0
+    return torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(size, dtype=torch.uint8)
+
+
+@operator("flashcart::gated_feed_forward_bwd")
+def gated_feed_forward_bwd(grad: Tensor, x: Tensor, w_in: Tensor, w_out: Tensor, saved: Tensor, act: int,
+                           act_scale: float, scale_in: float, scale_out: float, need_x: bool, need_w_in: bool,
+                           need_w_out: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(gradient of x, of w_in, of w_out), empty where not needed."""
+    desc, n = _ffn_desc("gated_feed_forward_bwd", x, w_in, w_out, act, act_scale, scale_in, scale_out)
+    if grad.shape != x.shape:
+        raise ValueError(f"gated_feed_forward_bwd: grad {tuple(grad.shape)} and x {tuple(x.shape)} differ in shape.")
+    x = _lib.contig("x", x, x.dtype)
+    g = _lib.contig("grad", grad, x.dtype)
+    w_in, w_out = _lib.contig("w_in", w_in, x.dtype), _lib.contig("w_out", w_out, x.dtype)
+    saved = _lib.contig("saved", saved, torch.uint8)
+    _same_device(x, grad=g, w_in=w_in, w_out=w_out, saved=saved)
+    lib = _lib.load()
+    desc.aligned = _aligned(g, x, w_in, w_out)
+    if saved.numel() != lib.fc_ffn_saved(desc, n):
+        raise ValueError(f"gated_feed_forward_bwd: saved holds {saved.numel()} bytes, not the {lib.fc_ffn_saved(desc, n)} "
+                         "of a forward pass with save=True.")
+    if saved.data_ptr() % 16:
+        saved = saved.clone()
+    empty = torch.zeros_like if n == 0 else torch.empty_like
+    gx, gwi, gwo = (empty(t) if need else t.new_empty(0)
+                    for t, need in ((x, need_x), (w_in, need_w_in), (w_out, need_w_out)))
+    if n == 0:
+        return gx, gwi, gwo
+    size = lib.fc_ffn_bwd_workspace(desc, n, int(need_x), int(need_w_in), int(need_w_out))
+    ws = _workspace(x, size)
+    _lib_call("fc_ffn_bwd", desc, n, g.data_ptr(), x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), saved.data_ptr(),
+              gx.data_ptr() if need_x else None, gwi.data_ptr() if need_w_in else None,
+              gwo.data_ptr() if need_w_out else None, ws.data_ptr(), size, _lib.stream_of(x))
+    return gx, gwi, gwo
+
+
+@gated_feed_forward_bwd.register_fake
+def _(grad, x, w_in, w_out, saved, act, act_scale, scale_in, scale_out, need_x, need_w_in, need_w_out):
+    return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if need else t.new_empty(0)
+                 for t, need in ((x, need_x), (w_in, need_w_in), (w_out, need_w_out)))
+
+
+def _ffn_setup(ctx, inputs, output):
+    x, w_in, w_out = inputs[:3]
+    ctx.save_for_backward(x, w_in, w_out, output[1])
+    ctx.cfg = inputs[3:7]
+    ctx.save = inputs[7]
+    ctx.mark_non_differentiable(output[1])
+
+
+def _ffn_backward(ctx, grad, _):
+    x, w_in, w_out, saved = ctx.saved_tensors
+    need = [bool(v) for v in ctx.needs_input_grad[:3]]
+    if not any(need):
+        return (None,) * 8
+    if not ctx.save:
+        raise RuntimeError("gated_feed_forward was called with save=False: its gradients cannot be formed.")
+    grads = gated_feed_forward_bwd(grad, x, w_in, w_out, saved, *ctx.cfg, *need)
+    return (*(g if n else None for g, n in zip(grads, need)), *(None,) * 5)
+
+
+def _ffn_bwd_setup(ctx, inputs, output):
+    pass
+
+
+def _ffn_dbwd(ctx, *cots):
+    raise NotImplementedError("second derivatives of gated_feed_forward are not provided "
+                              "(its backward pass was run with create_graph=True).")
+
+
+_register_autograd(gated_feed_forward, _ffn_backward, _ffn_setup)
+_register_autograd(gated_feed_forward_bwd, _ffn_dbwd, _ffn_bwd_setup)

@@ -1,4 +1,5 @@
-"""Node-wise functions in float32, bfloat16 and float16: embedding lookup, residual dropout.
+"""Node-wise functions in float32, bfloat16 and float16: embedding lookup, gated
+feed-forward block, residual dropout.
 
 They have no counterpart among the reference's kernels (it composes torch operations). Each is a registered operator
 (``torch.ops.flashcart.*``) with an autograd formula, runs on the current stream and allocates through torch, so it can
@@ -12,7 +13,7 @@ import torch
 from flashcart_amd.nn import _node_ops
 from flashcart_amd.o3._ops import param_alias
 
-__all__ = ["dropout_add", "embedding"]
+__all__ = ["dropout_add", "embedding", "gated_feed_forward"]
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
@@ -39,6 +40,30 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         if not 0 <= padding < rows:
             raise ValueError(f"padding_idx={padding_idx} is outside the table of {rows} rows.")
     return _node_ops.embedding(ids, param_alias(table), float(scale), padding)
+
+
+def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
+                       act_scale: float = 1.0, scale_in: float = 1.0, scale_out: float = 1.0) -> torch.Tensor:
+    """``scale_out * (act_scale * act(gate) * up) @ w_out.T`` with ``[gate | up] = scale_in * x @ w_in.T``.
+
+    Args:
+        x: (..., width).
+        w_in: (2 hidden, width), the gate's rows first.
+        w_out: (width, hidden).
+        act: "silu", "sigmoid" or "gelu" (erf form).
+        act_scale, scale_in, scale_out: factors, as the rescaled activations and linear layers of this package have them.
+
+    Sums are float32. For bfloat16 and float16 the hidden values ``act(gate) * up`` and, in the backward pass, the
+    gradients of gate and up are rounded to that type, being operands of the matrix instructions; the activation and its
+    derivative are formed from unrounded values. float32 products keep float32 accuracy (operands below 2^-116 lose
+    bits). In training the block keeps the hidden values and the activation's factors: 8 bytes per hidden value (14 for
+    float32). There are no second derivatives.
+    """
+    if act not in _node_ops.ACTIVATIONS:
+        raise ValueError(f"act must be one of {sorted(_node_ops.ACTIVATIONS)}, got {act!r}.")
+    save = torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad)
+    return _node_ops.gated_feed_forward(x, param_alias(w_in), param_alias(w_out), _node_ops.ACTIVATIONS[act],
+                                        float(act_scale), float(scale_in), float(scale_out), save)[0]
 
 
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng: torch.Tensor) -> torch.Tensor:

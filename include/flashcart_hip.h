@@ -514,6 +514,27 @@ int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t width, cons
 int fc_dropout_add(int32_t dtype, int64_t n, const void* x, const void* residual, double p, const int64_t* rng,
                    void* out, void* stream);
 
+/* Gated feed-forward block: [gate | up] = scale_in x W_in^T, h = act_scale act(gate) up, y = scale_out h W_out^T; x, y
+ * (n, width), W_in (2 hidden, width) with the gate's rows first, W_out (width, hidden), all of one type. act: 0 silu,
+ * 1 sigmoid, 2 gelu (erf form). `aligned`: x, w_in, w_out and grad are aligned to 16 bytes (otherwise they are copied).
+ * width and hidden are at most 2^20, n below 2^27. */
+typedef struct fc_ffn_desc {
+  int32_t dtype, act, width, hidden, aligned;
+  float act_scale, scale_in, scale_out;
+} fc_ffn_desc;
+
+/* Sizes in bytes; `saved` and the workspaces are aligned to 16. In training `saved` (fc_ffn_saved bytes) receives h and
+ * the activation's factors, which the backward pass reads; NULL otherwise (save = 0 in the workspace query). */
+int64_t fc_ffn_saved(const fc_ffn_desc* desc, int64_t n);
+int64_t fc_ffn_fwd_workspace(const fc_ffn_desc* desc, int64_t n, int32_t save);
+int fc_ffn_fwd(const fc_ffn_desc* desc, int64_t n, const void* x, const void* w_in, const void* w_out, void* y,
+               void* saved, void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients, each formed when its pointer is non-NULL (n >= 1 where a weight's gradient is asked for). */
+int64_t fc_ffn_bwd_workspace(const fc_ffn_desc* desc, int64_t n, int32_t need_x, int32_t need_w_in, int32_t need_w_out);
+int fc_ffn_bwd(const fc_ffn_desc* desc, int64_t n, const void* grad, const void* x, const void* w_in, const void* w_out,
+               const void* saved, void* grad_x, void* grad_w_in, void* grad_w_out, void* workspace,
+               int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,8 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="ROCm devices only"):
         F.embedding(torch.zeros(2, dtype=torch.int64), table)
     with pytest.raises(RuntimeError, match="ROCm devices only"):
+        F.gated_feed_forward(torch.zeros(2, 4), torch.zeros(6, 4), torch.zeros(4, 3))
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
         F.dropout_add(table, None, 0.5, rng)
 
 
@@ -43,6 +45,8 @@ def test_fake_tensors_have_the_shapes():
         ids, table = torch.empty(2, 5, dtype=torch.int64), torch.empty(7, 3, dtype=torch.bfloat16)
         assert F.embedding(ids, table).shape == (2, 5, 3)
         x = torch.empty(4, 6, dtype=torch.float16)
+        w_in, w_out = torch.empty(20, 6, dtype=torch.float16, requires_grad=True), torch.empty(6, 10, dtype=torch.float16)
+        assert F.gated_feed_forward(x, w_in, w_out).shape == (4, 6)
         assert F.dropout_add(x, x, 0.1, torch.empty(2, dtype=torch.int64)).shape == (4, 6)
 
 
@@ -62,4 +66,16 @@ def test_library_refuses_bad_arguments():
     for p in (-0.1, 1.1, float("nan")):
         assert lib.fc_dropout_add(0, 1, 16, None, p, 16, 16, None) == bad_desc
     assert lib.fc_dropout_add(0, 1, 16, None, 0.5, None, 16, None) == null
+    desc = _lib.FfnDesc(0, 0, 8, 16, 1, 1.0, 1.0, 1.0)
+    assert lib.fc_ffn_saved(desc, 3) == 3 * 16 * 14 and lib.fc_ffn_saved(desc, -1) == -shape
+    size = lib.fc_ffn_fwd_workspace(desc, 3, 1)
+    assert size > 0 and lib.fc_ffn_fwd_workspace(desc, 3, 0) > size
+    assert lib.fc_ffn_fwd(desc, 3, 16, 16, 16, 16, 16, 16, size - 1, None) == workspace
+    assert lib.fc_ffn_fwd(desc, 3, 16, 16, 16, None, 16, 16, size, None) == null
+    assert lib.fc_ffn_fwd(desc, 3, 18, 16, 16, 16, 16, 16, size, None) == bad_desc
+    assert lib.fc_ffn_bwd(desc, 3, 16, 16, 16, 16, None, 16, None, None, 16, 1 << 20, None) == null
+    for bad, code in ((dict(dtype=3), bad_desc), (dict(act=3), bad_desc), (dict(width=0), shape),
+                      (dict(hidden=(1 << 20) + 1), shape)):
+        fields = dict(dtype=1, act=0, width=8, hidden=16, aligned=1, act_scale=1.0, scale_in=1.0, scale_out=1.0)
+        assert lib.fc_ffn_saved(_lib.FfnDesc(**{**fields, **bad}), 3) == -code
     assert lib.fc_dropout_add(0, 0, None, None, 0.5, None, None, None) == 0
