@@ -129,11 +129,13 @@ struct Loader {
     }
   }
   // the step at k0 of the plane that starts `plane` elements behind the first
+  // (segments J .. J + C - 1 of the wave)
+  template <int J, int C>
   __device__ __forceinline__ void load(const Opnd& o, int k0, int64_t plane, lds_char* dst, int wave) const {
     const int64_t shift = 2 * (plane + (TR ? (int64_t)k0 * o.ld : k0));
     const int left = o.k - k0;
 #pragma unroll
-    for (int j = 0; j < SEGS; ++j) {
+    for (int j = J; j < J + C; ++j) {
       __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base[j] + shift), 0, kOutOfRange, 0x00020000);
       const uint32_t at = (left >= 64 || kl[TR ? j : 0] < left) ? off[j] : kOutOfRange;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (wave + NW * j) * 1024),
@@ -158,18 +160,20 @@ struct Reader {
       for (int j = 0; j < F; ++j) at[j] = k * (R * 2) + (((r0 >> 4) + j) ^ f) * 32 + (r & 3) * 8;
     }
   }
-  __device__ __forceinline__ void read(const lds_char* tile, int s, s16x8 (&x)[F]) const {
+  // C of the blocks, from block J on
+  template <int J, int C>
+  __device__ __forceinline__ void read(const lds_char* tile, int s, s16x8 (&x)[C]) const {
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
+    for (int j = J; j < J + C; ++j) {
       if constexpr (!TR) {
-        x[j] = *(const __attribute__((address_space(3))) s16x8*)(tile + at[s] + j * 16 * 128);
+        x[j - J] = *(const __attribute__((address_space(3))) s16x8*)(tile + at[s] + j * 16 * 128);
       } else {
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const lds_char* p = tile + at[j] + s * 32 * (R * 2);
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
         // k + 4: for R = 64 bit 1 of k is as before, bit 2 is not part of the permutation
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * (R * 2)));
-        x[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        x[j - J] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       }
     }
   }
@@ -305,40 +309,115 @@ struct FfnTile {
 
     const int s0 = (int)((int64_t)g.steps * split / g.splits), s1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
     const int per_pair = F32 ? g.steps / 6 : g.steps;
-    auto fetch = [&](int s, lds_char* at) {
+    // the tiles of step s, or zeros past the end; A's and B's parts of them
+    auto fetch = [&](int s, lds_char* at, bool a, bool b) {
       int pa = 0, pb = 0, k = s;
       if constexpr (F32) {
         const int i = s / per_pair;
         k = s - i * per_pair;
         plane_pair(i, pa, pb);
       }
-      la.load(g.A, 64 * k, pa * g.A.plane, at, wave);
-      lb.load(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
+      if (s >= s1) k = g.steps;
+      if (a) la.template load<0, la.SEGS>(g.A, 64 * k, pa * g.A.plane, at, wave);
+      if (b) lb.template load<0, lb.SEGS>(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
     };
-    // One step from `at`, while the next one's tiles go to `next`. The two are separate arrays and every access names
-    // one of them, so that no read waits for the loads into the other.
-    auto step = [&](int s, const lds_char* at, lds_char* next) {
-      // this step's tiles have arrived, and everyone has read the other buffer
+    // The two LDS stages are separate arrays and every access names one of them, so that no read waits for the loads into
+    // the other. Pairs of steps without a branch inside: where their number is odd the last one multiplies zeros.
+    if constexpr (T::NW == 8) {
+      // Two waves of each SIMD take turns: one multiplies while the other reads LDS, then they change places at a
+      // barrier. A step is four such phases, of a quarter of the wave's outputs each:
+      //   1 reads rows 0 (a half of its rows), multiplies them with columns 0;   2 reads columns 1, rows 0 x columns 1;
+      //   3 reads rows 1, rows 1 x columns 1;   4 reads columns 0 of the NEXT step, rows 1 x columns 0.
+      // A stage has been read by all when phase 4 begins: the loads of the step after next go there in phase 4 and in
+      // phase 1 of the next step, and have to be there by the end of its phase 3.
+      constexpr int MH = T::MF / 2, NH = T::NF / 2;
+      s16x8 a[2][MH], p[2][NH], q[2][NH];
+      auto turn = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto read_done = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        turn();
+        __builtin_amdgcn_s_setprio(1);
+      };
+      auto multiply = [&](auto mi, auto nj, s16x8 (&b)[2][NH]) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < MH; ++i)
+#pragma unroll
+            for (int j = 0; j < NH; ++j)
+              acc[mi * MH + i][nj * NH + j] = mfma16<MT>(b[ks][j], a[ks][i], acc[mi * MH + i][nj * NH + j]);
+        __builtin_amdgcn_s_setprio(0);
+        turn();
+      };
+      constexpr std::integral_constant<int, 0> c0{};
+      constexpr std::integral_constant<int, 1> c1{};
+      constexpr int BO = T::BM * 128;
+      auto step = [&](int s, lds_char* at, lds_char* next, s16x8 (&b0)[2][NH], s16x8 (&b1)[2][NH]) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) ra.template read<0, MH>(at, ks, a[ks]);
+        fetch(s + 1, next, false, true);
+        read_done();
+        multiply(c0, c0, b0);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) rb.template read<NH, NH>(at + BO, ks, b1[ks]);
+        read_done();
+        multiply(c0, c1, b1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) ra.template read<MH, MH>(at, ks, a[ks]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        read_done();
+        multiply(c1, c1, b1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) rb.template read<0, NH>(next + BO, ks, b1[ks]);
+        fetch(s + 2, at, true, false);
+        read_done();
+        multiply(c1, c0, b0);
+      };
+      fetch(s0, lds0, true, true);
+      fetch(s0 + 1, lds1, true, false);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (s + 1 < s1) fetch(s + 1, next);
+      __builtin_amdgcn_s_barrier();
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        s16x8 a[T::MF], b[T::NF];
-        ra.read(at, ks, a);
-        rb.read(at + T::BM * 128, ks, b);
-#pragma unroll
-        for (int i = 0; i < T::MF; ++i)
-#pragma unroll
-          for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(b[j], a[i], acc[i][j]);
+      for (int ks = 0; ks < 2; ++ks) rb.template read<0, NH>(lds0 + BO, ks, p[ks]);
+      if (wave >= 4) turn();
+#pragma unroll 1
+      for (int s = s0; s < s1; s += 2) {
+        step(s, lds0, lds1, p, q);
+        step(s + 1, lds1, lds0, q, p);
       }
-    };
-    if (s0 < s1) fetch(s0, lds0);
-    for (int s = s0; s < s1; s += 2) {
-      step(s, lds0, lds1);
-      if (s + 1 >= s1) break;
-      step(s + 1, lds1, lds0);
+      if (wave < 4) turn();
+    } else {
+      auto step = [&](int s, const lds_char* at, lds_char* next) {
+        // this step's tiles have arrived, and everyone has read the other stage
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(s + 1, next, true, true);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          s16x8 a[T::MF], b[T::NF];
+          ra.template read<0, T::MF>(at, ks, a);
+          rb.template read<0, T::NF>(at + T::BM * 128, ks, b);
+#pragma unroll
+          for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+            for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(b[j], a[i], acc[i][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      fetch(s0, lds0, true, true);
+#pragma unroll 1
+      for (int s = s0; s < s1; s += 2) {
+        step(s, lds0, lds1);
+        step(s + 1, lds1, lds0);
+      }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int r = lane & 15, q4 = 4 * (lane >> 4);
     const int row0 = m0 + wm * T::TM + r;
     float scale = g.scale;
