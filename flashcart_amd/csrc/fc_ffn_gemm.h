@@ -128,14 +128,14 @@ struct Loader {
       }
     }
   }
-  // the step at k0 of the plane that starts `plane` elements behind the first
-  // (segments J .. J + C - 1 of the wave)
-  template <int J, int C>
+  // the step at k0 of the plane that starts `plane` elements behind the first; the segments of the wave in MASK
+  template <int MASK>
   __device__ __forceinline__ void load(const Opnd& o, int k0, int64_t plane, lds_char* dst, int wave) const {
     const int64_t shift = 2 * (plane + (TR ? (int64_t)k0 * o.ld : k0));
     const int left = o.k - k0;
 #pragma unroll
-    for (int j = J; j < J + C; ++j) {
+    for (int j = 0; j < SEGS; ++j) {
+      if (!(MASK >> j & 1)) continue;
       __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base[j] + shift), 0, kOutOfRange, 0x00020000);
       const uint32_t at = (left >= 64 || kl[TR ? j : 0] < left) ? off[j] : kOutOfRange;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (wave + NW * j) * 1024),
@@ -309,8 +309,8 @@ struct FfnTile {
 
     const int s0 = (int)((int64_t)g.steps * split / g.splits), s1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
     const int per_pair = F32 ? g.steps / 6 : g.steps;
-    // the tiles of step s, or zeros past the end; A's and B's parts of them
-    auto fetch = [&](int s, lds_char* at, bool a, bool b) {
+    // segments MA of A's tile and MB of B's of step s, zeros past the end
+    auto fetch = [&](int s, lds_char* at, auto ma, auto mb) {
       int pa = 0, pb = 0, k = s;
       if constexpr (F32) {
         const int i = s / per_pair;
@@ -318,76 +318,78 @@ struct FfnTile {
         plane_pair(i, pa, pb);
       }
       if (s >= s1) k = g.steps;
-      if (a) la.template load<0, la.SEGS>(g.A, 64 * k, pa * g.A.plane, at, wave);
-      if (b) lb.template load<0, lb.SEGS>(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
+      la.template load<ma>(g.A, 64 * k, pa * g.A.plane, at, wave);
+      lb.template load<mb>(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
     };
+    constexpr std::integral_constant<int, 15> all{};
     // The two LDS stages are separate arrays and every access names one of them, so that no read waits for the loads into
     // the other. Pairs of steps without a branch inside: where their number is odd the last one multiplies zeros.
     if constexpr (T::NW == 8) {
       // Two waves of each SIMD take turns: one multiplies while the other reads LDS, then they change places at a
-      // barrier. A step is four such phases, of a quarter of the wave's outputs each:
-      //   1 reads rows 0 (a half of its rows), multiplies them with columns 0;   2 reads columns 1, rows 0 x columns 1;
-      //   3 reads rows 1, rows 1 x columns 1;   4 reads columns 0 of the NEXT step, rows 1 x columns 0.
-      // A stage has been read by all when phase 4 begins: the loads of the step after next go there in phase 4 and in
-      // phase 1 of the next step, and have to be there by the end of its phase 3.
-      constexpr int MH = T::MF / 2, NH = T::NF / 2;
-      s16x8 a[2][MH], p[2][NH], q[2][NH];
+      // barrier. A step is two such phases. Where A is (rows, K), phase 1 reads the first half of the wave's rows and all
+      // its columns and phase 2 the other rows; where A is (K, rows) the phases are the halves of the step's k. What
+      // everyone has read in one phase is loaded again from the next phase on, for the step after next: a load has four
+      // turns (32 products each) to arrive. It is waited for, by all waves, one turn before it is read.
+      constexpr int MH = ATR ? T::MF : T::MF / 2, KH = ATR ? 1 : 2;
+      constexpr std::integral_constant<int, ATR ? 3 : 5> a1{};
+      constexpr std::integral_constant<int, ATR ? 12 : 10> a2{};
+      constexpr std::integral_constant<int, ATR ? 3 : 15> b1{};
+      constexpr std::integral_constant<int, ATR ? 12 : 0> b2{};
+      static_assert(T::MF == 8 && T::NF == 4, "segments of the halves");
+      static_assert(!ATR || BTR, "halves of k are separate segments in the (K, rows) form alone");
+      s16x8 a[KH][MH], c[KH][T::NF];
       auto turn = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       };
+      // 8 loads are younger than the oldest that the next turn reads
       auto read_done = [&]() {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
         turn();
         __builtin_amdgcn_s_setprio(1);
       };
-      auto multiply = [&](auto mi, auto nj, s16x8 (&b)[2][NH]) {
+      auto multiply = [&](auto m0) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < KH; ++ks)
 #pragma unroll
           for (int i = 0; i < MH; ++i)
 #pragma unroll
-            for (int j = 0; j < NH; ++j)
-              acc[mi * MH + i][nj * NH + j] = mfma16<MT>(b[ks][j], a[ks][i], acc[mi * MH + i][nj * NH + j]);
+            for (int j = 0; j < T::NF; ++j) acc[m0 + i][j] = mfma16<MT>(c[ks][j], a[ks][i], acc[m0 + i][j]);
         __builtin_amdgcn_s_setprio(0);
         turn();
       };
-      constexpr std::integral_constant<int, 0> c0{};
-      constexpr std::integral_constant<int, 1> c1{};
       constexpr int BO = T::BM * 128;
-      auto step = [&](int s, lds_char* at, lds_char* next, s16x8 (&b0)[2][NH], s16x8 (&b1)[2][NH]) {
+      auto step = [&](int s, lds_char* at, lds_char* next) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) ra.template read<0, MH>(at, ks, a[ks]);
-        fetch(s + 1, next, false, true);
+        for (int ks = 0; ks < KH; ++ks) {
+          rb.template read<0, T::NF>(at + BO, ks, c[ks]);
+          ra.template read<0, MH>(at, ks, a[ks]);
+        }
+        fetch(s + 1, next, a2, b2);
         read_done();
-        multiply(c0, c0, b0);
+        multiply(std::integral_constant<int, 0>{});
+        if constexpr (ATR) {
+          rb.template read<0, T::NF>(at + BO, 1, c[0]);
+          ra.template read<0, MH>(at, 1, a[0]);
+        } else {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) rb.template read<NH, NH>(at + BO, ks, b1[ks]);
+          for (int ks = 0; ks < KH; ++ks) ra.template read<MH, MH>(at, ks, a[ks]);
+        }
+        fetch(s + 2, at, a1, b1);
         read_done();
-        multiply(c0, c1, b1);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) ra.template read<MH, MH>(at, ks, a[ks]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        read_done();
-        multiply(c1, c1, b1);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) rb.template read<0, NH>(next + BO, ks, b1[ks]);
-        fetch(s + 2, at, true, false);
-        read_done();
-        multiply(c1, c0, b0);
+        multiply(std::integral_constant<int, ATR ? 0 : MH>{});
       };
-      fetch(s0, lds0, true, true);
-      fetch(s0 + 1, lds1, true, false);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) rb.template read<0, NH>(lds0 + BO, ks, p[ks]);
+      fetch(s0, lds0, a1, b1);
+      fetch(s0, lds0, a2, b2);
+      fetch(s0 + 1, lds1, a1, b1);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      turn();
       if (wave >= 4) turn();
 #pragma unroll 1
       for (int s = s0; s < s1; s += 2) {
-        step(s, lds0, lds1, p, q);
-        step(s + 1, lds1, lds0, q, p);
+        step(s, lds0, lds1);
+        step(s + 1, lds1, lds0);
       }
       if (wave < 4) turn();
     } else {
@@ -396,7 +398,7 @@ struct FfnTile {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        fetch(s + 1, next, true, true);
+        fetch(s + 1, next, all, all);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -410,7 +412,7 @@ struct FfnTile {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      fetch(s0, lds0, true, true);
+      fetch(s0, lds0, all, all);
 #pragma unroll 1
       for (int s = s0; s < s1; s += 2) {
         step(s, lds0, lds1);
