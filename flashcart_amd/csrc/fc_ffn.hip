@@ -51,10 +51,21 @@ __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
   put4<MT, std::is_same_v<T, float>>(dst + 4, it.plane, hi);
 }
 
-// ---- sum over the parts of a split K loop ----
-template <class OT, bool F32, bool ATR, bool BTR>
-__global__ void __launch_bounds__(256) ffn_sum_kernel(FfnJob g) {
-  const int64_t chunks = g.N / 4, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// ---- sums over the parts of split K loops ----
+struct SumArgs {
+  FfnJob job[3];
+  int32_t base[3];  // first workgroup of each
+  int32_t count;
+};
+
+template <class OT, bool F32>
+__global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
+  int which = 0;
+#pragma unroll
+  for (int q = 1; q < 3; ++q)
+    if (q < a.count && (int)blockIdx.x >= a.base[q]) which = q;
+  const FfnJob& g = a.job[which];
+  const int64_t chunks = g.N / 4, t = (int64_t)(blockIdx.x - a.base[which]) * 256 + threadIdx.x;
   if (t >= g.M * chunks) return;
   int64_t row = t / chunks;
   const int64_t col = (t - row * chunks) * 4, m = row;
@@ -75,74 +86,147 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(FfnJob g) {
       if (!(fabsf(x) < __builtin_inff())) {  // again in plain float32, as where the sum is not split
         x = 0.f;
         const int k_end = max(g.A.k, g.B.k);
-        for (int k = 0; k < k_end; ++k) x = fmaf(g.scale * plane_sum<ATR>(g.A, m, k), plane_sum<BTR>(g.B, col + v, k), x);
+        for (int k = 0; k < k_end; ++k) {
+          const float u = g.a_tr ? plane_sum<true>(g.A, m, k) : plane_sum<false>(g.A, m, k);
+          const float w = g.b_tr ? plane_sum<true>(g.B, col + v, k) : plane_sum<false>(g.B, col + v, k);
+          x = fmaf(g.scale * u, w, x);
+        }
       }
     }
     out[col + v] = from_f32<OT>(x);
   }
 }
 
-using TileL = Tile<256, 256, 2, 4>;
-using TileM = Tile<128, 128, 2, 2>;
-using TileS = Tile<64, 64, 2, 2>;
+using TileL = Tile<256, 256, 2, 4, 2>;
+using TileM = Tile<128, 128, 2, 2, 2>;
+using TileS = Tile<64, 64, 2, 2, 4>;
 
-template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI>
-__global__ void __launch_bounds__(T::NT) ffn_gemm_kernel(FfnJob g) {
+// The products of one launch: workgroups from `first` on take the second.
+template <class T, class MT, bool F32, bool ATR1, bool BTR1, int EPI1, bool ATR2, bool BTR2, int EPI2>
+__global__ void __launch_bounds__(T::NT) ffn_gemm_kernel(FfnJob g1, FfnJob g2, int first) {
   __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
-  FfnTile<T, MT, F32, ATR, BTR, EPI>::run(g, blockIdx.x, (lds_char*)lds0, (lds_char*)lds1);
+  __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
+  lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
+  lds_char* const l3 = (lds_char*)lds3;
+  constexpr bool SAME = ATR1 == ATR2 && BTR1 == BTR2 && EPI1 == EPI2;
+  if (SAME || (int)blockIdx.x < first) {
+    FfnTile<T, MT, F32, ATR1, BTR1, EPI1>::run(g1, blockIdx.x, l0, l1, l2, l3);
+  } else {
+    if constexpr (!SAME)
+      FfnTile<T, MT, F32, ATR2, BTR2, EPI2>::run(g2, blockIdx.x - first, l0, l1, l2, l3);
+  }
 }
 
 static int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <class T>
-static void count_tiles(FfnJob& g, bool gate) {
-  g.tiles_m = cdiv(g.M, T::BM);
-  g.tiles_n = cdiv(g.N, gate ? T::BN / 2 : T::BN);
+static int64_t blocks_of(const FfnJob& g) { return (int64_t)g.tiles_m * g.tiles_n * g.splits; }
+
+static void set_tiles(FfnJob& g, int kind, bool gate) {
+  const int bm = kind == 2 ? 256 : kind == 1 ? 128 : 64, bn = gate ? bm / 2 : bm;
+  g.tiles_m = cdiv(g.M, bm);
+  g.tiles_n = cdiv(g.N, bn);
 }
 
-// Tile size: the largest that still fills the device; splits of the K loop (plain outputs only) where even the smallest
-// does not.
-static int plan_job(FfnJob& g, bool f32, bool gate, bool can_split) {
+// What a workgroup of each tile size takes, in us: a step of 64 k when it has its CU's loads to itself, the CU's time a
+// step takes when the device is full, and filling the pipeline and writing the tile. Measured in bf16: chains of steps on
+// few CUs (n = 30,000, width = hidden = 64), full devices at 1,024 to 16,384 rows. The 64 x 64 tile is bound by what the L2
+// caches deliver, the 256 x 256 tile by the matrix cores.
+struct TileCost {
+  double step, full, end;
+  int resident;
+};
+constexpr TileCost kTileCost[3] = {{0.28, 0.28, 0.8, 2}, {0.65, 0.55, 2.5, 2}, {1.25, 1.5, 9.0, 1}};
+
+// Tile size and splits of the K loops (plain outputs only) of one launch: those of the least time by the costs above, a
+// split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them.
+static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, bool f32, bool gate) {
   const int cus = device_cu_count();
-  g.steps = cdiv(g.A.k > g.B.k ? g.A.k : g.B.k, 64) * (f32 ? 6 : 1);
-  g.splits = 1;
-  int kind = 2;
-  count_tiles<TileL>(g, gate);
-  if ((int64_t)g.tiles_m * g.tiles_n < cus / 2) {
-    kind = 1;
-    count_tiles<TileM>(g, gate);
-    if ((int64_t)g.tiles_m * g.tiles_n < cus / 2) {
-      kind = 0;
-      count_tiles<TileS>(g, gate);
+  for (int q = 0; q < count; ++q) jobs[q]->steps = cdiv(jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k, 64) * (f32 ? 6 : 1);
+  int best_kind = 0, best_splits[2] = {1, 1};
+  double best = 1e30;
+  for (int kind = 0; kind < 3; ++kind) {
+    const TileCost& c = kTileCost[kind];
+    for (double most = 1e9; most > 2; most = most > 1e8 ? 128 : most / 2) {  // of a workgroup's steps
+      double load = 0, longest = 0, sums = 0;
+      int64_t blocks = 0;
+      int splits[2] = {1, 1};
+      for (int q = 0; q < count; ++q) {
+        FfnJob& g = *jobs[q];
+        if (g.M == 0) continue;
+        set_tiles(g, kind, gate);
+        double end = c.end * (can_split[q] ? 1 : 2.5) * (f32 ? 1.5 : 1);
+        if (can_split[q] && g.steps * c.step > most) {
+          splits[q] = (int)(g.steps * c.step / most) + 1;
+          if (splits[q] > g.steps / 4) splits[q] = g.steps / 4 > 1 ? g.steps / 4 : 1;
+        }
+        if (splits[q] > 1) {
+          end *= 1.5;
+          sums += 8e-6 / 3 * splits[q] * g.M * g.N;
+        }
+        const int64_t n = (int64_t)g.tiles_m * g.tiles_n * splits[q];
+        const double steps = (double)g.steps / splits[q];
+        blocks += n;
+        load += n * (steps * c.full + end) / cus;
+        const double t = steps * c.step + end;
+        longest = t > longest ? t : longest;
+      }
+      double time = blocks > (int64_t)cus * c.resident ? load + 0.5 * longest : load > longest ? load : longest;
+      if (sums > 0) time += sums + 3.5;
+      if (time < best) {
+        best = time;
+        best_kind = kind;
+        for (int q = 0; q < count; ++q) best_splits[q] = splits[q];
+      }
     }
   }
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
-  if (can_split && tiles < cus && g.steps >= 8) {
-    g.splits = (int)(2 * cus / tiles);
-    if (g.splits > g.steps / 4) g.splits = g.steps / 4;
-    if (g.splits < 1) g.splits = 1;
+  for (int q = 0; q < count; ++q) {
+    set_tiles(*jobs[q], best_kind, gate);
+    jobs[q]->splits = best_splits[q];
   }
-  return kind;
+  return best_kind;
 }
 static int64_t partial_bytes(const FfnJob& g) { return g.splits > 1 ? 4ll * g.splits * g.M * g.N : 0; }
 
-template <class MT, bool F32, bool ATR, bool BTR, int EPI>
-static int launch(const FfnJob& g, int kind, hipStream_t s) {
-  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+// One launch of up to two products (the second may have no outputs).
+template <class MT, bool F32, bool ATR1, bool BTR1, int EPI1, bool ATR2 = ATR1, bool BTR2 = BTR1, int EPI2 = EPI1>
+static int launch(const FfnJob& g1, const FfnJob& g2, int kind, hipStream_t s) {
+  const int64_t first = g1.M > 0 ? blocks_of(g1) : 0, blocks = first + (g2.M > 0 ? blocks_of(g2) : 0);
   if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
+  if (blocks == 0) return FC_OK;
   const dim3 grid((unsigned)blocks);
-  if (kind == 2) hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR, BTR, EPI>), grid, dim3(TileL::NT), 0, s, g);
-  else if (kind == 1) hipLaunchKernelGGL((ffn_gemm_kernel<TileM, MT, F32, ATR, BTR, EPI>), grid, dim3(TileM::NT), 0, s, g);
-  else hipLaunchKernelGGL((ffn_gemm_kernel<TileS, MT, F32, ATR, BTR, EPI>), grid, dim3(TileS::NT), 0, s, g);
+  const int b = (int)first;
+  if (kind == 2)
+    hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileL::NT), 0, s,
+                       g1, g2, b);
+  else if (kind == 1)
+    hipLaunchKernelGGL((ffn_gemm_kernel<TileM, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileM::NT), 0, s,
+                       g1, g2, b);
+  else
+    hipLaunchKernelGGL((ffn_gemm_kernel<TileS, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileS::NT), 0, s,
+                       g1, g2, b);
   FC_LAUNCH_CHECK();
-  if constexpr (EPI == EPI_OUT) {
-    if (g.splits > 1) {
-      using OT = std::conditional_t<F32, float, MT>;
-      hipLaunchKernelGGL((ffn_sum_kernel<OT, F32, ATR, BTR>), dim3(cdiv((int64_t)g.M * (g.N / 4), 256)), dim3(256), 0, s, g);
-      FC_LAUNCH_CHECK();
-    }
+  return FC_OK;
+}
+
+// The sums of the products with a split K loop, in one launch.
+template <class MT, bool F32>
+static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
+  SumArgs a{};
+  int64_t blocks = 0;
+  for (int q = 0; q < count; ++q) {
+    const FfnJob& g = *jobs[q];
+    if (g.M == 0 || g.splits <= 1) continue;
+    a.base[a.count] = (int32_t)blocks;
+    a.job[a.count++] = g;
+    blocks += cdiv((int64_t)g.M * (g.N / 4), 256);
   }
+  if (blocks == 0) return FC_OK;
+  if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
+  using OT = std::conditional_t<F32, float, MT>;
+  hipLaunchKernelGGL((ffn_sum_kernel<OT, F32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  FC_LAUNCH_CHECK();
   return FC_OK;
 }
 
@@ -254,7 +338,11 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   g.saved = saved ? keep + f.h_bytes() : nullptr;
   g.act = f.d.act;
   g.act_scale = f.d.act_scale;
-  p.gate_kind = plan_job(g, f.f32, true, false);
+  {
+    FfnJob* jobs[] = {&g};
+    const bool split[] = {false};
+    p.gate_kind = plan_launch(jobs, split, 1, f.f32, true);
+  }
   FfnJob& o = p.out;
   Opnd h{};
   h.p = (const uint16_t*)keep;
@@ -265,14 +353,18 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   o.M = (int32_t)f.n;
   o.N = (int32_t)f.wp;
   set_out(o, y, f.n, f.w, f.d.scale_out);
-  p.out_kind = plan_job(o, f.f32, false, true);
+  {
+    FfnJob* jobs[] = {&o};
+    const bool split[] = {true};
+    p.out_kind = plan_launch(jobs, split, 1, f.f32, false);
+  }
   o.partial = (float*)f.take(partial_bytes(o));
   return p;
 }
 
 struct FfnBwd {
-  FfnJob dh{}, dx{}, dwi{}, dwo{};
-  int dh_kind = 0, dx_kind = 0, dwi_kind = 0, dwo_kind = 0;
+  FfnJob dh{}, dx{}, dwi{}, dwo{};  // (absent where M = 0)
+  int first_kind = 0, second_kind = 0;  // dwo and dh run together, and dwi and dx: the long ones first
 };
 static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in, const void* w_out, const void* saved,
                        int need, void* gx, void* gwi, void* gwo) {
@@ -299,7 +391,6 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     g.saved = saved ? (char*)saved + f.h_bytes() : nullptr;
     g.dpre = (uint16_t*)dpre.p;
     g.dpre_plane = dpre.plane;
-    p.dh_kind = plan_job(g, f.f32, false, false);
   }
   if (nx) {
     const Opnd oi = f.w_in(w_in);
@@ -309,8 +400,6 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     g.M = (int32_t)f.n;
     g.N = (int32_t)f.wp;
     set_out(g, gx, f.n, f.w, f.d.scale_in);
-    p.dx_kind = plan_job(g, f.f32, false, true);
-    g.partial = (float*)f.take(partial_bytes(g));
   }
   if (ni) {
     const Opnd ox = f.x(x);
@@ -322,8 +411,6 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     set_out(g, gwi, 2 * f.hid, f.w, f.d.scale_in);
     g.gap_at = (int32_t)f.hid;
     g.gap = (int32_t)(f.hp - f.hid);
-    p.dwi_kind = plan_job(g, f.f32, false, true);
-    g.partial = (float*)f.take(partial_bytes(g));
   }
   if (no) {
     FfnJob& g = p.dwo;
@@ -332,9 +419,16 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     g.M = (int32_t)f.wp;
     g.N = (int32_t)f.hp;
     set_out(g, gwo, f.w, f.hid, f.d.scale_out);
-    p.dwo_kind = plan_job(g, f.f32, false, true);
-    g.partial = (float*)f.take(partial_bytes(g));
+    g.a_tr = g.b_tr = 1;
   }
+  p.dx.b_tr = p.dwi.a_tr = p.dwi.b_tr = 1;
+  FfnJob* one[] = {&p.dwo, &p.dh};
+  const bool split_one[] = {true, false};
+  p.first_kind = plan_launch(one, split_one, 2, f.f32, false);
+  FfnJob* two[] = {&p.dwi, &p.dx};
+  const bool split_two[] = {true, true};
+  p.second_kind = plan_launch(two, split_two, 2, f.f32, false);
+  for (FfnJob* g : {&p.dwo, &p.dwi, &p.dx}) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
   return p;
 }
 
@@ -384,8 +478,10 @@ extern "C" int fc_ffn_fwd(const fc_ffn_desc* d, int64_t n, const void* x, const 
   return with_operand(d->dtype, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
-    const int r = launch<MT, F32, false, false, EPI_GATE>(p.gate, p.gate_kind, s);
-    return r != FC_OK ? r : launch<MT, F32, false, false, EPI_OUT>(p.out, p.out_kind, s);
+    const FfnJob none{}, *sums[] = {&p.out};
+    int r = launch<MT, F32, false, false, EPI_GATE>(p.gate, none, p.gate_kind, s);
+    if (r == FC_OK) r = launch<MT, F32, false, false, EPI_OUT>(p.out, none, p.out_kind, s);
+    return r != FC_OK ? r : launch_sums<MT, F32>(sums, 1, s);
   });
 }
 
@@ -418,11 +514,10 @@ extern "C" int fc_ffn_bwd(const fc_ffn_desc* d, int64_t n, const void* grad, con
   return with_operand(d->dtype, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
-    int r = FC_OK;
-    if (gx || gwi) r = launch<MT, F32, false, true, EPI_DH>(p.dh, p.dh_kind, s);
-    if (r == FC_OK && gwo) r = launch<MT, F32, true, true, EPI_OUT>(p.dwo, p.dwo_kind, s);
-    if (r == FC_OK && gwi) r = launch<MT, F32, true, true, EPI_OUT>(p.dwi, p.dwi_kind, s);
-    if (r == FC_OK && gx) r = launch<MT, F32, false, true, EPI_OUT>(p.dx, p.dx_kind, s);
+    const FfnJob* sums[] = {&p.dwo, &p.dwi, &p.dx};
+    int r = launch<MT, F32, true, true, EPI_OUT, false, true, EPI_DH>(p.dwo, p.dh, p.first_kind, s);
+    if (r == FC_OK) r = launch<MT, F32, true, true, EPI_OUT, false, true, EPI_OUT>(p.dwi, p.dx, p.second_kind, s);
+    if (r == FC_OK) r = launch_sums<MT, F32>(sums, 3, s);
     return r;
   });
 }

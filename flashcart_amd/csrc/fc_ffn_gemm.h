@@ -46,7 +46,7 @@ struct FfnJob {
   Opnd A, B;
   int32_t M, N;          // outputs; for EPI_GATE N is the hidden size of one half, padded to 8
   int32_t tiles_m, tiles_n, splits, steps;  // steps: of 64 k, over all planes; a split takes steps / splits of them
-  int32_t block_base;
+  int32_t a_tr, b_tr;    // forms of A and B
   float scale;
   // EPI_OUT: out (., ld_out) of the operator's type; rows m >= gap_at are written gap rows earlier, rows in between not
   void* out;
@@ -83,11 +83,11 @@ __device__ __forceinline__ void ffn_act(int act, float g, float& f, float& d) {
   d = act == 0 ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
 }
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, NT = 64 * NW;
   static constexpr int TM = BM / WM, TN = BN / WN, MF = TM / 16, NF = TN / 16;
-  static constexpr int STAGE = (BM + BN) * 128;  // bytes
+  static constexpr int STAGE = (BM + BN) * 128, STAGES = STAGES_;  // bytes of LDS a stage, stages
 };
 
 // The part of a wave in bringing one (R rows, 64 k) operand tile to LDS: R / 8 segments of 1 KB, shared by the waves.
@@ -271,7 +271,8 @@ template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI>
 struct FfnTile {
   using OT = std::conditional_t<F32, float, MT>;
 
-  __device__ static __forceinline__ void run(const FfnJob& g, int block, lds_char* lds0, lds_char* lds1) {
+  __device__ static __forceinline__ void run(const FfnJob& g, int block, lds_char* lds0, lds_char* lds1, lds_char* lds2,
+                                         lds_char* lds3) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / T::WN, wn = wave % T::WN;
     // block -> split, tile. Consecutive blocks go to the 8 XCDs in turn: each XCD takes a run of tiles, in groups of 8
@@ -323,7 +324,7 @@ struct FfnTile {
     };
     constexpr std::integral_constant<int, 15> all{};
     // The two LDS stages are separate arrays and every access names one of them, so that no read waits for the loads into
-    // the other. Pairs of steps without a branch inside: where their number is odd the last one multiplies zeros.
+    // the other. As many steps as there are stages without a branch inside: steps past the end multiply zeros.
     if constexpr (T::NW == 8) {
       // Two waves of each SIMD take turns: one multiplies while the other reads LDS, then they change places at a
       // barrier. A step is two such phases. Where A is (rows, K), phase 1 reads the first half of the wave's rows and all
@@ -393,12 +394,15 @@ struct FfnTile {
       }
       if (wave < 4) turn();
     } else {
+      // One barrier a step; the loads run STAGES - 1 steps ahead.
+      constexpr int AHEAD = T::STAGES - 1;
       auto step = [&](int s, const lds_char* at, lds_char* next) {
-        // this step's tiles have arrived, and everyone has read the other stage
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // this step's tiles have arrived, and everyone has read the stage of the step before
+        if constexpr (AHEAD == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 1) * (la.SEGS + lb.SEGS)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        fetch(s + 1, next, all, all);
+        fetch(s + AHEAD, next, all, all);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -413,10 +417,22 @@ struct FfnTile {
         __builtin_amdgcn_sched_barrier(0);
       };
       fetch(s0, lds0, all, all);
+      if constexpr (T::STAGES == 4) {
+        fetch(s0 + 1, lds1, all, all);
+        fetch(s0 + 2, lds2, all, all);
 #pragma unroll 1
-      for (int s = s0; s < s1; s += 2) {
-        step(s, lds0, lds1);
-        step(s + 1, lds1, lds0);
+        for (int s = s0; s < s1; s += 4) {
+          step(s, lds0, lds3);
+          step(s + 1, lds1, lds0);
+          step(s + 2, lds2, lds1);
+          step(s + 3, lds3, lds2);
+        }
+      } else {
+#pragma unroll 1
+        for (int s = s0; s < s1; s += 2) {
+          step(s, lds0, lds1);
+          step(s + 1, lds1, lds0);
+        }
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

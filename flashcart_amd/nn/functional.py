@@ -62,7 +62,7 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
     if act not in _node_ops.ACTIVATIONS:
         raise ValueError(f"act must be one of {sorted(_node_ops.ACTIVATIONS)}, got {act!r}.")
     save = torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad)
-    return _node_ops.gated_feed_forward(x, param_alias(w_in), param_alias(w_out), _node_ops.ACTIVATIONS[act],
+    return _node_ops.gated_feed_forward(param_alias(x), param_alias(w_in), param_alias(w_out), _node_ops.ACTIVATIONS[act],
                                         float(act_scale), float(scale_in), float(scale_out), save)[0]
 
 
@@ -79,4 +79,4 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng
         rng: int64 tensor (seed, offset) on x's device. The caller advances the offset from call to call (on the device
             where the call is captured into a graph): the same pair gives the same mask.
     """
-    return _node_ops.dropout_add(x, residual, float(p), rng)
+    return _node_ops.dropout_add(param_alias(x), param_alias(residual), float(p), rng)
