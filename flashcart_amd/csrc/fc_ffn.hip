@@ -54,24 +54,37 @@ __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
 // ---- sums over the parts of split K loops ----
 struct SumArgs {
   FfnJob job[3];
-  int32_t base[3];  // first workgroup of each
+  int32_t base[3];    // first workgroup of each
+  int32_t groups[3];  // lanes that share the parts of an output
   int32_t count;
 };
 
+// A workgroup forms 256 / groups times 4 outputs: the lanes of an output add every groups-th part, their sums are added in
+// order.
 template <class OT, bool F32>
 __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
+  __shared__ f32x4v part[256];
   int which = 0;
 #pragma unroll
   for (int q = 1; q < 3; ++q)
     if (q < a.count && (int)blockIdx.x >= a.base[q]) which = q;
   const FfnJob& g = a.job[which];
-  const int64_t chunks = g.N / 4, t = (int64_t)(blockIdx.x - a.base[which]) * 256 + threadIdx.x;
-  if (t >= g.M * chunks) return;
-  int64_t row = t / chunks;
-  const int64_t col = (t - row * chunks) * 4, m = row;
+  const int groups = a.groups[which], per = 256 / groups, grp = threadIdx.x / per;
+  const int64_t chunks = g.N / 4, t = (int64_t)(blockIdx.x - a.base[which]) * per + threadIdx.x % per;
+  const bool ok = t < g.M * chunks;
+  int64_t row = ok ? t / chunks : 0;
+  const int64_t col = ok ? (t - row * chunks) * 4 : 0, m = row;
   f32x4v s{0.f, 0.f, 0.f, 0.f};
   const float* p = g.partial + row * g.N + col;
-  for (int k = 0; k < g.splits; ++k) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+#pragma unroll 4
+  for (int k = grp; k < g.splits; k += groups) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+  if (groups > 1) {
+    part[threadIdx.x] = s;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int k = 1; k < groups; ++k) s += part[k * per + threadIdx.x];
+  }
+  if (!ok) return;
   if (row >= g.gap_at) {
     if (row < g.gap_at + g.gap) return;
     row -= g.gap;
@@ -218,9 +231,12 @@ static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
   for (int q = 0; q < count; ++q) {
     const FfnJob& g = *jobs[q];
     if (g.M == 0 || g.splits <= 1) continue;
+    int groups = 1;
+    while (groups < 16 && groups * 4 <= g.splits) groups *= 2;
     a.base[a.count] = (int32_t)blocks;
+    a.groups[a.count] = groups;
     a.job[a.count++] = g;
-    blocks += cdiv((int64_t)g.M * (g.N / 4), 256);
+    blocks += cdiv((int64_t)g.M * (g.N / 4), 256 / groups);
   }
   if (blocks == 0) return FC_OK;
   if (blocks > 0x7fffffff) return FC_ERR_SHAPE;

@@ -78,7 +78,7 @@ __device__ __forceinline__ void ffn_act(int act, float g, float& f, float& d) {
     d = cdf + g * __expf(-0.5f * g * g) * 0.3989422804014327f;
     return;
   }
-  const float s = 1.f / (1.f + __expf(-g));
+  const float s = __builtin_amdgcn_rcpf(1.f + __expf(-g));
   f = act == 0 ? g * s : s;
   d = act == 0 ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
 }
@@ -179,46 +179,68 @@ struct Reader {
   }
 };
 
-__device__ __forceinline__ uint64_t pack4(const uint16_t (&x)[4]) {
-  return (uint64_t)(x[0] | (uint32_t)x[1] << 16) | (uint64_t)(x[2] | (uint32_t)x[3] << 16) << 32;
-}
+// Two values of the 16-bit type, round to nearest even, a in the low half.
 template <class T>
-__device__ __forceinline__ uint16_t bits16(float x) {
-  return from_f32<T>(x).v;
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, f16_t>) {
+    return from_f32<f16_t>(a).v | (uint32_t)from_f32<f16_t>(b).v << 16;
+  } else {
+    uint32_t u;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(u) : "v"(a), "v"(b));
+    return u;
+  }
 }
 
 // Three bf16 numbers whose sum is x. What rounds to infinity is cut off instead, so that only an infinite or NaN x has
 // parts that are not finite, and its other parts are zero.
 __device__ __forceinline__ void split3(float x, uint16_t& h, uint16_t& m, uint16_t& l) {
-  h = bits16<bf16_t>(x);
+  h = from_f32<bf16_t>(x).v;
   if ((h & 0x7fff) == 0x7f80) h = (uint16_t)(__float_as_uint(x) >> 16);
   const float r = (h & 0x7f80) == 0x7f80 ? 0.f : x - to_f32(bf16_t{h});
-  m = bits16<bf16_t>(r);
-  l = bits16<bf16_t>(r - to_f32(bf16_t{m}));
+  m = from_f32<bf16_t>(r).v;
+  l = from_f32<bf16_t>(r - to_f32(bf16_t{m})).v;
 }
 
 // Four consecutive values of a (n, ld) matrix of the operator's operand form.
 template <class MT, bool F32>
 __device__ __forceinline__ void put4(uint16_t* p, int64_t plane, const float (&x)[4]) {
-  uint16_t h[4], m[4], l[4];
-  if constexpr (F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) split3(x[i], h[i], m[i], l[i]);
-    *(uint64_t*)(p + plane) = pack4(m);
-    *(uint64_t*)(p + 2 * plane) = pack4(l);
+  if constexpr (!F32) {
+    *(uint2*)p = make_uint2(pack2<MT>(x[0], x[1]), pack2<MT>(x[2], x[3]));
   } else {
+    uint32_t h[2], m[2], l[2];
+    const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = bits16<MT>(x[i]);
+    for (int i = 0; i < 4; ++i) sum = fmaf(x[i], 0.f, sum);
+    if (most < 0x1.fep127f && sum == 0.f) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float a = x[2 * i], b = x[2 * i + 1];
+        h[i] = pack2<bf16_t>(a, b);
+        const float ra = a - __uint_as_float(h[i] << 16), rb = b - __uint_as_float(h[i] & 0xffff0000u);
+        m[i] = pack2<bf16_t>(ra, rb);
+        l[i] = pack2<bf16_t>(ra - __uint_as_float(m[i] << 16), rb - __uint_as_float(m[i] & 0xffff0000u));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint16_t u[2], v[2], w[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) split3(x[2 * i + q], u[q], v[q], w[q]);
+        h[i] = u[0] | (uint32_t)u[1] << 16;
+        m[i] = v[0] | (uint32_t)v[1] << 16;
+        l[i] = w[0] | (uint32_t)w[1] << 16;
+      }
+    }
+    *(uint2*)p = make_uint2(h[0], h[1]);
+    *(uint2*)(p + plane) = make_uint2(m[0], m[1]);
+    *(uint2*)(p + 2 * plane) = make_uint2(l[0], l[1]);
   }
-  *(uint64_t*)p = pack4(h);
 }
 
-// Factors kept for the backward pass. For 16-bit types they keep 24 bits (a bf16 number cut off and the next 8 bits of
-// each of the pair in one more uint16), so that their rounding does not add to those of dpre and of the gradients.
-__device__ __forceinline__ uint32_t round24(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return (u & 0x7f800000u) == 0x7f800000u ? u : u + 0x7f + ((u >> 8) & 1);
-}
+// Factors kept for the backward pass. For 16-bit types they keep 24 bits (the upper half of a float32 and the next 8 bits
+// of each of the pair in one more uint16), so that their rounding does not add to those of dpre and of the gradients.
+// (v_perm_b32: bytes 0 to 3 are those of its second operand, 4 to 7 those of the first.)
 template <bool F32>
 __device__ __forceinline__ void put_factors(void* saved, int64_t at, int64_t count, const float (&a)[4],
                                             const float (&b)[4]) {
@@ -227,37 +249,50 @@ __device__ __forceinline__ void put_factors(void* saved, int64_t at, int64_t cou
     *(float4*)p = make_float4(a[0], a[1], a[2], a[3]);
     *(float4*)(p + count) = make_float4(b[0], b[1], b[2], b[3]);
   } else {
-    uint16_t ah[4], bh[4], lo[4];
+    uint32_t u[4], v[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t ua = round24(a[i]), ub = round24(b[i]);
-      ah[i] = (uint16_t)(ua >> 16);
-      bh[i] = (uint16_t)(ub >> 16);
-      lo[i] = (uint16_t)(((ua >> 8) & 255) | (ub & 0xff00));
+      u[i] = __float_as_uint(a[i]) + 0x80;  // (infinite and NaN stay so: the lowest bits of such a value are zero)
+      v[i] = __float_as_uint(b[i]) + 0x80;
+      lo[i] = __builtin_amdgcn_perm(v[i], u[i], 0x0c0c0501);
     }
     uint16_t* p = (uint16_t*)saved + at;
-    *(uint64_t*)p = pack4(ah);
-    *(uint64_t*)(p + count) = pack4(bh);
-    *(uint64_t*)(p + 2 * count) = pack4(lo);
+    *(uint2*)p = make_uint2(__builtin_amdgcn_perm(u[1], u[0], 0x07060302), __builtin_amdgcn_perm(u[3], u[2], 0x07060302));
+    *(uint2*)(p + count) =
+        make_uint2(__builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302));
+    *(uint2*)(p + 2 * count) =
+        make_uint2(__builtin_amdgcn_perm(lo[1], lo[0], 0x05040100), __builtin_amdgcn_perm(lo[3], lo[2], 0x05040100));
   }
 }
 template <bool F32>
-__device__ __forceinline__ void get_factors(const void* saved, int64_t at, int64_t count, float (&a)[4], float (&b)[4]) {
-  if constexpr (F32) {
-    const float4 u = *(const float4*)((const float*)saved + at), v = *(const float4*)((const float*)saved + count + at);
-    a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
-    b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
-  } else {
+struct Factors {
+  uint2 x[3];
+  __device__ __forceinline__ void load(const void* saved, int64_t at, int64_t count) {
     const uint16_t* p = (const uint16_t*)saved + at;
-    const uint64_t ah = *(const uint64_t*)p, bh = *(const uint64_t*)(p + count), lo = *(const uint64_t*)(p + 2 * count);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[i] = *(const uint2*)(p + i * count);
+  }
+  __device__ __forceinline__ void get(float (&a)[4], float (&b)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t x = (uint32_t)(lo >> (16 * i)) & 0xffff;
-      a[i] = __uint_as_float(((uint32_t)(ah >> (16 * i)) << 16) | (x & 255) << 8);
-      b[i] = __uint_as_float(((uint32_t)(bh >> (16 * i)) << 16) | (x & 0xff00));
+      const uint32_t u = i < 2 ? x[0].x : x[0].y, v = i < 2 ? x[1].x : x[1].y, lo = i < 2 ? x[2].x : x[2].y;
+      a[i] = __uint_as_float(__builtin_amdgcn_perm(u, lo, i % 2 ? 0x0706020c : 0x0504000c));
+      b[i] = __uint_as_float(__builtin_amdgcn_perm(v, lo, i % 2 ? 0x0706030c : 0x0504010c));
     }
   }
-}
+};
+template <>
+struct Factors<true> {
+  float4 x[2];
+  __device__ __forceinline__ void load(const void* saved, int64_t at, int64_t count) {
+    x[0] = *(const float4*)((const float*)saved + at);
+    x[1] = *(const float4*)((const float*)saved + count + at);
+  }
+  __device__ __forceinline__ void get(float (&a)[4], float (&b)[4]) const {
+    a[0] = x[0].x; a[1] = x[0].y; a[2] = x[0].z; a[3] = x[0].w;
+    b[0] = x[1].x; b[1] = x[1].y; b[2] = x[1].z; b[3] = x[1].w;
+  }
+};
 
 // A float32 operand's value from its planes.
 template <bool TR>
@@ -309,18 +344,44 @@ struct FfnTile {
       for (int j = 0; j < T::NF; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
     const int s0 = (int)((int64_t)g.steps * split / g.splits), s1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
+    // Where the next load of some segments is: k, and the planes (float32: the pair, smallest products first).
+    struct Cursor {
+      int left, k, pair;  // left: steps before the end
+      int64_t a, b;       // elements to the planes
+    };
     const int per_pair = F32 ? g.steps / 6 : g.steps;
-    // segments MA of A's tile and MB of B's of step s, zeros past the end
-    auto fetch = [&](int s, lds_char* at, auto ma, auto mb) {
-      int pa = 0, pb = 0, k = s;
+    auto place = [&](Cursor& c) {
       if constexpr (F32) {
-        const int i = s / per_pair;
-        k = s - i * per_pair;
-        plane_pair(i, pa, pb);
+        int pa, pb;
+        plane_pair(c.pair, pa, pb);
+        c.a = pa * g.A.plane;
+        c.b = pb * g.B.plane;
+      } else {
+        c.a = c.b = 0;
       }
-      if (s >= s1) k = g.steps;
-      la.template load<ma>(g.A, 64 * k, pa * g.A.plane, at, wave);
-      lb.template load<mb>(g.B, 64 * k, pb * g.B.plane, at + T::BM * 128, wave);
+    };
+    auto cursor_at = [&](int s) {
+      Cursor c;
+      c.left = s1 - s;
+      c.pair = F32 ? s / per_pair : 0;
+      c.k = 64 * (s - c.pair * per_pair);
+      place(c);
+      return c;
+    };
+    // segments MA of A's tile and MB of B's at the cursor, zeros past the end; the cursor goes to the next step
+    auto fetch = [&](Cursor& c, lds_char* at, auto ma, auto mb) {
+      const int k = c.left > 0 ? c.k : 64 * per_pair;
+      la.template load<ma>(g.A, k, c.a, at, wave);
+      lb.template load<mb>(g.B, k, c.b, at + T::BM * 128, wave);
+      --c.left;
+      c.k += 64;
+      if constexpr (F32) {
+        if (c.k == 64 * per_pair) {
+          c.k = 0;
+          ++c.pair;
+          place(c);
+        }
+      }
     };
     constexpr std::integral_constant<int, 15> all{};
     // The two LDS stages are separate arrays and every access names one of them, so that no read waits for the loads into
@@ -339,6 +400,7 @@ struct FfnTile {
       static_assert(T::MF == 8 && T::NF == 4, "segments of the halves");
       static_assert(!ATR || BTR, "halves of k are separate segments in the (K, rows) form alone");
       s16x8 a[KH][MH], c[KH][T::NF];
+      Cursor first = cursor_at(s0), second = first;  // of the segments that phase 1 reads, and phase 2
       auto turn = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
@@ -361,13 +423,13 @@ struct FfnTile {
         turn();
       };
       constexpr int BO = T::BM * 128;
-      auto step = [&](int s, lds_char* at, lds_char* next) {
+      auto step = [&](lds_char* at, lds_char* next) {
 #pragma unroll
         for (int ks = 0; ks < KH; ++ks) {
           rb.template read<0, T::NF>(at + BO, ks, c[ks]);
           ra.template read<0, MH>(at, ks, a[ks]);
         }
-        fetch(s + 1, next, a2, b2);
+        fetch(second, next, a2, b2);
         read_done();
         multiply(std::integral_constant<int, 0>{});
         if constexpr (ATR) {
@@ -377,32 +439,33 @@ struct FfnTile {
 #pragma unroll
           for (int ks = 0; ks < KH; ++ks) ra.template read<MH, MH>(at, ks, a[ks]);
         }
-        fetch(s + 2, at, a1, b1);
+        fetch(first, at, a1, b1);
         read_done();
         multiply(std::integral_constant<int, ATR ? 0 : MH>{});
       };
-      fetch(s0, lds0, a1, b1);
-      fetch(s0, lds0, a2, b2);
-      fetch(s0 + 1, lds1, a1, b1);
+      fetch(first, lds0, a1, b1);
+      fetch(second, lds0, a2, b2);
+      fetch(first, lds1, a1, b1);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       turn();
       if (wave >= 4) turn();
 #pragma unroll 1
       for (int s = s0; s < s1; s += 2) {
-        step(s, lds0, lds1);
-        step(s + 1, lds1, lds0);
+        step(lds0, lds1);
+        step(lds1, lds0);
       }
       if (wave < 4) turn();
     } else {
       // One barrier a step; the loads run STAGES - 1 steps ahead.
       constexpr int AHEAD = T::STAGES - 1;
-      auto step = [&](int s, const lds_char* at, lds_char* next) {
+      Cursor next_load = cursor_at(s0);
+      auto step = [&](const lds_char* at, lds_char* next) {
         // this step's tiles have arrived, and everyone has read the stage of the step before
         if constexpr (AHEAD == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 1) * (la.SEGS + lb.SEGS)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        fetch(s + AHEAD, next, all, all);
+        fetch(next_load, next, all, all);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -416,22 +479,22 @@ struct FfnTile {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
-      fetch(s0, lds0, all, all);
+      fetch(next_load, lds0, all, all);
       if constexpr (T::STAGES == 4) {
-        fetch(s0 + 1, lds1, all, all);
-        fetch(s0 + 2, lds2, all, all);
+        fetch(next_load, lds1, all, all);
+        fetch(next_load, lds2, all, all);
 #pragma unroll 1
         for (int s = s0; s < s1; s += 4) {
-          step(s, lds0, lds3);
-          step(s + 1, lds1, lds0);
-          step(s + 2, lds2, lds1);
-          step(s + 3, lds3, lds2);
+          step(lds0, lds3);
+          step(lds1, lds0);
+          step(lds2, lds1);
+          step(lds3, lds2);
         }
       } else {
 #pragma unroll 1
         for (int s = s0; s < s1; s += 2) {
-          step(s, lds0, lds1);
-          step(s + 1, lds1, lds0);
+          step(lds0, lds1);
+          step(lds1, lds0);
         }
       }
     }
@@ -545,17 +608,28 @@ struct FfnTile {
         }
       }
     } else {
+      // the factors of the next 16 rows are loaded before this one's results are stored
       const int64_t count = (int64_t)g.M * g.N;
+      Factors<F32> f[2][T::NF];
+      auto load = [&](int i, Factors<F32> (&x)[T::NF]) {
+        const int64_t row = min(row0 + 16 * i, g.M - 1);
+#pragma unroll
+        for (int j = 0; j < T::NF; ++j)
+          x[j].load(g.saved, row * g.N + min(n0 + wn * T::TN + 16 * j + q4, g.N - 4), count);
+      };
+      load(0, f[0]);
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
         const int64_t row = row0 + 16 * i;
+        if (i + 1 < T::MF) load(i + 1, f[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
         if (row >= g.M) continue;
 #pragma unroll
         for (int j = 0; j < T::NF; ++j) {
           const int col = n0 + wn * T::TN + 16 * j + q4;
           if (col >= g.N) continue;
           float a[4], b[4], dg[4], du[4];
-          get_factors<F32>(g.saved, row * g.N + col, count, a, b);
+          f[i & 1][j].get(a, b);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const float dh = acc[i][j][v] * scale;
