@@ -9,6 +9,9 @@ Tensor ranks: the default library holds the kernels of ranks 0..3 (the reference
 ``--l-max 4``) builds ``libflashcart_hip_l4.so`` with ranks 0..4 beside it, from headers generated
 into ``_build_l4/generated`` (several minutes: the rank-4 products are long unrolled kernels);
 ``flashcart_amd._lib`` loads it when ``FLASHCART_KERNEL_L_MAX=4`` is set.
+
+``libflashcart_torch.so`` (host code, g++) registers the node-wise operators of ``flashcart_amd.nn.functional`` with PyTorch;
+it opens whichever of the two libraries is in use.
 """
 
 from __future__ import annotations
@@ -24,6 +27,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libflashcart_hip.so")
+TORCH_LIB = os.path.join(HERE, "libflashcart_torch.so")
 ROOT = os.path.dirname(HERE)
 _ENV_L_MAX = "FLASHCART_KERNEL_L_MAX"
 
@@ -65,7 +69,7 @@ def _sources():
 
 def _deps_digest(gen: str) -> str:
     h = hashlib.sha256()
-    for d in (CSRC, gen, os.path.join(ROOT, "include")):
+    for d in (CSRC, os.path.join(CSRC, "torch"), gen, os.path.join(ROOT, "include")):
         for f in sorted(os.listdir(d)):
             if f.endswith((".h", ".hip", ".cpp")):
                 with open(os.path.join(d, f), "rb") as fh:
@@ -86,6 +90,24 @@ def _compile(src: str, gen: str, build_dir: str) -> str:
     return obj
 
 
+def _build_torch() -> None:
+    """Compile the PyTorch operators (``csrc/torch``) against the installed torch."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(HIPCC))
+    tmp = TORCH_LIB + ".tmp"
+    cmd = ["g++", "-O2", "-fPIC", "-std=c++17", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include_paths()),
+           f"-I{os.path.join(rocm, 'include')}", os.path.join(CSRC, "torch", "node_ops.cpp"), "-o", tmp, f"-L{lib}",
+           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for the PyTorch operators:\n{res.stderr[-6000:]}")
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(jobs: int | None = None, force: bool = True, verbose: bool = False, l_max: int | None = None) -> str:
     """Compile the library (always recompiles when ``force``) and return its path. ``l_max``
     (default: ``FLASHCART_KERNEL_L_MAX``, else 3) selects the rank-3 or the rank-4 library."""
@@ -99,14 +121,17 @@ def build(jobs: int | None = None, force: bool = True, verbose: bool = False, l_
     os.makedirs(build_dir, exist_ok=True)
     digest = _deps_digest(gen)
     stamp = os.path.join(build_dir, "stamp")
-    if not force and os.path.exists(lib_path) and os.path.exists(stamp) and open(stamp).read() == digest:
+    if (not force and os.path.exists(lib_path) and os.path.exists(TORCH_LIB) and os.path.exists(stamp)
+            and open(stamp).read() == digest):
         return lib_path
     srcs = _sources()
     jobs = jobs or min(8, os.cpu_count() or 4)
     # the longest units (the products of the highest in1 rank) first
     srcs.sort(key=lambda p: (not os.path.basename(p).startswith("fc_tp_l"), -ord(os.path.basename(p)[-5])))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        with_torch = ex.submit(_build_torch)
         objs = list(ex.map(lambda p: _compile(p, gen, build_dir), srcs))
+        with_torch.result()
     tmp = lib_path + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)

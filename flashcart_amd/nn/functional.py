@@ -11,7 +11,6 @@ from typing import Optional
 import torch
 
 from flashcart_amd.nn import _node_ops
-from flashcart_amd.o3._ops import param_alias
 
 __all__ = ["dropout_add", "embedding", "gated_feed_forward"]
 
@@ -39,7 +38,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         padding = padding_idx + rows if padding_idx < 0 else padding_idx
         if not 0 <= padding < rows:
             raise ValueError(f"padding_idx={padding_idx} is outside the table of {rows} rows.")
-    return _node_ops.embedding(ids, param_alias(table), float(scale), padding)
+    return _node_ops.ops().embedding.default(ids, table, float(scale), padding)
 
 
 def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
@@ -62,8 +61,8 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
     if act not in _node_ops.ACTIVATIONS:
         raise ValueError(f"act must be one of {sorted(_node_ops.ACTIVATIONS)}, got {act!r}.")
     save = torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad)
-    return _node_ops.gated_feed_forward(param_alias(x), param_alias(w_in), param_alias(w_out), _node_ops.ACTIVATIONS[act],
-                                        float(act_scale), float(scale_in), float(scale_out), save)[0]
+    return _node_ops.ops().gated_feed_forward.default(x, w_in, w_out, _node_ops.ACTIVATIONS[act], float(act_scale),
+                                                      float(scale_in), float(scale_out), save)[0]
 
 
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng: torch.Tensor) -> torch.Tensor:
@@ -79,4 +78,4 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng
         rng: int64 tensor (seed, offset) on x's device. The caller advances the offset from call to call (on the device
             where the call is captured into a graph): the same pair gives the same mask.
     """
-    return _node_ops.dropout_add(param_alias(x), param_alias(residual), float(p), rng)
+    return _node_ops.ops().dropout_add.default(x, residual, float(p), rng)

@@ -79,3 +79,23 @@ def test_library_refuses_bad_arguments():
         fields = dict(dtype=1, act=0, width=8, hidden=16, aligned=1, act_scale=1.0, scale_in=1.0, scale_out=1.0)
         assert lib.fc_ffn_saved(_lib.FfnDesc(**{**fields, **bad}), 3) == -code
     assert lib.fc_dropout_add(0, 0, None, None, 0.5, None, None, None) == 0
+
+
+def test_compilers_see_the_operators():
+    """One graph with the operators themselves in it (which then end in their own error on the CPU)."""
+    seen = []
+
+    def backend(graph, inputs):
+        seen.extend(str(n.target) for n in graph.graph.nodes if n.op == "call_function")
+        return graph.forward
+
+    def block(ids, table, w_in, w_out, rng):
+        e = F.embedding(ids, table, 2.0, 0)
+        return F.dropout_add(F.gated_feed_forward(e, w_in, w_out), e, 0.1, rng)
+
+    rng = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        torch.compile(block, backend=backend, fullgraph=True)(rng, torch.zeros(3, 4), torch.zeros(6, 4),
+                                                              torch.zeros(4, 3), rng)
+    for name in ("embedding", "gated_feed_forward", "dropout_add"):
+        assert any(f"flashcart.{name}.default" in t for t in seen)
