@@ -10,7 +10,8 @@
 
 namespace fc {
 
-constexpr int kEmbTile = 2048;  // keys of a workgroup in the sort
+// Keys of a workgroup in the sort: 256 times the rounds, few where there are few keys.
+inline int emb_rounds(int64_t n) { return n <= 65536 ? 4 : 8; }
 
 // ---- forward: one 16-byte chunk of a row per thread ----
 template <class T, class I>
@@ -49,7 +50,8 @@ struct EmbSort {
   int32_t* order_out;
   int32_t* hist;    // (256, tiles): counts, then the keys of the digit in earlier tiles
   int32_t* total;   // (256)
-  int32_t shift;
+  int32_t shift, passes;
+  bool scanned;     // hist holds sums and total is there
   // table to be filled with zeros by the workgroups behind the tiles
   uint8_t* fill;
   int64_t fill_bytes;
@@ -75,6 +77,7 @@ __device__ void emb_fill(uint8_t* p, int64_t bytes) {
   if (done + threadIdx.x < bytes) p[done + threadIdx.x] = 0;
 }
 
+template <int ROUNDS>
 __global__ void __launch_bounds__(256) emb_hist_kernel(EmbSort a) {
   __shared__ int32_t cnt[256];
   const int t = threadIdx.x;
@@ -86,8 +89,9 @@ __global__ void __launch_bounds__(256) emb_hist_kernel(EmbSort a) {
   if (blockIdx.x == 0 && t == 0 && a.counter) *a.counter = 0;
   cnt[t] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kEmbTile;
-  for (int k = 0; k < kEmbTile / 256; ++k) {
+  const int64_t i0 = (int64_t)blockIdx.x * 256 * ROUNDS;
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
     const int64_t i = i0 + k * 256 + t;
     if (i < a.n) atomicAdd(&cnt[(emb_key(a, i) >> a.shift) & 255], 1);
   }
@@ -95,7 +99,8 @@ __global__ void __launch_bounds__(256) emb_hist_kernel(EmbSort a) {
   a.hist[(int64_t)t * a.tiles + blockIdx.x] = cnt[t];
 }
 
-// Exclusive sum over a workgroup of 256; every thread gets the total too.
+// Exclusive sum over a workgroup of NW waves; every thread gets the total too.
+template <int NW>
 __device__ __forceinline__ int block_scan(int v, int* wave_sums, int* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int s = v;
@@ -108,7 +113,7 @@ __device__ __forceinline__ int block_scan(int v, int* wave_sums, int* total) {
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < NW; ++k) {
     const int x = wave_sums[k];
     if (k < w) before += x;
     all += x;
@@ -127,7 +132,7 @@ __global__ void __launch_bounds__(256) emb_scan_kernel(EmbSort a) {
     const int i = k + threadIdx.x;
     const int v = i < a.tiles ? h[i] : 0;
     int all;
-    const int ex = block_scan(v, ws, &all);
+    const int ex = block_scan<4>(v, ws, &all);
     if (i < a.tiles) h[i] = base + ex;
     base += all;
   }
@@ -146,20 +151,31 @@ __device__ __forceinline__ uint64_t match_digit(uint32_t d, bool active) {
   return m;
 }
 
-// Stable placement: each wave ranks 512 consecutive keys, 64 at a time.
+// Stable placement: each wave ranks consecutive keys, 64 at a time.
+template <int ROUNDS>
 __global__ void __launch_bounds__(256) emb_scatter_kernel(EmbSort a) {
-  constexpr int ROUNDS = kEmbTile / 256;
   __shared__ int32_t cnt[4][256];
   __shared__ int32_t base[256];
   __shared__ int ws[4];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
 #pragma unroll
   for (int k = 0; k < 4; ++k) cnt[k][t] = 0;
+  int total, before;
+  if (a.scanned) {
+    total = a.total[t];
+    before = a.hist[(int64_t)t * a.tiles + blockIdx.x];
+  } else {  // few tiles: their counts are added here
+    total = before = 0;
+    for (int k = 0; k < a.tiles; ++k) {
+      const int c = a.hist[(int64_t)t * a.tiles + k];
+      before += k < (int)blockIdx.x ? c : 0;
+      total += c;
+    }
+  }
   int all;
-  const int ex = block_scan(a.total[t], ws, &all);
-  base[t] = ex + a.hist[(int64_t)t * a.tiles + blockIdx.x];
+  base[t] = block_scan<4>(total, ws, &all) + before;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kEmbTile + w * (kEmbTile / 4);
+  const int64_t i0 = ((int64_t)blockIdx.x * 4 + w) * 64 * ROUNDS;
   uint32_t key[ROUNDS];
   int rank[ROUNDS];
 #pragma unroll
@@ -193,6 +209,84 @@ __global__ void __launch_bounds__(256) emb_scatter_kernel(EmbSort a) {
     const int to = cnt[w][(key[k] >> a.shift) & 255] + rank[k];
     a.keys_out[to] = key[k];
     a.order_out[to] = a.ids ? (int32_t)i : a.order[i];
+  }
+}
+
+// Up to 1024 K tokens: all passes in one workgroup, in LDS; the other workgroups fill the table. 4,000 tokens of 300 rows:
+// 11 us, where two launches a pass take 20; at 16,384 tokens (K = 16) it would take 37, the launches 30.
+template <int K>
+__global__ void __launch_bounds__(1024) emb_sort_kernel(EmbSort a) {
+  __shared__ uint32_t skey[1024 * K];
+  __shared__ uint16_t sidx[1024 * K];
+  __shared__ int32_t cnt[16][256];
+  __shared__ int ws[16];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  if (blockIdx.x > 0) {
+    const int64_t b0 = (int64_t)(blockIdx.x - 1) * kEmbFillBytes;
+    emb_fill(a.fill + b0, min((int64_t)kEmbFillBytes, a.fill_bytes - b0));
+    return;
+  }
+  if (t == 0) *a.counter = 0;
+  const int n = (int)a.n, p0 = w * 64 * K + lane;
+  uint32_t key[K];
+  int idx[K], rank[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = p0 + 64 * k;
+    key[k] = p < n ? emb_key(a, p) : 0;
+    idx[k] = p;
+  }
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = 8 * pass;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) (&cnt[0][0])[t + 1024 * k] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool ok = p0 + 64 * k < n;
+      const uint32_t d = (key[k] >> shift) & 255;
+      const uint64_t m = match_digit(d, ok);
+      const int before = __popcll(m & ((1ull << lane) - 1));
+      rank[k] = ok ? cnt[w][d] + before : 0;
+      __builtin_amdgcn_wave_barrier();
+      if (ok && before == 0) cnt[w][d] += __popcll(m);
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    int total = 0;
+    if (t < 256)
+      for (int k = 0; k < 16; ++k) {
+        const int c = cnt[k][t];
+        cnt[k][t] = total;
+        total += c;
+      }
+    int all;
+    const int base = block_scan<16>(total, ws, &all);
+    if (t < 256)
+      for (int k = 0; k < 16; ++k) cnt[k][t] += base;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (p0 + 64 * k >= n) continue;
+      const int to = cnt[w][(key[k] >> shift) & 255] + rank[k];
+      skey[to] = key[k];
+      sidx[to] = (uint16_t)idx[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int p = p0 + 64 * k;
+      if (p >= n) continue;
+      key[k] = skey[p];
+      idx[k] = sidx[p];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = p0 + 64 * k;
+    if (p >= n) continue;
+    a.keys_out[p] = key[k];
+    a.order_out[p] = idx[k];
   }
 }
 
@@ -304,17 +398,21 @@ __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
     const int64_t p = a.joins[j];
     const int64_t first = (p + 1) * a.len;  // of the second piece: the run goes on here
     const uint32_t key = a.keys[first];
-    int64_t lo = first, hi = a.n;  // keys[lo] == key; the first larger key is in (lo, hi]
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.keys[mid] == key) lo = mid;
-      else hi = mid;
+    // The run's pieces are those that begin with its key: the last one lies in [last, hi]; 256 candidates a round, the
+    // next ones first, then spread over the rest.
+    int64_t last = p, hi = a.pieces - 1;
+    for (int64_t stride = 1; last < hi; stride = (hi - last + 255) / 256) {
+      const int64_t q = last + (threadIdx.x + 1) * stride;
+      const int c = __syncthreads_count(q <= hi && a.keys[q * a.len] == key);
+      last += c * stride;
+      if (c < 256) hi = min(hi, last + stride - 1);
     }
-    const int64_t last = lo / a.len, m = last - p + 1, span = (m + groups - 1) / groups;
+    const int64_t m = last - p + 1, span = (m + groups - 1) / groups;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     if (valid > 0)
+#pragma unroll 8
       for (int64_t q = p + grp * span; q < min(p + (grp + 1) * span, last + 1); ++q) {
         float x[V];
         load_f32<float, V>((q == p ? a.tail : a.head) + q * a.width + c0, valid, x);
@@ -345,7 +443,8 @@ struct EmbPlan {
 static EmbPlan emb_plan(int32_t dtype, int64_t n, int64_t rows, int64_t width) {
   EmbPlan p{};
   const int64_t V = 16 / node_dtype_size(dtype), cols = (width + V - 1) / V;
-  p.tiles = (n + kEmbTile - 1) / kEmbTile;
+  const int64_t tile = 256 * emb_rounds(n);
+  p.tiles = (n + tile - 1) / tile;
   int ct = 1;
   while (ct < 256 && ct < cols) ct *= 2;
   p.col_threads = ct;
@@ -436,23 +535,42 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   const int64_t table_bytes = rows * width * node_dtype_size(dtype);
   const int64_t fills = (table_bytes + kEmbFillBytes - 1) / kEmbFillBytes;
   if (p.tiles + fills > 0x7fffffff || p.col_blocks > 65535) return FC_ERR_SHAPE;
-  for (int k = 0; k < p.passes; ++k) {
-    a.ids = k == 0 ? ids : nullptr;
-    a.keys = (uint32_t*)(w + p.keys[(k + 1) & 1]);
-    a.order = (int32_t*)(w + p.order[(k + 1) & 1]);
-    a.keys_out = (uint32_t*)(w + p.keys[k & 1]);
-    a.order_out = (int32_t*)(w + p.order[k & 1]);
-    a.shift = 8 * k;
-    a.fill = (uint8_t*)grad_table;
-    a.fill_bytes = table_bytes;
-    const int64_t blocks = p.tiles + (k == 0 ? fills : 0);
-    hipLaunchKernelGGL(emb_hist_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+  a.fill = (uint8_t*)grad_table;
+  a.fill_bytes = table_bytes;
+  a.passes = p.passes;
+  int last = 0;
+  if (n > 0 && n <= 4096) {
+    a.ids = ids;
+    a.keys_out = (uint32_t*)(w + p.keys[0]);
+    a.order_out = (int32_t*)(w + p.order[0]);
+    const dim3 grid((unsigned)(1 + fills)), block(1024);
+    if (n <= 1024) hipLaunchKernelGGL((emb_sort_kernel<1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((emb_sort_kernel<4>), grid, block, 0, s, a);
     FC_LAUNCH_CHECK();
-    if (n == 0) return FC_OK;
-    hipLaunchKernelGGL(emb_scan_kernel, dim3(256), dim3(256), 0, s, a);
-    FC_LAUNCH_CHECK();
-    hipLaunchKernelGGL(emb_scatter_kernel, dim3((unsigned)p.tiles), dim3(256), 0, s, a);
-    FC_LAUNCH_CHECK();
+  } else {
+    last = (p.passes - 1) & 1;
+    a.scanned = p.tiles > 64;
+    const bool few = emb_rounds(n) == 4;
+    for (int k = 0; k < p.passes; ++k) {
+      a.ids = k == 0 ? ids : nullptr;
+      a.keys = (uint32_t*)(w + p.keys[(k + 1) & 1]);
+      a.order = (int32_t*)(w + p.order[(k + 1) & 1]);
+      a.keys_out = (uint32_t*)(w + p.keys[k & 1]);
+      a.order_out = (int32_t*)(w + p.order[k & 1]);
+      a.shift = 8 * k;
+      const int64_t blocks = p.tiles + (k == 0 ? fills : 0);
+      if (few) hipLaunchKernelGGL((emb_hist_kernel<4>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((emb_hist_kernel<8>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+      FC_LAUNCH_CHECK();
+      if (n == 0) return FC_OK;
+      if (a.scanned) {
+        hipLaunchKernelGGL(emb_scan_kernel, dim3(256), dim3(256), 0, s, a);
+        FC_LAUNCH_CHECK();
+      }
+      if (few) hipLaunchKernelGGL((emb_scatter_kernel<4>), dim3((unsigned)p.tiles), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((emb_scatter_kernel<8>), dim3((unsigned)p.tiles), dim3(256), 0, s, a);
+      FC_LAUNCH_CHECK();
+    }
   }
   EmbSum b{};
   b.n = n;
@@ -461,8 +579,8 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   b.pieces = (int32_t)p.pieces;
   b.len = (int32_t)p.len;
   b.col_threads = p.col_threads;
-  b.keys = (uint32_t*)(w + p.keys[(p.passes - 1) & 1]);
-  b.order = (int32_t*)(w + p.order[(p.passes - 1) & 1]);
+  b.keys = (uint32_t*)(w + p.keys[last]);
+  b.order = (int32_t*)(w + p.order[last]);
   b.grad = grad_out;
   b.out = grad_table;
   b.scale = scale;
@@ -476,8 +594,13 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
     hipLaunchKernelGGL((emb_piece_kernel<T>), dim3((unsigned)((p.pieces + groups - 1) / groups), p.col_blocks),
                        dim3(256), 0, s, b);
     FC_LAUNCH_CHECK();
-    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 512 ? p.pieces : 512), p.col_blocks),
-                       dim3(256), 0, s, b);
+    // narrow groups: more of them share the pieces of a run
+    EmbSum j = b;
+    j.col_threads = b.col_threads < 16 ? b.col_threads : 16;
+    const int64_t cols = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), wide = (cols + j.col_threads - 1) / j.col_threads;
+    if (wide > 65535) return FC_ERR_SHAPE;
+    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 512 ? p.pieces : 512), (unsigned)wide), dim3(256),
+                       0, s, j);
     FC_LAUNCH_CHECK();
     return FC_OK;
   });
