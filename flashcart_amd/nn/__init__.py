@@ -1,4 +1,5 @@
-"""Network layers: radial basis/cutoff, interaction, product, gates, norms, readout."""
+"""Network layers: radial basis/cutoff, interaction, product, gates, norms, readout; node-wise embedding, feed-forward
+block and dropout (their functions: ``flashcart_amd.nn.functional``)."""
 
 from flashcart_amd.nn.radial import BesselBasis, ChebyshevBasis, PolynomialCutoff
 from flashcart_amd.nn.layers import (
@@ -10,6 +11,12 @@ from flashcart_amd.nn.layers import (
     RescaledSiLULayer,
     RMSLayerNorm,
     ScaleShiftEnergyLayer,
+)
+from flashcart_amd.nn.node_layers import (
+    EmbeddingLayer,
+    GatedFeedForwardLayer,
+    NodeNetwork,
+    ResidualDropoutLayer,
 )
 
 __all__ = [
@@ -24,4 +31,8 @@ __all__ = [
     "RescaledSiLULayer",
     "RMSLayerNorm",
     "ScaleShiftEnergyLayer",
+    "EmbeddingLayer",
+    "GatedFeedForwardLayer",
+    "NodeNetwork",
+    "ResidualDropoutLayer",
 ]
