@@ -9,10 +9,10 @@
 
 namespace fc {
 
-// ---- operands whose rows are not a multiple of 16 bytes, and float32 operands: a padded copy, split into planes ----
+// ---- operands whose rows are not a multiple of 16 bytes, and those in planes: a padded copy ----
 struct PrepItem {
   const void* src;
-  uint16_t* dst;
+  char* dst;
   int64_t cols, ld, plane;  // of src; of dst
   int32_t rows, rows_out, gap_at, gap;  // dst row r is src row r (r < gap_at) or r - gap (r >= gap_at + gap), else zeros
   int32_t block_base;
@@ -22,7 +22,7 @@ struct PrepArgs {
   int32_t count;
 };
 
-template <class T>
+template <class T, class MT>
 __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
   int k = 0;
 #pragma unroll
@@ -45,10 +45,9 @@ __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
     for (int i = 0; i < 8; ++i) x[i] = from >= 0 && c0 + i < it.cols ? to_f32(src[i]) : 0.f;
   }
   const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-  uint16_t* dst = it.dst + row * it.ld + c0;
-  using MT = std::conditional_t<std::is_same_v<T, float>, bf16_t, T>;
-  put4<MT, std::is_same_v<T, float>>(dst, it.plane, lo);
-  put4<MT, std::is_same_v<T, float>>(dst + 4, it.plane, hi);
+  const int64_t at = row * it.ld + c0;
+  put4<MT, std::is_same_v<T, float>>(it.dst, at, it.plane, lo);
+  put4<MT, std::is_same_v<T, float>>(it.dst, at + 4, it.plane, hi);
 }
 
 // ---- sums over the parts of split K loops ----
@@ -61,8 +60,10 @@ struct SumArgs {
 
 // A workgroup forms 256 / groups times 4 outputs: the lanes of an output add every groups-th part, their sums are added in
 // order.
-template <class OT, bool F32>
+template <class MT, bool F32>
 __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
+  using OT = std::conditional_t<F32, float, MT>;
+  constexpr int ES = std::is_same_v<MT, float> ? 4 : 2;
   __shared__ f32x4v part[256];
   int which = 0;
 #pragma unroll
@@ -96,12 +97,12 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
     if (col + v >= g.n_out) break;
     float x = s[v] * g.scale;
     if constexpr (F32) {
-      if (!(fabsf(x) < __builtin_inff())) {  // again in plain float32, as where the sum is not split
+      if (!(fabsf(x) < __builtin_inff())) {  // again, as where the sum is not split
         x = 0.f;
         const int k_end = max(g.A.k, g.B.k);
         for (int k = 0; k < k_end; ++k) {
-          const float u = g.a_tr ? plane_sum<true>(g.A, m, k) : plane_sum<false>(g.A, m, k);
-          const float w = g.b_tr ? plane_sum<true>(g.B, col + v, k) : plane_sum<false>(g.B, col + v, k);
+          const float u = g.a_tr ? value_of<ES, true>(g.A, m, k) : value_of<ES, false>(g.A, m, k);
+          const float w = g.b_tr ? value_of<ES, true>(g.B, col + v, k) : value_of<ES, false>(g.B, col + v, k);
           x = fmaf(g.scale * u, w, x);
         }
       }
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
   }
 }
 
+// (native float32 has no 256 x 256 tile: planes take over before it would fill the device)
 using TileL = Tile<256, 256, 2, 4, 2>;
 using TileM = Tile<128, 128, 2, 2, 2>;
 using TileS = Tile<64, 64, 2, 2, 4>;
@@ -151,16 +153,23 @@ struct TileCost {
   int resident;
 };
 constexpr TileCost kTileCost[3] = {{0.28, 0.28, 0.8, 2}, {0.65, 0.55, 2.5, 2}, {1.25, 1.5, 9.0, 1}};
+// native float32, 32 k a step: bound by the matrix cores
+constexpr TileCost kNativeCost[2] = {{0.45, 0.5, 1.0, 2}, {1.8, 1.8, 3.0, 2}};
+
+enum Form { FORM_16, FORM_NATIVE, FORM_PLANES };
 
 // Tile size and splits of the K loops (plain outputs only) of one launch: those of the least time by the costs above, a
 // split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them.
-static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, bool f32, bool gate) {
+static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Form form, bool gate) {
   const int cus = device_cu_count();
-  for (int q = 0; q < count; ++q) jobs[q]->steps = cdiv(jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k, 64) * (f32 ? 6 : 1);
+  for (int q = 0; q < count; ++q) {
+    const int k = jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k;
+    jobs[q]->steps = form == FORM_NATIVE ? cdiv(k, 32) : cdiv(k, 64) * (form == FORM_PLANES ? 6 : 1);
+  }
   int best_kind = 0, best_splits[2] = {1, 1};
   double best = 1e30;
-  for (int kind = 0; kind < 3; ++kind) {
-    const TileCost& c = kTileCost[kind];
+  for (int kind = 0; kind < (form == FORM_NATIVE ? 2 : 3); ++kind) {
+    const TileCost& c = form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
     for (double most = 1e9; most > 2; most = most > 1e8 ? 128 : most / 2) {  // of a workgroup's steps
       double load = 0, longest = 0, sums = 0;
       int64_t blocks = 0;
@@ -169,7 +178,7 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, bo
         FfnJob& g = *jobs[q];
         if (g.M == 0) continue;
         set_tiles(g, kind, gate);
-        double end = c.end * (can_split[q] ? 1 : 2.5) * (f32 ? 1.5 : 1);
+        double end = c.end * (can_split[q] ? 1 : 2.5) * (form == FORM_PLANES ? 1.5 : 1);
         if (can_split[q] && g.steps * c.step > most) {
           splits[q] = (int)(g.steps * c.step / most) + 1;
           if (splits[q] > g.steps / 4) splits[q] = g.steps / 4 > 1 ? g.steps / 4 : 1;
@@ -210,10 +219,15 @@ static int launch(const FfnJob& g1, const FfnJob& g2, int kind, hipStream_t s) {
   if (blocks == 0) return FC_OK;
   const dim3 grid((unsigned)blocks);
   const int b = (int)first;
-  if (kind == 2)
-    hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileL::NT), 0, s,
-                       g1, g2, b);
-  else if (kind == 1)
+  if constexpr (!std::is_same_v<MT, float>) {
+    if (kind == 2) {
+      hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileL::NT), 0,
+                         s, g1, g2, b);
+      FC_LAUNCH_CHECK();
+      return FC_OK;
+    }
+  }
+  if (kind == 1)
     hipLaunchKernelGGL((ffn_gemm_kernel<TileM, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileM::NT), 0, s,
                        g1, g2, b);
   else
@@ -240,28 +254,36 @@ static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
   }
   if (blocks == 0) return FC_OK;
   if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
-  using OT = std::conditional_t<F32, float, MT>;
-  hipLaunchKernelGGL((ffn_sum_kernel<OT, F32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((ffn_sum_kernel<MT, F32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
   FC_LAUNCH_CHECK();
   return FC_OK;
 }
 
 static int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
+// float32 in planes where the products are large and the operands are used often enough for their splitting to pay.
+// Forward and backward, us, planes against native: 16,384 x 1,024 x 2,048 4,230 / 4,750, 2,048 x 1,024 x 2,048 746 / 858,
+// 4,096 x 512 x 1,024 433 / 371, 25,000 x 128 x 512 504 / 405, 512 x 512 x 512 101 / 64, 6 x 966 x 6,967 276 / 223.
+static Form form_of(const fc_ffn_desc& d, int64_t n) {
+  if (d.dtype != FC_F32) return FORM_16;
+  const bool large = n >= 1024 && d.width >= 512 && d.hidden >= 512 && (double)n * d.width * d.hidden >= 3.2e9;
+  return large ? FORM_PLANES : FORM_NATIVE;
+}
+
 // What is where, for one call; pointers are null where only sizes are asked for.
 struct Ffn {
   const fc_ffn_desc& d;
-  int64_t n, w, hid, wp, hp, esize;
-  bool f32;
-  int planes;
+  int64_t n, w, hid, wp, hp;
+  Form form;
+  int64_t esize;  // bytes of an element of an operand, over all planes
   char* ws;
   int64_t at = 0;
   PrepArgs prep{};
   int64_t prep_blocks = 0;
 
   Ffn(const fc_ffn_desc& desc, int64_t rows, void* workspace)
-      : d(desc), n(rows), w(desc.width), hid(desc.hidden), wp(up8(w)), hp(up8(hid)), esize(node_dtype_size(desc.dtype)),
-        f32(desc.dtype == FC_F32), planes(f32 ? 3 : 1), ws((char*)workspace) {}
+      : d(desc), n(rows), w(desc.width), hid(desc.hidden), wp(up8(w)), hp(up8(hid)), form(form_of(desc, rows)),
+        esize(form == FORM_16 ? 2 : form == FORM_NATIVE ? 4 : 6), ws((char*)workspace) {}
 
   char* take(int64_t bytes) {
     char* p = ws + at;
@@ -273,14 +295,14 @@ struct Ffn {
     const int64_t ld = up8(cols);
     Opnd o{};
     o.ld = ld;
-    if (!f32 && d.aligned && ld == cols && rows == rows_out) {
-      o.p = (const uint16_t*)src;
+    if (form != FORM_PLANES && d.aligned && ld == cols && rows == rows_out) {
+      o.p = (const char*)src;
       return o;
     }
     PrepItem& it = prep.it[prep.count++];
     o.plane = rows_out * ld;
     it.src = src;
-    it.dst = (uint16_t*)take(2 * planes * o.plane);
+    it.dst = take(esize * o.plane);
     it.cols = cols;
     it.ld = ld;
     it.plane = o.plane;
@@ -300,15 +322,15 @@ struct Ffn {
     if (prep.count == 0) return FC_OK;
     if (prep_blocks > 0x7fffffff) return FC_ERR_SHAPE;
     const dim3 grid((unsigned)prep_blocks), block(256);
-    return with_dtype(d.dtype, [&](auto t) -> int {
-      using T = decltype(t);
-      hipLaunchKernelGGL((ffn_prep_kernel<T>), grid, block, 0, s, prep);
-      FC_LAUNCH_CHECK();
-      return FC_OK;
-    });
+    if (d.dtype == FC_BF16) hipLaunchKernelGGL((ffn_prep_kernel<bf16_t, bf16_t>), grid, block, 0, s, prep);
+    else if (d.dtype == FC_F16) hipLaunchKernelGGL((ffn_prep_kernel<f16_t, f16_t>), grid, block, 0, s, prep);
+    else if (form == FORM_NATIVE) hipLaunchKernelGGL((ffn_prep_kernel<float, float>), grid, block, 0, s, prep);
+    else hipLaunchKernelGGL((ffn_prep_kernel<float, bf16_t>), grid, block, 0, s, prep);
+    FC_LAUNCH_CHECK();
+    return FC_OK;
   }
-  int64_t h_bytes() const { return 2 * planes * n * hp; }
-  int64_t factor_bytes() const { return (f32 ? 8 : 6) * n * hp; }
+  int64_t h_bytes() const { return esize * n * hp; }
+  int64_t factor_bytes() const { return (form == FORM_16 ? 6 : 8) * n * hp; }
 };
 
 static Opnd view(Opnd o, int64_t rows, int64_t k) {
@@ -349,7 +371,7 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   g.N = (int32_t)f.hp;
   g.n_out = (int32_t)f.hid;
   g.scale = f.d.scale_in;
-  g.h = (uint16_t*)keep;
+  g.h = keep;
   g.h_plane = f.n * f.hp;
   g.saved = saved ? keep + f.h_bytes() : nullptr;
   g.act = f.d.act;
@@ -357,11 +379,11 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   {
     FfnJob* jobs[] = {&g};
     const bool split[] = {false};
-    p.gate_kind = plan_launch(jobs, split, 1, f.f32, true);
+    p.gate_kind = plan_launch(jobs, split, 1, f.form, true);
   }
   FfnJob& o = p.out;
   Opnd h{};
-  h.p = (const uint16_t*)keep;
+  h.p = keep;
   h.ld = f.hp;
   h.plane = f.n * f.hp;
   o.A = view(h, f.n, f.hp);
@@ -372,7 +394,7 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   {
     FfnJob* jobs[] = {&o};
     const bool split[] = {true};
-    p.out_kind = plan_launch(jobs, split, 1, f.f32, false);
+    p.out_kind = plan_launch(jobs, split, 1, f.form, false);
   }
   o.partial = (float*)f.take(partial_bytes(o));
   return p;
@@ -388,7 +410,7 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
   const bool nx = need & 1, ni = need & 2, no = need & 4;
   const Opnd og = f.x(grad);
   Opnd h{};
-  h.p = (const uint16_t*)saved;
+  h.p = (const char*)saved;
   h.ld = f.hp;
   h.plane = f.n * f.hp;
   Opnd dpre{};
@@ -396,7 +418,8 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     const Opnd oo = f.w_out(w_out);
     dpre.ld = 2 * f.hp;
     dpre.plane = f.n * 2 * f.hp;
-    dpre.p = (const uint16_t*)f.take(2 * f.planes * dpre.plane);
+    char* const dpre_at = f.take(f.esize * dpre.plane);
+    dpre.p = dpre_at;
     FfnJob& g = p.dh;
     g.A = view(og, f.n, f.wp);
     g.B = view(oo, f.hp, f.w);
@@ -405,7 +428,7 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     g.n_out = (int32_t)f.hid;
     g.scale = f.d.scale_out;
     g.saved = saved ? (char*)saved + f.h_bytes() : nullptr;
-    g.dpre = (uint16_t*)dpre.p;
+    g.dpre = dpre_at;
     g.dpre_plane = dpre.plane;
   }
   if (nx) {
@@ -440,18 +463,19 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
   p.dx.b_tr = p.dwi.a_tr = p.dwi.b_tr = 1;
   FfnJob* one[] = {&p.dwo, &p.dh};
   const bool split_one[] = {true, false};
-  p.first_kind = plan_launch(one, split_one, 2, f.f32, false);
+  p.first_kind = plan_launch(one, split_one, 2, f.form, false);
   FfnJob* two[] = {&p.dwi, &p.dx};
   const bool split_two[] = {true, true};
-  p.second_kind = plan_launch(two, split_two, 2, f.f32, false);
+  p.second_kind = plan_launch(two, split_two, 2, f.form, false);
   for (FfnJob* g : {&p.dwo, &p.dwi, &p.dx}) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
   return p;
 }
 
-// f(operand type, is it float32 in planes)
+// f(type of the operands in memory, is the operator's type float32)
 template <class F>
-static int with_operand(int32_t dtype, F&& f) {
-  if (dtype == FC_F32) return f(bf16_t{}, std::true_type{});
+static int with_operand(int32_t dtype, Form form, F&& f) {
+  if (form == FORM_NATIVE) return f(float{}, std::true_type{});
+  if (form == FORM_PLANES) return f(bf16_t{}, std::true_type{});
   if (dtype == FC_BF16) return f(bf16_t{}, std::false_type{});
   return f(f16_t{}, std::false_type{});
 }
@@ -466,7 +490,7 @@ extern "C" int64_t fc_ffn_saved(const fc_ffn_desc* d, int64_t n) {
   const int st = ffn_check(d, n);
   if (st != FC_OK) return -st;
   Ffn f(*d, n, nullptr);
-  return f.h_bytes() + f.factor_bytes();
+  return d->dtype == FC_F32 ? 14 * n * f.hp : f.h_bytes() + f.factor_bytes();
 }
 
 extern "C" int64_t fc_ffn_fwd_workspace(const fc_ffn_desc* d, int64_t n, int32_t save) {
@@ -491,7 +515,7 @@ extern "C" int fc_ffn_fwd(const fc_ffn_desc* d, int64_t n, const void* x, const 
   hipStream_t s = (hipStream_t)stream;
   st = f.run_prep(s);
   if (st != FC_OK) return st;
-  return with_operand(d->dtype, [&](auto m, auto is32) -> int {
+  return with_operand(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
     const FfnJob none{}, *sums[] = {&p.out};
@@ -527,7 +551,7 @@ extern "C" int fc_ffn_bwd(const fc_ffn_desc* d, int64_t n, const void* grad, con
   hipStream_t s = (hipStream_t)stream;
   st = f.run_prep(s);
   if (st != FC_OK) return st;
-  return with_operand(d->dtype, [&](auto m, auto is32) -> int {
+  return with_operand(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
     const FfnJob* sums[] = {&p.dwo, &p.dwi, &p.dx};

@@ -2,11 +2,13 @@
 // matrix instructions with float32 accumulation, with the block's elementwise steps in the epilogues.
 //
 // Operands lie as (rows, K), or as (K, rows) ("TR"), so that no operand of the backward pass is transposed in memory.
-// float32 operands come as three bf16 planes (x = h + m + l, each the nearest bf16 of what the ones before it leave: the
-// split is exact); the K loop then runs over the six plane pairs of relative size 1, 2^-8, 2^-16, smallest first, and
-// what is left out is below 2^-24 of a product. A result that comes out infinite or NaN is formed again in plain float32.
+// float32 has two forms. "Native": float32 operands on the float32 matrix instructions. "Planes", for large products: three
+// bf16 planes (x = h + m + l, each the nearest bf16 of what the ones before it leave: the split is exact); the K loop then
+// runs over the six plane pairs of relative size 1, 2^-8, 2^-16, smallest first, and what is left out is below 2^-24 of a
+// product. A float32 result that comes out infinite or NaN is formed again from scaled operands, one product after the
+// other: it follows the IEEE rules, and stays finite where only the unscaled sum does not.
 //
-// Tiles of BM x BN outputs and 64 k, by waves of 16x16x32 instructions. Both operand tiles go from memory to LDS without
+// Tiles of BM x BN outputs and 64 k (32 in native float32), by waves of 16x16x32 (16x16x4) instructions. Both operand tiles go from memory to LDS without
 // passing through registers, one step ahead of the products. Chunks of 16 bytes are permuted on the way so that the
 // reads of the fragments spread over the banks: a (rows, 64) tile is read 16 bytes a lane, a (64, rows) tile by the
 // transposing LDS read, whose group of 16 lanes takes 4 k x 16 rows and returns 4 consecutive k of one row to each.
@@ -23,9 +25,16 @@ typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
+// The products of two fragments: 32 k of 16-bit operands, 16 k of float32 ones (four instructions; in each, the lanes of a
+// group of 16 take one k of their four).
 template <class MT>
-__device__ __forceinline__ f32x4v mfma16(const s16x8& a, const s16x8& b, const f32x4v& c) {
-  if constexpr (std::is_same_v<MT, f16_t>)
+__device__ __forceinline__ f32x4v mfma16(const s16x8& a, const s16x8& b, f32x4v c) {
+  if constexpr (std::is_same_v<MT, float>) {
+    const f32x4v u = __builtin_bit_cast(f32x4v, a), v = __builtin_bit_cast(f32x4v, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(u[e], v[e], c, 0, 0, 0);
+    return c;
+  } else if constexpr (std::is_same_v<MT, f16_t>)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0,
@@ -35,7 +44,7 @@ __device__ __forceinline__ f32x4v mfma16(const s16x8& a, const s16x8& b, const f
 // One operand: `rows` output rows (or columns), k valid up to `k`; element (r, k) at p[r * ld + k], or p[k * ld + r].
 // ld is a multiple of 8 and p is aligned to 16 bytes; in the TR form `rows` is a multiple of 8 too.
 struct Opnd {
-  const uint16_t* p;
+  const char* p;
   int64_t ld, plane;  // elements; plane: from one bf16 plane to the next
   int32_t rows, k;
 };
@@ -54,10 +63,10 @@ struct FfnJob {
   int32_t n_out, m_out, gap_at, gap;
   float* partial;        // splits > 1: (splits, M, N)
   // EPI_GATE: h (n, N) and, in training, the factors a = c act(gate), b = c act'(gate) up; EPI_DH: a, b and dpre
-  uint16_t* h;
+  char* h;
   int64_t h_plane;
   void* saved;           // 16-bit types: (3, n, N) uint16; float32: (2, n, N) float
-  uint16_t* dpre;        // (n, 2 N)
+  char* dpre;            // (n, 2 N)
   int64_t dpre_plane;
   int32_t act;
   float act_scale;
@@ -90,14 +99,21 @@ struct Tile {
   static constexpr int STAGE = (BM + BN) * 128, STAGES = STAGES_;  // bytes of LDS a stage, stages
 };
 
-// The part of a wave in bringing one (R rows, 64 k) operand tile to LDS: R / 8 segments of 1 KB, shared by the waves.
-template <int R, int NW, bool TR>
+// The part of a wave in bringing one operand tile of R rows and 128 bytes of k to LDS: R / 8 segments of 1 KB, shared by the
+// waves. ES: bytes of an element.
+template <int R, int NW, int ES, bool TR>
 struct Loader {
-  static constexpr int SEGS = R / 8 / NW;
+  static constexpr int SEGS = R / 8 / NW, CE = 16 / ES, KS = 128 / ES;  // elements of a chunk, k of a step
   static_assert(R % (8 * NW) == 0, "segments");
   const char* base[SEGS];
   uint32_t off[SEGS];
   int kl[TR ? SEGS : 1];  // k of the lane's chunk, counted from the step's first
+
+  // Where 16 bytes of row k are in a (K, rows) tile: how `c`, the index of 32 (float32: 64) bytes of the row, is permuted.
+  __device__ static __forceinline__ int permute(int k, int c) {
+    if constexpr (ES == 4) return c ^ ((k >> 2) & 3);
+    else return c ^ (R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2));
+  }
 
   // HALF > 0: rows r with r % (2 HALF) >= HALF come from `up` rows further on (gate and up rows of one weight)
   template <int HALF>
@@ -113,17 +129,16 @@ struct Loader {
           row = row / (2 * HALF) * HALF + row % HALF;
           if (second) first += up;
         }
-        base[j] = (const char*)(o.p + first * o.ld);
+        base[j] = o.p + ES * first * o.ld;
         row = min(row, o.rows - 1 - r0);
-        off[j] = (uint32_t)row * (uint32_t)(o.ld * 2) + 16 * ((lane & 7) ^ (lane >> 3));
-        kl[0] = 8 * ((lane & 7) ^ (lane >> 3));
+        off[j] = (uint32_t)row * (uint32_t)(o.ld * ES) + 16 * ((lane & 7) ^ (lane >> 3));
+        kl[0] = CE * ((lane & 7) ^ (lane >> 3));
       } else {
-        constexpr int CPR = R / 8;  // chunks per row
+        constexpr int CPR = R / CE, CPP = ES == 4 ? 4 : 2;  // chunks of a row, and of what is permuted as one
         const int k = seg * (64 / CPR) + lane / CPR, phys = lane % CPR;
-        const int f = R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
-        const int col = min(r0 + 8 * ((((phys >> 1) ^ f) << 1) | (phys & 1)), o.rows - 8);
-        base[j] = (const char*)o.p;
-        off[j] = (uint32_t)k * (uint32_t)(o.ld * 2) + 2 * col;
+        const int col = min(r0 + CE * (permute(k, phys / CPP) * CPP + phys % CPP), o.rows - CE);
+        base[j] = o.p;
+        off[j] = (uint32_t)k * (uint32_t)(o.ld * ES) + ES * col;
         kl[j] = k;
       }
     }
@@ -131,21 +146,21 @@ struct Loader {
   // the step at k0 of the plane that starts `plane` elements behind the first; the segments of the wave in MASK
   template <int MASK>
   __device__ __forceinline__ void load(const Opnd& o, int k0, int64_t plane, lds_char* dst, int wave) const {
-    const int64_t shift = 2 * (plane + (TR ? (int64_t)k0 * o.ld : k0));
+    const int64_t shift = ES * (plane + (TR ? (int64_t)k0 * o.ld : k0));
     const int left = o.k - k0;
 #pragma unroll
     for (int j = 0; j < SEGS; ++j) {
       if (!(MASK >> j & 1)) continue;
       __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base[j] + shift), 0, kOutOfRange, 0x00020000);
-      const uint32_t at = (left >= 64 || kl[TR ? j : 0] < left) ? off[j] : kOutOfRange;
+      const uint32_t at = (left >= KS || kl[TR ? j : 0] < left) ? off[j] : kOutOfRange;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (wave + NW * j) * 1024),
                                                16, at, 0, 0, 0);
     }
   }
 };
 
-// Fragments of a wave: F blocks of 16 rows from row `r0` of an operand tile of R rows; s: which 32 k of the step.
-template <int R, int F, bool TR>
+// Fragments of a wave: F blocks of 16 rows from row `r0` of an operand tile of R rows; s: which half of the step's k.
+template <int R, int F, int ES, bool TR>
 struct Reader {
   uint32_t at[TR ? F : 2];
   __device__ __forceinline__ void init(int r0, int lane) {
@@ -153,11 +168,14 @@ struct Reader {
     if constexpr (!TR) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) at[s] = (r0 + r) * 128 + 16 * ((4 * s + g) ^ (r & 7));
+    } else if constexpr (ES == 4) {
+      const int k = 4 * g;
+#pragma unroll
+      for (int j = 0; j < F; ++j) at[j] = k * (R * 4) + Loader<R, 1, ES, TR>::permute(k, (r0 >> 4) + j) * 64 + r * 4;
     } else {
       const int k = 8 * g + (r >> 2);
-      const int f = R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
 #pragma unroll
-      for (int j = 0; j < F; ++j) at[j] = k * (R * 2) + (((r0 >> 4) + j) ^ f) * 32 + (r & 3) * 8;
+      for (int j = 0; j < F; ++j) at[j] = k * (R * 2) + Loader<R, 1, ES, TR>::permute(k, (r0 >> 4) + j) * 32 + (r & 3) * 8;
     }
   }
   // C of the blocks, from block J on
@@ -167,6 +185,12 @@ struct Reader {
     for (int j = J; j < J + C; ++j) {
       if constexpr (!TR) {
         x[j - J] = *(const __attribute__((address_space(3))) s16x8*)(tile + at[s] + j * 16 * 128);
+      } else if constexpr (ES == 4) {
+        const lds_char* p = tile + at[j] + s * 16 * (R * 4);
+        f32x4v v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = *(const __attribute__((address_space(3))) float*)(p + e * (R * 4));
+        x[j - J] = __builtin_bit_cast(s16x8, v);
       } else {
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const lds_char* p = tile + at[j] + s * 32 * (R * 2);
@@ -201,11 +225,13 @@ __device__ __forceinline__ void split3(float x, uint16_t& h, uint16_t& m, uint16
   l = from_f32<bf16_t>(r - to_f32(bf16_t{m})).v;
 }
 
-// Four consecutive values of a (n, ld) matrix of the operator's operand form.
+// Four consecutive values, from element `at` on, of a matrix in the operator's operand form.
 template <class MT, bool F32>
-__device__ __forceinline__ void put4(uint16_t* p, int64_t plane, const float (&x)[4]) {
-  if constexpr (!F32) {
-    *(uint2*)p = make_uint2(pack2<MT>(x[0], x[1]), pack2<MT>(x[2], x[3]));
+__device__ __forceinline__ void put4(char* matrix, int64_t at, int64_t plane, const float (&x)[4]) {
+  if constexpr (std::is_same_v<MT, float>) {
+    *(float4*)(matrix + 4 * at) = make_float4(x[0], x[1], x[2], x[3]);
+  } else if constexpr (!F32) {
+    *(uint2*)(matrix + 2 * at) = make_uint2(pack2<MT>(x[0], x[1]), pack2<MT>(x[2], x[3]));
   } else {
     uint32_t h[2], m[2], l[2];
     const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
@@ -232,6 +258,7 @@ __device__ __forceinline__ void put4(uint16_t* p, int64_t plane, const float (&x
         l[i] = w[0] | (uint32_t)w[1] << 16;
       }
     }
+    uint16_t* p = (uint16_t*)matrix + at;
     *(uint2*)p = make_uint2(h[0], h[1]);
     *(uint2*)(p + plane) = make_uint2(m[0], m[1]);
     *(uint2*)(p + 2 * plane) = make_uint2(l[0], l[1]);
@@ -294,17 +321,21 @@ struct Factors<true> {
   }
 };
 
-// A float32 operand's value from its planes.
-template <bool TR>
-__device__ __forceinline__ float plane_sum(const Opnd& o, int64_t r, int k) {
+// A float32 operand's value, native (ES = 4) or in planes.
+template <int ES, bool TR>
+__device__ __forceinline__ float value_of(const Opnd& o, int64_t r, int k) {
   if (k >= o.k) return 0.f;
-  const uint16_t* p = o.p + (TR ? (int64_t)k * o.ld + r : r * o.ld + k);
+  const int64_t at = TR ? (int64_t)k * o.ld + r : r * o.ld + k;
+  if constexpr (ES == 4) return ((const float*)o.p)[at];
+  const uint16_t* p = (const uint16_t*)o.p + at;
   return to_f32(bf16_t{p[0]}) + (to_f32(bf16_t{p[o.plane]}) + to_f32(bf16_t{p[2 * o.plane]}));
 }
 
 template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI>
 struct FfnTile {
   using OT = std::conditional_t<F32, float, MT>;
+  static constexpr bool PLANES = F32 && !std::is_same_v<MT, float>;
+  static constexpr int ES = std::is_same_v<MT, float> ? 4 : 2, KS = 128 / ES;
 
   __device__ static __forceinline__ void run(const FfnJob& g, int block, lds_char* lds0, lds_char* lds1, lds_char* lds2,
                                          lds_char* lds3) {
@@ -328,12 +359,12 @@ struct FfnTile {
     constexpr int BNO = EPI == EPI_GATE ? T::BN / 2 : T::BN;  // output columns of a tile
     const int m0 = mt * T::BM, n0 = nt * BNO;
 
-    Loader<T::BM, T::NW, ATR> la;
-    Loader<T::BN, T::NW, BTR> lb;
+    Loader<T::BM, T::NW, ES, ATR> la;
+    Loader<T::BN, T::NW, ES, BTR> lb;
     la.template init<0>(g.A, m0, wave, lane, 0);
     lb.template init<EPI == EPI_GATE ? T::TN / 2 : 0>(g.B, n0, wave, lane, g.N);
-    Reader<T::BM, T::MF, ATR> ra;
-    Reader<T::BN, T::NF, BTR> rb;
+    Reader<T::BM, T::MF, ES, ATR> ra;
+    Reader<T::BN, T::NF, ES, BTR> rb;
     ra.init(wm * T::TM, lane);
     rb.init(wn * T::TN, lane);
 
@@ -349,9 +380,9 @@ struct FfnTile {
       int left, k, pair;  // left: steps before the end
       int64_t a, b;       // elements to the planes
     };
-    const int per_pair = F32 ? g.steps / 6 : g.steps;
+    const int per_pair = PLANES ? g.steps / 6 : g.steps;
     auto place = [&](Cursor& c) {
-      if constexpr (F32) {
+      if constexpr (PLANES) {
         int pa, pb;
         plane_pair(c.pair, pa, pb);
         c.a = pa * g.A.plane;
@@ -363,20 +394,20 @@ struct FfnTile {
     auto cursor_at = [&](int s) {
       Cursor c;
       c.left = s1 - s;
-      c.pair = F32 ? s / per_pair : 0;
-      c.k = 64 * (s - c.pair * per_pair);
+      c.pair = PLANES ? s / per_pair : 0;
+      c.k = KS * (s - c.pair * per_pair);
       place(c);
       return c;
     };
     // segments MA of A's tile and MB of B's at the cursor, zeros past the end; the cursor goes to the next step
     auto fetch = [&](Cursor& c, lds_char* at, auto ma, auto mb) {
-      const int k = c.left > 0 ? c.k : 64 * per_pair;
+      const int k = c.left > 0 ? c.k : KS * per_pair;
       la.template load<ma>(g.A, k, c.a, at, wave);
       lb.template load<mb>(g.B, k, c.b, at + T::BM * 128, wave);
       --c.left;
-      c.k += 64;
-      if constexpr (F32) {
-        if (c.k == 64 * per_pair) {
+      c.k += KS;
+      if constexpr (PLANES) {
+        if (c.k == KS * per_pair) {
           c.k = 0;
           ++c.pair;
           place(c);
@@ -479,6 +510,29 @@ struct FfnTile {
         }
         __builtin_amdgcn_sched_barrier(0);
       };
+      // The float32 instructions round after every product: sums of 256 k are kept apart and added (relative error of a
+      // sum of 6,000 normal products 1.05e-6 in one chain, 3e-7 so).
+      constexpr bool CHUNKS = std::is_same_v<MT, float>;
+      constexpr int EVERY = 256 / (KS * T::STAGES);
+      f32x4v sum[CHUNKS ? T::MF : 1][T::NF];
+      int turn = 0;
+      auto flush = [&](bool now) {
+        if constexpr (CHUNKS) {
+          if (!now) return;
+#pragma unroll
+          for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+            for (int j = 0; j < T::NF; ++j) {
+              sum[i][j] += acc[i][j];
+              acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+      };
+      if constexpr (CHUNKS)
+#pragma unroll
+        for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+          for (int j = 0; j < T::NF; ++j) sum[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
       fetch(next_load, lds0, all, all);
       if constexpr (T::STAGES == 4) {
         fetch(next_load, lds1, all, all);
@@ -489,13 +543,21 @@ struct FfnTile {
           step(lds1, lds0);
           step(lds2, lds1);
           step(lds3, lds2);
+          flush(++turn % EVERY == 0);
         }
       } else {
 #pragma unroll 1
         for (int s = s0; s < s1; s += 2) {
           step(lds0, lds1);
           step(lds1, lds0);
+          flush(++turn % EVERY == 0);
         }
+      }
+      if constexpr (CHUNKS) {
+#pragma unroll
+        for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+          for (int j = 0; j < T::NF; ++j) acc[i][j] += sum[i][j];
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -539,8 +601,8 @@ struct FfnTile {
         const int row = min(m0 + wm * T::TM + i * 16 + r, g.A.rows - 1);
 #pragma unroll 1
         for (int k = q; k < k_end + q; k += 4)
-          c = __builtin_amdgcn_mfma_f32_16x16x4f32(plane_sum<BTR>(g.B, col, k),
-                                                   g.scale * plane_sum<ATR>(g.A, row, k), c, 0, 0, 0);
+          c = __builtin_amdgcn_mfma_f32_16x16x4f32(value_of<ES, BTR>(g.B, col, k),
+                                                   g.scale * value_of<ES, ATR>(g.A, row, k), c, 0, 0, 0);
         acc[i][j] = c;
       }
     }
@@ -603,7 +665,7 @@ struct FfnTile {
             if (col + v >= g.n_out) h[v] = 0.f;  // pad columns take part in the next product
           }
           const int64_t at = row * g.N + col;
-          put4<MT, F32>(g.h + at, g.h_plane, h);
+          put4<MT, F32>(g.h, at, g.h_plane, h);
           if (g.saved) put_factors<F32>(g.saved, at, count, a, b);
         }
       }
@@ -636,9 +698,9 @@ struct FfnTile {
             dg[v] = col + v < g.n_out ? dh * b[v] : 0.f;
             du[v] = col + v < g.n_out ? dh * a[v] : 0.f;
           }
-          uint16_t* p = g.dpre + row * 2 * g.N + col;
-          put4<MT, F32>(p, g.dpre_plane, dg);
-          put4<MT, F32>(p + g.N, g.dpre_plane, du);
+          const int64_t at = row * 2 * g.N + col;
+          put4<MT, F32>(g.dpre, at, g.dpre_plane, dg);
+          put4<MT, F32>(g.dpre, at + g.N, g.dpre_plane, du);
         }
       }
     }

@@ -59,7 +59,8 @@ def _check(got, want, dtype):
 # small; hidden large, n small), the largest tiles with and without ragged edges
 SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (17, 33, 19), (64, 128, 512), (130, 96, 200), (257, 519, 103),
          (1000, 64, 72), (300, 256, 1032), (5, 2056, 40), (70, 40, 3001), (9001, 24, 16), (2049, 136, 264),
-         (4096, 512, 1024), (4100, 520, 1100), (16, 1024, 2048), (48, 2048, 1000), (33, 72, 4099)]
+         (4096, 512, 1024), (4100, 520, 1100), (16, 1024, 2048), (48, 2048, 1000), (33, 72, 4099),
+         (8200, 520, 1032)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -142,8 +143,9 @@ def test_subsets_of_gradients_and_layouts(dtype):
     assert not none["dw_in"].any() and not none["dw_out"].any()
 
 
+# (the last: float32 in three bf16 parts)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,width,hidden", [(70, 48, 80), (4, 260, 70), (700, 24, 16)])
+@pytest.mark.parametrize("n,width,hidden", [(70, 48, 80), (4, 260, 70), (700, 24, 16), (8200, 520, 1028)])
 def test_values_that_are_not_finite(n, width, hidden, dtype):
     """An infinite or NaN element reaches what the formulas say and nothing else."""
     (x, w_in, w_out), grad = _inputs(n, width, hidden, dtype, seed=2)
