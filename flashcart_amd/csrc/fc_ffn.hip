@@ -59,7 +59,8 @@ struct SumArgs {
 };
 
 // A workgroup forms 256 / groups times 4 outputs: the lanes of an output add every groups-th part, their sums are added in
-// order.
+// order. Where the product has an epilogue of its own, it follows here; with the gate's, a lane's second output is the other
+// projection's.
 template <class MT, bool F32>
 __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
   using OT = std::conditional_t<F32, float, MT>;
@@ -71,21 +72,55 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
     if (q < a.count && (int)blockIdx.x >= a.base[q]) which = q;
   const FfnJob& g = a.job[which];
   const int groups = a.groups[which], per = 256 / groups, grp = threadIdx.x / per;
-  const int64_t chunks = g.N / 4, t = (int64_t)(blockIdx.x - a.base[which]) * per + threadIdx.x % per;
+  const int cols = g.finish == EPI_GATE ? g.N / 2 : g.N;
+  const int64_t chunks = cols / 4, t = (int64_t)(blockIdx.x - a.base[which]) * per + threadIdx.x % per;
   const bool ok = t < g.M * chunks;
   int64_t row = ok ? t / chunks : 0;
-  const int64_t col = ok ? (t - row * chunks) * 4 : 0, m = row;
-  f32x4v s{0.f, 0.f, 0.f, 0.f};
-  const float* p = g.partial + row * g.N + col;
+  const int col = ok ? (int)(t - row * chunks) * 4 : 0;
+  // the sums, scaled; every lane of the workgroup takes part
+  auto total = [&](int c, float (&x)[4]) {
+    f32x4v s{0.f, 0.f, 0.f, 0.f};
+    const float* p = g.partial + row * g.N + c;
 #pragma unroll 4
-  for (int k = grp; k < g.splits; k += groups) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
-  if (groups > 1) {
-    part[threadIdx.x] = s;
-    __syncthreads();
-    if (grp > 0) return;
-    for (int k = 1; k < groups; ++k) s += part[k * per + threadIdx.x];
+    for (int k = grp; k < g.splits; k += groups) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+    if (groups > 1) {
+      part[threadIdx.x] = s;
+      __syncthreads();
+      if (grp == 0)
+        for (int k = 1; k < groups; ++k) s += part[k * per + threadIdx.x];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      x[v] = s[v] * g.scale;
+      if constexpr (F32) {
+        if (ok && grp == 0 && !(fabsf(x[v]) < __builtin_inff())) {  // again, as where the sum is not split
+          x[v] = 0.f;
+          const int k_end = max(g.A.k, g.B.k), m = (int)row, n = min(c + v, g.B.rows - 1);
+          for (int k = 0; k < k_end; ++k) {
+            const float u = g.a_tr ? value_of<ES, true>(g.A, m, k) : value_of<ES, false>(g.A, m, k);
+            const float w = g.b_tr ? value_of<ES, true>(g.B, n, k) : value_of<ES, false>(g.B, n, k);
+            x[v] = fmaf(g.scale * u, w, x[v]);
+          }
+        }
+      }
+    }
+  };
+  float x[4];
+  total(col, x);
+  if (g.finish == EPI_GATE) {
+    float up[4];
+    total(cols + col, up);
+    if (ok && grp == 0) finish_gate<MT, F32>(g, row, col, cols, x, up);
+    return;
   }
-  if (!ok) return;
+  if (!ok || grp > 0) return;
+  if (g.finish == EPI_DH) {
+    Factors<F32> f;
+    f.load(g.saved, row * g.N + col, (int64_t)g.M * g.N);
+    finish_dh<MT, F32>(g, row, col, f, x);
+    return;
+  }
   if (row >= g.gap_at) {
     if (row < g.gap_at + g.gap) return;
     row -= g.gap;
@@ -93,22 +128,8 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
   if (row >= g.m_out) return;
   OT* out = (OT*)g.out + row * g.ld_out;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    if (col + v >= g.n_out) break;
-    float x = s[v] * g.scale;
-    if constexpr (F32) {
-      if (!(fabsf(x) < __builtin_inff())) {  // again, as where the sum is not split
-        x = 0.f;
-        const int k_end = max(g.A.k, g.B.k);
-        for (int k = 0; k < k_end; ++k) {
-          const float u = g.a_tr ? value_of<ES, true>(g.A, m, k) : value_of<ES, false>(g.A, m, k);
-          const float w = g.b_tr ? value_of<ES, true>(g.B, col + v, k) : value_of<ES, false>(g.B, col + v, k);
-          x = fmaf(g.scale * u, w, x);
-        }
-      }
-    }
-    out[col + v] = from_f32<OT>(x);
-  }
+  for (int v = 0; v < 4; ++v)
+    if (col + v < g.n_out) out[col + v] = from_f32<OT>(x[v]);
 }
 
 // (native float32 has no 256 x 256 tile: planes take over before it would fill the device)
@@ -116,9 +137,10 @@ using TileL = Tile<256, 256, 2, 4, 2>;
 using TileM = Tile<128, 128, 2, 2, 2>;
 using TileS = Tile<64, 64, 2, 2, 4>;
 
-// The products of one launch: workgroups from `first` on take the second.
+// The products of one launch. The first `front` workgroups take the one with the longer sums, g1 or (swapped) g2, the others
+// the other one.
 template <class T, class MT, bool F32, bool ATR1, bool BTR1, int EPI1, bool ATR2, bool BTR2, int EPI2>
-__global__ void __launch_bounds__(T::NT) ffn_gemm_kernel(FfnJob g1, FfnJob g2, int first) {
+__global__ void __launch_bounds__(T::NT, 2) ffn_gemm_kernel(FfnJob g1, FfnJob g2, int front, bool swapped) {
   __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
@@ -126,11 +148,12 @@ __global__ void __launch_bounds__(T::NT) ffn_gemm_kernel(FfnJob g1, FfnJob g2, i
   lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
   lds_char* const l3 = (lds_char*)lds3;
   constexpr bool SAME = ATR1 == ATR2 && BTR1 == BTR2 && EPI1 == EPI2;
-  if (SAME || (int)blockIdx.x < first) {
-    FfnTile<T, MT, F32, ATR1, BTR1, EPI1>::run(g1, blockIdx.x, l0, l1, l2, l3);
+  const bool in_front = (int)blockIdx.x < front;
+  const int block = in_front ? blockIdx.x : blockIdx.x - front;
+  if (SAME || in_front != swapped) {
+    FfnTile<T, MT, F32, ATR1, BTR1, EPI1>::run(g1, block, l0, l1, l2, l3);
   } else {
-    if constexpr (!SAME)
-      FfnTile<T, MT, F32, ATR2, BTR2, EPI2>::run(g2, blockIdx.x - first, l0, l1, l2, l3);
+    if constexpr (!SAME) FfnTile<T, MT, F32, ATR2, BTR2, EPI2>::run(g2, block, l0, l1, l2, l3);
   }
 }
 
@@ -150,17 +173,16 @@ static void set_tiles(FfnJob& g, int kind, bool gate) {
 // caches deliver, the 256 x 256 tile by the matrix cores.
 struct TileCost {
   double step, full, end;
-  int resident;
 };
-constexpr TileCost kTileCost[3] = {{0.28, 0.28, 0.8, 2}, {0.65, 0.55, 2.5, 2}, {1.25, 1.5, 9.0, 1}};
+constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8}, {0.65, 0.55, 2.5}, {1.25, 1.5, 9.0}};
 // native float32, 32 k a step: bound by the matrix cores
-constexpr TileCost kNativeCost[2] = {{0.45, 0.5, 1.0, 2}, {1.8, 1.8, 3.0, 2}};
+constexpr TileCost kNativeCost[2] = {{0.6, 0.62, 1.0}, {2.05, 1.85, 5.0}};
 
 enum Form { FORM_16, FORM_NATIVE, FORM_PLANES };
 
 // Tile size and splits of the K loops (plain outputs only) of one launch: those of the least time by the costs above, a
 // split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them.
-static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Form form, bool gate) {
+static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Form form, bool gate, double* time_us) {
   const int cus = device_cu_count();
   for (int q = 0; q < count; ++q) {
     const int k = jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k;
@@ -170,7 +192,11 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
   double best = 1e30;
   for (int kind = 0; kind < (form == FORM_NATIVE ? 2 : 3); ++kind) {
     const TileCost& c = form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
-    for (double most = 1e9; most > 2; most = most > 1e8 ? 128 : most / 2) {  // of a workgroup's steps
+    double chain = 0;  // the longest sum that may be split
+    for (int q = 0; q < count; ++q)
+      if (jobs[q]->M > 0 && can_split[q] && jobs[q]->steps * c.step > chain) chain = jobs[q]->steps * c.step;
+    double most = chain + 1;  // of a workgroup's steps
+    do {
       double load = 0, longest = 0, sums = 0;
       int64_t blocks = 0;
       int splits[2] = {1, 1};
@@ -194,19 +220,24 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
         const double t = steps * c.step + end;
         longest = t > longest ? t : longest;
       }
-      double time = blocks > (int64_t)cus * c.resident ? load + 0.5 * longest : load > longest ? load : longest;
+      // whole rounds of workgroups where the matrix cores bound them, something between where the caches do
+      const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
+      if (blocks > cus) load *= form == FORM_NATIVE ? rounds : 0.5 + 0.5 * rounds;
+      double time = load > longest ? load : longest;
       if (sums > 0) time += sums + 3.5;
       if (time < best) {
         best = time;
         best_kind = kind;
         for (int q = 0; q < count; ++q) best_splits[q] = splits[q];
       }
-    }
+      most /= 2;
+    } while (most > 2);
   }
   for (int q = 0; q < count; ++q) {
     set_tiles(*jobs[q], best_kind, gate);
     jobs[q]->splits = best_splits[q];
   }
+  *time_us = best;
   return best_kind;
 }
 static int64_t partial_bytes(const FfnJob& g) { return g.splits > 1 ? 4ll * g.splits * g.M * g.N : 0; }
@@ -214,25 +245,26 @@ static int64_t partial_bytes(const FfnJob& g) { return g.splits > 1 ? 4ll * g.sp
 // One launch of up to two products (the second may have no outputs).
 template <class MT, bool F32, bool ATR1, bool BTR1, int EPI1, bool ATR2 = ATR1, bool BTR2 = BTR1, int EPI2 = EPI1>
 static int launch(const FfnJob& g1, const FfnJob& g2, int kind, hipStream_t s) {
-  const int64_t first = g1.M > 0 ? blocks_of(g1) : 0, blocks = first + (g2.M > 0 ? blocks_of(g2) : 0);
+  const int64_t blocks1 = g1.M > 0 ? blocks_of(g1) : 0, blocks2 = g2.M > 0 ? blocks_of(g2) : 0, blocks = blocks1 + blocks2;
   if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
   if (blocks == 0) return FC_OK;
   const dim3 grid((unsigned)blocks);
-  const int b = (int)first;
+  const bool swapped = blocks2 > 0 && (blocks1 == 0 || g2.steps / g2.splits > g1.steps / g1.splits);
+  const int front = (int)(swapped ? blocks2 : blocks1);
   if constexpr (!std::is_same_v<MT, float>) {
     if (kind == 2) {
       hipLaunchKernelGGL((ffn_gemm_kernel<TileL, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileL::NT), 0,
-                         s, g1, g2, b);
+                         s, g1, g2, front, swapped);
       FC_LAUNCH_CHECK();
       return FC_OK;
     }
   }
   if (kind == 1)
     hipLaunchKernelGGL((ffn_gemm_kernel<TileM, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileM::NT), 0, s,
-                       g1, g2, b);
+                       g1, g2, front, swapped);
   else
     hipLaunchKernelGGL((ffn_gemm_kernel<TileS, MT, F32, ATR1, BTR1, EPI1, ATR2, BTR2, EPI2>), grid, dim3(TileS::NT), 0, s,
-                       g1, g2, b);
+                       g1, g2, front, swapped);
   FC_LAUNCH_CHECK();
   return FC_OK;
 }
@@ -250,7 +282,7 @@ static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
     a.base[a.count] = (int32_t)blocks;
     a.groups[a.count] = groups;
     a.job[a.count++] = g;
-    blocks += cdiv((int64_t)g.M * (g.N / 4), 256 / groups);
+    blocks += cdiv((int64_t)g.M * ((g.finish == EPI_GATE ? g.N / 2 : g.N) / 4), 256 / groups);
   }
   if (blocks == 0) return FC_OK;
   if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
@@ -377,9 +409,21 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   g.act = f.d.act;
   g.act_scale = f.d.act_scale;
   {
-    FfnJob* jobs[] = {&g};
-    const bool split[] = {false};
-    p.gate_kind = plan_launch(jobs, split, 1, f.form, true);
+    // few tiles and long sums: as a plain product with a split K loop, the activation after the sum of its parts
+    FfnJob plain = g;
+    plain.N = (int32_t)(2 * f.hp);
+    plain.B.rows = plain.N;
+    plain.finish = EPI_GATE;
+    FfnJob *fused[] = {&g}, *split[] = {&plain};
+    const bool no[] = {false}, yes[] = {true};
+    double time, plain_time;
+    p.gate_kind = plan_launch(fused, no, 1, f.form, true, &time);
+    const int kind = plan_launch(split, yes, 1, f.form, false, &plain_time);
+    if (plain.splits > 1 && plain_time < time) {
+      g = plain;
+      p.gate_kind = kind;
+      g.partial = (float*)f.take(partial_bytes(g));
+    }
   }
   FfnJob& o = p.out;
   Opnd h{};
@@ -391,10 +435,12 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
   o.M = (int32_t)f.n;
   o.N = (int32_t)f.wp;
   set_out(o, y, f.n, f.w, f.d.scale_out);
+  o.finish = EPI_OUT;
   {
     FfnJob* jobs[] = {&o};
-    const bool split[] = {true};
-    p.out_kind = plan_launch(jobs, split, 1, f.form, false);
+    const bool yes[] = {true};
+    double time;
+    p.out_kind = plan_launch(jobs, yes, 1, f.form, false, &time);
   }
   o.partial = (float*)f.take(partial_bytes(o));
   return p;
@@ -461,13 +507,26 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     g.a_tr = g.b_tr = 1;
   }
   p.dx.b_tr = p.dwi.a_tr = p.dwi.b_tr = 1;
-  FfnJob* one[] = {&p.dwo, &p.dh};
-  const bool split_one[] = {true, false};
-  p.first_kind = plan_launch(one, split_one, 2, f.form, false);
+  p.dwo.finish = p.dwi.finish = p.dx.finish = EPI_OUT;
+  p.dh.b_tr = 1;
+  double time, plain_time;
+  const bool split_dwo[] = {true, false}, split_both[] = {true, true};
+  {
+    // (as for the gate: the hidden gradient with a split K loop, where that is faster)
+    FfnJob dwo = p.dwo, dh = p.dh;
+    dh.finish = EPI_DH;
+    FfnJob *fused[] = {&p.dwo, &p.dh}, *split[] = {&dwo, &dh};
+    p.first_kind = plan_launch(fused, split_dwo, 2, f.form, false, &time);
+    const int kind = plan_launch(split, split_both, 2, f.form, false, &plain_time);
+    if (dh.splits > 1 && plain_time + 3.5 < time) {
+      p.dwo = dwo;
+      p.dh = dh;
+      p.first_kind = kind;
+    }
+  }
   FfnJob* two[] = {&p.dwi, &p.dx};
-  const bool split_two[] = {true, true};
-  p.second_kind = plan_launch(two, split_two, 2, f.form, false);
-  for (FfnJob* g : {&p.dwo, &p.dwi, &p.dx}) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
+  p.second_kind = plan_launch(two, split_both, 2, f.form, false, &time);
+  for (FfnJob* g : {&p.dwo, &p.dh, &p.dwi, &p.dx}) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
   return p;
 }
 
@@ -518,8 +577,10 @@ extern "C" int fc_ffn_fwd(const fc_ffn_desc* d, int64_t n, const void* x, const 
   return with_operand(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
-    const FfnJob none{}, *sums[] = {&p.out};
-    int r = launch<MT, F32, false, false, EPI_GATE>(p.gate, none, p.gate_kind, s);
+    const FfnJob none{}, *gates[] = {&p.gate}, *sums[] = {&p.out};
+    int r = p.gate.splits > 1 ? launch<MT, F32, false, false, EPI_OUT>(p.gate, none, p.gate_kind, s)
+                              : launch<MT, F32, false, false, EPI_GATE>(p.gate, none, p.gate_kind, s);
+    if (r == FC_OK) r = launch_sums<MT, F32>(gates, 1, s);
     if (r == FC_OK) r = launch<MT, F32, false, false, EPI_OUT>(p.out, none, p.out_kind, s);
     return r != FC_OK ? r : launch_sums<MT, F32>(sums, 1, s);
   });
@@ -554,8 +615,10 @@ extern "C" int fc_ffn_bwd(const fc_ffn_desc* d, int64_t n, const void* grad, con
   return with_operand(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);
     constexpr bool F32 = decltype(is32)::value;
-    const FfnJob* sums[] = {&p.dwo, &p.dwi, &p.dx};
-    int r = launch<MT, F32, true, true, EPI_OUT, false, true, EPI_DH>(p.dwo, p.dh, p.first_kind, s);
+    const FfnJob *hidden[] = {&p.dh}, *sums[] = {&p.dwo, &p.dwi, &p.dx};
+    int r = p.dh.splits > 1 ? launch<MT, F32, true, true, EPI_OUT, false, true, EPI_OUT>(p.dwo, p.dh, p.first_kind, s)
+                            : launch<MT, F32, true, true, EPI_OUT, false, true, EPI_DH>(p.dwo, p.dh, p.first_kind, s);
+    if (r == FC_OK) r = launch_sums<MT, F32>(hidden, 1, s);
     if (r == FC_OK) r = launch<MT, F32, true, true, EPI_OUT, false, true, EPI_OUT>(p.dwi, p.dx, p.second_kind, s);
     if (r == FC_OK) r = launch_sums<MT, F32>(sums, 3, s);
     return r;

@@ -56,6 +56,7 @@ struct FfnJob {
   int32_t M, N;          // outputs; for EPI_GATE N is the hidden size of one half, padded to 8
   int32_t tiles_m, tiles_n, splits, steps;  // steps: of 64 k, over all planes; a split takes steps / splits of them
   int32_t a_tr, b_tr;    // forms of A and B
+  int32_t finish;        // splits > 1: the epilogue that the sum of the parts goes through
   float scale;
   // EPI_OUT: out (., ld_out) of the operator's type; rows m >= gap_at are written gap rows earlier, rows in between not
   void* out;
@@ -321,6 +322,39 @@ struct Factors<true> {
   }
 };
 
+// The epilogues of the first products, for four columns from `col` on of row `row`; hp: columns of h, padded to 8; pad columns
+// take part in the next product as zeros.
+template <class MT, bool F32>
+__device__ __forceinline__ void finish_gate(const FfnJob& g, int64_t row, int col, int hp, const float (&gate)[4],
+                                            const float (&up)[4]) {
+  float a[4], b[4], h[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    float f, d;
+    ffn_act(g.act, gate[v], f, d);
+    a[v] = g.act_scale * f;
+    b[v] = g.act_scale * d * up[v];
+    h[v] = col + v < g.n_out ? a[v] * up[v] : 0.f;
+  }
+  const int64_t at = row * hp + col;
+  put4<MT, F32>(g.h, at, g.h_plane, h);
+  if (g.saved) put_factors<F32>(g.saved, at, (int64_t)g.M * hp, a, b);
+}
+template <class MT, bool F32>
+__device__ __forceinline__ void finish_dh(const FfnJob& g, int64_t row, int col, const Factors<F32>& f,
+                                          const float (&dh)[4]) {
+  float a[4], b[4], dg[4], du[4];
+  f.get(a, b);
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    dg[v] = col + v < g.n_out ? dh[v] * b[v] : 0.f;
+    du[v] = col + v < g.n_out ? dh[v] * a[v] : 0.f;
+  }
+  const int64_t at = row * 2 * g.N + col;
+  put4<MT, F32>(g.dpre, at, g.dpre_plane, dg);
+  put4<MT, F32>(g.dpre, at + g.N, g.dpre_plane, du);
+}
+
 // A float32 operand's value, native (ES = 4) or in planes.
 template <int ES, bool TR>
 __device__ __forceinline__ float value_of(const Opnd& o, int64_t r, int k) {
@@ -487,29 +521,7 @@ struct FfnTile {
       }
       if (wave < 4) turn();
     } else {
-      // One barrier a step; the loads run STAGES - 1 steps ahead.
-      constexpr int AHEAD = T::STAGES - 1;
       Cursor next_load = cursor_at(s0);
-      auto step = [&](const lds_char* at, lds_char* next) {
-        // this step's tiles have arrived, and everyone has read the stage of the step before
-        if constexpr (AHEAD == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((AHEAD - 1) * (la.SEGS + lb.SEGS)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        fetch(next_load, next, all, all);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          s16x8 a[T::MF], b[T::NF];
-          ra.template read<0, T::MF>(at, ks, a);
-          rb.template read<0, T::NF>(at + T::BM * 128, ks, b);
-#pragma unroll
-          for (int i = 0; i < T::MF; ++i)
-#pragma unroll
-            for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(b[j], a[i], acc[i][j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      };
       // The float32 instructions round after every product: sums of 256 k are kept apart and added (relative error of a
       // sum of 6,000 normal products 1.05e-6 in one chain, 3e-7 so).
       constexpr bool CHUNKS = std::is_same_v<MT, float>;
@@ -533,19 +545,78 @@ struct FfnTile {
         for (int i = 0; i < T::MF; ++i)
 #pragma unroll
           for (int j = 0; j < T::NF; ++j) sum[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
-      fetch(next_load, lds0, all, all);
       if constexpr (T::STAGES == 4) {
+        // One barrier a step; its products run while the next step's fragments are read, the loads four steps ahead.
+        constexpr int LOADS = la.SEGS + lb.SEGS;
+        struct Frags {
+          s16x8 a[2][T::MF], b[2][T::NF];
+        };
+        auto read = [&](const lds_char* at, Frags& f) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            rb.template read<0, T::NF>(at + T::BM * 128, ks, f.b[ks]);
+            ra.template read<0, T::MF>(at, ks, f.a[ks]);
+          }
+        };
+        auto multiply = [&](const Frags& f) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+              for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(f.b[ks][j], f.a[ks][i], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        Frags f, g2;
+        auto step = [&](lds_char* at, const lds_char* next, const Frags& now, Frags& then) {
+          // the next step's tiles have arrived, and everyone has read this step's
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          read(next, then);
+          __builtin_amdgcn_sched_barrier(0);
+          fetch(next_load, at, all, all);
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(now);
+        };
+        fetch(next_load, lds0, all, all);
         fetch(next_load, lds1, all, all);
         fetch(next_load, lds2, all, all);
+        fetch(next_load, lds3, all, all);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * LOADS) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(lds0, f);
 #pragma unroll 1
         for (int s = s0; s < s1; s += 4) {
-          step(lds0, lds3);
-          step(lds1, lds0);
-          step(lds2, lds1);
-          step(lds3, lds2);
+          step(lds0, lds1, f, g2);
+          step(lds1, lds2, g2, f);
+          step(lds2, lds3, f, g2);
+          step(lds3, lds0, g2, f);
           flush(++turn % EVERY == 0);
         }
       } else {
+        // One barrier a step; the loads run one step ahead.
+        auto step = [&](const lds_char* at, lds_char* next) {
+          // this step's tiles have arrived, and everyone has read the other stage
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          fetch(next_load, next, all, all);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            s16x8 a[T::MF], b[T::NF];
+            ra.template read<0, T::MF>(at, ks, a);
+            rb.template read<0, T::NF>(at + T::BM * 128, ks, b);
+#pragma unroll
+            for (int i = 0; i < T::MF; ++i)
+#pragma unroll
+              for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(b[j], a[i], acc[i][j]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        fetch(next_load, lds0, all, all);
 #pragma unroll 1
         for (int s = s0; s < s1; s += 2) {
           step(lds0, lds1);
@@ -644,7 +715,6 @@ struct FfnTile {
       }
     } else if constexpr (EPI == EPI_GATE) {
       constexpr int HF = T::NF / 2;
-      const int64_t count = (int64_t)g.M * g.N;
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
         const int64_t row = row0 + 16 * i;
@@ -653,20 +723,13 @@ struct FfnTile {
         for (int j = 0; j < HF; ++j) {
           const int col = n0 + wn * (T::TN / 2) + 16 * j + q4;
           if (col >= g.N) continue;
-          float a[4], b[4], h[4];
+          float gate[4], up[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const float gate = acc[i][j][v] * scale, up = acc[i][j + HF][v] * scale;
-            float f, d;
-            ffn_act(g.act, gate, f, d);
-            a[v] = g.act_scale * f;
-            b[v] = g.act_scale * d * up;
-            h[v] = a[v] * up;
-            if (col + v >= g.n_out) h[v] = 0.f;  // pad columns take part in the next product
+            gate[v] = acc[i][j][v] * scale;
+            up[v] = acc[i][j + HF][v] * scale;
           }
-          const int64_t at = row * g.N + col;
-          put4<MT, F32>(g.h, at, g.h_plane, h);
-          if (g.saved) put_factors<F32>(g.saved, at, count, a, b);
+          finish_gate<MT, F32>(g, row, col, g.N, gate, up);
         }
       }
     } else {
@@ -690,17 +753,10 @@ struct FfnTile {
         for (int j = 0; j < T::NF; ++j) {
           const int col = n0 + wn * T::TN + 16 * j + q4;
           if (col >= g.N) continue;
-          float a[4], b[4], dg[4], du[4];
-          f[i & 1][j].get(a, b);
+          float dh[4];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float dh = acc[i][j][v] * scale;
-            dg[v] = col + v < g.n_out ? dh * b[v] : 0.f;
-            du[v] = col + v < g.n_out ? dh * a[v] : 0.f;
-          }
-          const int64_t at = row * 2 * g.N + col;
-          put4<MT, F32>(g.dpre, at, g.dpre_plane, dg);
-          put4<MT, F32>(g.dpre, at + g.N, g.dpre_plane, du);
+          for (int v = 0; v < 4; ++v) dh[v] = acc[i][j][v] * scale;
+          finish_dh<MT, F32>(g, row, col, f[i & 1][j], dh);
         }
       }
     }
