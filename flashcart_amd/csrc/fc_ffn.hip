@@ -172,11 +172,11 @@ static void set_tiles(FfnJob& g, int kind, bool gate) {
 // few CUs (n = 30,000, width = hidden = 64), full devices at 1,024 to 16,384 rows. The 64 x 64 tile is bound by what the L2
 // caches deliver, the 256 x 256 tile by the matrix cores.
 struct TileCost {
-  double step, full, end;
+  double step, full, end, fused;  // fused: the end with an epilogue of the block's elementwise steps
 };
-constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8}, {0.65, 0.55, 2.5}, {1.25, 1.5, 9.0}};
+constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8, 2.0}, {0.65, 0.55, 2.5, 6.25}, {1.25, 1.5, 9.0, 22.5}};
 // native float32, 32 k a step: bound by the matrix cores
-constexpr TileCost kNativeCost[2] = {{0.6, 0.62, 1.0}, {2.05, 1.85, 5.0}};
+constexpr TileCost kNativeCost[2] = {{0.5, 0.56, 1.0, 2.6}, {2.05, 1.85, 5.0, 6.5}};
 
 enum Form { FORM_16, FORM_NATIVE, FORM_PLANES };
 
@@ -204,7 +204,7 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
         FfnJob& g = *jobs[q];
         if (g.M == 0) continue;
         set_tiles(g, kind, gate);
-        double end = c.end * (can_split[q] ? 1 : 2.5) * (form == FORM_PLANES ? 1.5 : 1);
+        double end = (can_split[q] ? c.end : c.fused) * (form == FORM_PLANES ? 1.5 : 1);
         if (can_split[q] && g.steps * c.step > most) {
           splits[q] = (int)(g.steps * c.step / most) + 1;
           if (splits[q] > g.steps / 4) splits[q] = g.steps / 4 > 1 ? g.steps / 4 : 1;
@@ -220,9 +220,9 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
         const double t = steps * c.step + end;
         longest = t > longest ? t : longest;
       }
-      // whole rounds of workgroups where the matrix cores bound them, something between where the caches do
+      // whole rounds of workgroups where they are few and the matrix cores bound them, something between otherwise
       const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
-      if (blocks > cus) load *= form == FORM_NATIVE ? rounds : 0.5 + 0.5 * rounds;
+      if (blocks > cus) load *= form == FORM_NATIVE && blocks <= 2 * cus ? rounds : 0.5 + 0.5 * rounds;
       double time = load > longest ? load : longest;
       if (sums > 0) time += sums + 3.5;
       if (time < best) {

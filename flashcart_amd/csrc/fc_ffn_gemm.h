@@ -565,7 +565,6 @@ struct FfnTile {
             for (int i = 0; i < T::MF; ++i)
 #pragma unroll
               for (int j = 0; j < T::NF; ++j) acc[i][j] = mfma16<MT>(f.b[ks][j], f.a[ks][i], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
         };
         Frags f, g2;
         auto step = [&](lds_char* at, const lds_char* next, const Frags& now, Frags& then) {
@@ -574,10 +573,17 @@ struct FfnTile {
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           read(next, then);
-          __builtin_amdgcn_sched_barrier(0);
           fetch(next_load, at, all, all);
-          __builtin_amdgcn_sched_barrier(0);
           multiply(now);
+          // reads and loads are issued between the products
+          constexpr int PRODUCTS = 2 * T::MF * T::NF * (std::is_same_v<MT, float> ? 4 : 1);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / 8, 0);  // matrix
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);             // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);             // loads
+          }
+          __builtin_amdgcn_sched_barrier(0);
         };
         fetch(next_load, lds0, all, all);
         fetch(next_load, lds1, all, all);
