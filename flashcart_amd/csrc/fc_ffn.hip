@@ -197,7 +197,7 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
       if (jobs[q]->M > 0 && can_split[q] && jobs[q]->steps * c.step > chain) chain = jobs[q]->steps * c.step;
     double most = chain + 1;  // of a workgroup's steps
     do {
-      double load = 0, longest = 0, sums = 0;
+      double load = 0, sums = 0, steps[2] = {0, 0}, ends[2] = {0, 0};
       int64_t blocks = 0;
       int splits[2] = {1, 1};
       for (int q = 0; q < count; ++q) {
@@ -214,12 +214,16 @@ static int plan_launch(FfnJob* const* jobs, const bool* can_split, int count, Fo
           sums += 8e-6 / 3 * splits[q] * g.M * g.N;
         }
         const int64_t n = (int64_t)g.tiles_m * g.tiles_n * splits[q];
-        const double steps = (double)g.steps / splits[q];
+        steps[q] = (double)g.steps / splits[q];
+        ends[q] = end;
         blocks += n;
-        load += n * (steps * c.full + end) / cus;
-        const double t = steps * c.step + end;
-        longest = t > longest ? t : longest;
+        load += n * (steps[q] * c.full + end) / cus;
       }
+      // the longest workgroup, which shares its CU with another one where the device is full (not the largest tile)
+      const double shared = (kind < 2 ? 2 : 1) * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
+      double longest = 0;
+      for (int q = 0; q < count; ++q)
+        if (steps[q] * pace + ends[q] > longest) longest = steps[q] * pace + ends[q];
       // whole rounds of workgroups where they are few and the matrix cores bound them, something between otherwise
       const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
       if (blocks > cus) load *= form == FORM_NATIVE && blocks <= 2 * cus ? rounds : 0.5 + 0.5 * rounds;
