@@ -44,10 +44,7 @@ __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = from >= 0 && c0 + i < it.cols ? to_f32(src[i]) : 0.f;
   }
-  const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-  const int64_t at = row * it.ld + c0;
-  put4<MT, std::is_same_v<T, float>>(it.dst, at, it.plane, lo);
-  put4<MT, std::is_same_v<T, float>>(it.dst, at + 4, it.plane, hi);
+  put<MT, std::is_same_v<T, float>, 8>(it.dst, row * it.ld + c0, it.plane, x);
 }
 
 // ---- sums over the parts of split K loops ----
@@ -111,14 +108,14 @@ __global__ void __launch_bounds__(256) ffn_sum_kernel(SumArgs a) {
   if (g.finish == EPI_GATE) {
     float up[4];
     total(cols + col, up);
-    if (ok && grp == 0) finish_gate<MT, F32>(g, row, col, cols, x, up);
+    if (ok && grp == 0) finish_gate<MT, F32, 4>(g, row, col, cols, x, up);
     return;
   }
   if (!ok || grp > 0) return;
   if (g.finish == EPI_DH) {
-    Factors<F32> f;
+    Factors<F32, 4> f;
     f.load(g.saved, row * g.N + col, (int64_t)g.M * g.N);
-    finish_dh<MT, F32>(g, row, col, f, x);
+    finish_dh<MT, F32, 4>(g, row, col, f, x);
     return;
   }
   if (row >= g.gap_at) {

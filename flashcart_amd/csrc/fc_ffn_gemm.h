@@ -226,22 +226,39 @@ __device__ __forceinline__ void split3(float x, uint16_t& h, uint16_t& m, uint16
   l = from_f32<bf16_t>(r - to_f32(bf16_t{m})).v;
 }
 
-// Four consecutive values, from element `at` on, of a matrix in the operator's operand form.
-template <class MT, bool F32>
-__device__ __forceinline__ void put4(char* matrix, int64_t at, int64_t plane, const float (&x)[4]) {
-  if constexpr (std::is_same_v<MT, float>) {
-    *(float4*)(matrix + 4 * at) = make_float4(x[0], x[1], x[2], x[3]);
-  } else if constexpr (!F32) {
-    *(uint2*)(matrix + 2 * at) = make_uint2(pack2<MT>(x[0], x[1]), pack2<MT>(x[2], x[3]));
-  } else {
-    uint32_t h[2], m[2], l[2];
-    const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    float sum = 0.f;
+// V (4 or 8) consecutive 16-bit values.
+template <int V>
+__device__ __forceinline__ void put_words(void* p, const uint32_t (&x)[V / 2]) {
+  if constexpr (V == 8) *(uint4*)p = make_uint4(x[0], x[1], x[2], x[3]);
+  else *(uint2*)p = make_uint2(x[0], x[1]);
+}
+template <int V>
+__device__ __forceinline__ void put_floats(float* p, const float (&x)[V]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum = fmaf(x[i], 0.f, sum);
+  for (int i = 0; i < V; i += 4) *(float4*)(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+
+// V consecutive values, from element `at` on, of a matrix in the operator's operand form.
+template <class MT, bool F32, int V>
+__device__ __forceinline__ void put(char* matrix, int64_t at, int64_t plane, const float (&x)[V]) {
+  if constexpr (std::is_same_v<MT, float>) {
+    put_floats((float*)matrix + at, x);
+  } else if constexpr (!F32) {
+    uint32_t u[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) u[i] = pack2<MT>(x[2 * i], x[2 * i + 1]);
+    put_words<V>(matrix + 2 * at, u);
+  } else {
+    uint32_t h[V / 2], m[V / 2], l[V / 2];
+    float most = 0.f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      most = fmaxf(most, fabsf(x[i]));
+      sum = fmaf(x[i], 0.f, sum);
+    }
     if (most < 0x1.fep127f && sum == 0.f) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < V / 2; ++i) {
         const float a = x[2 * i], b = x[2 * i + 1];
         h[i] = pack2<bf16_t>(a, b);
         const float ra = a - __uint_as_float(h[i] << 16), rb = b - __uint_as_float(h[i] & 0xffff0000u);
@@ -250,7 +267,7 @@ __device__ __forceinline__ void put4(char* matrix, int64_t at, int64_t plane, co
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < V / 2; ++i) {
         uint16_t u[2], v[2], w[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) split3(x[2 * i + q], u[q], v[q], w[q]);
@@ -260,76 +277,85 @@ __device__ __forceinline__ void put4(char* matrix, int64_t at, int64_t plane, co
       }
     }
     uint16_t* p = (uint16_t*)matrix + at;
-    *(uint2*)p = make_uint2(h[0], h[1]);
-    *(uint2*)(p + plane) = make_uint2(m[0], m[1]);
-    *(uint2*)(p + 2 * plane) = make_uint2(l[0], l[1]);
+    put_words<V>(p, h);
+    put_words<V>(p + plane, m);
+    put_words<V>(p + 2 * plane, l);
   }
 }
 
 // Factors kept for the backward pass. For 16-bit types they keep 24 bits (the upper half of a float32 and the next 8 bits
 // of each of the pair in one more uint16), so that their rounding does not add to those of dpre and of the gradients.
 // (v_perm_b32: bytes 0 to 3 are those of its second operand, 4 to 7 those of the first.)
-template <bool F32>
-__device__ __forceinline__ void put_factors(void* saved, int64_t at, int64_t count, const float (&a)[4],
-                                            const float (&b)[4]) {
+template <bool F32, int V>
+__device__ __forceinline__ void put_factors(void* saved, int64_t at, int64_t count, const float (&a)[V],
+                                            const float (&b)[V]) {
   if constexpr (F32) {
-    float* p = (float*)saved + at;
-    *(float4*)p = make_float4(a[0], a[1], a[2], a[3]);
-    *(float4*)(p + count) = make_float4(b[0], b[1], b[2], b[3]);
+    put_floats((float*)saved + at, a);
+    put_floats((float*)saved + count + at, b);
   } else {
-    uint32_t u[4], v[4], lo[4];
+    uint32_t ah[V / 2], bh[V / 2], lo[V / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u[i] = __float_as_uint(a[i]) + 0x80;  // (infinite and NaN stay so: the lowest bits of such a value are zero)
-      v[i] = __float_as_uint(b[i]) + 0x80;
-      lo[i] = __builtin_amdgcn_perm(v[i], u[i], 0x0c0c0501);
+    for (int i = 0; i < V / 2; ++i) {
+      // (infinite and NaN stay so: the lowest bits of such a value are zero)
+      const uint32_t u0 = __float_as_uint(a[2 * i]) + 0x80, u1 = __float_as_uint(a[2 * i + 1]) + 0x80;
+      const uint32_t v0 = __float_as_uint(b[2 * i]) + 0x80, v1 = __float_as_uint(b[2 * i + 1]) + 0x80;
+      ah[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302);
+      bh[i] = __builtin_amdgcn_perm(v1, v0, 0x07060302);
+      lo[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v1, u1, 0x0c0c0501), __builtin_amdgcn_perm(v0, u0, 0x0c0c0501),
+                                    0x05040100);
     }
     uint16_t* p = (uint16_t*)saved + at;
-    *(uint2*)p = make_uint2(__builtin_amdgcn_perm(u[1], u[0], 0x07060302), __builtin_amdgcn_perm(u[3], u[2], 0x07060302));
-    *(uint2*)(p + count) =
-        make_uint2(__builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302));
-    *(uint2*)(p + 2 * count) =
-        make_uint2(__builtin_amdgcn_perm(lo[1], lo[0], 0x05040100), __builtin_amdgcn_perm(lo[3], lo[2], 0x05040100));
+    put_words<V>(p, ah);
+    put_words<V>(p + count, bh);
+    put_words<V>(p + 2 * count, lo);
   }
 }
-template <bool F32>
+template <bool F32, int V>
 struct Factors {
-  uint2 x[3];
+  uint32_t x[F32 ? 2 : 3][F32 ? V : V / 2];
   __device__ __forceinline__ void load(const void* saved, int64_t at, int64_t count) {
-    const uint16_t* p = (const uint16_t*)saved + at;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) x[i] = *(const uint2*)(p + i * count);
-  }
-  __device__ __forceinline__ void get(float (&a)[4], float (&b)[4]) const {
+    for (int i = 0; i < (F32 ? 2 : 3); ++i) {
+      const uint32_t* p = (const uint32_t*)((const char*)saved + (F32 ? 4 : 2) * (at + i * count));
+      constexpr int WORDS = sizeof(x[0]) / 4;
+      if constexpr (WORDS == 2) {
+        const uint2 v = *(const uint2*)p;
+        x[i][0] = v.x;
+        x[i][1] = v.y;
+      } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = i < 2 ? x[0].x : x[0].y, v = i < 2 ? x[1].x : x[1].y, lo = i < 2 ? x[2].x : x[2].y;
-      a[i] = __uint_as_float(__builtin_amdgcn_perm(u, lo, i % 2 ? 0x0706020c : 0x0504000c));
-      b[i] = __uint_as_float(__builtin_amdgcn_perm(v, lo, i % 2 ? 0x0706030c : 0x0504010c));
+        for (int k = 0; k < WORDS; k += 4) {
+          const uint4 v = *(const uint4*)(p + k);
+          x[i][k] = v.x;
+          x[i][k + 1] = v.y;
+          x[i][k + 2] = v.z;
+          x[i][k + 3] = v.w;
+        }
+      }
     }
   }
-};
-template <>
-struct Factors<true> {
-  float4 x[2];
-  __device__ __forceinline__ void load(const void* saved, int64_t at, int64_t count) {
-    x[0] = *(const float4*)((const float*)saved + at);
-    x[1] = *(const float4*)((const float*)saved + count + at);
-  }
-  __device__ __forceinline__ void get(float (&a)[4], float (&b)[4]) const {
-    a[0] = x[0].x; a[1] = x[0].y; a[2] = x[0].z; a[3] = x[0].w;
-    b[0] = x[1].x; b[1] = x[1].y; b[2] = x[1].z; b[3] = x[1].w;
+  __device__ __forceinline__ void get(float (&a)[V], float (&b)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (F32) {
+        a[i] = __uint_as_float(x[0][i]);
+        b[i] = __uint_as_float(x[1][i]);
+      } else {
+        a[i] = __uint_as_float(__builtin_amdgcn_perm(x[0][i / 2], x[2][i / 2], i % 2 ? 0x0706020c : 0x0504000c));
+        b[i] = __uint_as_float(__builtin_amdgcn_perm(x[1][i / 2], x[2][i / 2], i % 2 ? 0x0706030c : 0x0504010c));
+      }
+    }
   }
 };
 
-// The epilogues of the first products, for four columns from `col` on of row `row`; hp: columns of h, padded to 8; pad columns
+// The epilogues of the first products, for V columns from `col` on of row `row`; hp: columns of h, padded to 8; pad columns
 // take part in the next product as zeros.
-template <class MT, bool F32>
-__device__ __forceinline__ void finish_gate(const FfnJob& g, int64_t row, int col, int hp, const float (&gate)[4],
-                                            const float (&up)[4]) {
-  float a[4], b[4], h[4];
+template <class MT, bool F32, int V>
+__device__ __forceinline__ void finish_gate(const FfnJob& g, int64_t row, int col, int hp, const float (&gate)[V],
+                                            const float (&up)[V]) {
+  float a[V], b[V], h[V];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
+  for (int v = 0; v < V; ++v) {
     float f, d;
     ffn_act(g.act, gate[v], f, d);
     a[v] = g.act_scale * f;
@@ -337,22 +363,22 @@ __device__ __forceinline__ void finish_gate(const FfnJob& g, int64_t row, int co
     h[v] = col + v < g.n_out ? a[v] * up[v] : 0.f;
   }
   const int64_t at = row * hp + col;
-  put4<MT, F32>(g.h, at, g.h_plane, h);
-  if (g.saved) put_factors<F32>(g.saved, at, (int64_t)g.M * hp, a, b);
+  put<MT, F32, V>(g.h, at, g.h_plane, h);
+  if (g.saved) put_factors<F32, V>(g.saved, at, (int64_t)g.M * hp, a, b);
 }
-template <class MT, bool F32>
-__device__ __forceinline__ void finish_dh(const FfnJob& g, int64_t row, int col, const Factors<F32>& f,
-                                          const float (&dh)[4]) {
-  float a[4], b[4], dg[4], du[4];
+template <class MT, bool F32, int V>
+__device__ __forceinline__ void finish_dh(const FfnJob& g, int64_t row, int col, const Factors<F32, V>& f,
+                                          const float (&dh)[V]) {
+  float a[V], b[V], dg[V], du[V];
   f.get(a, b);
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
+  for (int v = 0; v < V; ++v) {
     dg[v] = col + v < g.n_out ? dh[v] * b[v] : 0.f;
     du[v] = col + v < g.n_out ? dh[v] * a[v] : 0.f;
   }
   const int64_t at = row * 2 * g.N + col;
-  put4<MT, F32>(g.dpre, at, g.dpre_plane, dg);
-  put4<MT, F32>(g.dpre, at + g.N, g.dpre_plane, du);
+  put<MT, F32, V>(g.dpre, at, g.dpre_plane, dg);
+  put<MT, F32, V>(g.dpre, at + g.N, g.dpre_plane, du);
 }
 
 // A float32 operand's value, native (ES = 4) or in planes.
@@ -638,8 +664,10 @@ struct FfnTile {
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const int r = lane & 15, q4 = 4 * (lane >> 4);
-    const int row0 = m0 + wm * T::TM + r;
+    // (anew, so that nothing of it is held in registers through the loop)
+    int again_tid = threadIdx.x;
+    asm volatile("" : "+v"(again_tid));
+    const int end_lane = again_tid & 63;
     float scale = g.scale;
     if constexpr (F32) {
       float probe = 0.f;
@@ -651,11 +679,13 @@ struct FfnTile {
           for (int v = 0; v < 4; ++v) probe = fmaf(acc[i][j][v], 0.f, probe);
       // (a split K loop leaves this to the sum over its parts)
       if (g.splits == 1 && __any(probe != probe)) {
-        again(g, m0, n0, wm, wn, lane, acc);
+        again(g, m0, n0, wm, wn, end_lane, acc);
         scale = 1.f;
       }
     }
-    epilogue(g, scale, split, row0, n0, wn, q4, acc);
+    __builtin_amdgcn_s_barrier();  // (everyone has read the stages, and their last loads have arrived)
+    asm volatile("" ::: "memory");
+    epilogue(g, scale, split, m0 + wm * T::TM, n0, wave, wn, end_lane, lds0, acc);
   }
 
   // In plain float32, scaled before the sum, which may stay finite where the sum of the unscaled products does not: lane
@@ -685,85 +715,97 @@ struct FfnTile {
     }
   }
 
-  __device__ static __forceinline__ void epilogue(const FfnJob& g, float scale, int split, int row0, int n0, int wn, int q4,
-                                                  f32x4v (&acc)[T::MF][T::NF]) {
+  // 16 rows of the wave's outputs at a time go through LDS, where a lane writes 4 columns of a row and takes 8, so that
+  // memory is read and written in whole lines: as they come out of the products, a store would write 32 bytes of each of
+  // 16 rows (16,384 x 2,048 x 5,632 in bf16: hidden gradient 640 us, of them 165 of stores).
+  __device__ static __forceinline__ void epilogue(const FfnJob& g, float scale, int split, int row0, int n0, int wave, int wn,
+                                                  int lane, lds_char* lds, f32x4v (&acc)[T::MF][T::NF]) {
+    typedef __attribute__((address_space(3))) f32x4v lds_f32x4;
+    constexpr int RS = T::TN * 4 + 16, COLS = EPI == EPI_GATE ? T::TN / 2 : T::TN;
+    constexpr int LPR = COLS / 8, RPP = 64 / LPR < 16 ? 64 / LPR : 16, PASSES = 16 / RPP;  // lanes a row, rows a pass
+    static_assert(T::NW * 16 * RS <= T::STAGE, "a stage holds 16 rows of each wave");
+    lds_char* const mine = lds + wave * 16 * RS;
+    lds_char* const to = mine + (lane & 15) * RS + (lane >> 4) * 16;
+    const int rl = lane / LPR, cl = lane % LPR * 8;
+    const lds_char* const from = mine + rl * RS + cl * 4;
+    const int col = n0 + wn * COLS + cl;
+    const bool on = rl < RPP;
+    auto stage = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < T::NF; ++j) *(lds_f32x4*)(to + 64 * j) = acc[i][j];
+    };
+    auto take = [&](const lds_char* p, float (&x)[8]) {
+      const f32x4v u = *(const lds_f32x4*)p, v = *(const lds_f32x4*)(p + 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = u[k] * scale;
+        x[4 + k] = v[k] * scale;
+      }
+    };
     if constexpr (EPI == EPI_OUT) {
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
-        int64_t row = row0 + 16 * i;
-        if (row >= g.M) continue;
-        if (g.splits > 1) {
-          float* p = g.partial + ((int64_t)split * g.M + row) * g.N;
+        stage(i);
 #pragma unroll
-          for (int j = 0; j < T::NF; ++j) {
-            const int col = n0 + wn * T::TN + 16 * j + q4;  // N is a multiple of 4
-            if (col < g.N) *(f32x4v*)(p + col) = acc[i][j];
+        for (int p = 0; p < PASSES; ++p) {
+          int64_t row = row0 + 16 * i + p * RPP + rl;
+          if (row >= g.M || col >= g.N) continue;
+          float x[8];
+          if (g.splits > 1) {  // unscaled
+            const f32x4v u = *(const lds_f32x4*)(from + p * RPP * RS), v = *(const lds_f32x4*)(from + p * RPP * RS + 16);
+            float* out = g.partial + ((int64_t)split * g.M + row) * g.N + col;
+            *(f32x4v*)out = u;
+            *(f32x4v*)(out + 4) = v;
+            continue;
           }
-          continue;
-        }
-        if (row >= g.gap_at) {
-          if (row < g.gap_at + g.gap) continue;
-          row -= g.gap;
-        }
-        if (row >= g.m_out) continue;
-        OT* p = (OT*)g.out + row * g.ld_out;
+          take(from + p * RPP * RS, x);
+          if (row >= g.gap_at) {
+            if (row < g.gap_at + g.gap) continue;
+            row -= g.gap;
+          }
+          if (row >= g.m_out) continue;
+          OT* out = (OT*)g.out + row * g.ld_out + col;
+          Pack<OT, 8> o;
 #pragma unroll
-        for (int j = 0; j < T::NF; ++j) {
-          const int col = n0 + wn * T::TN + 16 * j + q4;
-          Pack<OT, 4> o;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) o.v[v] = from_f32<OT>(acc[i][j][v] * scale);
-          if (col + 4 <= g.n_out) store_pack<OT, 4>(p + col, o);
+          for (int v = 0; v < 8; ++v) o.v[v] = from_f32<OT>(x[v]);
+          if (col + 8 <= g.n_out) store_pack<OT, 8>(out, o);
           else
-            for (int v = 0; v < 4; ++v)
-              if (col + v < g.n_out) p[col + v] = o.v[v];
+            for (int v = 0; v < 8; ++v)
+              if (col + v < g.n_out) out[v] = o.v[v];
         }
       }
     } else if constexpr (EPI == EPI_GATE) {
-      constexpr int HF = T::NF / 2;
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
-        const int64_t row = row0 + 16 * i;
-        if (row >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < HF; ++j) {
-          const int col = n0 + wn * (T::TN / 2) + 16 * j + q4;
-          if (col >= g.N) continue;
-          float gate[4], up[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            gate[v] = acc[i][j][v] * scale;
-            up[v] = acc[i][j + HF][v] * scale;
-          }
-          finish_gate<MT, F32>(g, row, col, g.N, gate, up);
-        }
+        stage(i);
+        const int64_t row = row0 + 16 * i + rl;
+        if (!on || row >= g.M || col >= g.N) continue;
+        float gate[8], up[8];
+        take(from, gate);
+        take(from + COLS * 4, up);
+        finish_gate<MT, F32, 8>(g, row, col, g.N, gate, up);
       }
     } else {
-      // the factors of the next 16 rows are loaded before this one's results are stored
+      // the factors of the next turns are loaded before these rows' results are stored
+      constexpr int TURNS = T::MF * PASSES, AHEAD = PLANES ? 1 : TURNS < 5 ? TURNS - 1 : 4;
       const int64_t count = (int64_t)g.M * g.N;
-      Factors<F32> f[2][T::NF];
-      auto load = [&](int i, Factors<F32> (&x)[T::NF]) {
-        const int64_t row = min(row0 + 16 * i, g.M - 1);
-#pragma unroll
-        for (int j = 0; j < T::NF; ++j)
-          x[j].load(g.saved, row * g.N + min(n0 + wn * T::TN + 16 * j + q4, g.N - 4), count);
+      Factors<F32, 8> f[AHEAD + 1];
+      auto load = [&](int t) {
+        const int64_t row = min(row0 + t * RPP + rl, g.M - 1);
+        f[t % (AHEAD + 1)].load(g.saved, row * g.N + min(col, g.N - 8), count);
       };
-      load(0, f[0]);
 #pragma unroll
-      for (int i = 0; i < T::MF; ++i) {
-        const int64_t row = row0 + 16 * i;
-        if (i + 1 < T::MF) load(i + 1, f[(i + 1) & 1]);
+      for (int t = 0; t < AHEAD; ++t) load(t);
+#pragma unroll
+      for (int t = 0; t < TURNS; ++t) {
+        if (t % PASSES == 0) stage(t / PASSES);
+        if (t + AHEAD < TURNS) load(t + AHEAD);
         __builtin_amdgcn_sched_barrier(0);
-        if (row >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < T::NF; ++j) {
-          const int col = n0 + wn * T::TN + 16 * j + q4;
-          if (col >= g.N) continue;
-          float dh[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) dh[v] = acc[i][j][v] * scale;
-          finish_dh<MT, F32>(g, row, col, f[i & 1][j], dh);
-        }
+        const int64_t row = row0 + t * RPP + rl;
+        if (row >= g.M || col >= g.N) continue;
+        float dh[8];
+        take(from + t % PASSES * RPP * RS, dh);
+        finish_dh<MT, F32, 8>(g, row, col, f[t % (AHEAD + 1)], dh);
       }
     }
   }
