@@ -295,11 +295,12 @@ static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
 static int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
 // float32 in planes where the products are large and the operands are used often enough for their splitting to pay.
-// Forward and backward, us, planes against native: 16,384 x 1,024 x 2,048 4,230 / 4,750, 2,048 x 1,024 x 2,048 746 / 858,
-// 4,096 x 512 x 1,024 433 / 371, 25,000 x 128 x 512 504 / 405, 512 x 512 x 512 101 / 64, 6 x 966 x 6,967 276 / 223.
+// Forward and backward, us, planes against native: 8,192 x 2,048 x 4,096 5,850 / 9,100, 2,048 x 1,024 x 2,048 542 / 719,
+// 1,024 x 1,024 x 2,048 326 / 373, 4,096 x 512 x 1,024 345 / 377, 583 x 736 x 3,680 352 / 347, 25,000 x 128 x 512 411 / 393,
+// 2,520 x 256 x 768 161 / 133, 512 x 512 x 512 84 / 62.
 static Form form_of(const fc_ffn_desc& d, int64_t n) {
   if (d.dtype != FC_F32) return FORM_16;
-  const bool large = n >= 1024 && d.width >= 512 && d.hidden >= 512 && (double)n * d.width * d.hidden >= 3.2e9;
+  const bool large = n >= 512 && d.width >= 512 && d.hidden >= 512 && (double)n * d.width * d.hidden >= 2e9;
   return large ? FORM_PLANES : FORM_NATIVE;
 }
 

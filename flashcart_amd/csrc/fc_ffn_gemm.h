@@ -75,9 +75,10 @@ struct FfnJob {
 
 constexpr uint32_t kOutOfRange = 0x7ffffff0u;  // byte offset that a buffer load answers with zeros
 
-__device__ __forceinline__ void plane_pair(int i, int& a, int& b) {  // smallest products first
-  a = i == 0 ? 0 : i == 1 ? 2 : i == 2 ? 1 : i == 3 ? 0 : i == 4 ? 1 : 0;
-  b = i == 0 ? 2 : i == 1 ? 0 : i == 2 ? 1 : i == 3 ? 1 : 0;
+// Planes of the pair i: 0 2, 2 0, 1 1, 0 1, 1 0, 0 0, the smallest products first.
+__device__ __forceinline__ void plane_pair(int i, int& a, int& b) {
+  a = (0x010120 >> (4 * i)) & 15;
+  b = (0x001102 >> (4 * i)) & 15;
 }
 
 // act(g) and its derivative; 0 silu, 1 sigmoid, 2 gelu (erf form)
@@ -434,7 +435,8 @@ struct FfnTile {
 #pragma unroll
       for (int j = 0; j < T::NF; ++j) acc[i][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
 
-    const int s0 = (int)((int64_t)g.steps * split / g.splits), s1 = (int)((int64_t)g.steps * (split + 1) / g.splits);
+    const int s0 = __builtin_amdgcn_readfirstlane((int)((int64_t)g.steps * split / g.splits));
+    const int s1 = __builtin_amdgcn_readfirstlane((int)((int64_t)g.steps * (split + 1) / g.splits));
     // Where the next load of some segments is: k, and the planes (float32: the pair, smallest products first).
     struct Cursor {
       int left, k, pair;  // left: steps before the end
@@ -445,8 +447,9 @@ struct FfnTile {
       if constexpr (PLANES) {
         int pa, pb;
         plane_pair(c.pair, pa, pb);
-        c.a = pa * g.A.plane;
-        c.b = pb * g.B.plane;
+        // (in scalar registers: a buffer's base that the compiler takes for different in the lanes costs a loop a load)
+        c.a = __builtin_amdgcn_readfirstlane(pa) * g.A.plane;
+        c.b = __builtin_amdgcn_readfirstlane(pb) * g.B.plane;
       } else {
         c.a = c.b = 0;
       }
@@ -454,7 +457,7 @@ struct FfnTile {
     auto cursor_at = [&](int s) {
       Cursor c;
       c.left = s1 - s;
-      c.pair = PLANES ? s / per_pair : 0;
+      c.pair = PLANES ? __builtin_amdgcn_readfirstlane(s / per_pair) : 0;
       c.k = KS * (s - c.pair * per_pair);
       place(c);
       return c;
