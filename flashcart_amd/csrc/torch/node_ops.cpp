@@ -278,7 +278,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_feed_forward_bwd(const Tensor& grad_, c
   if ((uintptr_t)saved.const_data_ptr() & 15) saved = saved.clone();
   d.aligned = aligned({&grad, &x, &w_in, &w_out});
   auto result = [&](const Tensor& t, bool need) {
-    return !need ? at::empty({0}, t.options()) : n == 0 ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options());
+    if (!need) return at::empty({0}, t.options());
+    return n == 0 ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options());
   };
   Tensor gx = result(x, need_x), gwi = result(w_in, need_w_in), gwo = result(w_out, need_w_out);
   if (n > 0) {

@@ -53,10 +53,10 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
         act_scale, scale_in, scale_out: factors, as the rescaled activations and linear layers of this package have them.
 
     Sums are float32. For bfloat16 and float16 the hidden values ``act(gate) * up`` and, in the backward pass, the
-    gradients of gate and up are rounded to that type, being operands of the matrix instructions; the activation and its
-    derivative are formed from unrounded values. float32 products keep float32 accuracy (operands below 2^-116 lose
-    bits). In training the block keeps the hidden values and the activation's factors: 8 bytes per hidden value (14 for
-    float32). There are no second derivatives.
+    gradients of gate and up are rounded to that type, being operands of the matrix instructions; the activation and
+    its derivative are formed from unrounded values. (float16: hidden values above 65,504 become infinite.) float32
+    products keep float32 accuracy (operands below 2^-116 lose bits). In training the block keeps the hidden values
+    and the activation's factors: 8 bytes per hidden value (14 for float32). There are no second derivatives.
     """
     if act not in _node_ops.ACTIVATIONS:
         raise ValueError(f"act must be one of {sorted(_node_ops.ACTIVATIONS)}, got {act!r}.")

@@ -68,11 +68,12 @@ def test_library_refuses_bad_arguments():
     assert lib.fc_dropout_add(0, 1, 16, None, 0.5, None, 16, None) == null
     desc = _lib.FfnDesc(0, 0, 8, 16, 1, 1.0, 1.0, 1.0)
     assert lib.fc_ffn_saved(desc, 3) == 3 * 16 * 14 and lib.fc_ffn_saved(desc, -1) == -shape
+    assert lib.fc_ffn_fwd(desc, 3, 18, 16, 16, 16, 16, 16, 1 << 20, None) == bad_desc  # not aligned
+    desc.aligned = 0  # every operand is copied
     size = lib.fc_ffn_fwd_workspace(desc, 3, 1)
     assert size > 0 and lib.fc_ffn_fwd_workspace(desc, 3, 0) > size
     assert lib.fc_ffn_fwd(desc, 3, 16, 16, 16, 16, 16, 16, size - 1, None) == workspace
     assert lib.fc_ffn_fwd(desc, 3, 16, 16, 16, None, 16, 16, size, None) == null
-    assert lib.fc_ffn_fwd(desc, 3, 18, 16, 16, 16, 16, 16, size, None) == bad_desc
     assert lib.fc_ffn_bwd(desc, 3, 16, 16, 16, 16, None, 16, None, None, 16, 1 << 20, None) == null
     for bad, code in ((dict(dtype=3), bad_desc), (dict(act=3), bad_desc), (dict(width=0), shape),
                       (dict(hidden=(1 << 20) + 1), shape)):
