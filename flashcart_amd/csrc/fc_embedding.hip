@@ -14,6 +14,13 @@ namespace fc {
 // Keys of a workgroup in the sort: 256 times the rounds, few where there are few keys.
 inline int emb_rounds(int64_t n) { return n <= 65536 ? 4 : 8; }
 
+// The first column of a chunk of V: the last chunk of a row overlaps the one before it, so that chunks are whole wherever a
+// row has V columns (the columns in both get the same value from both).
+template <int V>
+__device__ __forceinline__ int64_t chunk_start(int64_t c, int64_t width) {
+  return width >= V && c > width - V ? width - V : c;
+}
+
 // ---- forward: one 16-byte chunk of a row per thread ----
 template <class T, class I>
 __global__ void __launch_bounds__(256) embedding_fwd_kernel(I total, I chunks, int64_t rows, int64_t width,
@@ -24,7 +31,7 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(I total, I chunks, i
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= (int64_t)total) return;
   const I row = (I)t / chunks, chunk = (I)t - row * chunks;
-  const int64_t c0 = (int64_t)chunk * V;
+  const int64_t c0 = chunk_start<V>((int64_t)chunk * V, width);
   const int64_t id = ids[row];
   const bool ok = id >= 0 && id < rows;
   const T* src = table + (ok ? id : 0) * width + c0;
@@ -337,8 +344,9 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
   constexpr int V = 16 / sizeof(T), U = 4;
   const int groups = 256 / a.col_threads;
   const int64_t p = (int64_t)blockIdx.x * groups + threadIdx.x / a.col_threads;
-  const int64_t c0 = ((int64_t)blockIdx.y * a.col_threads + threadIdx.x % a.col_threads) * V;
-  if (p >= a.pieces || c0 >= a.width) return;
+  const int64_t first = ((int64_t)blockIdx.y * a.col_threads + threadIdx.x % a.col_threads) * V;
+  if (p >= a.pieces || first >= a.width) return;
+  const int64_t c0 = chunk_start<V>(first, a.width);
   const int valid = (int)min((int64_t)V, a.width - c0);
   const int64_t t0 = p * a.len, t1 = min(a.n, t0 + a.len);
   const T* grad = (const T*)a.grad + c0;
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
     if (run < (uint32_t)a.rows) {
       if (from_left || to_right) {
         store_f32<float, V>((from_left ? a.head : a.tail) + p * a.width + c0, valid, acc);
-        if (!from_left && c0 == 0) a.joins[atomicAdd(a.counter, 1)] = (int32_t)p;
+        if (!from_left && first == 0) a.joins[atomicAdd(a.counter, 1)] = (int32_t)p;
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] *= a.scale;
@@ -361,26 +369,49 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
   };
-  for (int64_t t = t0; t < t1; t += U) {
-    uint32_t key[U];
-    float g[U][V];
+  // the rows of the next U tokens are loaded before this U's are added, their numbers one step earlier still
+  uint32_t key[2][U], next_key[U];
+  int32_t next_row[U];
+  float g[2][U][V];
+  auto load_tokens = [&](int64_t t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t at = min(t + u, t1 - 1);
-      key[u] = a.keys[at];
-      load_f32<T, V>(grad + (int64_t)a.order[at] * a.width, valid, g[u]);
+      next_key[u] = a.keys[at];
+      next_row[u] = a.order[at];
     }
+  };
+  auto load_rows = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      key[buf][u] = next_key[u];
+      load_f32<T, V>(grad + (int64_t)next_row[u] * a.width, valid, g[buf][u]);
+    }
+  };
+  auto add = [&](int64_t t, int buf) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (t + u >= t1) break;
-      if (key[u] != run) {
+      if (key[buf][u] != run) {
         flush(false);
-        run = key[u];
+        run = key[buf][u];
         from_left = false;
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += g[u][i];
+      for (int i = 0; i < V; ++i) acc[i] += g[buf][u][i];
     }
+  };
+  load_tokens(t0);
+  load_rows(0);
+  load_tokens(t0 + U);
+  for (int64_t t = t0; t < t1; t += 2 * U) {
+    load_rows(1);
+    load_tokens(t + 2 * U);
+    add(t, 0);
+    if (t + U >= t1) break;
+    load_rows(0);
+    load_tokens(t + 3 * U);
+    add(t + U, 1);
   }
   flush(t1 < a.n && a.keys[t1] == run);
 }
@@ -392,8 +423,8 @@ __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float part[256 * V];
   const int groups = 256 / a.col_threads, grp = threadIdx.x / a.col_threads, ct = threadIdx.x % a.col_threads;
-  const int64_t c0 = ((int64_t)blockIdx.y * a.col_threads + ct) * V;
-  const int valid = (int)max((int64_t)0, min((int64_t)V, a.width - c0));
+  const int64_t first_col = ((int64_t)blockIdx.y * a.col_threads + ct) * V, c0 = chunk_start<V>(first_col, a.width);
+  const int valid = first_col < a.width ? (int)min((int64_t)V, a.width - c0) : 0;
   const int count = *a.counter;
   for (int j = blockIdx.x; j < count; j += gridDim.x) {
     const int64_t p = a.joins[j];
@@ -600,7 +631,7 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
     j.col_threads = b.col_threads < 16 ? b.col_threads : 16;
     const int64_t cols = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), wide = (cols + j.col_threads - 1) / j.col_threads;
     if (wide > 65535) return FC_ERR_SHAPE;
-    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 512 ? p.pieces : 512), (unsigned)wide), dim3(256),
+    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 2048 ? p.pieces : 2048), (unsigned)wide), dim3(256),
                        0, s, j);
     FC_LAUNCH_CHECK();
     return FC_OK;

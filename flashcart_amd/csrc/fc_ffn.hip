@@ -169,14 +169,15 @@ static void set_tiles(FfnJob& g, int kind, bool gate) {
 
 // What a workgroup of each tile size takes, in us: a step of 64 k when it has its CU's loads to itself, the CU's time a
 // step takes when the device is full, and filling the pipeline and writing the tile. Measured in bf16: chains of steps on
-// few CUs (n = 30,000, width = hidden = 64), full devices at 1,024 to 16,384 rows. The 64 x 64 tile is bound by what the L2
+// few CUs (n = 30,000, width = hidden = 64), full devices at 1,024 to 30,000 rows. (Of 14 sizes tried with each tile
+// throughout, the choice was within 3% of the best in 13; 128 x 128 tiles alone cost up to 20%, 64 x 64 up to 2 times.) The 64 x 64 tile is bound by what the L2
 // caches deliver, the 256 x 256 tile by the matrix cores.
 struct TileCost {
   double step, full, end, fused;  // fused: the end with an epilogue of the block's elementwise steps
 };
-constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8, 2.0}, {0.65, 0.55, 2.5, 6.25}, {1.25, 1.5, 9.0, 22.5}};
+constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8, 1.2}, {0.65, 0.55, 2.5, 3.2}, {1.25, 1.5, 9.0, 14.0}};
 // native float32, 32 k a step: bound by the matrix cores
-constexpr TileCost kNativeCost[2] = {{0.5, 0.56, 1.0, 2.6}, {2.05, 1.85, 5.0, 6.5}};
+constexpr TileCost kNativeCost[2] = {{0.5, 0.56, 1.0, 2.2}, {2.05, 1.85, 5.0, 6.0}};
 
 enum Form { FORM_16, FORM_NATIVE, FORM_PLANES };
 

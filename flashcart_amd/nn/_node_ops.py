@@ -72,7 +72,10 @@ def _gated_feed_forward_bwd(grad, x, w_in, w_out, saved, act, act_scale, scale_i
 _FAKES = {"embedding": _embedding, "embedding_bwd": _embedding_bwd, "dropout_add": _dropout_add,
           "gated_feed_forward": _gated_feed_forward, "gated_feed_forward_bwd": _gated_feed_forward_bwd}
 
-# With the import, so that a compiled function never meets the loading; a package that is not built yet says so at the
-# first call.
+# With the import, so that a compiled function never meets the loading. Where it fails (not built, built for another torch)
+# the first call says why; the rest of the package does not need it.
 if os.path.exists(TORCH_LIB_PATH) and os.path.exists(_lib.LIB_PATH):
-    _load()
+    try:
+        _load()
+    except (OSError, AttributeError, _lib.HipLibraryError):
+        pass
