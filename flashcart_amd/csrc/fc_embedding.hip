@@ -5,8 +5,13 @@
 // the gradient rows of its runs of equal indices in float32, in token order. Runs inside one piece are written at once;
 // runs that cross pieces leave one partial sum per piece, which a second kernel joins in piece order. Rows without
 // tokens are zero: the table is filled while the sort counts, since most rows of a large table have no token.
-// With the lookup: 16,384 tokens of 32,000 rows of 1,024 in bf16 73 us, 1,083,777 of 4 rows of 16 in float32 89 us.
+// Small tables need no sort: each wave keeps the sums of all rows in LDS, and a second kernel adds the waves' tables.
+// With the lookup: 16,384 tokens of 32,000 rows of 1,024 in bf16 69 us, 1,083,777 of 4 rows of 16 in float32 36 us.
 // Indices outside the table (a device-side check cannot raise) give rows of NaN and take no part in the gradient.
+#include <math.h>
+
+#include <algorithm>
+
 #include "fc_node.h"
 
 namespace fc {
@@ -313,16 +318,16 @@ struct EmbSum {
   int32_t* counter;
 };
 
-template <class T, int V>
-__device__ __forceinline__ void load_f32(const T* p, int valid, float (&x)[V]) {
-  if (valid >= V) {
-    const Pack<T, V> v = load_pack<T, V>(p);
+// A chunk of V elements, of which `valid` are there and more are asked for only where rows are narrower than V (WIDE false).
+// Without a branch, so that loads of several rows are under way together: a branch around a load ends in a wait for it
+// (32,126 rows of 2,082 in f16: pieces 53 us with one, 33 without).
+template <class T, int V, bool WIDE>
+__device__ __forceinline__ Pack<T, V> load_chunk(const T* p, int valid) {
+  if constexpr (WIDE) return load_pack<T, V>(p);
+  Pack<T, V> v;
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f32(v.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = i < valid ? to_f32(p[i]) : 0.f;
-  }
+  for (int i = 0; i < V; ++i) v.v[i] = p[min(i, valid - 1)];
+  return v;
 }
 template <class T, int V>
 __device__ __forceinline__ void store_f32(T* p, int valid, const float (&x)[V]) {
@@ -339,7 +344,7 @@ __device__ __forceinline__ void store_f32(T* p, int valid, const float (&x)[V]) 
 }
 
 // A group of col_threads lanes sums one piece over V columns each; U gradient rows are loaded ahead.
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
   constexpr int V = 16 / sizeof(T), U = 4;
   const int groups = 256 / a.col_threads;
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
   // the rows of the next U tokens are loaded before this U's are added, their numbers one step earlier still
   uint32_t key[2][U], next_key[U];
   int32_t next_row[U];
-  float g[2][U][V];
+  Pack<T, V> g[2][U];
   auto load_tokens = [&](int64_t t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       key[buf][u] = next_key[u];
-      load_f32<T, V>(grad + (int64_t)next_row[u] * a.width, valid, g[buf][u]);
+      g[buf][u] = load_chunk<T, V, WIDE>(grad + (int64_t)next_row[u] * a.width, valid);
     }
   };
   auto add = [&](int64_t t, int buf) {
@@ -398,7 +403,7 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
         from_left = false;
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += g[buf][u][i];
+      for (int i = 0; i < V; ++i) acc[i] += to_f32(g[buf][u].v[i]);
     }
   };
   load_tokens(t0);
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
 
 // A run of several pieces: tail of the first, heads of the others. Groups of lanes add consecutive spans of pieces, the
 // groups' sums are added in order.
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float part[256 * V];
@@ -444,12 +449,11 @@ __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     if (valid > 0)
-#pragma unroll 8
+#pragma unroll 2
       for (int64_t q = p + grp * span; q < min(p + (grp + 1) * span, last + 1); ++q) {
-        float x[V];
-        load_f32<float, V>((q == p ? a.tail : a.head) + q * a.width + c0, valid, x);
+        const Pack<float, V> x = load_chunk<float, V, WIDE>((q == p ? a.tail : a.head) + q * a.width + c0, valid);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += x[i];
+        for (int i = 0; i < V; ++i) acc[i] += x.v[i];
       }
 #pragma unroll
     for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = acc[i];
@@ -466,15 +470,154 @@ __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
   }
 }
 
+// ---- few rows: no sort ----
+struct EmbFew {
+  int64_t n, rows, width, padding, per;  // per: tokens of a workgroup
+  int32_t col_threads;                   // a power of two, <= 64
+  const int64_t* ids;
+  const void* grad;
+  void* out;
+  float scale;
+  float* part;  // (rows, chunks, workgroups, V)
+};
+
+// Each group of col_threads lanes of a wave keeps the sums of all rows over V columns a lane in LDS, and one row more for
+// tokens that add to none. A lane's 16-byte words lie at its own banks, whatever the row. Gradient rows are read once, in
+// order, not gathered; two batches of U tokens are under way. (LDS float adds instead of read, add and write: 126 us for
+// 16 at 1,083,777 of 4 rows of 16 in float32.)
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(64) emb_few_kernel(EmbFew a) {
+  constexpr int V = 16 / sizeof(T), Q = V / 4, U = 4;
+  extern __shared__ float4 sums[];  // (rows + 1, Q, 64)
+  const int lane = threadIdx.x, groups = 64 / a.col_threads, grp = lane / a.col_threads, ct = lane % a.col_threads;
+  const int rows = (int)a.rows;
+  const int64_t cols = (a.width + V - 1) / V, chunk = (int64_t)blockIdx.x * a.col_threads + ct;
+  const int64_t c0 = chunk_start<V>(min(chunk, cols - 1) * V, a.width);
+  const int valid = (int)min((int64_t)V, a.width - c0);
+  for (int k = 0; k < (rows + 1) * Q; ++k) sums[k * 64 + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int64_t t0 = blockIdx.y * a.per, t1 = min(a.n, t0 + a.per), batch = (int64_t)U * groups;
+  uint64_t id[2][U];
+  Pack<T, V> g[2][U];
+  auto load = [&](const int64_t* ids, const T* grad, int buf) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      id[buf][u] = (uint64_t)ids[u * groups];
+      g[buf][u] = load_chunk<T, V, WIDE>(grad + (int64_t)(u * groups) * a.width, valid);
+    }
+  };
+  auto add_row = [&](uint64_t x, const Pack<T, V>& v) {
+    const int row = x < (uint64_t)rows && x != (uint64_t)a.padding ? (int)x : rows;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      float4& to = sums[(row * Q + q) * 64 + lane];
+      float4 y = to;
+      y.x += to_f32(v.v[4 * q]);
+      y.y += to_f32(v.v[4 * q + 1]);
+      y.z += to_f32(v.v[4 * q + 2]);
+      y.w += to_f32(v.v[4 * q + 3]);
+      to = y;
+    }
+  };
+  auto add = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_row(id[buf][u], g[buf][u]);
+  };
+  const int64_t pairs = (t1 - t0) / (2 * batch);
+  const int64_t* ids = a.ids + t0 + grp;
+  const T* grad = (const T*)a.grad + (t0 + grp) * a.width + c0;
+  if (pairs > 0) load(ids, grad, 0);
+  for (int64_t k = 1; k <= pairs; ++k) {
+    load(ids + batch, grad + batch * a.width, 1);
+    add(0);
+    const int64_t on = k < pairs ? 2 * batch : 0;  // (the last pair's first batch is loaded again, and not used)
+    ids += on;
+    grad += on * a.width;
+    load(ids, grad, 0);
+    add(1);
+  }
+  for (int64_t t = t0 + pairs * 2 * batch; t < t1; t += groups) {  // a token behind the last adds to no row
+    const int64_t from = min(t + grp, t1 - 1);
+    const Pack<T, V> v = load_chunk<T, V, WIDE>((const T*)a.grad + from * a.width + c0, valid);
+    add_row(t + grp < t1 ? (uint64_t)a.ids[from] : ~0ull, v);
+  }
+  __syncthreads();
+  if (chunk >= cols) return;
+  for (int r = grp; r < rows; r += groups)
+    for (int q = 0; q < Q; ++q) {
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < groups; ++k) {
+        const float4 x = sums[(r * Q + q) * 64 + k * a.col_threads + ct];
+        y.x += x.x;
+        y.y += x.y;
+        y.z += x.z;
+        y.w += x.w;
+      }
+      *(float4*)(a.part + ((r * cols + chunk) * gridDim.y + blockIdx.y) * V + 4 * q) = y;
+    }
+}
+
+// One wave per chunk of V columns of a row: its partial sums in consecutive spans, the lanes' sums in a fixed order.
+template <class T>
+__global__ void __launch_bounds__(64) emb_few_join_kernel(EmbFew a, int64_t parts) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t cols = (a.width + V - 1) / V, r = blockIdx.x / cols, chunk = blockIdx.x - r * cols;
+  const float* part = a.part + blockIdx.x * parts * V;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int64_t k = threadIdx.x; k < parts; k += 64) {
+    const Pack<float, V> x = load_pack<float, V>(part + k * V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] += x.v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) acc[i] += __shfl_xor(acc[i], o, 64);
+    acc[i] *= a.scale;
+  }
+  const int64_t c0 = chunk_start<V>(chunk * V, a.width);
+  if (threadIdx.x == 0) store_f32<T, V>((T*)a.out + r * a.width + c0, (int)min((int64_t)V, a.width - c0), acc);
+}
+
 struct EmbPlan {
   int64_t tiles, pieces, len;
   int col_threads, col_blocks, passes;
   int64_t keys[2], order[2], hist, total, head, tail, joins, counter, bytes;
+  // few rows
+  bool few;
+  int few_threads, few_lds;
+  int64_t few_parts, few_per;
 };
+
+// Tables of up to 32 KB whose sums fit a wave's 64 KB of LDS. Backward kernels, us, against sorting: 1,083,777 of 4 rows of
+// 16 in float32 19 / 64, 25,000 of 63 of 128 19 / 24, 2,000 of 31 of 512 in bf16 19 / 17; of larger tables the partial sums
+// weigh more: 16,384 of 31 of 1,024 in bf16 32 / 30, 65,536 of 16 of 1,024 in float32 118 / 105, of 63 of 4,096 312 / 278.
+static void emb_plan_few(EmbPlan& p, int64_t n, int64_t rows, int64_t width, int64_t V) {
+  const int64_t cols = (width + V - 1) / V;
+  if (n == 0 || rows > 64 || (rows + 1) * V * 256 > (64 << 10) || rows * width * (16 / V) > (32 << 10)) return;
+  int ct = 1;
+  while (ct < 64 && ct < cols) ct *= 2;
+  const int64_t groups = 64 / ct, blocks = (cols + ct - 1) / ct, lds = (rows + 1) * V * 256;
+  const int64_t waves = 256 * std::min<int64_t>(8, (160 << 10) / lds);
+  // steps of a workgroup: a step's chain through LDS against the partial sums' bytes, and the waves that run at once
+  const double bytes = 8.0 * (double)n * rows * width / groups / 4.5e6;
+  int64_t steps = std::max<int64_t>({8, (int64_t)sqrt(bytes / 0.12), n * blocks / (groups * waves)});
+  steps = std::max((steps + 7) / 8 * 8, (n / groups + 65534) / 65535);
+  p.few = true;
+  p.few_threads = ct;
+  p.few_lds = (int)lds;
+  p.few_per = steps * groups;
+  p.few_parts = (n + p.few_per - 1) / p.few_per;
+  p.bytes = 4 * p.few_parts * rows * cols * V;
+}
 
 static EmbPlan emb_plan(int32_t dtype, int64_t n, int64_t rows, int64_t width) {
   EmbPlan p{};
   const int64_t V = 16 / node_dtype_size(dtype), cols = (width + V - 1) / V;
+  emb_plan_few(p, n, rows, width, V);
+  if (p.few) return p;
   const int64_t tile = 256 * emb_rounds(n);
   p.tiles = (n + tile - 1) / tile;
   int ct = 1;
@@ -556,6 +699,31 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   if (ws_bytes < p.bytes || !ws) return FC_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   char* w = (char*)ws;
+  if (p.few) {
+    EmbFew f{};
+    f.n = n;
+    f.rows = rows;
+    f.width = width;
+    f.padding = padding;
+    f.per = p.few_per;
+    f.col_threads = p.few_threads;
+    f.ids = ids;
+    f.grad = grad_out;
+    f.out = grad_table;
+    f.scale = scale;
+    f.part = (float*)w;
+    return with_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      const int64_t cols = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+      const dim3 grid((unsigned)((cols + p.few_threads - 1) / p.few_threads), (unsigned)p.few_parts);
+      if (width >= (int64_t)(16 / sizeof(T))) hipLaunchKernelGGL((emb_few_kernel<T, true>), grid, dim3(64), p.few_lds, s, f);
+      else hipLaunchKernelGGL((emb_few_kernel<T, false>), grid, dim3(64), p.few_lds, s, f);
+      FC_LAUNCH_CHECK();
+      hipLaunchKernelGGL((emb_few_join_kernel<T>), dim3((unsigned)(rows * cols)), dim3(64), 0, s, f, p.few_parts);
+      FC_LAUNCH_CHECK();
+      return FC_OK;
+    });
+  }
   EmbSort a{};
   a.n = n;
   a.rows = rows;
@@ -623,16 +791,19 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     const int groups = 256 / p.col_threads;
-    hipLaunchKernelGGL((emb_piece_kernel<T>), dim3((unsigned)((p.pieces + groups - 1) / groups), p.col_blocks),
-                       dim3(256), 0, s, b);
+    const bool whole = width >= (int64_t)(16 / sizeof(T));
+    const dim3 grid((unsigned)((p.pieces + groups - 1) / groups), p.col_blocks);
+    if (whole) hipLaunchKernelGGL((emb_piece_kernel<T, true>), grid, dim3(256), 0, s, b);
+    else hipLaunchKernelGGL((emb_piece_kernel<T, false>), grid, dim3(256), 0, s, b);
     FC_LAUNCH_CHECK();
     // narrow groups: more of them share the pieces of a run
     EmbSum j = b;
     j.col_threads = b.col_threads < 16 ? b.col_threads : 16;
     const int64_t cols = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), wide = (cols + j.col_threads - 1) / j.col_threads;
     if (wide > 65535) return FC_ERR_SHAPE;
-    hipLaunchKernelGGL((emb_join_kernel<T>), dim3((unsigned)(p.pieces < 2048 ? p.pieces : 2048), (unsigned)wide), dim3(256),
-                       0, s, j);
+    const dim3 joins((unsigned)(p.pieces < 2048 ? p.pieces : 2048), (unsigned)wide);
+    if (whole) hipLaunchKernelGGL((emb_join_kernel<T, true>), joins, dim3(256), 0, s, j);
+    else hipLaunchKernelGGL((emb_join_kernel<T, false>), joins, dim3(256), 0, s, j);
     FC_LAUNCH_CHECK();
     return FC_OK;
   });
