@@ -6,7 +6,7 @@
 // runs that cross pieces leave one partial sum per piece, which a second kernel joins in piece order. Rows without
 // tokens are zero: the table is filled while the sort counts, since most rows of a large table have no token.
 // Small tables need no sort: each wave keeps the sums of all rows in LDS, and a second kernel adds the waves' tables.
-// With the lookup: 16,384 tokens of 32,000 rows of 1,024 in bf16 69 us, 1,083,777 of 4 rows of 16 in float32 36 us.
+// With the lookup: 16,384 tokens of 32,000 rows of 1,024 in bf16 66-70 us, 1,083,777 of 4 rows of 16 in float32 36 us.
 // Indices outside the table (a device-side check cannot raise) give rows of NaN and take no part in the gradient.
 #include <math.h>
 
@@ -421,50 +421,86 @@ __global__ void __launch_bounds__(256) emb_piece_kernel(EmbSum a) {
   flush(t1 < a.n && a.keys[t1] == run);
 }
 
-// A run of several pieces: tail of the first, heads of the others. Groups of lanes add consecutive spans of pieces, the
-// groups' sums are added in order.
+// A run of several pieces: tail of the first, heads of the others. Runs of up to four pieces are added by one group of lanes
+// each, as many at once as there are for a workgroup; longer ones by the whole workgroup: its groups add consecutive spans
+// of pieces, the groups' sums are added in order. (351,854 tokens of 120,666 rows of 29 in f16, runs of three tokens: 10 us,
+// by whole workgroups only 59.)
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) emb_join_kernel(EmbSum a) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), SHORT = 4;
   __shared__ float part[256 * V];
+  __shared__ int32_t longer[256];  // first piece of a group's run, or -1
+  __shared__ uint32_t run[256];
   const int groups = 256 / a.col_threads, grp = threadIdx.x / a.col_threads, ct = threadIdx.x % a.col_threads;
   const int64_t first_col = ((int64_t)blockIdx.y * a.col_threads + ct) * V, c0 = chunk_start<V>(first_col, a.width);
   const int valid = first_col < a.width ? (int)min((int64_t)V, a.width - c0) : 0;
-  const int count = *a.counter;
-  for (int j = blockIdx.x; j < count; j += gridDim.x) {
-    const int64_t p = a.joins[j];
-    const int64_t first = (p + 1) * a.len;  // of the second piece: the run goes on here
-    const uint32_t key = a.keys[first];
-    // The run's pieces are those that begin with its key: the last one lies in [last, hi]; 256 candidates a round, the
-    // next ones first, then spread over the rest.
-    int64_t last = p, hi = a.pieces - 1;
-    for (int64_t stride = 1; last < hi; stride = (hi - last + 255) / 256) {
-      const int64_t q = last + (threadIdx.x + 1) * stride;
-      const int c = __syncthreads_count(q <= hi && a.keys[q * a.len] == key);
-      last += c * stride;
-      if (c < 256) hi = min(hi, last + stride - 1);
-    }
-    const int64_t m = last - p + 1, span = (m + groups - 1) / groups;
-    float acc[V];
+  const int count = *a.counter, batch = min(groups, (count + (int)gridDim.x - 1) / (int)gridDim.x);
+  auto store = [&](uint32_t key, float (&acc)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    if (valid > 0)
-#pragma unroll 2
-      for (int64_t q = p + grp * span; q < min(p + (grp + 1) * span, last + 1); ++q) {
-        const Pack<float, V> x = load_chunk<float, V, WIDE>((q == p ? a.tail : a.head) + q * a.width + c0, valid);
+    for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+    store_f32<T, V>((T*)a.out + (int64_t)key * a.width + c0, valid, acc);
+  };
+  for (int64_t j0 = (int64_t)blockIdx.x * batch; j0 < count; j0 += (int64_t)gridDim.x * batch) {
+    const int here = (int)min((int64_t)batch, count - j0);
+    if (grp < here) {
+      const int64_t p = a.joins[j0 + grp];
+      const uint32_t key = a.keys[(p + 1) * a.len];
+      int m = 2;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += x.v[i];
+      for (int k = 2; k <= SHORT; ++k)
+        m += p + k < a.pieces && a.keys[min(p + k, (int64_t)a.pieces - 1) * a.len] == key;
+      if (ct == 0) {
+        longer[grp] = m > SHORT ? (int32_t)p : -1;
+        run[grp] = key;
       }
+      if (m <= SHORT && valid > 0) {
+        float acc[V];
+        const Pack<float, V> x = load_chunk<float, V, WIDE>(a.tail + p * a.width + c0, valid);
 #pragma unroll
-    for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = acc[i];
+        for (int i = 0; i < V; ++i) acc[i] = x.v[i];
+        for (int k = 1; k < m; ++k) {
+          const Pack<float, V> y = load_chunk<float, V, WIDE>(a.head + (p + k) * a.width + c0, valid);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] += y.v[i];
+        }
+        store(key, acc);
+      }
+    }
     __syncthreads();
-    if (grp == 0 && valid > 0) {
-      for (int k = 1; k < groups; ++k)
+    for (int e = 0; e < here; ++e) {
+      const int64_t p = longer[e];
+      if (p < 0) continue;
+      const uint32_t key = run[e];
+      // The run's pieces are those that begin with its key: the last one lies in [last, hi]; 256 candidates a round, the
+      // next ones first, then spread over the rest.
+      int64_t last = p + SHORT, hi = a.pieces - 1;
+      for (int64_t stride = 1; last < hi; stride = (hi - last + 255) / 256) {
+        const int64_t q = last + (threadIdx.x + 1) * stride;
+        const int c = __syncthreads_count(q <= hi && a.keys[q * a.len] == key);
+        last += c * stride;
+        if (c < 256) hi = min(hi, last + stride - 1);
+      }
+      const int64_t m = last - p + 1, span = (m + groups - 1) / groups;
+      float acc[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += part[(k * a.col_threads + ct) * V + i];
+      for (int i = 0; i < V; ++i) acc[i] = 0.f;
+      if (valid > 0)
+#pragma unroll 2
+        for (int64_t q = p + grp * span; q < min(p + (grp + 1) * span, last + 1); ++q) {
+          const Pack<float, V> x = load_chunk<float, V, WIDE>((q == p ? a.tail : a.head) + q * a.width + c0, valid);
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] *= a.scale;
-      store_f32<T, V>((T*)a.out + (int64_t)key * a.width + c0, valid, acc);
+          for (int i = 0; i < V; ++i) acc[i] += x.v[i];
+        }
+#pragma unroll
+      for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = acc[i];
+      __syncthreads();
+      if (grp == 0 && valid > 0) {
+        for (int k = 1; k < groups; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] += part[(k * a.col_threads + ct) * V + i];
+        store(key, acc);
+      }
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -801,7 +837,7 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
     j.col_threads = b.col_threads < 16 ? b.col_threads : 16;
     const int64_t cols = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), wide = (cols + j.col_threads - 1) / j.col_threads;
     if (wide > 65535) return FC_ERR_SHAPE;
-    const dim3 joins((unsigned)(p.pieces < 2048 ? p.pieces : 2048), (unsigned)wide);
+    const dim3 joins((unsigned)(p.pieces < 4096 ? p.pieces : 4096), (unsigned)wide);
     if (whole) hipLaunchKernelGGL((emb_join_kernel<T, true>), joins, dim3(256), 0, s, j);
     else hipLaunchKernelGGL((emb_join_kernel<T, false>), joins, dim3(256), 0, s, j);
     FC_LAUNCH_CHECK();
