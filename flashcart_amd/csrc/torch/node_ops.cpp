@@ -67,11 +67,12 @@ Tensor bytes(const Tensor& like, int64_t size, const char* what) {
   return at::empty({size}, like.options().dtype(at::kByte));
 }
 
-// Whether autograd records a call with these inputs.
+// Whether a call with these inputs goes through its autograd formula: where autograd records it, and where an input carries
+// a forward-mode tangent (in either grad mode), which the formula refuses; below it the tangent would be lost.
 bool records(std::initializer_list<const Tensor*> inputs) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grad = at::GradMode::is_enabled();
   for (const Tensor* t : inputs)
-    if (t->defined() && t->requires_grad()) return true;
+    if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
 

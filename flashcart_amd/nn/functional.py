@@ -3,7 +3,8 @@ feed-forward block, residual dropout.
 
 They have no counterpart among the reference's kernels (it composes torch operations). Each is a registered operator
 (``torch.ops.flashcart.*``) with an autograd formula, runs on the current stream and allocates through torch, so it can
-be captured into a graph. There is no CPU path. Values are formed in float32 and rounded once to the tensors' type.
+be captured into a graph. There is no CPU path, and there are no forward-mode derivatives (an argument with a tangent is
+refused). Values are formed in float32 and rounded once to the tensors' type.
 """
 
 from typing import Optional

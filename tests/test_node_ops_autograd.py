@@ -1,0 +1,45 @@
+"""What the autograd formulas of the node-wise operators do around their kernels, seen on tensors without memory."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from flashcart_amd.nn import functional as F
+
+OPERATORS = ["embedding", "embedding_bwd", "dropout_add", "residual", "gated_feed_forward", "w_out"]
+
+
+def _call(name):
+    """The operator as a function of one differentiable argument, and that argument."""
+    ids, rng = torch.zeros(3, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)
+    x, w_in, w_out = torch.empty(5, 4), torch.empty(12, 4), torch.empty(4, 6)
+    return {
+        "embedding": (lambda t: F.embedding(ids, t, 2.0, 0), torch.empty(7, 4)),
+        "embedding_bwd": (lambda t: torch.ops.flashcart.embedding_bwd(t, ids, 7, 2.0, -1), torch.empty(3, 4)),
+        "dropout_add": (lambda t: F.dropout_add(t, None, 0.5, rng), x),
+        "residual": (lambda t: F.dropout_add(x, t, 0.5, rng), torch.empty(5, 4)),
+        "gated_feed_forward": (lambda t: F.gated_feed_forward(t, w_in, w_out), x),
+        "w_out": (lambda t: F.gated_feed_forward(x, w_in, t), w_out),
+    }[name]
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("enabled", [False, True])
+@pytest.mark.parametrize("name", OPERATORS)
+def test_forward_mode_is_refused(name, enabled, recorded):
+    """A tangent is never dropped: forward-mode derivatives, which the operators lack, raise."""
+    with FakeTensorMode(), forward_ad.dual_level(), torch.set_grad_enabled(enabled):
+        call, t = _call(name)
+        dual = forward_ad.make_dual(t.requires_grad_(recorded), torch.empty_like(t))
+        with pytest.raises(RuntimeError, match="jvp is not implemented"):
+            call(dual)
+        assert call(t).requires_grad == (enabled and recorded)  # (the level alone refuses nothing)
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_functional_forward_mode_is_refused(name):
+    with FakeTensorMode():
+        call, t = _call(name)
+        with pytest.raises(RuntimeError, match="functorch transforms"):
+            torch.func.jvp(call, (t,), (torch.empty_like(t),))
