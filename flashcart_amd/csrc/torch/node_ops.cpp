@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include "../../../include/flashcart_hip.h"
@@ -214,6 +215,21 @@ Tensor dropout_add_autograd(const Tensor& x, const optional<Tensor>& residual, d
   FCT_DISPATCHED(dropout_add, x, residual, p, rng);
 }
 
+// Seed and offset of one call; `state` goes on to the next offset. A call that the backward pass runs again would get other
+// numbers than the first time. (Asked here, when it runs, so that it holds in compiled functions too.)
+Tensor dropout_draw(Tensor& state) {
+  TORCH_CHECK(torch::autograd::get_current_graph_task_id() == -1,
+              "random numbers of a dropout call were asked for during a backward pass, as activation checkpointing does when "
+              "it runs a call again: those of the first run cannot be drawn again. Take rng = layer.draw() outside the "
+              "checkpointed function and pass it in.");
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && state.sizes() == at::IntArrayRef({2}),
+                    "dropout_draw: the state must be an int64 seed and offset, got ", state.scalar_type(), " ",
+                    state.sizes(), ".");
+  Tensor rng = state.clone();  // (kept for the backward pass)
+  state.select(0, 1).add_(1);
+  return rng;
+}
+
 // ---- gated feed-forward block ----
 
 fc_ffn_desc ffn_desc(const char* what, const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act,
@@ -394,6 +410,7 @@ TORCH_LIBRARY_FRAGMENT(flashcart, m) {
   m.def("embedding(Tensor ids, Tensor table, float scale, int padding) -> Tensor");
   m.def("embedding_bwd(Tensor grad, Tensor ids, int rows, float scale, int padding) -> Tensor");
   m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor rng) -> Tensor");
+  m.def("dropout_draw(Tensor(a!) state) -> Tensor");
   m.def("gated_feed_forward(Tensor x, Tensor w_in, Tensor w_out, int act, float act_scale, float scale_in, "
         "float scale_out, bool save) -> (Tensor, Tensor)");
   m.def("gated_feed_forward_bwd(Tensor grad, Tensor x, Tensor w_in, Tensor w_out, Tensor saved, int act, "
@@ -401,11 +418,12 @@ TORCH_LIBRARY_FRAGMENT(flashcart, m) {
         "(Tensor, Tensor, Tensor)");
 }
 
-// (on the CPU they end in their own error)
+// (on the CPU they end in their own error, dropout_draw aside)
 #define FCT_IMPLS(m)                                         \
   m.impl("embedding", TORCH_FN(embedding));                  \
   m.impl("embedding_bwd", TORCH_FN(embedding_bwd));          \
   m.impl("dropout_add", TORCH_FN(dropout_add));              \
+  m.impl("dropout_draw", TORCH_FN(dropout_draw));            \
   m.impl("gated_feed_forward", TORCH_FN(gated_feed_forward)); \
   m.impl("gated_feed_forward_bwd", TORCH_FN(gated_feed_forward_bwd));
 TORCH_LIBRARY_IMPL(flashcart, CUDA, m) { FCT_IMPLS(m) }

@@ -56,6 +56,10 @@ def _dropout_add(x, residual, p, rng):
     return _contiguous(x)
 
 
+def _dropout_draw(state):
+    return torch.empty_like(state)
+
+
 def _gated_feed_forward(x, w_in, w_out, act, act_scale, scale_in, scale_out, save):
     width, hidden = w_out.shape
     size = 0
@@ -70,7 +74,7 @@ def _gated_feed_forward_bwd(grad, x, w_in, w_out, saved, act, act_scale, scale_i
 
 
 _FAKES = {"embedding": _embedding, "embedding_bwd": _embedding_bwd, "dropout_add": _dropout_add,
-          "gated_feed_forward": _gated_feed_forward, "gated_feed_forward_bwd": _gated_feed_forward_bwd}
+          "dropout_draw": _dropout_draw, "gated_feed_forward": _gated_feed_forward, "gated_feed_forward_bwd": _gated_feed_forward_bwd}
 
 # With the import, so that a compiled function never meets the loading. Where it fails (not built, built for another torch)
 # the first call says why; the rest of the package does not need it.

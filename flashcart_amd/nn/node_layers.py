@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from flashcart_amd.nn import functional
+from flashcart_amd.nn import _node_ops, functional
 from flashcart_amd.nn.layers import SIGMOID_SCALE, SILU_SCALE
 
 _ACT_SCALE = {"silu": SILU_SCALE, "sigmoid": SIGMOID_SCALE, "gelu": 1.0}
@@ -49,7 +49,14 @@ class GatedFeedForwardLayer(nn.Module):
 class ResidualDropoutLayer(nn.Module):
     """``residual + dropout(x)`` in training, ``residual + x`` in evaluation. The generator's seed and offset are a buffer on
     the device that every training call advances there, so a captured graph draws new masks at each replay and a
-    checkpoint goes on where it stopped. Layers of one network need different seeds."""
+    checkpoint goes on where it stopped.
+
+    Layers of equal seed and offset draw the same mask: layers of one network need different seeds, and so do the processes
+    of data-parallel training (whose wrapper must not copy this buffer from one process to the others).
+
+    A call that is run again during the backward pass (activation checkpointing) has to draw the mask of the first run,
+    which the buffer no longer holds. Hand it to both: ``rng = layer.draw()`` before, ``layer(x, residual, rng)`` inside what
+    is run again. ``draw``, and so a training call without ``rng``, is refused during a backward pass."""
 
     def __init__(self, p: float, seed: int = 0):
         super().__init__()
@@ -58,16 +65,19 @@ class ResidualDropoutLayer(nn.Module):
         self.p = float(p)
         self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
+    def draw(self) -> torch.Tensor:
+        """Seed and offset of one call; the next one gets the next offset."""
+        return _node_ops.ops().dropout_draw.default(self.rng)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor, rng: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return residual + x
-        rng = self.rng.clone()  # (kept for the backward pass)
-        self.rng[1:].add_(1)
-        return functional.dropout_add(x, residual, self.p, rng)
+        return functional.dropout_add(x, residual, self.p, self.draw() if rng is None else rng)
 
 
 class NodeNetwork(nn.Module):
-    """Embedding, then ``depth`` blocks x + dropout(feed_forward(x))."""
+    """Embedding, then ``depth`` blocks x + dropout(feed_forward(x)). The dropouts' seeds are ``seed`` .. ``seed + depth - 1``:
+    networks that are not to share masks need seeds that far apart."""
 
     def __init__(self, n_rows: int, width: int, hidden: int, depth: int = 2, p: float = 0.0, activation: str = "silu",
                  padding_idx: Optional[int] = None, seed: int = 0):
@@ -76,8 +86,12 @@ class NodeNetwork(nn.Module):
         self.blocks = nn.ModuleList(GatedFeedForwardLayer(width, hidden, activation) for _ in range(depth))
         self.dropouts = nn.ModuleList(ResidualDropoutLayer(p, seed + k) for k in range(depth))
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+    def draw(self) -> torch.Tensor:
+        """Seeds and offsets (depth, 2) of one call, for calls under activation checkpointing (``ResidualDropoutLayer``)."""
+        return torch.stack([dropout.draw() for dropout in self.dropouts])
+
+    def forward(self, ids: torch.Tensor, rng: Optional[torch.Tensor] = None) -> torch.Tensor:
         x = self.embedding(ids)
-        for block, dropout in zip(self.blocks, self.dropouts):
-            x = dropout(block(x), x)
+        for k, (block, dropout) in enumerate(zip(self.blocks, self.dropouts)):
+            x = dropout(block(x), x, None if rng is None else rng[k])
         return x
