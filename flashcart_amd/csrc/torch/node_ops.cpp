@@ -352,6 +352,7 @@ struct FeedForwardNode : torch::autograd::Function<FeedForwardNode> {
     ctx->saved_data["scales"] = std::vector<double>{act_scale, scale_in, scale_out};
     ctx->saved_data["save"] = save;
     ctx->mark_non_differentiable({saved});
+    ctx->set_materialize_grads(false);  // (no zeros the size of `saved` as its gradient)
     return {y, saved};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {

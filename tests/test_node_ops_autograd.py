@@ -4,6 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from flashcart_amd.nn import functional as F
 
@@ -43,3 +44,55 @@ def test_functional_forward_mode_is_refused(name):
         call, t = _call(name)
         with pytest.raises(RuntimeError, match="functorch transforms"):
             torch.func.jvp(call, (t,), (torch.empty_like(t),))
+
+
+class _Calls(TorchDispatchMode):
+    """The operators that run, without queries of properties."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace != "prim":
+            self.names.append(func.name())
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_backward_passes_run_their_operator_alone(name):
+    """No zeros for outputs without a gradient (the block's kept values are the largest tensor of a training step)."""
+    with FakeTensorMode():
+        call, t = _call(name)
+        out = call(t.requires_grad_())
+        grad = torch.empty_like(out)
+        with _Calls() as calls:
+            torch.autograd.grad(out, t, grad)
+    if name == "residual":
+        assert calls.names == []
+    elif name == "embedding_bwd":  # its cotangent is looked up, but for ids that add to no row
+        assert "flashcart::embedding" in calls.names and not any("zeros" in n for n in calls.names)
+    else:
+        assert calls.names == [{"embedding": "flashcart::embedding_bwd", "dropout_add": "flashcart::dropout_add"}.get(
+            name, "flashcart::gated_feed_forward_bwd")]
+
+
+def test_block_without_a_gradient_of_its_output():
+    """A pass that reaches the block with no gradient of y gives none to its arguments."""
+    with FakeTensorMode():
+        call, t = _call("gated_feed_forward")
+
+        class Stop(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x):
+                return x.clone()
+
+            @staticmethod
+            def backward(ctx, grad):
+                return None
+
+        out = Stop.apply(call(t.requires_grad_()))
+        ones = torch.empty_like(out)
+        with _Calls() as calls:
+            (grad,) = torch.autograd.grad(out, t, ones, allow_unused=True)
+        assert grad is None and calls.names == []
