@@ -20,6 +20,7 @@ struct DropoutArgs {
   void* out;
   uint64_t threshold;
   float factor;
+  int64_t first;  // block of this launch
 };
 
 __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
@@ -39,7 +40,7 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k
 template <class T, bool RESIDUAL, bool ALL>
 __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs g) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t e0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+  const int64_t e0 = ((g.first + blockIdx.x) * 256 + threadIdx.x) * V;
   if (e0 >= g.n) return;
   const T* x = (const T*)g.x + e0;
   const T* res = (const T*)g.residual + (RESIDUAL ? e0 : 0);
@@ -89,19 +90,20 @@ extern "C" int fc_dropout_add(int32_t dtype, int64_t n, const void* x, const voi
   if (n < 0) return FC_ERR_SHAPE;
   if (n == 0) return FC_OK;
   if (!x || !rng || !out) return FC_ERR_NULL;
-  DropoutArgs g{n, x, residual, rng, out, (uint64_t)(p * 4294967296.0), (float)(1.0 / (1.0 - p))};
+  DropoutArgs g{n, x, residual, rng, out, (uint64_t)(p * 4294967296.0), (float)(1.0 / (1.0 - p)), 0};
+  if (n > INT64_MAX / 8) return FC_ERR_SHAPE;
   const int64_t blocks = (n * node_dtype_size(dtype) + 4095) / 4096;
-  if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks), block(256);
+  const dim3 block(256);
   hipStream_t s = (hipStream_t)stream;
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     const bool all = g.threshold == 0;
-    if (residual && all) hipLaunchKernelGGL((dropout_kernel<T, true, true>), grid, block, 0, s, g);
-    else if (residual) hipLaunchKernelGGL((dropout_kernel<T, true, false>), grid, block, 0, s, g);
-    else if (all) hipLaunchKernelGGL((dropout_kernel<T, false, true>), grid, block, 0, s, g);
-    else hipLaunchKernelGGL((dropout_kernel<T, false, false>), grid, block, 0, s, g);
-    FC_LAUNCH_CHECK();
-    return FC_OK;
+    return in_launches(blocks, [&](int64_t first, unsigned grid) {
+      g.first = first;
+      if (residual && all) hipLaunchKernelGGL((dropout_kernel<T, true, true>), dim3(grid), block, 0, s, g);
+      else if (residual) hipLaunchKernelGGL((dropout_kernel<T, true, false>), dim3(grid), block, 0, s, g);
+      else if (all) hipLaunchKernelGGL((dropout_kernel<T, false, true>), dim3(grid), block, 0, s, g);
+      else hipLaunchKernelGGL((dropout_kernel<T, false, false>), dim3(grid), block, 0, s, g);
+    });
   });
 }

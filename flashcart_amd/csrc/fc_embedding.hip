@@ -27,15 +27,15 @@ __device__ __forceinline__ int64_t chunk_start(int64_t c, int64_t width) {
 }
 
 // ---- forward: one 16-byte chunk of a row per thread ----
-template <class T, class I>
-__global__ void __launch_bounds__(256) embedding_fwd_kernel(I total, I chunks, int64_t rows, int64_t width,
+template <class T>
+__global__ void __launch_bounds__(256) embedding_fwd_kernel(uint32_t total, uint32_t chunks, int64_t rows, int64_t width,
                                                             const int64_t* __restrict__ ids,
                                                             const T* __restrict__ table, float scale,
                                                             T* __restrict__ out) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)total) return;
-  const I row = (I)t / chunks, chunk = (I)t - row * chunks;
+  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= total) return;
+  const uint32_t row = t / chunks, chunk = t - row * chunks;
   const int64_t c0 = chunk_start<V>((int64_t)chunk * V, width);
   const int64_t id = ids[row];
   const bool ok = id >= 0 && id < rows;
@@ -704,17 +704,16 @@ extern "C" int fc_embedding_fwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   if (!ids || !table || !out) return FC_ERR_NULL;
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const int64_t chunks = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T)), total = n * chunks;
-    if ((total + 255) / 256 > 0x7fffffff) return FC_ERR_SHAPE;
-    const dim3 grid((unsigned)((total + 255) / 256)), block(256);
-    hipStream_t s = (hipStream_t)stream;
-    if (total <= 0xffffffffll)
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, uint32_t>), grid, block, 0, s, (uint32_t)total, (uint32_t)chunks,
-                         rows, width, ids, (const T*)table, scale, (T*)out);
-    else
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, uint64_t>), grid, block, 0, s, (uint64_t)total, (uint64_t)chunks,
-                         rows, width, ids, (const T*)table, scale, (T*)out);
-    FC_LAUNCH_CHECK();
+    // (chunks < 2^30; a launch of whole tokens, kLaunchBlocks blocks of them where a row is not longer)
+    const int64_t chunks = (width + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    const int64_t tokens = std::max<int64_t>(1, kLaunchBlocks * 256 / chunks);
+    for (int64_t i = 0; i < n; i += tokens) {
+      const int64_t total = std::min(tokens, n - i) * chunks;
+      hipLaunchKernelGGL(embedding_fwd_kernel<T>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                         (uint32_t)total, (uint32_t)chunks, rows, width, ids + i, (const T*)table, scale,
+                         (T*)out + i * width);
+      FC_LAUNCH_CHECK();
+    }
     return FC_OK;
   });
 }
@@ -770,7 +769,7 @@ extern "C" int fc_embedding_bwd(int32_t dtype, int64_t n, int64_t rows, int64_t 
   a.counter = (int32_t*)(w + p.counter);
   const int64_t table_bytes = rows * width * node_dtype_size(dtype);
   const int64_t fills = (table_bytes + kEmbFillBytes - 1) / kEmbFillBytes;
-  if (p.tiles + fills > 0x7fffffff || p.col_blocks > 65535) return FC_ERR_SHAPE;
+  if (!grid_fits(p.tiles + fills + 1, 1024) || p.col_blocks > 65535) return FC_ERR_SHAPE;
   a.fill = (uint8_t*)grad_table;
   a.fill_bytes = table_bytes;
   a.passes = p.passes;

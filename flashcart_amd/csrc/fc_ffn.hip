@@ -18,21 +18,23 @@ struct PrepItem {
   char* dst;
   int64_t cols, ld, plane;  // of src; of dst
   int32_t rows, rows_out, gap_at, gap;  // dst row r is src row r (r < gap_at) or r - gap (r >= gap_at + gap), else zeros
-  int32_t block_base;
+  int64_t block_base;
 };
 struct PrepArgs {
   PrepItem it[4];
   int32_t count;
+  int64_t first;  // block of this launch
 };
 
 template <class T, class MT>
 __global__ void __launch_bounds__(256) ffn_prep_kernel(PrepArgs a) {
   int k = 0;
+  const int64_t block = a.first + blockIdx.x;
 #pragma unroll
   for (int q = 1; q < 4; ++q)
-    if (q < a.count && (int)blockIdx.x >= a.it[q].block_base) k = q;
+    if (q < a.count && block >= a.it[q].block_base) k = q;
   const PrepItem& it = a.it[k];
-  const int64_t chunks = it.ld / 8, t = (int64_t)(blockIdx.x - it.block_base) * 256 + threadIdx.x;
+  const int64_t chunks = it.ld / 8, t = (block - it.block_base) * 256 + threadIdx.x;
   if (t >= it.rows_out * chunks) return;
   const int64_t row = t / chunks, c0 = (t - row * chunks) * 8;
   int64_t from = row < it.gap_at ? row : row < it.gap_at + it.gap ? -1 : row - it.gap;
@@ -251,7 +253,7 @@ static int64_t partial_bytes(const FfnJob& g) { return g.splits > 1 ? 4ll * g.sp
 template <class MT, bool F32, bool ATR1, bool BTR1, int EPI1, bool ATR2 = ATR1, bool BTR2 = BTR1, int EPI2 = EPI1>
 static int launch(const FfnJob& g1, const FfnJob& g2, int kind, hipStream_t s) {
   const int64_t blocks1 = g1.M > 0 ? blocks_of(g1) : 0, blocks2 = g2.M > 0 ? blocks_of(g2) : 0, blocks = blocks1 + blocks2;
-  if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
+  if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
   if (blocks == 0) return FC_OK;
   const dim3 grid((unsigned)blocks);
   const bool swapped = blocks2 > 0 && (blocks1 == 0 || g2.steps / g2.splits > g1.steps / g1.splits);
@@ -290,7 +292,7 @@ static int launch_sums(const FfnJob* const* jobs, int count, hipStream_t s) {
     blocks += cdiv((int64_t)g.M * ((g.finish == EPI_GATE ? g.N / 2 : g.N) / 4), 256 / groups);
   }
   if (blocks == 0) return FC_OK;
-  if (blocks > 0x7fffffff) return FC_ERR_SHAPE;
+  if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
   hipLaunchKernelGGL((ffn_sum_kernel<MT, F32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
   FC_LAUNCH_CHECK();
   return FC_OK;
@@ -348,7 +350,7 @@ struct Ffn {
     it.rows_out = (int32_t)rows_out;
     it.gap_at = (int32_t)gap_at;
     it.gap = (int32_t)(gap_at < rows_out ? (rows_out - rows) / 2 : 0);
-    it.block_base = (int32_t)prep_blocks;
+    it.block_base = prep_blocks;
     prep_blocks += (o.plane / 8 + 255) / 256;
     o.p = it.dst;
     return o;
@@ -358,14 +360,14 @@ struct Ffn {
   Opnd w_in(const void* p) { return operand(p, 2 * hid, w, 2 * hp, hid); }
   int run_prep(hipStream_t s) {
     if (prep.count == 0) return FC_OK;
-    if (prep_blocks > 0x7fffffff) return FC_ERR_SHAPE;
-    const dim3 grid((unsigned)prep_blocks), block(256);
-    if (d.dtype == FC_BF16) hipLaunchKernelGGL((ffn_prep_kernel<bf16_t, bf16_t>), grid, block, 0, s, prep);
-    else if (d.dtype == FC_F16) hipLaunchKernelGGL((ffn_prep_kernel<f16_t, f16_t>), grid, block, 0, s, prep);
-    else if (form == FORM_NATIVE) hipLaunchKernelGGL((ffn_prep_kernel<float, float>), grid, block, 0, s, prep);
-    else hipLaunchKernelGGL((ffn_prep_kernel<float, bf16_t>), grid, block, 0, s, prep);
-    FC_LAUNCH_CHECK();
-    return FC_OK;
+    return in_launches(prep_blocks, [&](int64_t first, unsigned blocks) {
+      prep.first = first;
+      const dim3 grid(blocks), block(256);
+      if (d.dtype == FC_BF16) hipLaunchKernelGGL((ffn_prep_kernel<bf16_t, bf16_t>), grid, block, 0, s, prep);
+      else if (d.dtype == FC_F16) hipLaunchKernelGGL((ffn_prep_kernel<f16_t, f16_t>), grid, block, 0, s, prep);
+      else if (form == FORM_NATIVE) hipLaunchKernelGGL((ffn_prep_kernel<float, float>), grid, block, 0, s, prep);
+      else hipLaunchKernelGGL((ffn_prep_kernel<float, bf16_t>), grid, block, 0, s, prep);
+    });
   }
   int64_t h_bytes() const { return esize * n * hp; }
   int64_t factor_bytes() const { return (form == FORM_16 ? 6 : 8) * n * hp; }

@@ -55,6 +55,19 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
 inline bool node_dtype_ok(int32_t dtype) { return dtype == FC_F32 || dtype == FC_BF16 || dtype == FC_F16; }
 inline int64_t node_dtype_size(int32_t dtype) { return dtype == FC_F32 ? 4 : 2; }
 
+// A grid has below 2^32 threads a dimension. Work of more blocks than this goes in several launches, f(first block, blocks)
+// each, of GBs each.
+constexpr int64_t kLaunchBlocks = 1 << 20;
+template <class F>
+int in_launches(int64_t blocks, F&& f) {
+  for (int64_t b = 0; b < blocks; b += kLaunchBlocks) {
+    f(b, (unsigned)(blocks - b < kLaunchBlocks ? blocks - b : kLaunchBlocks));
+    FC_LAUNCH_CHECK();
+  }
+  return FC_OK;
+}
+inline bool grid_fits(int64_t blocks, int threads) { return blocks < (int64_t(1) << 32) / threads; }
+
 // f(T{}) for the element type of a checked dtype code.
 template <class F>
 int with_dtype(int32_t dtype, F&& f) {
