@@ -67,15 +67,40 @@ def _sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
 
 
-def _deps_digest(gen: str) -> str:
+def _digest(dirs, *more: str) -> str:
     h = hashlib.sha256()
-    for d in (CSRC, os.path.join(CSRC, "torch"), gen, os.path.join(ROOT, "include")):
+    for d in dirs:
         for f in sorted(os.listdir(d)):
             if f.endswith((".h", ".hip", ".cpp")):
                 with open(os.path.join(d, f), "rb") as fh:
                     h.update(f.encode() + fh.read())
-    h.update(" ".join(CFLAGS).encode() + repr(sorted(NO_CONTRACT.items())).encode())
+    h.update(" ".join(more).encode())
     return h.hexdigest()
+
+
+def _deps_digest(gen: str) -> str:
+    return _digest((CSRC, gen, os.path.join(ROOT, "include")), *CFLAGS, repr(sorted(NO_CONTRACT.items())))
+
+
+def _torch_digest() -> str:
+    """Sources of the PyTorch operators and the torch that they are compiled against: its ABI changes from version to
+    version."""
+    import torch
+
+    return _digest((os.path.join(CSRC, "torch"), os.path.join(ROOT, "include")), torch.__version__,
+                   os.path.dirname(torch.__file__), HIPCC)
+
+
+def _is_current(lib: str, stamp: str, digest: str) -> bool:
+    if not (os.path.exists(lib) and os.path.exists(stamp)):
+        return False
+    with open(stamp) as fh:
+        return fh.read() == digest
+
+
+def _write_stamp(stamp: str, digest: str) -> None:
+    with open(stamp, "w") as fh:
+        fh.write(digest)
 
 
 def _compile(src: str, gen: str, build_dir: str) -> str:
@@ -108,6 +133,15 @@ def _build_torch() -> None:
     os.replace(tmp, TORCH_LIB)
 
 
+def _link(objs, lib_path: str) -> None:
+    tmp = lib_path + ".tmp"
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed:\n{res.stderr[-4000:]}")
+    os.replace(tmp, lib_path)
+
+
 def build(jobs: int | None = None, force: bool = True, verbose: bool = False, l_max: int | None = None) -> str:
     """Compile the library (always recompiles when ``force``) and return its path. ``l_max``
     (default: ``FLASHCART_KERNEL_L_MAX``, else 3) selects the rank-3 or the rank-4 library."""
@@ -119,27 +153,26 @@ def build(jobs: int | None = None, force: bool = True, verbose: bool = False, l_
     gen, build_dir, lib_path = _variant(l_max)
     write_all(gen, 3 if l_max <= 3 else l_max)
     os.makedirs(build_dir, exist_ok=True)
-    digest = _deps_digest(gen)
-    stamp = os.path.join(build_dir, "stamp")
-    if (not force and os.path.exists(lib_path) and os.path.exists(TORCH_LIB) and os.path.exists(stamp)
-            and open(stamp).read() == digest):
-        return lib_path
-    srcs = _sources()
+    os.makedirs(BUILD, exist_ok=True)
+    digest, torch_digest = _deps_digest(gen), _torch_digest()
+    # (the PyTorch operators are one library beside both variants)
+    stamp, torch_stamp = os.path.join(build_dir, "stamp"), os.path.join(BUILD, "torch_stamp")
+    kernels = force or not _is_current(lib_path, stamp, digest)
+    with_torch = force or not _is_current(TORCH_LIB, torch_stamp, torch_digest)
+    srcs = _sources() if kernels else []
     jobs = jobs or min(8, os.cpu_count() or 4)
     # the longest units (the products of the highest in1 rank) first
     srcs.sort(key=lambda p: (not os.path.basename(p).startswith("fc_tp_l"), -ord(os.path.basename(p)[-5])))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        with_torch = ex.submit(_build_torch)
+        operators = ex.submit(_build_torch) if with_torch else None
         objs = list(ex.map(lambda p: _compile(p, gen, build_dir), srcs))
-        with_torch.result()
-    tmp = lib_path + ".tmp"
-    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"link failed:\n{res.stderr[-4000:]}")
-    os.replace(tmp, lib_path)
-    with open(stamp, "w") as fh:
-        fh.write(digest)
+        if operators is not None:
+            operators.result()
+            _write_stamp(torch_stamp, torch_digest)
+    if not kernels:
+        return lib_path
+    _link(objs, lib_path)
+    _write_stamp(stamp, digest)
     if verbose:
         print(f"built {lib_path}")
     return lib_path
