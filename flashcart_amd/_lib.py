@@ -84,9 +84,6 @@ class FfnDesc(ctypes.Structure):
                 ("act_scale", c_f32), ("scale_in", c_f32), ("scale_out", c_f32)]
 
 
-# Element types of the node-wise operators (fc_dtype).
-NODE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
 BASIS_CHEBYSHEV_AFFINE = 0
 BASIS_CHEBYSHEV_COSINE = 1
 BASIS_BESSEL = 2

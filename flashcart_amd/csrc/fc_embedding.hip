@@ -640,7 +640,7 @@ static void emb_plan_few(EmbPlan& p, int64_t n, int64_t rows, int64_t width, int
   // steps of a workgroup: a step's chain through LDS against the partial sums' bytes, and the waves that run at once
   const double bytes = 8.0 * (double)n * rows * width / groups / 4.5e6;
   int64_t steps = std::max<int64_t>({8, (int64_t)sqrt(bytes / 0.12), n * blocks / (groups * waves)});
-  steps = std::max((steps + 7) / 8 * 8, (n / groups + 65534) / 65535);
+  steps = (steps + 7) / 8 * 8;  // (a grid of few thousand workgroups: what 2,048 waves at once or 8 steps each leave)
   p.few = true;
   p.few_threads = ct;
   p.few_lds = (int)lds;
