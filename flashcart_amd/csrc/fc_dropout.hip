@@ -5,7 +5,7 @@
 // device, so a captured graph sees the values of each replay. A dropped element is written as if x were 0 whatever it
 // holds (infinities and NaN included). The sum is formed in float32 and rounded once.
 //
-// Bound by memory: 16,384 x 4,096 in bf16 70 us with a residual (5.8 TB/s), 56 us without; the generator's 20 wide products a
+// Bound by memory: 16,384 x 4,096 in bf16 70-71 us with a residual (5.7 TB/s), 56-57 us without; the generator's 20 wide products a
 // block of four elements run beside the loads.
 #include "fc_node.h"
 

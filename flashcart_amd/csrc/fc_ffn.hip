@@ -3,8 +3,9 @@
 //   dx = s_in [d gate | d up] W_in,  dW_in = s_in [d gate | d up]^T x,  dW_out = s_out g^T h.
 // Two products forward (the first forms gate and up of the same hidden columns in one workgroup and applies the
 // activation and the product in its epilogue), four backward (the first applies the factors a and b, kept from the
-// forward pass, in its epilogue). h and [d gate | d up] are rounded to the operator's type between the products, as
-// operands of the 16-bit matrix instructions; everything else is float32 until an output is rounded.
+// forward pass, in its epilogue). In 16-bit types h and [d gate | d up] are rounded to the type between the products, as
+// operands of the matrix instructions, and the factors a and b are kept with 16 significant bits; everything else is
+// float32 until an output is rounded.
 //
 // Bound by the matrix cores where n is large (16,384 x 2,048 x 5,632 in bf16, forward and backward: 2.83-3.0 ms, 1,130-1,200
 // TFLOP/s, the cores busy 57-72%), by the weights' bytes where it is small (1 x 4,096 x 10,240: 61 us, 4.1 TB/s).

@@ -491,7 +491,8 @@ int64_t fc_neighbor_list_device_noalloc(int64_t n, const double* pos, const doub
 /* ------------------------------------------------------------------------- */
 /* Node-wise operators of three element types (no counterpart in the reference,  */
 /* which composes them of torch calls on float32). Values are held in float32    */
-/* in the kernels and rounded once to the element type. Pointers need the        */
+/* in the kernels and outputs rounded once to the element type; between its      */
+/* products the feed-forward block rounds too (see there). Pointers need the     */
 /* alignment of one element.                                                     */
 /* ------------------------------------------------------------------------- */
 typedef enum fc_dtype { FC_F32 = 0, FC_BF16 = 1, FC_F16 = 2 } fc_dtype;
@@ -516,7 +517,9 @@ int fc_dropout_add(int32_t dtype, int64_t n, const void* x, const void* residual
 
 /* Gated feed-forward block: [gate | up] = scale_in x W_in^T, h = act_scale act(gate) up, y = scale_out h W_out^T; x, y
  * (n, width), W_in (2 hidden, width) with the gate's rows first, W_out (width, hidden), all of one type. act: 0 silu,
- * 1 sigmoid, 2 gelu (erf form). `aligned`: x, w_in, w_out and grad are aligned to 16 bytes (otherwise they are copied).
+ * 1 sigmoid, 2 gelu (erf form). In 16-bit types h and the gradients of gate and up are rounded to the type between the
+ * products, and the activation's factors are kept with 16 significant bits. `aligned`: x, w_in, w_out and grad are aligned
+ * to 16 bytes (otherwise they are copied).
  * width and hidden are at most 2^20, n below 2^27. */
 typedef struct fc_ffn_desc {
   int32_t dtype, act, width, hidden, aligned;

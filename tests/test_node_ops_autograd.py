@@ -96,3 +96,16 @@ def test_block_without_a_gradient_of_its_output():
         with _Calls() as calls:
             (grad,) = torch.autograd.grad(out, t, ones, allow_unused=True)
         assert grad is None and calls.names == []
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,width,hidden", [(1, 1, 1), (7, 24, 40), (600, 520, 523), (2000, 1024, 1024), (0, 8, 8)])
+def test_kept_bytes_of_fake_tensors(n, width, hidden, dtype):
+    """The shape-only operator keeps as many bytes as the library asks for, in every form of the products."""
+    from flashcart_amd import _lib
+    code = [torch.float32, torch.bfloat16, torch.float16].index(dtype)
+    want = _lib.load().fc_ffn_saved(_lib.FfnDesc(code, 0, width, hidden, 1, 1.0, 1.0, 1.0), n)
+    with FakeTensorMode():
+        x, w_in, w_out = (torch.empty(*s, dtype=dtype) for s in ((n, width), (2 * hidden, width), (width, hidden)))
+        saved = torch.ops.flashcart.gated_feed_forward(x, w_in, w_out, 0, 1.0, 1.0, 1.0, True)[1]
+    assert saved.numel() == want
