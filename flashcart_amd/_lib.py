@@ -84,6 +84,11 @@ class FfnDesc(ctypes.Structure):
                 ("act_scale", c_f32), ("scale_in", c_f32), ("scale_out", c_f32)]
 
 
+class DenseDesc(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("act", c_i32), ("in_", c_i32), ("out", c_i32), ("groups", c_i32), ("aligned", c_i32),
+                ("act_scale", c_f32), ("scale", c_f32)]
+
+
 BASIS_CHEBYSHEV_AFFINE = 0
 BASIS_CHEBYSHEV_COSINE = 1
 BASIS_BESSEL = 2
@@ -159,6 +164,17 @@ _SIGNATURES = {
     "fc_ffn_fwd": (c_int, [ctypes.POINTER(FfnDesc), c_i64] + [c_vp] * 6 + [c_i64, c_vp]),
     "fc_ffn_bwd_workspace": (c_i64, [ctypes.POINTER(FfnDesc), c_i64, c_i32, c_i32, c_i32]),
     "fc_ffn_bwd": (c_int, [ctypes.POINTER(FfnDesc), c_i64] + [c_vp] * 9 + [c_i64, c_vp]),
+    "fc_node_dense_saved": (c_i64, [ctypes.POINTER(DenseDesc), c_i64]),
+    "fc_node_dense_fwd_workspace": (c_i64, [ctypes.POINTER(DenseDesc), c_i64]),
+    "fc_node_dense_fwd": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 8 + [c_i64, c_vp]),
+    "fc_node_dense_bwd_workspace": (c_i64, [ctypes.POINTER(DenseDesc), c_i64, c_i32, c_i32, c_i32]),
+    "fc_node_dense_bwd": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 9 + [c_i64, c_vp]),
+    "fc_quantized_dense_workspace": (c_i64, [ctypes.POINTER(DenseDesc), c_i64]),
+    "fc_quantized_dense": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 8 + [c_i64, c_vp]),
+    "fc_row_norm_fwd": (c_int, [c_i32, c_i64, c_i64, c_vp, c_vp, c_vp, c_f32, c_vp, c_vp, c_vp, c_vp]),
+    "fc_row_norm_quantize": (c_int, [c_i32, c_i32, c_i64, c_i64, c_vp, c_vp, c_vp, c_f32, c_vp, c_vp, c_vp, c_vp]),
+    "fc_row_norm_bwd_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i32]),
+    "fc_row_norm_bwd": (c_int, [c_i32, c_i64, c_i64] + [c_vp] * 8 + [c_i64, c_vp]),
     "fc_neighbor_list": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp]),
     "fc_neighbor_list_device_workspace": (c_i64, [c_i64]),
     "fc_neighbor_list_device": (c_i64, [c_i64, c_vp, c_vp, c_vp, ctypes.c_double, c_i64, c_vp, c_vp, c_vp, c_vp,

@@ -17,6 +17,7 @@ it opens whichever of the two libraries is in use.
 from __future__ import annotations
 
 import argparse
+import glob
 import hashlib
 import os
 import subprocess
@@ -125,8 +126,8 @@ def _build_torch() -> None:
     tmp = TORCH_LIB + ".tmp"
     cmd = ["g++", "-O2", "-fPIC", "-std=c++17", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include_paths()),
-           f"-I{os.path.join(rocm, 'include')}", os.path.join(CSRC, "torch", "node_ops.cpp"), "-o", tmp, f"-L{lib}",
-           "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+           f"-I{os.path.join(rocm, 'include')}", *sorted(glob.glob(os.path.join(CSRC, "torch", "*.cpp"))), "-o", tmp,
+           f"-L{lib}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for the PyTorch operators:\n{res.stderr[-6000:]}")

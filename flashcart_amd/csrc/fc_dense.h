@@ -1,0 +1,264 @@
+// Dense layers (included by fc_dense.hip, fc_dense_bwd.hip): y = residual + c act(s x W^T + b), one weight for all rows or
+// one for each group of rows, and
+//   dz = c g act'(z),  dx = s dz W,  dW = s dz^T x,  db = sum of the rows of dz,  d residual = g.
+// The products are those of fc_ffn_gemm.h; bias, activation and residual are applied in the epilogue, before the one
+// rounding of y. In 16-bit types dz is rounded to the type, as operand of the matrix instructions (one rounding more than an
+// exact sum's: gradients of x and W are 1.4 times as far off as a rounding); act'(z) is kept for it with 16 significant bits.
+//
+// Groups: the rows offsets[e] .. offsets[e + 1] - 1 have weight e. The offsets stay on the device: a workgroup finds its
+// group and tile from them, the grid is the most that any offsets can need.
+#pragma once
+
+#include "fc_gemm_plan.h"
+
+namespace fc {
+
+enum { ACT_NONE = 3 };
+
+// act'(z), kept in float32, or with 24 bits as (upper 16, next 8) in two arrays.
+template <bool F32, int V>
+__device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t count, const float (&d)[V]) {
+  if constexpr (F32) {
+    put_floats((float*)factor + at, d);
+  } else {
+    uint32_t hi[V / 2], lo[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const uint32_t u0 = __float_as_uint(d[2 * i]) + 0x80, u1 = __float_as_uint(d[2 * i + 1]) + 0x80;
+      hi[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302);
+      const uint32_t pair = __builtin_amdgcn_perm(u1, u0, 0x0c0c0501);
+      if (i % 2 == 0) lo[i / 2] = pair;
+      else lo[i / 2] |= pair << 16;
+    }
+    put_words<V>(factor + 2 * at, hi);
+    char* const p = factor + 2 * count + at;
+    if constexpr (V == 8) *(uint2*)p = make_uint2(lo[0], lo[1]);
+    else *(uint32_t*)p = lo[0];
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void get_factor(const char* factor, int64_t at, int64_t count, float (&d)[8]) {
+  if constexpr (F32) {
+    const float4 u = *(const float4*)((const float*)factor + at), v = *(const float4*)((const float*)factor + at + 4);
+    d[0] = u.x, d[1] = u.y, d[2] = u.z, d[3] = u.w, d[4] = v.x, d[5] = v.y, d[6] = v.z, d[7] = v.w;
+  } else {
+    const uint4 h = *(const uint4*)(factor + 2 * at);
+    const uint2 l = *(const uint2*)(factor + 2 * count + at);
+    const uint32_t hi[4] = {h.x, h.y, h.z, h.w}, lo[2] = {l.x, l.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // (bytes: 4 to 7 of the first operand, 0 to 3 of the second, 0x0c zero)
+      d[i] = __uint_as_float(__builtin_amdgcn_perm(hi[i / 2], lo[i / 4],
+                                                   (i % 2 ? 0x07060000u : 0x05040000u) | (uint32_t)(i % 4) << 8 | 0x0cu));
+  }
+}
+
+// One product of a dense layer. For groups the pointers are those of the whole call, and a workgroup shifts them.
+struct DenseJob : GemmJob {
+  const void* bias;              // (groups, n_out), or null
+  const void* residual;          // (rows, n_out), or null
+  const float *row_scale, *col_scale;  // of 8-bit operands
+  char* factor;                  // act'(z), (rows, N), or null
+  int64_t factor_at, factor_count;
+  int32_t act;
+  float act_scale;
+  const int64_t* offsets;        // (groups + 1)
+  int32_t groups;
+  int32_t unit;                  // > 0: sums over a group's rows, in parts of so many
+  int64_t rows, b_stride, out_stride;  // rows of the call; elements from one group's B, and output, to the next one's
+
+  template <int V>
+  struct Cols {
+    float bias[V], scale[V];
+  };
+  // What the columns col .. col + V - 1 have in common in all rows; columns past the last have its values.
+  template <class OT, bool EIGHT, int V>
+  __device__ __forceinline__ Cols<V> columns(int col) const {
+    Cols<V> c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int at = min(col + v, n_out - 1);
+      c.bias[v] = bias ? to_f32(((const OT*)bias)[at]) : 0.f;
+      c.scale[v] = EIGHT ? col_scale[at] : 1.f;
+    }
+    return c;
+  }
+  // y of V columns from x = s x W^T
+  template <class OT, bool F32, bool EIGHT, int V>
+  __device__ __forceinline__ void finish(int64_t row, int col, const Cols<V>& c, const float (&x)[V]) const {
+    const int64_t at = row * ld_out + col;
+    const bool whole = col + V <= n_out;
+    float res[V];
+    if (residual) {
+      const OT* p = (const OT*)residual + at;
+      if (whole) {
+        const Pack<OT, V> r = load_pack<OT, V>(p);
+#pragma unroll
+        for (int v = 0; v < V; ++v) res[v] = to_f32(r.v[v]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) res[v] = col + v < n_out ? to_f32(p[v]) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) res[v] = 0.f;
+    }
+    float row_factor = 1.f;
+    if constexpr (EIGHT) row_factor = row_scale[row];
+    float d[V];
+    Pack<OT, V> o;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float z = EIGHT ? fmaf(x[v] * row_factor, c.scale[v], c.bias[v]) : x[v] + c.bias[v];
+      float f = z;
+      d[v] = 1.f;
+      if (act != ACT_NONE) ffn_act(act, z, f, d[v]);
+      o.v[v] = from_f32<OT>(residual ? fmaf(act_scale, f, res[v]) : act_scale * f);
+    }
+    OT* p = (OT*)out + at;
+    if (whole) {
+      store_pack<OT, V>(p, o);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (col + v < n_out) p[v] = o.v[v];
+    }
+    if constexpr (!EIGHT) {
+      if (factor) put_factor<F32, V>(factor, factor_at + row * N + col, factor_count, d);
+    }
+  }
+};
+
+// Where unit `t` of the groups' rows is, or (BY_GROUP) group `t`'s first: of the units of `size` rows (an empty group has `least` of them), counted group by
+// group. Offsets are taken into [0, n] and as their running maximum, so that the groups' rows are apart whatever they hold.
+struct GroupUnit {
+  int group, index;   // -1: there are fewer units than that; index within the group
+  int64_t row, rows;  // the group's first row and its rows
+  int total;          // units of all groups
+  int before;         // units of the groups before it
+  int slot;           // the same, of those that have more than one
+  int64_t begin, end; // rows of all groups
+};
+template <bool BY_GROUP = false>
+__device__ __forceinline__ GroupUnit find_unit(const int64_t* offsets, int groups, int64_t n, int size, int least, int t,
+                                               bool want_total) {
+  const int lane = threadIdx.x & 63;
+  auto clamped = [&](int64_t v) { return v < 0 ? 0 : v > n ? n : v; };
+  GroupUnit u{-1, 0, 0, 0, 0, 0, 0, 0, 0};
+  int64_t last = clamped(offsets[0]);
+  u.begin = last;
+  int units = 0, several = 0;
+  for (int b = 0; b < groups; b += 64) {
+    int64_t end = b + lane < groups ? clamped(offsets[b + lane + 1]) : 0;
+    end = end > last ? end : last;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int64_t v = __shfl_up(end, o, 64);
+      if (lane >= o && v > end) end = v;
+    }
+    int64_t begin = __shfl_up(end, 1, 64);
+    if (lane == 0) begin = last;
+    int count = (int)((end - begin + size - 1) / size);
+    if (count < least) count = least;
+    if (b + lane >= groups) count = 0;
+    int upto = count, more = count > 1 ? count : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int v = __shfl_up(upto, o, 64), w = __shfl_up(more, o, 64);
+      if (lane >= o) {
+        upto += v;
+        more += w;
+      }
+    }
+    const uint64_t hit = __ballot(BY_GROUP ? b + lane == t : t >= units + upto - count && t < units + upto);
+    if (hit && u.group < 0) {
+      const int at = __builtin_ctzll(hit);
+      const int own = __shfl(count, at, 64);
+      u.group = b + at;
+      u.before = units + __shfl(upto, at, 64) - own;
+      u.index = BY_GROUP ? 0 : t - u.before;
+      u.row = __shfl(begin, at, 64);
+      u.rows = __shfl(end, at, 64) - u.row;
+      u.slot = several + __shfl(more, at, 64) - (own > 1 ? own : 0);
+      if (!want_total) break;
+    }
+    units += __shfl(upto, 63, 64);
+    several += __shfl(more, 63, 64);
+    last = __shfl(end, 63, 64);
+  }
+  auto uniform64 = [](int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+  };
+  u.group = __builtin_amdgcn_readfirstlane(u.group);
+  u.index = __builtin_amdgcn_readfirstlane(u.index);
+  u.before = __builtin_amdgcn_readfirstlane(u.before);
+  u.slot = __builtin_amdgcn_readfirstlane(u.slot);
+  u.total = __builtin_amdgcn_readfirstlane(units);
+  u.begin = uniform64(u.begin);
+  u.end = uniform64(last);
+  u.row = uniform64(u.row);
+  u.rows = uniform64(u.rows);
+  return u;
+}
+
+// One workgroup's tile of a job with groups. A job over rows has a tile for every T::BM rows of a group; one with `unit`
+// sums over a group's rows, the parts of a group of more than one to `partial`, in the groups' order.
+template <class T, class MT, bool F32, bool ATR, bool BTR, int EPI, class OT_ = void>
+struct GroupTile {
+  using Base = FfnTile<T, MT, F32, ATR, BTR, EPI, OT_>;
+  using OT = typename Base::OT;
+  __device__ static __forceinline__ void run(const DenseJob& arg, int block, int blocks, lds_char* l0, lds_char* l1, lds_char* l2,
+                                             lds_char* l3) {
+    constexpr bool SUMS = ATR;
+    DenseJob g = arg;
+    const int size = SUMS ? g.unit : T::BM, least = SUMS ? 1 : 0, per = SUMS ? g.tiles_m * g.tiles_n : g.tiles_n;
+    // block -> tile as without groups: a run of tiles for each XCD
+    const GroupUnit all = find_unit(g.offsets, g.groups, g.rows, size, least, -1, true);
+    const int total = all.total * per;
+    if constexpr (!SUMS) {  // rows of no group
+      for (int64_t r = block; r < g.rows - (all.end - all.begin); r += blocks) {
+        OT* const out = (OT*)g.out + (r < all.begin ? r : r + (all.end - all.begin)) * g.ld_out;
+        for (int c = threadIdx.x; c < g.n_out; c += T::NT) out[c] = from_f32<OT>(0.f);
+      }
+    }
+    if (block >= total) return;
+    int tile = block;
+    if (total >= 64) {
+      const int each = total / 8, rest = total % 8, x = tile % 8;
+      tile = x * each + min(x, rest) + tile / 8;
+    }
+    const GroupUnit u = find_unit(g.offsets, g.groups, g.rows, size, least, tile / per, false);
+    int tiles_m = g.tiles_m, in;
+    if constexpr (SUMS) {
+      const int64_t row = u.row + (int64_t)u.index * g.unit, left = u.rows - (int64_t)u.index * g.unit;
+      const int k = (int)(left < g.unit ? left : g.unit);
+      g.A.p += Base::ES * row * g.A.ld;
+      g.B.p += Base::ES * row * g.B.ld;
+      g.A.k = g.B.k = k;
+      g.steps = max(1, (k + Base::KS - 1) / Base::KS) * (Base::PLANES ? 6 : 1);
+      if (u.rows > g.unit) {
+        g.splits = 2;
+        g.partial += (int64_t)(u.slot + u.index) * g.M * g.N;
+      } else {
+        g.splits = 1;
+        g.out = (OT*)g.out + u.group * g.out_stride;
+      }
+      in = tile - tile / per * per;
+    } else {
+      g.A.p += Base::ES * u.row * g.A.ld;
+      g.A.rows = g.M = g.m_out = (int)u.rows;
+      g.B.p += Base::ES * u.group * g.b_stride;
+      g.out = (OT*)g.out + u.row * g.ld_out;
+      if constexpr (EPI == EPI_DENSE) {
+        if (g.bias) g.bias = (const OT*)g.bias + (int64_t)u.group * g.n_out;
+        g.factor_at = u.row * g.N;
+      }
+      tiles_m = (int)((u.rows + T::BM - 1) / T::BM);
+      in = tile - u.before * per;
+    }
+    const int group = in / (8 * g.tiles_n), rest = in - group * 8 * g.tiles_n, gm = min(8, tiles_m - group * 8);
+    Base::run_tile(g, group * 8 + rest % gm, rest / gm, 0, 0, g.steps, l0, l1, l2, l3);
+  }
+};
+
+}  // namespace fc

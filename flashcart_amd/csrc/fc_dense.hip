@@ -1,0 +1,206 @@
+// Dense layers forward (fc_dense.h), in three types, with one weight or one for each group of rows, and in 8 bits:
+//   y = residual + c act(s (x_scale x) (w_scale W)^T + b)  with e4m3 x and W, a float32 scale for each of their rows, and y in 16 bits.
+#include "fc_dense_plan.h"
+
+namespace fc {
+
+template <class T, class MT, bool F32, class OT, bool GROUPS>
+__global__ void __launch_bounds__(T::NT, 2) dense_fwd_kernel(DenseJob g) {
+  __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
+  lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
+  lds_char* const l3 = (lds_char*)lds3;
+  if constexpr (GROUPS) GroupTile<T, MT, F32, false, false, EPI_DENSE, OT>::run(g, blockIdx.x, gridDim.x, l0, l1, l2, l3);
+  else FfnTile<T, MT, F32, false, false, EPI_DENSE, OT>::run(g, blockIdx.x, l0, l1, l2, l3);
+}
+
+// ---- sums over the parts of a split K loop, with the epilogue ----
+// A workgroup forms 256 / groups times 4 outputs: the lanes of an output add every groups-th part, their sums are added in
+// order.
+template <class MT, bool F32, class OT>
+__global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups) {
+  constexpr int ES = std::is_same_v<MT, float> ? 4 : 2;
+  constexpr bool EIGHT = std::is_same_v<MT, e4m3_t>;
+  __shared__ f32x4v part[256];
+  const int per = 256 / groups, grp = threadIdx.x / per;
+  const int64_t chunks = g.N / 4, t = (int64_t)blockIdx.x * per + threadIdx.x % per;
+  const bool ok = t < g.M * chunks;
+  const int64_t row = ok ? t / chunks : 0;
+  const int col = ok ? (int)(t - row * chunks) * 4 : 0;
+  f32x4v s{0.f, 0.f, 0.f, 0.f};
+  const float* p = g.partial + row * g.N + col;
+#pragma unroll 4
+  for (int k = grp; k < g.splits; k += groups) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+  if (groups > 1) {
+    part[threadIdx.x] = s;
+    __syncthreads();
+    if (grp == 0)
+      for (int k = 1; k < groups; ++k) s += part[k * per + threadIdx.x];
+  }
+  if (!ok || grp > 0) return;
+  float x[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    x[v] = s[v] * g.scale;
+    if constexpr (F32) {
+      if (!(fabsf(x[v]) < __builtin_inff())) {  // again, scaled before the sum, as where it is not split
+        x[v] = 0.f;
+        const int k_end = max(g.A.k, g.B.k), n = min(col + v, g.B.rows - 1);
+        for (int k = 0; k < k_end; ++k)
+          x[v] = fmaf(g.scale * value_of<ES, false>(g.A, row, k), value_of<ES, false>(g.B, n, k), x[v]);
+      }
+    }
+  }
+  g.finish<OT, F32, EIGHT, 4>(row, col, g.columns<OT, EIGHT, 4>(col), x);
+}
+
+struct DenseFwd {
+  DenseJob job{};
+  int kind = 0;
+};
+static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const void* bias, const void* residual,
+                           const void* offsets, void* y, void* saved) {
+  DenseFwd p;
+  DenseJob& g = p.job;
+  g.A = view(f.x(x), f.n, f.ip);
+  g.B = view(f.weight(weight), f.out, f.ip);
+  g.M = (int32_t)f.n;
+  g.N = (int32_t)f.op;
+  set_out(g, y, f.n, f.out, f.d.scale);
+  g.bias = bias;
+  g.residual = residual;
+  g.act = f.d.act;
+  g.act_scale = f.d.act_scale;
+  g.factor = (char*)saved;
+  g.factor_count = f.n * f.op;
+  if (f.d.groups > 0) {
+    f.grouped(g, offsets, f.out * f.ip, 0);
+    p.kind = plan_groups(&g, nullptr, f);
+    return p;
+  }
+  DenseJob split = g;
+  DenseJob *fused[] = {&g}, *parts[] = {&split};
+  const bool no[] = {false}, yes[] = {true};
+  double time, split_time;
+  p.kind = plan_launch(fused, no, 1, f.form, false, &time);
+  const int kind = plan_launch(parts, yes, 1, f.form, false, &split_time);
+  if (split.splits > 1 && split_time < time) {
+    g = split;
+    p.kind = kind;
+    g.partial = (float*)f.take(partial_bytes(g));
+  }
+  return p;
+}
+
+template <class MT, bool F32, class OT, bool GROUPS>
+static int launch_tiles(const DenseJob& g, int kind, hipStream_t s) {
+  const int bm = kind == 2 ? 256 : kind == 1 ? 128 : 64;
+  const int64_t blocks = GROUPS ? group_blocks(g, bm) : blocks_of(g);
+  if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks);
+  if constexpr (!std::is_same_v<MT, float>) {
+    if (kind == 2) {
+      hipLaunchKernelGGL((dense_fwd_kernel<TileL, MT, F32, OT, GROUPS>), grid, dim3(TileL::NT), 0, s, g);
+      FC_LAUNCH_CHECK();
+      return FC_OK;
+    }
+  }
+  if (kind == 1) hipLaunchKernelGGL((dense_fwd_kernel<TileM, MT, F32, OT, GROUPS>), grid, dim3(TileM::NT), 0, s, g);
+  else hipLaunchKernelGGL((dense_fwd_kernel<TileS, MT, F32, OT, GROUPS>), grid, dim3(TileS::NT), 0, s, g);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+template <class MT, bool F32, class OT>
+static int launch_dense(const DenseFwd& p, hipStream_t s) {
+  const DenseJob& g = p.job;
+  if constexpr (!std::is_same_v<MT, e4m3_t>) {
+    if (g.groups > 0) return launch_tiles<MT, F32, OT, true>(g, p.kind, s);
+  }
+  const int r = launch_tiles<MT, F32, OT, false>(g, p.kind, s);
+  if (r != FC_OK || g.splits == 1) return r;
+  int groups = 1;
+  while (groups < 16 && groups * 4 <= g.splits) groups *= 2;
+  const int64_t blocks = cdiv((int64_t)g.M * (g.N / 4), 256 / groups);
+  if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
+  hipLaunchKernelGGL((dense_sum_kernel<MT, F32, OT>), dim3((unsigned)blocks), dim3(256), 0, s, g, groups);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" int64_t fc_node_dense_saved(const fc_dense_desc* d, int64_t n) {
+  const int st = dense_check(d, n);
+  return st != FC_OK ? -st : Dense(*d, n, nullptr).factor_bytes();
+}
+
+extern "C" int64_t fc_node_dense_fwd_workspace(const fc_dense_desc* d, int64_t n) {
+  const int st = dense_check(d, n);
+  if (st != FC_OK) return -st;
+  if (n == 0) return 0;
+  Dense f(*d, n, nullptr);
+  plan_dense(f, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+  return f.at;
+}
+
+extern "C" int fc_node_dense_fwd(const fc_dense_desc* d, int64_t n, const void* x, const void* weight, const void* bias,
+                                 const void* residual, const int64_t* offsets, void* y, void* saved, void* ws,
+                                 int64_t ws_bytes, void* stream) {
+  int st = dense_check(d, n);
+  if (st != FC_OK) return st;
+  if (d->groups > 0 && residual) return FC_ERR_BAD_DESC;
+  if (n == 0) return FC_OK;
+  if (!x || !weight || !y || (d->groups > 0 && !offsets)) return FC_ERR_NULL;
+  if (d->aligned && !(aligned16(x) && aligned16(weight))) return FC_ERR_BAD_DESC;
+  Dense f(*d, n, ws);
+  const DenseFwd p = plan_dense(f, x, weight, bias, residual, offsets, y, d->act == ACT_NONE ? nullptr : saved);
+  if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
+  if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  st = f.run_pad(s);
+  if (st != FC_OK) return st;
+  return with_operand_form(d->dtype, f.form, [&](auto m, auto is32) -> int {
+    using MT = decltype(m);
+    constexpr bool F32 = decltype(is32)::value;
+    return launch_dense<MT, F32, std::conditional_t<F32, float, MT>>(p, s);
+  });
+}
+
+static int eight_check(const fc_dense_desc* d, int64_t n) {
+  const int st = dense_check(d, n);
+  return st != FC_OK ? st : d->groups != 0 || d->dtype == FC_F32 ? FC_ERR_BAD_DESC : FC_OK;
+}
+
+extern "C" int64_t fc_quantized_dense_workspace(const fc_dense_desc* d, int64_t n) {
+  const int st = eight_check(d, n);
+  if (st != FC_OK) return -st;
+  if (n == 0) return 0;
+  Dense f(*d, n, nullptr, true);
+  plan_dense(f, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+  return f.at;
+}
+
+extern "C" int fc_quantized_dense(const fc_dense_desc* d, int64_t n, const void* x, const float* x_scale,
+                                  const void* weight, const float* weight_scale, const void* bias, const void* residual,
+                                  void* y, void* ws, int64_t ws_bytes, void* stream) {
+  int st = eight_check(d, n);
+  if (st != FC_OK) return st;
+  if (n == 0) return FC_OK;
+  if (!x || !x_scale || !weight || !weight_scale || !y) return FC_ERR_NULL;
+  if (d->aligned && !(aligned16(x) && aligned16(weight))) return FC_ERR_BAD_DESC;
+  Dense f(*d, n, ws, true);
+  DenseFwd p = plan_dense(f, x, weight, bias, residual, nullptr, y, nullptr);
+  p.job.row_scale = x_scale;
+  p.job.col_scale = weight_scale;
+  if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
+  if (!aligned16(ws)) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  st = f.run_pad(s);
+  if (st != FC_OK) return st;
+  return d->dtype == FC_BF16 ? launch_dense<e4m3_t, false, bf16_t>(p, s) : launch_dense<e4m3_t, false, f16_t>(p, s);
+}

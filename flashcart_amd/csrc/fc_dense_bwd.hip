@@ -1,0 +1,355 @@
+// Dense layers backward (fc_dense.h): dz and the bias' gradient in one pass over the incoming gradient, then the products
+// for dx and dW in one launch, the one with the longer sums first.
+#include "fc_dense_plan.h"
+
+namespace fc {
+
+// ---- dz = c g act'(z) as operand of the products, and the sums of its columns over 64 rows each ----
+constexpr int kDzRows = 64, kDzCols = 256;
+
+struct DzArgs {
+  const void* grad;         // (n, out)
+  const char* factor;       // act'(z), or null
+  int64_t factor_count;
+  char* dz;                 // (n, op) in the operands' form, or null
+  int64_t plane;
+  float* sums;              // (chunks, op), or null
+  int32_t out, op, col_blocks;
+  float act_scale;
+  const int64_t* offsets;   // or null
+  int32_t groups;
+  int64_t rows;
+};
+
+// A workgroup takes 64 rows (of one group) by 256 columns, a thread 8 columns of every 8th row.
+template <class T, class MT>
+__global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
+  constexpr bool F32 = std::is_same_v<T, float>;
+  __shared__ float part[8][kDzCols + 8];
+  const int chunk = blockIdx.x / a.col_blocks, cb = blockIdx.x - chunk * a.col_blocks;
+  int64_t r0 = (int64_t)chunk * kDzRows, r1 = min(r0 + kDzRows, a.rows);
+  if (a.offsets) {
+    const GroupUnit u = find_unit(a.offsets, a.groups, a.rows, kDzRows, 0, chunk, false);
+    if (u.group < 0) return;
+    r0 = u.row + (int64_t)u.index * kDzRows;
+    r1 = min(r0 + kDzRows, u.row + u.rows);
+  }
+  const int cl = threadIdx.x % 32 * 8, col = cb * kDzCols + cl;
+  float sum[8] = {};
+  if (col < a.op) {
+#pragma unroll 4
+    for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += 8) {
+      const T* p = (const T*)a.grad + r * a.out + col;
+      float x[8];
+      if (col + 8 <= a.out) {
+        const Pack<T, 8> v = load_pack<T, 8>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = col + i < a.out ? to_f32(p[i]) : 0.f;
+      }
+      if (a.factor) {
+        float d[8];
+        get_factor<F32>(a.factor, r * a.op + col, a.factor_count, d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = col + i < a.out ? x[i] * d[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= a.act_scale;
+        sum[i] += x[i];
+      }
+      if (a.dz) put<MT, F32, 8>(a.dz, r * a.op + col, a.plane, x);
+    }
+  }
+  if (!a.sums) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[threadIdx.x / 32][cl + i] = sum[i];
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s += part[k][threadIdx.x];
+  const int c = cb * kDzCols + threadIdx.x;
+  if (c < a.op) a.sums[(int64_t)chunk * a.op + c] = s;
+}
+
+// The bias' gradient: 32 columns of a group, 8 lanes each; the chunks of a group are added in a fixed order.
+template <class T>
+__global__ void __launch_bounds__(256) dense_db_kernel(DzArgs a, void* out, int64_t chunks) {
+  __shared__ float part[8][33];
+  const int blocks = (a.out + 31) / 32, e = blockIdx.x / blocks, cl = threadIdx.x % 32, grp = threadIdx.x / 32;
+  const int c = (blockIdx.x - e * blocks) * 32 + cl;
+  int64_t c0 = 0, c1 = chunks;
+  if (a.offsets) {
+    const GroupUnit u = find_unit<true>(a.offsets, a.groups, a.rows, kDzRows, 0, e, false);
+    c0 = u.before;
+    c1 = c0 + (u.rows + kDzRows - 1) / kDzRows;
+  }
+  float s = 0.f;
+  if (c < a.out) {
+#pragma unroll 4
+    for (int64_t k = c0 + grp; k < c1; k += 8) s += a.sums[k * a.op + c];
+  }
+  part[grp][cl] = s;
+  __syncthreads();
+  if (grp > 0 || c >= a.out) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += part[k][cl];
+  ((T*)out)[(int64_t)e * a.out + c] = from_f32<T>(s);
+}
+
+// ---- the products: g1 forms dW (sums over rows), g2 dx. The first `front` workgroups take the one with the longer sums ----
+template <class T, class MT, bool F32, bool GROUPS>
+__global__ void __launch_bounds__(T::NT, 2) dense_bwd_kernel(DenseJob g1, DenseJob g2, int front, bool swapped) {
+  __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
+  lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
+  lds_char* const l3 = (lds_char*)lds3;
+  const bool in_front = (int)blockIdx.x < front;
+  const int block = in_front ? blockIdx.x : blockIdx.x - front, blocks = in_front ? front : gridDim.x - front;
+  if (in_front != swapped) {
+    if constexpr (GROUPS) GroupTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, blocks, l0, l1, l2, l3);
+    else FfnTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, l0, l1, l2, l3);
+  } else {
+    if constexpr (GROUPS) GroupTile<T, MT, F32, false, true, EPI_OUT>::run(g2, block, blocks, l0, l1, l2, l3);
+    else FfnTile<T, MT, F32, false, true, EPI_OUT>::run(g2, block, l0, l1, l2, l3);
+  }
+}
+
+// ---- sums over the parts of split sums: dW (first; with groups that alone) and dx ----
+struct BwdSums {
+  DenseJob job[2];
+  int64_t base;      // first workgroup of the second
+  int32_t lanes[2];  // that share the parts of an output
+};
+template <class MT, bool F32, bool GROUPS>
+__global__ void __launch_bounds__(256) dense_bwd_sum_kernel(BwdSums a) {
+  using OT = std::conditional_t<F32, float, MT>;
+  constexpr int ES = std::is_same_v<MT, float> ? 4 : 2;
+  __shared__ f32x4v part[256];
+  const bool dx = !GROUPS && blockIdx.x >= a.base;
+  DenseJob g = a.job[dx];
+  const int lanes = a.lanes[dx], per = 256 / lanes, grp = threadIdx.x / per;
+  const int64_t chunks = g.N / 4;
+  int64_t block = dx ? blockIdx.x - a.base : blockIdx.x;
+  if constexpr (GROUPS) {
+    const int64_t each = (g.M * chunks + per - 1) / per;
+    const int e = (int)(block / each);
+    block -= e * each;
+    const GroupUnit u = find_unit<true>(g.offsets, g.groups, g.rows, g.unit, 1, e, false);
+    if (u.rows <= g.unit) return;
+    g.splits = (int)((u.rows + g.unit - 1) / g.unit);
+    g.partial += (int64_t)u.slot * g.M * g.N;
+    g.A.p += ES * u.row * g.A.ld;
+    g.B.p += ES * u.row * g.B.ld;
+    g.A.k = g.B.k = (int)u.rows;
+    g.out = (OT*)g.out + e * g.out_stride;
+  }
+  const int64_t t = block * per + threadIdx.x % per;
+  const bool ok = t < g.M * chunks;
+  const int64_t row = ok ? t / chunks : 0;
+  const int col = ok ? (int)(t - row * chunks) * 4 : 0;
+  f32x4v s{0.f, 0.f, 0.f, 0.f};
+  const float* p = g.partial + row * g.N + col;
+#pragma unroll 4
+  for (int k = grp; k < g.splits; k += lanes) s += *(const f32x4v*)(p + (int64_t)k * g.M * g.N);
+  if (lanes > 1) {
+    part[threadIdx.x] = s;
+    __syncthreads();
+    if (grp == 0)
+      for (int k = 1; k < lanes; ++k) s += part[k * per + threadIdx.x];
+  }
+  if (!ok || grp > 0 || row >= g.m_out) return;
+  OT* const out = (OT*)g.out + row * g.ld_out;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    if (col + v >= g.n_out) continue;
+    float x = s[v] * g.scale;
+    if constexpr (F32) {
+      if (!(fabsf(x) < __builtin_inff())) {  // again, scaled before the sum, as where it is not split
+        x = 0.f;
+        const int k_end = max(g.A.k, g.B.k), m = (int)row, n = col + v;
+        for (int k = 0; k < k_end; ++k) {
+          const float u = dx ? value_of<ES, false>(g.A, m, k) : value_of<ES, true>(g.A, m, k);
+          x = fmaf(g.scale * u, value_of<ES, true>(g.B, n, k), x);
+        }
+      }
+    }
+    out[col + v] = from_f32<OT>(x);
+  }
+}
+
+struct DenseBwd {
+  DzArgs dz{};
+  bool run_dz = false;
+  int64_t chunks = 0;
+  DenseJob dw{}, dx{};  // (absent where M = 0)
+  int kind = 0;
+};
+static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const void* weight, const void* saved,
+                               const void* offsets, int need, void* gx, void* gw) {
+  DenseBwd p;
+  const bool nx = need & 1, nw = need & 2, nb = need & 4, groups = f.d.groups > 0;
+  const bool factor = f.d.act != ACT_NONE, plain = !factor && f.d.act_scale == 1.f && f.direct(f.out, f.op);
+  p.chunks = (f.n + kDzRows - 1) / kDzRows;
+  if (groups && nb) p.chunks = f.n / kDzRows + f.d.groups;
+  Opnd dz{};
+  dz.ld = f.op;
+  dz.plane = f.n * f.op;
+  dz.p = (const char*)grad;
+  DzArgs& a = p.dz;
+  if ((nx || nw) && !plain) {
+    a.dz = f.take(f.esize * dz.plane);
+    dz.p = a.dz;
+    p.run_dz = true;
+  }
+  if (nb) {
+    a.sums = (float*)f.take(4 * p.chunks * f.op);
+    p.run_dz = true;
+    if (groups) {
+      a.offsets = (const int64_t*)offsets;
+      a.groups = f.d.groups;
+    }
+  }
+  a.grad = grad;
+  a.factor = factor ? (const char*)saved : nullptr;
+  a.factor_count = a.plane = f.n * f.op;
+  a.out = (int32_t)f.out;
+  a.op = (int32_t)f.op;
+  a.col_blocks = cdiv(f.op, kDzCols);
+  a.act_scale = f.d.act_scale;
+  a.rows = f.n;
+  if (nx) {
+    DenseJob& g = p.dx;
+    g.A = view(dz, f.n, f.op);
+    g.B = view(f.weight(weight), f.ip, f.out);
+    g.M = (int32_t)f.n;
+    g.N = (int32_t)f.ip;
+    set_out(g, gx, f.n, f.in, f.d.scale);
+    g.b_tr = 1;
+    if (groups) f.grouped(g, offsets, f.out * f.ip, 0);
+  }
+  if (nw) {
+    DenseJob& g = p.dw;
+    g.A = view(dz, f.op, f.n);
+    g.B = view(f.x(x), f.ip, f.n);
+    g.M = (int32_t)f.op;
+    g.N = (int32_t)f.ip;
+    set_out(g, gw, f.out, f.in, f.d.scale);
+    g.a_tr = g.b_tr = 1;
+    if (groups) f.grouped(g, offsets, 0, f.out * f.in);
+  }
+  if (!nx && !nw) return p;
+  if (groups) {
+    p.kind = plan_groups(nx ? &p.dx : nullptr, nw ? &p.dw : nullptr, f);
+    if (nw && p.dw.unit < f.n) p.dw.partial = (float*)f.take(group_partial_bytes(p.dw));
+    return p;
+  }
+  DenseJob* jobs[] = {&p.dw, &p.dx};
+  const bool yes[] = {true, true};
+  double time;
+  p.kind = plan_launch(jobs, yes, 2, f.form, false, &time);
+  for (DenseJob* g : jobs) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
+  return p;
+}
+
+template <class MT, bool F32, bool GROUPS>
+static int launch_products(const DenseBwd& p, hipStream_t s) {
+  const DenseJob &g1 = p.dw, &g2 = p.dx;
+  const int bm = p.kind == 2 ? 256 : p.kind == 1 ? 128 : 64;
+  const int64_t blocks1 = g1.M == 0 ? 0 : GROUPS ? group_blocks(g1, bm) : blocks_of(g1);
+  const int64_t blocks2 = g2.M == 0 ? 0 : GROUPS ? group_blocks(g2, bm) : blocks_of(g2), blocks = blocks1 + blocks2;
+  if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks);
+  const int steps1 = g1.M == 0 ? 0 : GROUPS ? g1.unit / 64 : g1.steps / g1.splits;
+  const bool swapped = blocks2 > 0 && (blocks1 == 0 || g2.steps / g2.splits > steps1);
+  const int front = (int)(swapped ? blocks2 : blocks1);
+  if constexpr (!std::is_same_v<MT, float>) {
+    if (p.kind == 2)
+      hipLaunchKernelGGL((dense_bwd_kernel<TileL, MT, F32, GROUPS>), grid, dim3(TileL::NT), 0, s, g1, g2, front, swapped);
+  }
+  if (p.kind == 1)
+    hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, front, swapped);
+  else if (p.kind == 0)
+    hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, front, swapped);
+  FC_LAUNCH_CHECK();
+  // the sums of split sums
+  BwdSums a{};
+  int64_t sum_blocks = 0;
+  auto add = [&](int q, const DenseJob& g, int splits, int64_t times) {
+    int lanes = 1;
+    while (lanes < 16 && lanes * 4 <= splits) lanes *= 2;
+    a.job[q] = g;
+    a.lanes[q] = lanes;
+    sum_blocks += times * cdiv((int64_t)g.M * (g.N / 4), 256 / lanes);
+  };
+  if (GROUPS) {
+    if (g1.M > 0 && g1.unit < g1.rows) add(0, g1, cdiv(g1.rows, (int64_t)g1.unit * g1.groups), g1.groups);
+    a.base = sum_blocks;
+  } else {
+    if (g1.M > 0 && g1.splits > 1) add(0, g1, g1.splits, 1);
+    a.base = sum_blocks;
+    if (g2.M > 0 && g2.splits > 1) add(1, g2, g2.splits, 1);
+  }
+  if (sum_blocks == 0) return FC_OK;
+  if (!grid_fits(sum_blocks, 256)) return FC_ERR_SHAPE;
+  hipLaunchKernelGGL((dense_bwd_sum_kernel<MT, F32, GROUPS>), dim3((unsigned)sum_blocks), dim3(256), 0, s, a);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" int64_t fc_node_dense_bwd_workspace(const fc_dense_desc* d, int64_t n, int32_t need_x, int32_t need_weight,
+                                               int32_t need_bias) {
+  const int st = dense_check(d, n);
+  if (st != FC_OK) return -st;
+  if (n == 0) return 0;
+  Dense f(*d, n, nullptr);
+  plan_dense_bwd(f, nullptr, nullptr, nullptr, nullptr, nullptr,
+                 (need_x != 0) | 2 * (need_weight != 0) | 4 * (need_bias != 0), nullptr, nullptr);
+  return f.at;
+}
+
+extern "C" int fc_node_dense_bwd(const fc_dense_desc* d, int64_t n, const void* grad, const void* x, const void* weight,
+                                 const void* saved, const int64_t* offsets, void* gx, void* gw, void* gb, void* ws,
+                                 int64_t ws_bytes, void* stream) {
+  int st = dense_check(d, n);
+  if (st != FC_OK) return st;
+  const int need = (gx != nullptr) | 2 * (gw != nullptr) | 4 * (gb != nullptr);
+  if (n == 0 || need == 0) return n == 0 && (gw || gb) ? FC_ERR_SHAPE : FC_OK;
+  if (!grad || (gx && !weight) || (gw && !x) || (d->act != ACT_NONE && !saved) || (d->groups > 0 && !offsets))
+    return FC_ERR_NULL;
+  if (d->aligned && !(aligned16(grad) && aligned16(x) && aligned16(weight))) return FC_ERR_BAD_DESC;
+  Dense f(*d, n, ws);
+  const DenseBwd p = plan_dense_bwd(f, grad, x, weight, saved, offsets, need, gx, gw);
+  if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
+  if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  st = f.run_pad(s);
+  if (st != FC_OK) return st;
+  return with_operand_form(d->dtype, f.form, [&](auto m, auto is32) -> int {
+    using MT = decltype(m);
+    constexpr bool F32 = decltype(is32)::value;
+    using T = std::conditional_t<F32, float, MT>;
+    if (p.run_dz) {
+      const int64_t blocks = p.chunks * p.dz.col_blocks;
+      if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
+      hipLaunchKernelGGL((dense_dz_kernel<T, MT>), dim3((unsigned)blocks), dim3(256), 0, s, p.dz);
+      FC_LAUNCH_CHECK();
+    }
+    if (gb) {
+      const int64_t blocks = (int64_t)(f.d.groups > 0 ? f.d.groups : 1) * cdiv(f.out, 32);
+      if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
+      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, p.dz, gb, p.chunks);
+      FC_LAUNCH_CHECK();
+    }
+    if (!gx && !gw) return FC_OK;
+    return d->groups > 0 ? launch_products<MT, F32, true>(p, s) : launch_products<MT, F32, false>(p, s);
+  });
+}

@@ -14,6 +14,9 @@ struct bf16_t {
 struct f16_t {
   uint16_t v;
 };
+struct e4m3_t {
+  uint8_t v;
+};
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(bf16_t x) { return __uint_as_float((uint32_t)x.v << 16); }

@@ -1,0 +1,488 @@
+// Root-mean-square norm of rows with the residual's addition: total = x + residual in the tensors' type,
+//   y = w total r,  r = 1 / sqrt(mean(total^2) + eps),
+// y being the norm of the total as it is stored, so that the backward pass, which reads the stored total, differentiates what
+// was computed. With xhat = r total and g the gradient of y
+//   dx = g_total + r (w g - xhat mean(w g xhat)),  dw = sum over the rows of g xhat.
+// In 8 bits y is written as round(y / s) in e4m3 with s = max(|y|, 2^-100) / 448 for each row.
+//
+// Bound by memory: every tensor is read or written once. A row is held in registers by a group of 16 to 256 lanes, 16
+// bytes a lane and load; squares, means and dw are summed in float32. dw: a workgroup adds up the rows it takes, in
+// registers, and a second launch adds the workgroups' sums: a fixed order. Rows too wide for that (above 16,384 16-bit or
+// 8,192 float32 elements; half as many backward) are read again instead.
+#include "fc_node.h"
+
+namespace fc {
+
+struct RowNorm {
+  const void *x, *residual, *weight;
+  void *total, *y;
+  float *rstd, *scale;
+  int64_t n, width, first;  // first: block of this launch
+  float eps;
+};
+
+template <class T>
+constexpr int kChunk = 16 / sizeof(T);  // elements of a load
+
+// The elements c .. c + 15 / sizeof(T) of a row, zeros past its end.
+template <class T>
+__device__ __forceinline__ Pack<T, kChunk<T>> load_chunk(const T* row, int64_t c, int64_t width) {
+  constexpr int V = kChunk<T>;
+  if (c + V <= width) return load_pack<T, V>(row + c);
+  Pack<T, V> p;
+#pragma unroll
+  for (int i = 0; i < V; ++i) p.v[i] = c + i < width ? row[c + i] : T{};
+  return p;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t width, const Pack<T, V>& p) {
+  if (c + V <= width) {
+    store_pack<T, V>(row + c, p);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (c + i < width) row[c + i] = p.v[i];
+}
+
+// A sum, or largest value, over the L lanes of a row; every lane gets it. Called by all threads of a workgroup of NT.
+template <int L, int NT, bool MAX>
+__device__ __forceinline__ float over_row(float v, float* lds) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) / 2; o > 0; o /= 2) {
+    const float w = __shfl_xor(v, o, 64);
+    v = MAX ? fmaxf(v, w) : v + w;
+  }
+  if constexpr (L > 64) {
+    constexpr int W = L / 64;
+    const int wave = threadIdx.x / 64;
+    __syncthreads();  // (the last call's values have been read)
+    if (threadIdx.x % 64 == 0) lds[wave] = v;
+    __syncthreads();
+    const int w0 = wave / W * W;
+    v = lds[w0];
+#pragma unroll
+    for (int k = 1; k < W; ++k) v = MAX ? fmaxf(v, lds[w0 + k]) : v + lds[w0 + k];
+  }
+  return v;
+}
+
+__device__ __forceinline__ float row_scale(float most) { return fmaxf(most, 0x1p-100f) / 448.f; }
+
+// e4m3 numbers of 4 values, to nearest even; beyond 448 the largest number, NaN stays.
+__device__ __forceinline__ uint32_t pack_e4m3(const float (&x)[4], float inv) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = x[i] * inv;
+    v[i] = v[i] > 448.f ? 448.f : v[i] < -448.f ? -448.f : v[i];
+  }
+  int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], u, true);
+}
+template <int V>
+__device__ __forceinline__ Pack<uint8_t, V> to_e4m3(const float (&x)[V], float inv) {
+  Pack<uint8_t, V> p;
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    const float q[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+    w[i / 4] = pack_e4m3(q, inv);
+  }
+  memcpy(&p, w, V);
+  return p;
+}
+
+enum { NORM = 0, NORM_EIGHT = 1, ROW_EIGHT = 2 };
+
+// L lanes a row, K chunks a lane.
+template <class T, int L, int K, int MODE>
+__global__ void __launch_bounds__(256) row_norm_fwd_kernel(RowNorm g) {
+  constexpr int V = kChunk<T>, R = 256 / L;
+  __shared__ float lds[4];
+  const int lane = threadIdx.x % L;
+  const int64_t row = (g.first + blockIdx.x) * R + threadIdx.x / L, at = row * g.width;
+  const bool on = row < g.n;
+  float t[K][V];
+  float sum = 0.f;
+  Pack<T, V> xp[K], rp[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t c = ((int64_t)k * L + lane) * V;
+    xp[k] = rp[k] = Pack<T, V>{};
+    if (on && c < g.width) {
+      xp[k] = load_chunk((const T*)g.x + at, c, g.width);
+      if (g.residual) rp[k] = load_chunk((const T*)g.residual + at, c, g.width);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t c = ((int64_t)k * L + lane) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[k][i] = to_f32(xp[k].v[i]);
+    if (g.residual) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        xp[k].v[i] = from_f32<T>(t[k][i] + to_f32(rp[k].v[i]));
+        t[k][i] = to_f32(xp[k].v[i]);
+      }
+      if (on && c < g.width) store_chunk<T, V>((T*)g.total + at, c, g.width, xp[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum = fmaf(t[k][i], t[k][i], sum);
+  }
+  if constexpr (MODE != ROW_EIGHT) {
+    const float r = 1.f / sqrtf(over_row<L, 256, false>(sum, lds) / (float)g.width + g.eps);
+    if (g.rstd && on && lane == 0) g.rstd[row] = r;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = ((int64_t)k * L + lane) * V;
+      if (g.weight) {
+        const Pack<T, V> w = c < g.width ? load_chunk((const T*)g.weight, c, g.width) : Pack<T, V>{};
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[k][i] *= r * to_f32(w.v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[k][i] *= r;
+      }
+    }
+  }
+  if constexpr (MODE == NORM) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = ((int64_t)k * L + lane) * V;
+      Pack<T, V> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(t[k][i]);
+      if (on && c < g.width) store_chunk<T, V>((T*)g.y + at, c, g.width, o);
+    }
+  } else {
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(t[k][i]));
+    const float scale = row_scale(over_row<L, 256, true>(most, lds)), inv = 1.f / scale;
+    if (on && lane == 0) g.scale[row] = scale;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = ((int64_t)k * L + lane) * V;
+      if (on && c < g.width) store_chunk<uint8_t, V>((uint8_t*)g.y + at, c, g.width, to_e4m3<V>(t[k], inv));
+    }
+  }
+}
+
+// Rows of any width, a workgroup each: the row is read once for each step.
+template <class T, int MODE>
+__global__ void __launch_bounds__(1024) row_norm_wide_kernel(RowNorm g) {
+  constexpr int V = kChunk<T>, NT = 1024;
+  __shared__ float lds[NT / 64];
+  const int64_t row = g.first + blockIdx.x, at = row * g.width;
+  const T* const x = (const T*)g.x + at;
+  const T* const t = g.residual ? (const T*)g.total + at : x;
+  float r = 1.f;
+  if (MODE != ROW_EIGHT) {
+    float sum = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      Pack<T, V> v = load_chunk(x, c, g.width);
+      if (g.residual) {
+        const Pack<T, V> q = load_chunk((const T*)g.residual + at, c, g.width);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v.v[i] = from_f32<T>(to_f32(v.v[i]) + to_f32(q.v[i]));
+        store_chunk<T, V>((T*)g.total + at, c, g.width, v);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum = fmaf(to_f32(v.v[i]), to_f32(v.v[i]), sum);
+    }
+    r = 1.f / sqrtf(over_row<NT, NT, false>(sum, lds) / (float)g.width + g.eps);
+    if (g.rstd && threadIdx.x == 0) g.rstd[row] = r;
+  }
+  // (a thread reads back the elements that it wrote)
+  auto values = [&](int64_t c, float (&v)[V]) {
+    const Pack<T, V> p = load_chunk(t, c, g.width);
+    Pack<T, V> w{};
+    if (g.weight) w = load_chunk((const T*)g.weight, c, g.width);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(p.v[i]) * (g.weight ? r * to_f32(w.v[i]) : r);
+  };
+  if constexpr (MODE == NORM) {
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      float v[V];
+      values(c, v);
+      Pack<T, V> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(v[i]);
+      store_chunk<T, V>((T*)g.y + at, c, g.width, o);
+    }
+  } else {
+    float most = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      float v[V];
+      values(c, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(v[i]));
+    }
+    const float scale = row_scale(over_row<NT, NT, true>(most, lds)), inv = 1.f / scale;
+    if (threadIdx.x == 0) g.scale[row] = scale;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      float v[V];
+      values(c, v);
+      store_chunk<uint8_t, V>((uint8_t*)g.y + at, c, g.width, to_e4m3<V>(v, inv));
+    }
+  }
+}
+
+struct RowNormBwd {
+  const void *grad, *grad_total, *total, *weight;
+  const float* rstd;
+  void* dx;     // or null
+  float* sums;  // (blocks, width), or null
+  int64_t n, width;
+};
+
+template <class T, int L, int K>
+__global__ void __launch_bounds__(256) row_norm_bwd_kernel(RowNormBwd g) {
+  constexpr int V = kChunk<T>, R = 256 / L;
+  __shared__ float lds[4];
+  __shared__ float part[R > 1 ? 256 * V : 1];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  float dw[K][V];
+  Pack<T, V> wp[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t c = ((int64_t)k * L + lane) * V;
+    wp[k] = Pack<T, V>{};
+    if (g.weight && c < g.width) wp[k] = load_chunk((const T*)g.weight, c, g.width);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
+  }
+  for (int64_t first = (int64_t)blockIdx.x * R; first < g.n; first += (int64_t)gridDim.x * R) {
+    const int64_t row = first + group, at = row * g.width;
+    const bool on = row < g.n;
+    Pack<T, V> gp[K], tp[K], ap[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = ((int64_t)k * L + lane) * V;
+      gp[k] = tp[k] = ap[k] = Pack<T, V>{};
+      if (on && c < g.width) {
+        gp[k] = load_chunk((const T*)g.grad + at, c, g.width);
+        tp[k] = load_chunk((const T*)g.total + at, c, g.width);
+        if (g.grad_total && g.dx) ap[k] = load_chunk((const T*)g.grad_total + at, c, g.width);
+      }
+    }
+    const float r = on ? g.rstd[row] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float q = to_f32(gp[k].v[i]), p = q * (r * to_f32(tp[k].v[i]));
+        dw[k][i] += p;
+        sum = g.weight ? fmaf(p, to_f32(wp[k].v[i]), sum) : sum + p;
+      }
+    if (!g.dx) continue;
+    const float mean = over_row<L, 256, false>(sum, lds) / (float)g.width;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = ((int64_t)k * L + lane) * V;
+      Pack<T, V> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float q = to_f32(gp[k].v[i]), gw = g.weight ? q * to_f32(wp[k].v[i]) : q;
+        o.v[i] = from_f32<T>(fmaf(r, gw - (r * to_f32(tp[k].v[i])) * mean, to_f32(ap[k].v[i])));
+      }
+      if (on && c < g.width) store_chunk<T, V>((T*)g.dx + at, c, g.width, o);
+    }
+  }
+  if (!g.sums) return;
+  float* const out = g.sums + (int64_t)blockIdx.x * g.width;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t c = ((int64_t)k * L + lane) * V;
+    if constexpr (R > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = dw[k][i];
+      __syncthreads();
+      if (group > 0) continue;
+      for (int q = 1; q < R; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[k][i] += part[(q * L + lane) * V + i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < g.width) out[c + i] = dw[k][i];
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024) row_norm_wide_bwd_kernel(RowNormBwd g) {
+  constexpr int V = kChunk<T>, NT = 1024;
+  __shared__ float lds[NT / 64];
+  float* const out = g.sums ? g.sums + (int64_t)blockIdx.x * g.width : nullptr;
+  for (int64_t row = blockIdx.x; row < g.n; row += gridDim.x) {
+    const int64_t at = row * g.width;
+    const T *const grad = (const T*)g.grad + at, *const total = (const T*)g.total + at;
+    const float r = g.rstd[row];
+    float sum = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      const Pack<T, V> q = load_chunk(grad, c, g.width), t = load_chunk(total, c, g.width);
+      Pack<T, V> w{};
+      if (g.weight) w = load_chunk((const T*)g.weight, c, g.width);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float p = to_f32(q.v[i]) * (r * to_f32(t.v[i]));
+        sum = g.weight ? fmaf(p, to_f32(w.v[i]), sum) : sum + p;
+        if (out && c + i < g.width) out[c + i] = row == blockIdx.x ? p : out[c + i] + p;
+      }
+    }
+    if (!g.dx) continue;
+    const float mean = over_row<NT, NT, false>(sum, lds) / (float)g.width;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
+      const Pack<T, V> q = load_chunk(grad, c, g.width), t = load_chunk(total, c, g.width);
+      Pack<T, V> w{}, a{}, o;
+      if (g.weight) w = load_chunk((const T*)g.weight, c, g.width);
+      if (g.grad_total) a = load_chunk((const T*)g.grad_total + at, c, g.width);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float gw = g.weight ? to_f32(q.v[i]) * to_f32(w.v[i]) : to_f32(q.v[i]);
+        o.v[i] = from_f32<T>(fmaf(r, gw - (r * to_f32(t.v[i])) * mean, to_f32(a.v[i])));
+      }
+      store_chunk<T, V>((T*)g.dx + at, c, g.width, o);
+    }
+  }
+}
+
+// The workgroups' sums added up: 32 columns by 32 lanes that take every 32nd row.
+template <class T>
+__global__ void __launch_bounds__(1024) row_norm_dw_kernel(const float* sums, int64_t rows, int64_t width, T* out) {
+  __shared__ float part[32][33];
+  const int cl = threadIdx.x % 32, grp = threadIdx.x / 32;
+  const int64_t c = (int64_t)blockIdx.x * 32 + cl;
+  float s = 0.f;
+  if (c < width) {
+#pragma unroll 8
+    for (int64_t k = grp; k < rows; k += 32) s += sums[k * width + c];
+  }
+  part[grp][cl] = s;
+  __syncthreads();
+  if (grp > 0 || c >= width) return;
+#pragma unroll
+  for (int k = 1; k < 32; ++k) s += part[k][cl];
+  out[c] = from_f32<T>(s);
+}
+
+// f(lanes of a row, chunks of a lane) for rows of so many chunks; false where they do not fit into registers. Few rows: more
+// lanes for each.
+template <int MOST, class F>
+static bool with_row(int64_t chunks, int64_t n, F&& f) {
+  auto lanes = [&](auto l) {
+    constexpr int L = decltype(l)::value;
+    const int64_t k = (chunks + L - 1) / L;
+    if (k <= 1) f(l, std::integral_constant<int, 1>{});
+    else if (k <= 2) f(l, std::integral_constant<int, 2>{});
+    else if (k <= 4 || MOST == 4) f(l, std::integral_constant<int, 4>{});
+    else f(l, std::integral_constant<int, MOST>{});
+  };
+  const int64_t most = n < 1024 ? 2 : MOST;
+  if (chunks > 256 * MOST) return false;
+  if (chunks <= 16 * most) lanes(std::integral_constant<int, 16>{});
+  else if (chunks <= 64 * most) lanes(std::integral_constant<int, 64>{});
+  else if (chunks <= 128 * most) lanes(std::integral_constant<int, 128>{});
+  else lanes(std::integral_constant<int, 256>{});
+  return true;
+}
+
+static int row_norm_check(int32_t dtype, int64_t n, int64_t width) {
+  if (!node_dtype_ok(dtype)) return FC_ERR_BAD_DESC;
+  return n < 0 || n > 0x7fffffff || width < 1 || width > (1 << 20) ? FC_ERR_SHAPE : FC_OK;
+}
+
+template <int MODE>
+static int run_fwd(int32_t dtype, RowNorm g, hipStream_t s) {
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    int st = FC_OK;
+    const bool fits = with_row<8>((g.width + kChunk<T> - 1) / kChunk<T>, g.n, [&](auto l, auto k) {
+      constexpr int L = decltype(l)::value, K = decltype(k)::value;
+      st = in_launches((g.n + 256 / L - 1) / (256 / L), [&](int64_t first, unsigned grid) {
+        g.first = first;
+        hipLaunchKernelGGL((row_norm_fwd_kernel<T, L, K, MODE>), dim3(grid), dim3(256), 0, s, g);
+      });
+    });
+    if (fits) return st;
+    return in_launches(g.n, [&](int64_t first, unsigned grid) {
+      g.first = first;
+      hipLaunchKernelGGL((row_norm_wide_kernel<T, MODE>), dim3(grid), dim3(1024), 0, s, g);
+    });
+  });
+}
+
+// Workgroups of a backward pass with dw: each adds a row to the second launch.
+static int64_t bwd_blocks(int64_t n) { return n < 512 ? n : 512; }
+
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" int fc_row_norm_fwd(int32_t dtype, int64_t n, int64_t width, const void* x, const void* residual,
+                               const void* weight, float eps, void* total, void* y, float* rstd, void* stream) {
+  const int st = row_norm_check(dtype, n, width);
+  if (st != FC_OK) return st;
+  if (n == 0) return FC_OK;
+  if (!x || !y || (residual && !total)) return FC_ERR_NULL;
+  return run_fwd<NORM>(dtype, RowNorm{x, residual, weight, total, y, rstd, nullptr, n, width, 0, eps}, (hipStream_t)stream);
+}
+
+extern "C" int fc_row_norm_quantize(int32_t dtype, int32_t norm, int64_t n, int64_t width, const void* x,
+                                    const void* residual, const void* weight, float eps, void* total, void* q,
+                                    float* scale, void* stream) {
+  const int st = row_norm_check(dtype, n, width);
+  if (st != FC_OK) return st;
+  if (!norm && (residual || weight)) return FC_ERR_BAD_DESC;
+  if (n == 0) return FC_OK;
+  if (!x || !q || !scale || (residual && !total)) return FC_ERR_NULL;
+  const RowNorm g{x, residual, weight, total, q, nullptr, scale, n, width, 0, eps};
+  return norm ? run_fwd<NORM_EIGHT>(dtype, g, (hipStream_t)stream) : run_fwd<ROW_EIGHT>(dtype, g, (hipStream_t)stream);
+}
+
+extern "C" int64_t fc_row_norm_bwd_workspace(int32_t dtype, int64_t n, int64_t width, int32_t need_weight) {
+  const int st = row_norm_check(dtype, n, width);
+  if (st != FC_OK) return -st;
+  return need_weight ? 4 * bwd_blocks(n) * width : 0;
+}
+
+extern "C" int fc_row_norm_bwd(int32_t dtype, int64_t n, int64_t width, const void* grad, const void* grad_total,
+                               const void* total, const void* weight, const float* rstd, void* grad_x, void* grad_weight,
+                               void* ws, int64_t ws_bytes, void* stream) {
+  const int st = row_norm_check(dtype, n, width);
+  if (st != FC_OK) return st;
+  if (!grad_x && !grad_weight) return FC_OK;
+  if (n == 0) return grad_weight ? FC_ERR_SHAPE : FC_OK;
+  if (!grad || !total || !rstd) return FC_ERR_NULL;
+  const int64_t need = grad_weight ? 4 * bwd_blocks(n) * width : 0;
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return FC_ERR_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const RowNormBwd g{grad, grad_total, total, weight, rstd, grad_x, grad_weight ? (float*)ws : nullptr, n, width};
+    int64_t blocks = 0;
+    const bool fits = with_row<4>((width + kChunk<T> - 1) / kChunk<T>, n, [&](auto l, auto k) {
+      constexpr int L = decltype(l)::value, K = decltype(k)::value;
+      blocks = (n + 256 / L - 1) / (256 / L);
+      if (grad_weight) blocks = bwd_blocks(blocks);
+      else if (blocks > kLaunchBlocks) blocks = kLaunchBlocks;
+      hipLaunchKernelGGL((row_norm_bwd_kernel<T, L, K>), dim3((unsigned)blocks), dim3(256), 0, s, g);
+    });
+    if (!fits) {
+      blocks = bwd_blocks(n);
+      hipLaunchKernelGGL((row_norm_wide_bwd_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, g);
+    }
+    FC_LAUNCH_CHECK();
+    if (!grad_weight) return FC_OK;
+    hipLaunchKernelGGL((row_norm_dw_kernel<T>), dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, s, (const float*)ws,
+                       blocks, width, (T*)grad_weight);
+    FC_LAUNCH_CHECK();
+    return FC_OK;
+  });
+}

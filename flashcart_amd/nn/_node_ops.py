@@ -1,6 +1,6 @@
 """The registered operators of ``flashcart_amd.nn.functional`` (``torch.ops.flashcart.embedding``, ``dropout_add``,
-``gated_feed_forward`` and their backward passes). They are C++ operators over the C entry points
-(``csrc/torch/node_ops.cpp``, ``libflashcart_torch.so``); here they are loaded and given their shape-only
+``gated_feed_forward``, ``rms_norm_add``, ``node_dense``, ..., and their backward passes). They are C++ operators over the
+C entry points (``csrc/torch``, ``libflashcart_torch.so``); here they are loaded and given their shape-only
 implementations."""
 
 from __future__ import annotations
@@ -13,6 +13,7 @@ import torch
 from flashcart_amd import _lib
 
 ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2}
+NO_ACTIVATION = 3
 
 TORCH_LIB_PATH = os.path.join(os.path.dirname(_lib.LIB_PATH), "libflashcart_torch.so")
 
@@ -73,8 +74,46 @@ def _gated_feed_forward_bwd(grad, x, w_in, w_out, saved, act, act_scale, scale_i
     return _contiguous(x, need_x), _contiguous(w_in, need_w_in), _contiguous(w_out, need_w_out)
 
 
+def _rms_norm_add(x, residual, weight, eps, save):
+    total = _contiguous(x, residual is not None)
+    return _contiguous(x), total, x.new_empty(x.numel() // x.shape[-1] if save else 0, dtype=torch.float32)
+
+
+def _rms_norm_add_bwd(grad, grad_total, total, weight, rstd, need_x, need_weight):
+    return _contiguous(total, need_x), total.new_empty(total.shape[-1] if need_weight else 0)
+
+
+def _quantize_rows(x):
+    return (torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+def _rms_norm_add_quantized(x, residual, weight, eps):
+    return (*_quantize_rows(x), _contiguous(x, residual is not None))
+
+
+def _node_dense(x, weight, bias, residual, offsets, act, act_scale, scale, save):
+    out = weight.shape[-2]
+    size = 0
+    if save and act != NO_ACTIVATION:  # the activation's derivative
+        size = x.numel() // weight.shape[-1] * ((out + 7) // 8 * 8) * (4 if x.dtype == torch.float32 else 3)
+    return x.new_empty((*x.shape[:-1], out)), x.new_empty(size, dtype=torch.uint8)
+
+
+def _node_dense_bwd(grad, x, weight, saved, offsets, act, act_scale, scale, need_x, need_weight, need_bias):
+    return _contiguous(x, need_x), _contiguous(weight, need_weight), x.new_empty(weight.shape[:-1] if need_bias else 0)
+
+
+def _quantized_dense(x, x_scale, weight, weight_scale, bias, residual, act, act_scale, scale, dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=dtype)
+
+
 _FAKES = {"embedding": _embedding, "embedding_bwd": _embedding_bwd, "dropout_add": _dropout_add,
-          "dropout_draw": _dropout_draw, "gated_feed_forward": _gated_feed_forward, "gated_feed_forward_bwd": _gated_feed_forward_bwd}
+          "dropout_draw": _dropout_draw, "gated_feed_forward": _gated_feed_forward,
+          "gated_feed_forward_bwd": _gated_feed_forward_bwd, "rms_norm_add": _rms_norm_add,
+          "rms_norm_add_bwd": _rms_norm_add_bwd, "rms_norm_add_quantized": _rms_norm_add_quantized,
+          "quantize_rows": _quantize_rows, "node_dense": _node_dense, "node_dense_bwd": _node_dense_bwd,
+          "quantized_dense": _quantized_dense}
 
 # With the import, so that a compiled function never meets the loading. Where it fails (not built, built for another torch)
 # the first call says why; the rest of the package does not need it.

@@ -1,20 +1,22 @@
 """Node-wise functions in float32, bfloat16 and float16: embedding lookup, gated
-feed-forward block, residual dropout.
+feed-forward block, residual dropout, root-mean-square norm, dense layers (also with a weight for each group of rows), and
+the norm and dense layers of 8-bit inference.
 
 They have no counterpart among the reference's kernels (it composes torch operations). Each is a registered operator
 (``torch.ops.flashcart.*``) with an autograd formula, runs on the current stream and allocates through torch, so it can
 be captured into a graph. There is no CPU path, and there are no forward-mode derivatives (an argument with a tangent is
-refused). Values are formed in float32 and outputs rounded once to the tensors' type; what the feed-forward block rounds
-between its products stands there. None has an autocast rule: under ``torch.autocast`` the arguments keep their types.
+refused). Values are formed in float32 and outputs rounded once to the tensors' type; what the feed-forward block and the
+dense layers round between their products stands there. None has an autocast rule: under ``torch.autocast`` the arguments keep their types.
 """
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from flashcart_amd.nn import _node_ops
 
-__all__ = ["dropout_add", "embedding", "gated_feed_forward"]
+__all__ = ["dense", "dropout_add", "embedding", "gated_feed_forward", "grouped_dense", "quantize_rows", "quantized_dense",
+           "rms_norm_add", "rms_norm_add_quantized"]
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
@@ -84,3 +86,110 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng
             where the call is captured into a graph): the same pair gives the same mask.
     """
     return _node_ops.ops().dropout_add.default(x, residual, float(p), rng)
+
+
+def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _activation(act: Optional[str]) -> int:
+    if act is None:
+        return _node_ops.NO_ACTIVATION
+    if act not in _node_ops.ACTIVATIONS:
+        raise ValueError(f"act must be None or one of {sorted(_node_ops.ACTIVATIONS)}, got {act!r}.")
+    return _node_ops.ACTIVATIONS[act]
+
+
+def rms_norm_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(weight * total / sqrt(mean(total^2) + eps), total)`` with ``total = x + residual``.
+
+    Args:
+        x: (..., width).
+        residual: as x, or None: the total is x itself.
+        weight: (width) of x's type, or None for ones.
+
+    The norm is that of the total as it is returned, rounded to the tensors' type. Both outputs have gradients; the
+    weight's adds its rows in float32 in an order that the sizes fix. There are no second derivatives. A row of zeros with
+    ``eps=0`` gives NaN.
+    """
+    y, total, _ = _node_ops.ops().rms_norm_add.default(x, residual, weight, float(eps), _wants_grad(x, residual, weight))
+    return y, x if residual is None else total
+
+
+def rms_norm_add_quantized(x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                           weight: Optional[torch.Tensor] = None,
+                           eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``rms_norm_add`` with its norm in 8 bits, for inference: (q, scale, total), the norm being ``q * scale[..., None]``.
+
+    q is float8_e4m3fn, ``round(y / scale)`` of the unrounded norm y; scale (float32) is ``max(|y|, 2^-100) / 448`` over the
+    row. A row with an infinity has an infinite scale, and NaN for its values. There are no gradients: arguments that
+    require them are refused where autograd records.
+    """
+    q, scale, total = _node_ops.ops().rms_norm_add_quantized.default(x, residual, weight, float(eps))
+    return q, scale, x if residual is None else total
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of the rows of x (..., width), as ``rms_norm_add_quantized`` gives them for its norm: the operands of
+    ``quantized_dense``. A weight is laid out so once."""
+    return _node_ops.ops().quantize_rows.default(x)
+
+
+def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
+          act_scale: float = 1.0, scale: float = 1.0, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``residual + act_scale * act(scale * x @ weight.T + bias)``.
+
+    Args:
+        x: (..., in).
+        weight: (out, in).
+        bias: (out) or None.
+        act: "silu", "sigmoid", "gelu" (erf form) or None.
+        act_scale, scale: factors, as the rescaled activations and linear layers of this package have them.
+        residual: (..., out) or None.
+
+    Sums are float32, and bias, activation and residual are applied before the one rounding of the output. For bfloat16
+    and float16 the gradient of the activation's argument is rounded to that type in the backward pass, being an operand of
+    the matrix instructions (gradients of x and weight are 1.4 times as far from exact ones as one rounding); the
+    activation's derivative is kept for it with 16 significant bits, 3 bytes an output (float32: all, 4). float32 products
+    keep float32 accuracy, as in ``gated_feed_forward``; so does the activation. There are no second derivatives.
+    """
+    return _node_ops.ops().node_dense.default(x, weight, bias, residual, None, _activation(act), float(act_scale),
+                                              float(scale), _wants_grad(x, weight, bias))[0]
+
+
+def grouped_dense(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  act: Optional[str] = None, act_scale: float = 1.0, scale: float = 1.0) -> torch.Tensor:
+    """``act_scale * act(scale * x[r] @ weight[e].T + bias[e])`` for each row r of group e, as ``dense`` without a residual.
+
+    Args:
+        x: (rows, in), the rows of a group together.
+        weight: (groups, out, in).
+        offsets: (groups + 1) int64 or int32 on x's device: group e has the rows ``offsets[e]`` to ``offsets[e + 1] - 1``.
+            They are not read on the host. Groups may be empty; rows in front of the first and behind the last give zeros
+            and take no part in gradients. Offsets outside the rows are taken as the nearest inside, one smaller than those
+            before it as the largest of them.
+        bias: (groups, out) or None.
+
+    Returns:
+        (rows, out). The gradients of a group without rows are zero.
+    """
+    if offsets is None:
+        raise TypeError("`offsets` must be a tensor.")
+    return _node_ops.ops().node_dense.default(x, weight, bias, None, offsets, _activation(act), float(act_scale),
+                                              float(scale), _wants_grad(x, weight, bias))[0]
+
+
+def quantized_dense(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                    bias: Optional[torch.Tensor] = None, act: Optional[str] = None, act_scale: float = 1.0,
+                    scale: float = 1.0, residual: Optional[torch.Tensor] = None,
+                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``dense`` in 8 bits, for inference: x (..., in) and weight (out, in) in float8_e4m3fn with a float32 scale for each
+    row, (...) and (out), as ``rms_norm_add_quantized`` and ``quantize_rows`` give them.
+
+    Bias, residual and output have the type ``dtype``, bfloat16 or float16. The 8-bit matrix instructions add eight products
+    with 13 bits below the largest's leading bit and those sums in float32: about 1.5e-5 of the output, below its rounding.
+    There are no gradients: arguments that require them are refused where autograd records.
+    """
+    return _node_ops.ops().quantized_dense.default(x, x_scale, weight, weight_scale, bias, residual, _activation(act),
+                                                   float(act_scale), float(scale), dtype)

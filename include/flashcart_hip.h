@@ -538,6 +538,59 @@ int fc_ffn_bwd(const fc_ffn_desc* desc, int64_t n, const void* grad, const void*
                const void* saved, void* grad_x, void* grad_w_in, void* grad_w_out, void* workspace,
                int64_t workspace_bytes, void* stream);
 
+/* Dense layer: y = residual + act_scale act(scale x W^T + bias), x (n, in), W (out, in), bias (out), residual and y
+ * (n, out), all of one type; bias and residual may be NULL. act: as above, 3 none. groups > 0: W (groups, out, in), bias
+ * (groups, out), no residual; row r has weight e where offsets[e] <= r < offsets[e + 1]; offsets: groups + 1 int64 on the
+ * device, taken into [0, n] and as their running maximum; rows of no group give zeros. In 16-bit types the gradient of
+ * act's argument is rounded to the type between the products, and act's derivative is kept with 16 significant bits.
+ * `aligned`: x, W and grad are aligned to 16 bytes (otherwise they are copied). in and out are at most 2^20, n below 2^27,
+ * groups at most 2^16 with (groups + 1) out below 2^30. */
+typedef struct fc_dense_desc {
+  int32_t dtype, act, in, out, groups, aligned;
+  float act_scale, scale;
+} fc_dense_desc;
+
+/* Sizes in bytes; `saved` and the workspaces are aligned to 16. In training `saved` (fc_node_dense_saved bytes, 0 without
+ * an activation) receives what the backward pass reads; NULL otherwise. */
+int64_t fc_node_dense_saved(const fc_dense_desc* desc, int64_t n);
+int64_t fc_node_dense_fwd_workspace(const fc_dense_desc* desc, int64_t n);
+int fc_node_dense_fwd(const fc_dense_desc* desc, int64_t n, const void* x, const void* weight, const void* bias,
+                      const void* residual, const int64_t* offsets, void* y, void* saved, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+/* Gradients, each formed when its pointer is non-NULL (n >= 1 where one of weight or bias is asked for); the residual's
+ * is grad. Zero for groups without rows, and for rows of no group. */
+int64_t fc_node_dense_bwd_workspace(const fc_dense_desc* desc, int64_t n, int32_t need_x, int32_t need_weight,
+                                    int32_t need_bias);
+int fc_node_dense_bwd(const fc_dense_desc* desc, int64_t n, const void* grad, const void* x, const void* weight,
+                      const void* saved, const int64_t* offsets, void* grad_x, void* grad_weight, void* grad_bias,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same without groups on e4m3 operands (OCP, 448 the largest) x and W with a float32 scale for each of their rows,
+ * the values being x[r, :] x_scale[r] and W[c, :] weight_scale[c]; bias, residual and y of desc's type, one of 16 bits: the
+ * 8-bit matrix instructions add with about 16. */
+int64_t fc_quantized_dense_workspace(const fc_dense_desc* desc, int64_t n);
+int fc_quantized_dense(const fc_dense_desc* desc, int64_t n, const void* x, const float* x_scale, const void* weight,
+                       const float* weight_scale, const void* bias, const void* residual, void* y, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of rows: total = x + residual, rounded to the type; y = weight total / sqrt(mean(total^2) + eps),
+ * with the total as it is stored. x, residual, total, y (n, width), weight (width), all of one type; residual, and with it
+ * total, may be NULL (total is x), weight too (ones). rstd (n) float32 receives 1 / sqrt(...) where it is non-NULL. width
+ * is at most 2^20, n below 2^31. */
+int fc_row_norm_fwd(int32_t dtype, int64_t n, int64_t width, const void* x, const void* residual, const void* weight,
+                    float eps, void* total, void* y, float* rstd, void* stream);
+/* The same with y in e4m3 and a scale for each row, max(largest |y|, 2^-100) / 448: q = round(y / scale). norm = 0: y is
+ * the row of x itself (no residual, weight, total or eps). */
+int fc_row_norm_quantize(int32_t dtype, int32_t norm, int64_t n, int64_t width, const void* x, const void* residual,
+                         const void* weight, float eps, void* total, void* q, float* scale, void* stream);
+/* grad_x = grad_total + rstd (weight grad - xhat mean(weight grad xhat)) with xhat = rstd total (also the residual's
+ * gradient), grad_weight = sum over rows of grad xhat, in a fixed order; each where its pointer is non-NULL. grad_total may
+ * be NULL. The workspace is in bytes, its base aligned to 16. */
+int64_t fc_row_norm_bwd_workspace(int32_t dtype, int64_t n, int64_t width, int32_t need_weight);
+int fc_row_norm_bwd(int32_t dtype, int64_t n, int64_t width, const void* grad, const void* grad_total, const void* total,
+                    const void* weight, const float* rstd, void* grad_x, void* grad_weight, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,5 @@
-"""Node-wise operators in float64: embedding and its gradient, residual dropout, the gated feed-forward block. No
-counterpart in the reference; stated from the formulas."""
+"""Node-wise operators in float64: embedding and its gradient, residual dropout, the gated feed-forward block, the
+root-mean-square norm, dense layers. No counterpart in the reference; stated from the formulas."""
 
 import math
 
@@ -102,4 +102,103 @@ def gated_feed_forward(x, w_in, w_out, act, c, s_in, s_out, grad=None, mid=0.0, 
     res["dx"] = (dx, bound(dx, abs(s_in) * ((e_d + (2 * hidden + 3) * f * dpre.abs()) @ w_in.abs())))
     res["dw_in"] = (dwi, bound(dwi, abs(s_in) * ((e_d + (n + 3) * f * dpre.abs()).t() @ x.abs())))
     res["dw_out"] = (dwo, bound(dwo, abs(s_out) * (g.abs().t() @ (e_h + (n + 3) * f * h.abs()))))
+    return res
+
+
+def rms_norm_add(x, residual, weight, eps, grad=None, grad_total=None, end=0.0, tiny=0.0):
+    """{name: (value, bound)} of the total (as it is stored, in x's type), y, and with ``grad`` the gradients dx and dw.
+
+    The bound is what a float32 evaluation may be off: y is a product of three factors whose square sum has relative error
+    (width / 2 + 2) 2^-24 at most, halved by the root; ``end`` and ``tiny`` as in ``gated_feed_forward``."""
+    f = 2.0 ** -24
+    n, width = x.shape
+    total = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    t = total.double()
+    w = t.new_ones(width) if weight is None else weight.double()
+    r = 1 / torch.sqrt((t * t).mean(1, keepdim=True) + eps)
+    e_r = (0.5 * (width / 2 + 2) + 4) * f
+    y = t * r * w
+    res = {"total": (t, torch.zeros_like(t)), "y": (y, (end + e_r + 2 * f) * y.abs() + tiny)}
+    if grad is None:
+        return res
+    g, xhat = grad.double(), t * r
+    gw = g * w
+    mean, size = (gw * xhat).mean(1, keepdim=True), (gw * xhat).abs().mean(1, keepdim=True)
+    dx = r * (gw - xhat * mean)
+    e_dx = r * (((e_r + 4 * f) * (gw.abs() + 2 * xhat.abs() * mean.abs())) + xhat.abs() * (width + e_r / f) * f * size)
+    if grad_total is not None:
+        dx = dx + grad_total.double()
+    res["dx"] = (dx, (end + f) * dx.abs() + e_dx + tiny)
+    terms = g * xhat
+    res["dw"] = (terms.sum(0), end * terms.sum(0).abs() + ((e_r + (n + 2) * f) * terms.abs()).sum(0) + tiny)
+    return res
+
+
+def e4m3_rows(y):
+    """(values of the 8-bit numbers, scale) of rows of float64 values: the nearest of the e4m3 numbers, ties to even."""
+    scale = y.abs().amax(1).clamp_min(2.0 ** -100) / 448
+    v = y / scale[:, None]
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 3)
+    return (torch.round(v / step) * step).clamp(-448, 448), scale
+
+
+def dense(x, weight, bias, residual, act, c, s, grad=None, mid=0.0, end=0.0, kept=0.0, tiny=0.0):
+    """{name: (value, bound)} of y and, with ``grad``, of dx, dw and db. Roundings as in ``gated_feed_forward``."""
+    f = 2.0 ** -24
+    x, w = x.double(), weight.double()
+    n, (out, width) = x.shape[0], w.shape
+    z = s * (x @ w.t())
+    e_z = (width + 3) * f * abs(s) * (x.abs() @ w.abs().t())
+    if bias is not None:
+        z = z + bias.double()
+    e_z = e_z + f * z.abs()
+    if act is None:
+        a, d, e_a, e_d = z, torch.ones_like(z), e_z, torch.zeros_like(z)
+    else:
+        a, d = activation(z, act)
+        e_a, e_d = 1.13 * e_z + 16 * f * (1 + z.abs()), 0.8 * e_z + 16 * f * (1 + z.abs())
+    y, e_y = c * a, abs(c) * (e_a + 2 * f * a.abs())
+    if residual is not None:
+        y = y + residual.double()
+        e_y = e_y + f * y.abs()
+    res = {"y": (y, end * y.abs() + e_y + tiny)}
+    if grad is None:
+        return res
+    g = grad.double()
+    dz = c * g * d
+    e_dz = (c * g).abs() * (e_d + (kept if act else 0.0) * d.abs() + 3 * f * d.abs())
+    m_dz = e_dz + mid * dz.abs() + tiny  # as an operand
+    dx, dw, db = s * (dz @ w), s * (dz.t() @ x), dz.sum(0)
+
+    def bound(value, size):
+        return end * value.abs() + size + tiny
+
+    res["dx"] = (dx, bound(dx, abs(s) * ((m_dz + (out + 3) * f * dz.abs()) @ w.abs())))
+    res["dw"] = (dw, bound(dw, abs(s) * ((m_dz + (n + 3) * f * dz.abs()).t() @ x.abs())))
+    res["db"] = (db, bound(db, (e_dz + (n + 3) * f * dz.abs()).sum(0)))
+    return res
+
+
+def group_rows(offsets, rows):
+    """The [first, end) rows of each group: offsets inside the rows, none smaller than one before it."""
+    ends, last = [], 0
+    for v in offsets.tolist():
+        last = max(last, min(max(v, 0), rows))
+        ends.append(last)
+    return list(zip(ends, ends[1:]))
+
+
+def grouped_dense(x, weight, offsets, bias, act, c, s, grad=None, **roundings):
+    """``dense`` group by group; rows of no group are zero in y and dx."""
+    rows, (groups, out, width) = x.shape[0], weight.shape
+    shapes = {"y": (rows, out), "dx": (rows, width), "dw": (groups, out, width), "db": (groups, out)}
+    res = {k: tuple(torch.zeros(v, dtype=torch.float64) for _ in range(2))
+           for k, v in shapes.items() if k == "y" or grad is not None}
+    for e, (a, b) in enumerate(group_rows(offsets, rows)):
+        part = dense(x[a:b], weight[e], None if bias is None else bias[e], None, act, c, s,
+                     None if grad is None else grad[a:b], **roundings)
+        for k, v in part.items():
+            at = slice(a, b) if k in ("y", "dx") else e
+            for to, value in zip(res[k], v):
+                to[at] = value
     return res
