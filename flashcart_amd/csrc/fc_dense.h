@@ -3,7 +3,7 @@
 //   dz = c g act'(z),  dx = s dz W,  dW = s dz^T x,  db = sum of the rows of dz,  d residual = g.
 // The products are those of fc_ffn_gemm.h; bias, activation and residual are applied in the epilogue, before the one
 // rounding of y. In 16-bit types dz is rounded to the type, as operand of the matrix instructions (one rounding more than an
-// exact sum's: gradients of x and W are 1.4 times as far off as a rounding); act'(z) is kept for it with 16 significant bits.
+// exact sum's: gradients of x and W are 1.4 times as far off as a rounding).
 //
 // Groups: the rows offsets[e] .. offsets[e + 1] - 1 have weight e. The offsets stay on the device: a workgroup finds its
 // group and tile from them, the grid is the most that any offsets can need.
@@ -15,11 +15,20 @@ namespace fc {
 
 enum { ACT_NONE = 3 };
 
-// act'(z), kept in float32, or with 24 bits as (upper 16, next 8) in two arrays.
-template <bool F32, int V>
+// act'(z) as it is kept for the backward pass: in float32; in float16 beside bfloat16 operands (its rounding is an eighth of
+// theirs); beside float16 ones with 24 bits, (upper 16, next 8) in two arrays.
+template <class OT>
+constexpr int kFactorBytes = std::is_same_v<OT, float> ? 4 : std::is_same_v<OT, bf16_t> ? 2 : 3;
+
+template <class OT, int V>
 __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t count, const float (&d)[V]) {
-  if constexpr (F32) {
+  if constexpr (std::is_same_v<OT, float>) {
     put_floats((float*)factor + at, d);
+  } else if constexpr (std::is_same_v<OT, bf16_t>) {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2<f16_t>(d[2 * i], d[2 * i + 1]);
+    put_words<V>(factor + 2 * at, w);
   } else {
     uint32_t hi[V / 2], lo[V / 4];
 #pragma unroll
@@ -36,11 +45,15 @@ __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t cou
     else *(uint32_t*)p = lo[0];
   }
 }
-template <bool F32>
+template <class OT>
 __device__ __forceinline__ void get_factor(const char* factor, int64_t at, int64_t count, float (&d)[8]) {
-  if constexpr (F32) {
+  if constexpr (std::is_same_v<OT, float>) {
     const float4 u = *(const float4*)((const float*)factor + at), v = *(const float4*)((const float*)factor + at + 4);
     d[0] = u.x, d[1] = u.y, d[2] = u.z, d[3] = u.w, d[4] = v.x, d[5] = v.y, d[6] = v.z, d[7] = v.w;
+  } else if constexpr (std::is_same_v<OT, bf16_t>) {
+    const Pack<f16_t, 8> p = *(const Pack<f16_t, 8>*)__builtin_assume_aligned(factor + 2 * at, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = to_f32(p.v[i]);
   } else {
     const uint4 h = *(const uint4*)(factor + 2 * at);
     const uint2 l = *(const uint2*)(factor + 2 * count + at);
@@ -66,66 +79,130 @@ struct DenseJob : GemmJob {
   int32_t unit;                  // > 0: sums over a group's rows, in parts of so many
   int64_t rows, b_stride, out_stride;  // rows of the call; elements from one group's B, and output, to the next one's
 
-  template <int V>
-  struct Cols {
-    float bias[V], scale[V];
-  };
-  // What the columns col .. col + V - 1 have in common in all rows; columns past the last have its values.
-  template <class OT, bool EIGHT, int V>
-  __device__ __forceinline__ Cols<V> columns(int col) const {
-    Cols<V> c;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int at = min(col + v, n_out - 1);
-      c.bias[v] = bias ? to_f32(((const OT*)bias)[at]) : 0.f;
-      c.scale[v] = EIGHT ? col_scale[at] : 1.f;
-    }
-    return c;
-  }
-  // y of V columns from x = s x W^T
+  // V columns from `col` on of the rows that a lane finishes one after the other:
+  // where it is, what its columns have in common in all rows, and the residuals of its next rows, loaded ahead.
   template <class OT, bool F32, bool EIGHT, int V>
-  __device__ __forceinline__ void finish(int64_t row, int col, const Cols<V>& c, const float (&x)[V]) const {
-    const int64_t at = row * ld_out + col;
-    const bool whole = col + V <= n_out;
-    float res[V];
-    if (residual) {
-      const OT* p = (const OT*)residual + at;
-      if (whole) {
-        const Pack<OT, V> r = load_pack<OT, V>(p);
+  struct Line {
+    OT* out;
+    const OT* res;
+    int64_t factor_at;
+    float bias[V], col_scale[V];
+    float lin, one, act_scale;  // silu, sigmoid: act(z) = s(z) (lin z + one), s the logistic function; times act_scale
+    int col_at;
+    bool whole;
+    Pack<OT, V> next[2];
+
+    __device__ __forceinline__ void init(const DenseJob& g, int64_t row, int col) {
+      out = (OT*)g.out + row * g.ld_out + col;
+      res = g.residual ? (const OT*)g.residual + row * g.ld_out + col : nullptr;
+      factor_at = g.factor_at + row * g.N + col;
+      col_at = col;
+      whole = col + V <= g.n_out;
+      lin = g.act == 1 ? 0.f : 1.f;
+      one = 1.f - lin;
+      act_scale = g.act_scale;
+      Pack<OT, V> b{};
+      Pack<float, V> c{};
+      if (g.bias) b = part(g, (const OT*)g.bias + col);
+      if constexpr (EIGHT) c = part(g, g.col_scale + col);
 #pragma unroll
-        for (int v = 0; v < V; ++v) res[v] = to_f32(r.v[v]);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) res[v] = col + v < n_out ? to_f32(p[v]) : 0.f;
+      for (int v = 0; v < V; ++v) {
+        bias[v] = to_f32(b.v[v]);
+        col_scale[v] = EIGHT ? c.v[v] : 1.f;
       }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) res[v] = 0.f;
     }
-    float row_factor = 1.f;
-    if constexpr (EIGHT) row_factor = row_scale[row];
-    float d[V];
-    Pack<OT, V> o;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float z = EIGHT ? fmaf(x[v] * row_factor, c.scale[v], c.bias[v]) : x[v] + c.bias[v];
-      float f = z;
-      d[v] = 1.f;
-      if (act != ACT_NONE) ffn_act(act, z, f, d[v]);
-      o.v[v] = from_f32<OT>(residual ? fmaf(act_scale, f, res[v]) : act_scale * f);
-    }
-    OT* p = (OT*)out + at;
-    if (whole) {
-      store_pack<OT, V>(p, o);
-    } else {
+    // the V elements from p on, as far as there are columns
+    template <class E>
+    __device__ __forceinline__ Pack<E, V> part(const DenseJob& g, const E* p) const {
+      Pack<E, V> r{};
+      if (whole) return load_pack<E, V>(p);
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (col + v < n_out) p[v] = o.v[v];
+        if (col_at + v < g.n_out) r.v[v] = p[v];
+      return r;
     }
-    if constexpr (!EIGHT) {
-      if (factor) put_factor<F32, V>(factor, factor_at + row * N + col, factor_count, d);
+    // the residuals of this turn's rows: `row`, row + step, ... of PASSES
+    template <int PASSES>
+    __device__ __forceinline__ void ahead(const DenseJob& g, bool inside, int64_t row, int step) {
+      if (!g.residual) return;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        if (inside && row + p * step < g.M) next[p] = part(g, res + p * step * g.ld_out);
+      }
     }
-  }
+    // y of those rows from x = s x W^T; the cursor goes on to the next turn, 16 rows further
+    template <int PASSES>
+    __device__ __forceinline__ void finish(const DenseJob& g, bool inside, int64_t row, int step,
+                                           float (&x)[PASSES][V]) {
+      static_assert(PASSES <= 2, "residuals ahead");
+      Pack<OT, V> r[PASSES];
+      const bool with_res = g.residual != nullptr;
+      if (with_res) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) r[p] = next[p];
+        res += 16 * g.ld_out;
+        ahead<PASSES>(g, inside, row + 16, step);
+      }
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const bool ok = inside && row + p * step < g.M;
+        float d[V];
+        float row_scale = 1.f;
+        if constexpr (EIGHT) row_scale = g.row_scale[ok ? row + p * step : 0];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if constexpr (EIGHT) x[p][v] = fmaf(x[p][v] * row_scale, col_scale[v], bias[v]);
+          else x[p][v] += bias[v];
+        }
+        if (g.act == ACT_NONE) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[p][v] *= act_scale;
+        } else if (g.act == 2) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float f;
+            ffn_act(2, x[p][v], f, d[v]);
+            x[p][v] = act_scale * f;
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float z = x[p][v], s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), q = fmaf(lin, z, one);
+            d[v] = s * fmaf(q, 1.f - s, lin);
+            x[p][v] = act_scale * (s * q);
+          }
+        }
+        if (with_res) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[p][v] += to_f32(r[p].v[v]);
+        }
+        if (!ok) continue;
+        OT* const to = out + p * step * g.ld_out;
+        if (whole) {
+          Pack<OT, V> o;
+          if constexpr (std::is_same_v<OT, float>) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) o.v[v] = x[p][v];
+          } else {
+            uint32_t w[V / 2];
+#pragma unroll
+            for (int v = 0; v < V / 2; ++v) w[v] = pack2<OT>(x[p][2 * v], x[p][2 * v + 1]);
+            memcpy(&o, w, sizeof(o));
+          }
+          store_pack<OT, V>(to, o);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (col_at + v < g.n_out) to[v] = from_f32<OT>(x[p][v]);
+        }
+        if constexpr (!EIGHT) {
+          if (g.factor) put_factor<OT, V>(g.factor, factor_at + (int64_t)p * step * g.N, g.factor_count, d);
+        }
+      }
+      out += 16 * g.ld_out;
+      factor_at += 16 * (int64_t)g.N;
+    }
+  };
 };
 
 // Where unit `t` of the groups' rows is, or (BY_GROUP) group `t`'s first: of the units of `size` rows (an empty group has `least` of them), counted group by

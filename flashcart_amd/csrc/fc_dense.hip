@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups) 
       for (int k = 1; k < groups; ++k) s += part[k * per + threadIdx.x];
   }
   if (!ok || grp > 0) return;
-  float x[4];
+  float y[1][4], (&x)[4] = y[0];
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     x[v] = s[v] * g.scale;
@@ -53,7 +53,10 @@ __global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups) 
       }
     }
   }
-  g.finish<OT, F32, EIGHT, 4>(row, col, g.columns<OT, EIGHT, 4>(col), x);
+  DenseJob::Line<OT, F32, EIGHT, 4> line;
+  line.init(g, row, col);
+  line.template ahead<1>(g, true, row, 0);
+  line.template finish<1>(g, true, row, 0, y);
 }
 
 struct DenseFwd {

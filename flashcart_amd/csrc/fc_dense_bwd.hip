@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
       }
       if (a.factor) {
         float d[8];
-        get_factor<F32>(a.factor, r * a.op + col, a.factor_count, d);
+        get_factor<T>(a.factor, r * a.op + col, a.factor_count, d);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = col + i < a.out ? x[i] * d[i] : 0.f;
       }

@@ -125,7 +125,9 @@ struct Dense {
       else hipLaunchKernelGGL((dense_pad_kernel<float, bf16_t>), grid, block, 0, s, pad);
     });
   }
-  int64_t factor_bytes() const { return d.act == ACT_NONE ? 0 : (form == FORM_16 ? 3 : 4) * n * op; }
+  int64_t factor_bytes() const {
+    return d.act == ACT_NONE ? 0 : (d.dtype == FC_F32 ? 4 : d.dtype == FC_BF16 ? 2 : 3) * n * op;
+  }
   void grouped(DenseJob& g, const void* offsets, int64_t b_stride, int64_t out_stride) const {
     g.offsets = (const int64_t*)offsets;
     g.groups = d.groups;

@@ -801,12 +801,12 @@ struct FfnTile {
 #pragma unroll
       for (int j = 0; j < T::NF; ++j) *(lds_f32x4*)(to + 64 * j) = acc[i][j];
     };
-    auto take = [&](const lds_char* p, float (&x)[8]) {
+    auto take = [&](const lds_char* p, float (&x)[8], float factor) {
       const f32x4v u = *(const lds_f32x4*)p, v = *(const lds_f32x4*)(p + 16);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        x[k] = u[k] * scale;
-        x[4 + k] = v[k] * scale;
+        x[k] = u[k] * factor;
+        x[4 + k] = v[k] * factor;
       }
     };
     if constexpr (EPI == EPI_OUT) {
@@ -825,7 +825,7 @@ struct FfnTile {
             *(f32x4v*)(out + 4) = v;
             continue;
           }
-          take(from + p * RPP * RS, x);
+          take(from + p * RPP * RS, x, scale);
           if (row >= g.gap_at) {
             if (row < g.gap_at + g.gap) continue;
             row -= g.gap;
@@ -842,25 +842,26 @@ struct FfnTile {
         }
       }
     } else if constexpr (EPI == EPI_DENSE) {
-      const auto cols = g.template columns<OT, EIGHT, 8>(min(col, g.N - 8));
+      typename Job::template Line<OT, F32, EIGHT, 8> line;
+      line.init(g, row0 + rl, min(col, g.N - 8));
+      const bool inside = on && col < g.N;
+      line.template ahead<PASSES>(g, inside, row0 + rl, RPP);
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
         stage(i);
+        float x[PASSES][8];
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-          const int64_t row = row0 + 16 * i + p * RPP + rl;
-          if (row >= g.M || col >= g.N) continue;
-          const lds_char* const at = from + p * RPP * RS;
-          if (g.splits > 1) {  // unscaled
-            float* out = g.partial + ((int64_t)split * g.M + row) * g.N + col;
-            *(f32x4v*)out = *(const lds_f32x4*)at;
-            *(f32x4v*)(out + 4) = *(const lds_f32x4*)(at + 16);
-            continue;
+        for (int p = 0; p < PASSES; ++p) take(from + p * RPP * RS, x[p], g.splits > 1 ? 1.f : scale);
+        if (g.splits > 1) {  // unscaled
+#pragma unroll
+          for (int p = 0; p < PASSES; ++p) {
+            const int64_t row = row0 + 16 * i + p * RPP + rl;
+            if (!inside || row >= g.M) continue;
+            put_floats<8>(g.partial + ((int64_t)split * g.M + row) * g.N + col, x[p]);
           }
-          float x[8];
-          take(at, x);
-          g.template finish<OT, F32, EIGHT, 8>(row, col, cols, x);
+          continue;
         }
+        line.template finish<PASSES>(g, inside, row0 + 16 * i + rl, RPP, x);
       }
     } else if constexpr (EPI == EPI_GATE) {
 #pragma unroll
@@ -869,8 +870,8 @@ struct FfnTile {
         const int64_t row = row0 + 16 * i + rl;
         if (!on || row >= g.M || col >= g.N) continue;
         float gate[8], up[8];
-        take(from, gate);
-        take(from + COLS * 4, up);
+        take(from, gate, scale);
+        take(from + COLS * 4, up, scale);
         finish_gate<MT, F32, 8>(g, row, col, g.N, gate, up);
       }
     } else {
@@ -892,7 +893,7 @@ struct FfnTile {
         const int64_t row = row0 + t * RPP + rl;
         if (row >= g.M || col >= g.N) continue;
         float dh[8];
-        take(from + t % PASSES * RPP * RS, dh);
+        take(from + t % PASSES * RPP * RS, dh, scale);
         finish_dh<MT, F32, 8>(g, row, col, f[t % (AHEAD + 1)], dh);
       }
     }

@@ -96,7 +96,7 @@ def _node_dense(x, weight, bias, residual, offsets, act, act_scale, scale, save)
     out = weight.shape[-2]
     size = 0
     if save and act != NO_ACTIVATION:  # the activation's derivative
-        size = x.numel() // weight.shape[-1] * ((out + 7) // 8 * 8) * (4 if x.dtype == torch.float32 else 3)
+        size = x.numel() // weight.shape[-1] * ((out + 7) // 8 * 8) * {torch.float32: 4, torch.float16: 3}.get(x.dtype, 2)
     return x.new_empty((*x.shape[:-1], out)), x.new_empty(size, dtype=torch.uint8)
 
 

@@ -191,7 +191,7 @@ def test_library_refuses_bad_arguments():
     good = dict(dtype=1, act=0, in_=8, out=16, groups=0, aligned=0, act_scale=1.0, scale=1.0)
     d = _lib.DenseDesc(**good)
     size = lib.fc_node_dense_fwd_workspace(d, 3)
-    assert size >= 0 and lib.fc_node_dense_saved(d, 3) == 3 * 16 * 3 and lib.fc_node_dense_saved(d, -1) == -shape
+    assert size >= 0 and lib.fc_node_dense_saved(d, 3) == 3 * 16 * 2 and lib.fc_node_dense_saved(d, -1) == -shape
     assert lib.fc_node_dense_fwd(d, 3, 16, None, None, None, None, 16, None, 16, size, None) == null
     big = lib.fc_node_dense_fwd_workspace(d, 1000)  # (operands are copied)
     assert big > 0 and lib.fc_node_dense_fwd(d, 1000, 16, 16, None, None, None, 16, None, 16, big - 1, None) == workspace

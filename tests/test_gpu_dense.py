@@ -43,8 +43,8 @@ def _roundings(dtype):
     u = torch.finfo(dtype).eps / 2
     if dtype == torch.float32:
         return dict(mid=0.0, end=u, kept=0.0, tiny=2.0 ** -140)
-    # the kept derivative holds 16 significant bits
-    return dict(mid=u, end=u, kept=2.0 ** -17, tiny=2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    # the kept derivative holds 11 significant bits beside bfloat16, 16 beside float16 (below 2^-14 all to 2^-24 of one)
+    return dict(mid=u, end=u, kept=2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -17, tiny=2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
 
 
 def _check(got, want, dtype):
