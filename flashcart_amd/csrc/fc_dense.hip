@@ -1,5 +1,6 @@
 // Dense layers forward (fc_dense.h), in three types, with one weight or one for each group of rows, and in 8 bits:
 //   y = residual + c act(s (x_scale x) (w_scale W)^T + b)  with e4m3 x and W, a float32 scale for each of their rows, and y in 16 bits.
+#include "fc_dense_few.h"
 #include "fc_dense_plan.h"
 
 namespace fc {
@@ -62,13 +63,38 @@ __global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups) 
 struct DenseFwd {
   DenseJob job{};
   int kind = 0;
+  bool few = false;
 };
+// Whether the kernel for few rows is faster than tiles. It reads x again for every 16 columns, and has less of the weight on
+// its way than the tiles; it needs no copy of operands whose rows are not a multiple of 16 bytes. us, few / tiles, out of
+// in -> out: bf16, one row 256 -> 512 3.4 / 4.8, 1,024 -> 4,096 4.4 / 6.8, 2,048 -> 8,192 11.6 / 9.8, 4,096 -> 10,240 20 / 16,
+// 1,031 -> 4,096 8.0 / 15.8; 16 rows 4,097 -> 4,096 29 / 28; 32 rows 1,024 -> 4,096 6.1 / 6.8, 2,048 -> 1,024 8.6 / 8.9.
+// float32, one row 2,048 -> 8,192 15 / 28, 4,096 -> 10,240 52 / 59, 4,096 -> 64 11.5 / 8.8; 32 rows 4,097 -> 4,096 29 / 53.
+// Groups: 16 of 2,048 -> 1,024 with 64 rows 20 / 14, 64 of 1,031 -> 512 with 32 rows 24 / 39 and with 512 41 / 47,
+// 8 of 4,099 -> 1,000 with 128 rows 66 / 41.
+static bool few_rows(const Dense& f) {
+  if (f.form == FORM_PLANES) return false;
+  const bool direct = f.direct(f.in, f.ip);
+  if (f.d.groups > 0) return !direct && f.n <= 8 * (int64_t)f.d.groups;
+  if (f.n > kFewRows) return false;
+  const int64_t blocks = (f.n + 15) / 16, k = blocks * f.in;
+  if (f.form == FORM_NATIVE) return k <= (direct ? 2048 : 16384) || (blocks == 1 && f.out >= 4096);
+  return direct ? k <= 2048 && k * f.out <= 1 << 23 : k <= 4096;
+}
 static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const void* bias, const void* residual,
                            const void* offsets, void* y, void* saved) {
   DenseFwd p;
   DenseJob& g = p.job;
-  g.A = view(f.x(x), f.n, f.ip);
-  g.B = view(f.weight(weight), f.out, f.ip);
+  p.few = few_rows(f);
+  if (p.few) {
+    g.A.p = (const char*)x;
+    g.B.p = (const char*)weight;
+    g.A.ld = g.B.ld = f.in;
+    g.A.k = (int32_t)f.in;
+  } else {
+    g.A = view(f.x(x), f.n, f.ip);
+    g.B = view(f.weight(weight), f.out, f.ip);
+  }
   g.M = (int32_t)f.n;
   g.N = (int32_t)f.op;
   set_out(g, y, f.n, f.out, f.d.scale);
@@ -79,16 +105,18 @@ static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const vo
   g.factor = (char*)saved;
   g.factor_count = f.n * f.op;
   if (f.d.groups > 0) {
-    f.grouped(g, offsets, f.out * f.ip, 0);
+    f.grouped(g, offsets, f.out * (p.few ? f.in : f.ip), 0);
+    if (p.few) return p;
     p.kind = plan_groups(&g, nullptr, f);
     return p;
   }
+  if (p.few) return p;
   DenseJob split = g;
   DenseJob *fused[] = {&g}, *parts[] = {&split};
   const bool no[] = {false}, yes[] = {true};
   double time, split_time;
-  p.kind = plan_launch(fused, no, 1, f.form, false, &time);
-  const int kind = plan_launch(parts, yes, 1, f.form, false, &split_time);
+  p.kind = plan_launch(fused, no, 1, f.form, false, true, &time);
+  const int kind = plan_launch(parts, yes, 1, f.form, false, true, &split_time);
   if (split.splits > 1 && split_time < time) {
     g = split;
     p.kind = kind;
@@ -99,7 +127,7 @@ static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const vo
 
 template <class MT, bool F32, class OT, bool GROUPS>
 static int launch_tiles(const DenseJob& g, int kind, hipStream_t s) {
-  const int bm = kind == 2 ? 256 : kind == 1 ? 128 : 64;
+  const int bm = tile_rows(kind);
   const int64_t blocks = GROUPS ? group_blocks(g, bm) : blocks_of(g);
   if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
   const dim3 grid((unsigned)blocks);
@@ -110,8 +138,20 @@ static int launch_tiles(const DenseJob& g, int kind, hipStream_t s) {
       return FC_OK;
     }
   }
-  if (kind == 1) hipLaunchKernelGGL((dense_fwd_kernel<TileM, MT, F32, OT, GROUPS>), grid, dim3(TileM::NT), 0, s, g);
+  if (kind == 3) hipLaunchKernelGGL((dense_fwd_kernel<TileX, MT, F32, OT, GROUPS>), grid, dim3(TileX::NT), 0, s, g);
+  else if (kind == 1) hipLaunchKernelGGL((dense_fwd_kernel<TileM, MT, F32, OT, GROUPS>), grid, dim3(TileM::NT), 0, s, g);
   else hipLaunchKernelGGL((dense_fwd_kernel<TileS, MT, F32, OT, GROUPS>), grid, dim3(TileS::NT), 0, s, g);
+  FC_LAUNCH_CHECK();
+  return FC_OK;
+}
+
+template <class MT, class OT, bool GROUPS>
+static int launch_few(const DenseJob& g, hipStream_t s) {
+  const int64_t blocks = (int64_t)(GROUPS ? g.groups : 1) * cdiv(g.n_out, 16);
+  if (!grid_fits(blocks, 64 * kFewWaves)) return FC_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
+  if (GROUPS || g.M <= 16) hipLaunchKernelGGL((dense_few_kernel<MT, OT, 1, GROUPS>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((dense_few_kernel<MT, OT, 2, GROUPS>), grid, block, 0, s, g);
   FC_LAUNCH_CHECK();
   return FC_OK;
 }
@@ -119,6 +159,14 @@ static int launch_tiles(const DenseJob& g, int kind, hipStream_t s) {
 template <class MT, bool F32, class OT>
 static int launch_dense(const DenseFwd& p, hipStream_t s) {
   const DenseJob& g = p.job;
+  if (p.few) {
+    if constexpr (!(F32 && std::is_same_v<MT, bf16_t>)) {
+      if constexpr (!std::is_same_v<MT, e4m3_t>) {
+        if (g.groups > 0) return launch_few<MT, OT, true>(g, s);
+      }
+      return launch_few<MT, OT, false>(g, s);
+    }
+  }
   if constexpr (!std::is_same_v<MT, e4m3_t>) {
     if (g.groups > 0) return launch_tiles<MT, F32, OT, true>(g, p.kind, s);
   }

@@ -4,8 +4,8 @@
 
 namespace fc {
 
-// ---- dz = c g act'(z) as operand of the products, and the sums of its columns over 64 rows each ----
-constexpr int kDzRows = 64, kDzCols = 256;
+// ---- dz = c g act'(z) as operand of the products, and the sums of its columns over 32 rows each ----
+constexpr int kDzRows = 32, kDzCols = 256;
 
 struct DzArgs {
   const void* grad;         // (n, out)
@@ -21,10 +21,12 @@ struct DzArgs {
   int64_t rows;
 };
 
-// A workgroup takes 64 rows (of one group) by 256 columns, a thread 8 columns of every 8th row.
+// A workgroup takes 32 rows (of one group) by 256 columns, a thread 8 columns of every 8th row, all loaded before the first is
+// stored.
 template <class T, class MT>
 __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   constexpr bool F32 = std::is_same_v<T, float>;
+  constexpr int N = kDzRows / 8;
   __shared__ float part[8][kDzCols + 8];
   const int chunk = blockIdx.x / a.col_blocks, cb = blockIdx.x - chunk * a.col_blocks;
   int64_t r0 = (int64_t)chunk * kDzRows, r1 = min(r0 + kDzRows, a.rows);
@@ -37,26 +39,30 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   const int cl = threadIdx.x % 32 * 8, col = cb * kDzCols + cl;
   float sum[8] = {};
   if (col < a.op) {
-#pragma unroll 4
-    for (int64_t r = r0 + threadIdx.x / 32; r < r1; r += 8) {
-      const T* p = (const T*)a.grad + r * a.out + col;
-      float x[8];
-      if (col + 8 <= a.out) {
-        const Pack<T, 8> v = load_pack<T, 8>(p);
+    const int64_t first = r0 + threadIdx.x / 32;
+    Pack<T, 8> v[N];
+    float d[N][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
+    for (int k = 0; k < N; ++k) {
+      const int64_t r = min(first + 8 * k, r1 - 1);
+      const T* p = (const T*)a.grad + r * a.out + col;
+      if (col + 8 <= a.out) {
+        v[k] = load_pack<T, 8>(p);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = col + i < a.out ? to_f32(p[i]) : 0.f;
+        for (int i = 0; i < 8; ++i) v[k].v[i] = col + i < a.out ? p[i] : T{};
       }
-      if (a.factor) {
-        float d[8];
-        get_factor<T>(a.factor, r * a.op + col, a.factor_count, d);
+      if (a.factor) get_factor<T>(a.factor, r * a.op + col, a.factor_count, d[k]);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = col + i < a.out ? x[i] * d[i] : 0.f;
-      }
+    for (int k = 0; k < N; ++k) {
+      const int64_t r = first + 8 * k;
+      if (r >= r1) break;
+      float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        x[i] = to_f32(v[k].v[i]);
+        if (a.factor) x[i] = col + i < a.out ? x[i] * d[k][i] : 0.f;
         x[i] *= a.act_scale;
         sum[i] += x[i];
       }
@@ -74,10 +80,10 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   if (c < a.op) a.sums[(int64_t)chunk * a.op + c] = s;
 }
 
-// The bias' gradient: 32 columns of a group, 8 lanes each; the chunks of a group are added in a fixed order.
+// The bias' gradient: 32 columns of a group, 32 lanes each; the chunks of a group are added in a fixed order.
 template <class T>
-__global__ void __launch_bounds__(256) dense_db_kernel(DzArgs a, void* out, int64_t chunks) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) dense_db_kernel(DzArgs a, void* out, int64_t chunks) {
+  __shared__ float part[32][33];
   const int blocks = (a.out + 31) / 32, e = blockIdx.x / blocks, cl = threadIdx.x % 32, grp = threadIdx.x / 32;
   const int c = (blockIdx.x - e * blocks) * 32 + cl;
   int64_t c0 = 0, c1 = chunks;
@@ -88,14 +94,14 @@ __global__ void __launch_bounds__(256) dense_db_kernel(DzArgs a, void* out, int6
   }
   float s = 0.f;
   if (c < a.out) {
-#pragma unroll 4
-    for (int64_t k = c0 + grp; k < c1; k += 8) s += a.sums[k * a.op + c];
+#pragma unroll 8
+    for (int64_t k = c0 + grp; k < c1; k += 32) s += a.sums[k * a.op + c];
   }
   part[grp][cl] = s;
   __syncthreads();
   if (grp > 0 || c >= a.out) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) s += part[k][cl];
+  for (int k = 1; k < 32; ++k) s += part[k][cl];
   ((T*)out)[(int64_t)e * a.out + c] = from_f32<T>(s);
 }
 
@@ -251,7 +257,7 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
   DenseJob* jobs[] = {&p.dw, &p.dx};
   const bool yes[] = {true, true};
   double time;
-  p.kind = plan_launch(jobs, yes, 2, f.form, false, &time);
+  p.kind = plan_launch(jobs, yes, 2, f.form, false, true, &time);
   for (DenseJob* g : jobs) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
   return p;
 }
@@ -259,7 +265,7 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
 template <class MT, bool F32, bool GROUPS>
 static int launch_products(const DenseBwd& p, hipStream_t s) {
   const DenseJob &g1 = p.dw, &g2 = p.dx;
-  const int bm = p.kind == 2 ? 256 : p.kind == 1 ? 128 : 64;
+  const int bm = tile_rows(p.kind);
   const int64_t blocks1 = g1.M == 0 ? 0 : GROUPS ? group_blocks(g1, bm) : blocks_of(g1);
   const int64_t blocks2 = g2.M == 0 ? 0 : GROUPS ? group_blocks(g2, bm) : blocks_of(g2), blocks = blocks1 + blocks2;
   if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
@@ -273,6 +279,8 @@ static int launch_products(const DenseBwd& p, hipStream_t s) {
   }
   if (p.kind == 1)
     hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, front, swapped);
+  else if (p.kind == 3)
+    hipLaunchKernelGGL((dense_bwd_kernel<TileX, MT, F32, GROUPS>), grid, dim3(TileX::NT), 0, s, g1, g2, front, swapped);
   else if (p.kind == 0)
     hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, front, swapped);
   FC_LAUNCH_CHECK();
@@ -345,8 +353,8 @@ extern "C" int fc_node_dense_bwd(const fc_dense_desc* d, int64_t n, const void* 
     }
     if (gb) {
       const int64_t blocks = (int64_t)(f.d.groups > 0 ? f.d.groups : 1) * cdiv(f.out, 32);
-      if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
-      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, p.dz, gb, p.chunks);
+      if (!grid_fits(blocks, 1024)) return FC_ERR_SHAPE;
+      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, p.dz, gb, p.chunks);
       FC_LAUNCH_CHECK();
     }
     if (!gx && !gw) return FC_OK;

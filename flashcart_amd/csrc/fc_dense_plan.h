@@ -148,17 +148,19 @@ inline int plan_groups(DenseJob* rows, DenseJob* sums, const Dense& f) {
   int64_t best_unit = 0;
   double best = 1e30;
   if (rows) rows->steps = steps_of(rows->A.k > rows->B.k ? rows->A.k : rows->B.k, f.form);
-  for (int kind = 0; kind < (f.form == FORM_NATIVE ? 2 : 3); ++kind) {
+  for (int kind = 0; kind < kKinds; ++kind) {
+    if (f.form == FORM_NATIVE && kind == 2) continue;
     const TileCost& c = f.form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
-    const int bm = kind == 2 ? 256 : kind == 1 ? 128 : 64;
-    double row_blocks = 0, row_load = 0, row_chain = 0;
+    const int bm = tile_rows(kind);
+    double row_blocks = 0, row_load = 0, row_chain = 0, row_alone = 0;
     if (rows) {
       row_blocks = (f.n / (double)bm + 0.5 * groups) * cdiv(rows->N, bm);
       row_chain = rows->steps;
       row_load = row_blocks * (rows->steps * c.full + c.fused);
+      row_alone = row_blocks * (rows->steps * c.step + kLatency[kind][!sums]);
     }
     for (int64_t unit = (f.n + per - 1) / per * per;;) {
-      double blocks = row_blocks, load = row_load, chain = row_chain, extra = 0;
+      double blocks = row_blocks, load = row_load, chain = row_chain, alone = row_alone, extra = 0;
       if (sums) {
         const double tiles = (double)cdiv(sums->M, bm) * cdiv(sums->N, bm);
         const double parts = each > unit ? f.n / (double)unit + 0.5 * groups : groups;
@@ -167,14 +169,18 @@ inline int plan_groups(DenseJob* rows, DenseJob* sums, const Dense& f) {
         const double longest = planes * (double)(unit < 2 * each ? unit : 2 * each) / per;
         blocks += parts * tiles;
         load += parts * tiles * (steps * c.full + c.end) + (f.d.groups - groups) * tiles * c.end;
+        alone += parts * tiles * (steps * c.step + kLatency[kind][0]);
         if (longest > chain) chain = longest;
         if (each * 2 > unit) extra = 8e-6 / 3 * (2.0 * f.n / unit) * sums->M * sums->N + 3.5;
       }
-      const double shared = (kind < 2 ? 2 : 1) * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
+      const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
       const double longest = chain * pace + c.fused;
       load /= cus;
       if (blocks > cus) load *= 0.5 + 0.5 * (double)(int64_t)((blocks + cus - 1) / cus) * cus / blocks;
-      const double time = (load > longest ? load : longest) + extra;
+      double time = load > longest ? load : longest;
+      const double rounds = (double)(int64_t)(blocks / (cus * kShare[kind]) + 1) / blocks;
+      if (alone * rounds > time) time = alone * rounds;
+      time += extra;
       if (time < best) {
         best = time;
         best_kind = kind;

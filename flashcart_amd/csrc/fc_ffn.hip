@@ -314,8 +314,8 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
     FfnJob *fused[] = {&g}, *split[] = {&plain};
     const bool no[] = {false}, yes[] = {true};
     double time, plain_time;
-    p.gate_kind = plan_launch(fused, no, 1, f.form, true, &time);
-    const int kind = plan_launch(split, yes, 1, f.form, false, &plain_time);
+    p.gate_kind = plan_launch(fused, no, 1, f.form, true, false, &time);
+    const int kind = plan_launch(split, yes, 1, f.form, false, false, &plain_time);
     if (plain.splits > 1 && plain_time < time) {
       g = plain;
       p.gate_kind = kind;
@@ -337,7 +337,7 @@ static FfnFwd plan_fwd(Ffn& f, const void* x, const void* w_in, const void* w_ou
     FfnJob* jobs[] = {&o};
     const bool yes[] = {true};
     double time;
-    p.out_kind = plan_launch(jobs, yes, 1, f.form, false, &time);
+    p.out_kind = plan_launch(jobs, yes, 1, f.form, false, false, &time);
   }
   o.partial = (float*)f.take(partial_bytes(o));
   return p;
@@ -413,8 +413,8 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     FfnJob dwo = p.dwo, dh = p.dh;
     dh.finish = EPI_DH;
     FfnJob *fused[] = {&p.dwo, &p.dh}, *split[] = {&dwo, &dh};
-    p.first_kind = plan_launch(fused, split_dwo, 2, f.form, false, &time);
-    const int kind = plan_launch(split, split_both, 2, f.form, false, &plain_time);
+    p.first_kind = plan_launch(fused, split_dwo, 2, f.form, false, false, &time);
+    const int kind = plan_launch(split, split_both, 2, f.form, false, false, &plain_time);
     if (dh.splits > 1 && plain_time + 3.5 < time) {
       p.dwo = dwo;
       p.dh = dh;
@@ -422,7 +422,7 @@ static FfnBwd plan_bwd(Ffn& f, const void* grad, const void* x, const void* w_in
     }
   }
   FfnJob* two[] = {&p.dwi, &p.dx};
-  p.second_kind = plan_launch(two, split_both, 2, f.form, false, &time);
+  p.second_kind = plan_launch(two, split_both, 2, f.form, false, false, &time);
   for (FfnJob* g : {&p.dwo, &p.dh, &p.dwi, &p.dx}) g->partial = (float*)f.take(g->M > 0 ? partial_bytes(*g) : 0);
   return p;
 }

@@ -595,7 +595,7 @@ struct FfnTile {
       // The float32 instructions round after every product: sums of 256 k are kept apart and added (relative error of a
       // sum of 6,000 normal products 1.05e-6 in one chain, 3e-7 so).
       constexpr bool CHUNKS = std::is_same_v<MT, float>;
-      constexpr int EVERY = 256 / (KS * T::STAGES);
+      constexpr int EVERY = CHUNKS ? 256 / (KS * T::STAGES) : 1;
       f32x4v sum[CHUNKS ? T::MF : 1][T::NF];
       int turn = 0;
       auto flush = [&](bool now) {

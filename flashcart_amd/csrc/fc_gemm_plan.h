@@ -9,6 +9,7 @@ namespace fc {
 using TileL = Tile<256, 256, 2, 4, 2>;
 using TileM = Tile<128, 128, 2, 2, 2>;
 using TileS = Tile<64, 64, 2, 2, 4>;
+using TileX = Tile<64, 64, 2, 2, 2>;  // (of the dense layers alone)
 
 inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
 
@@ -33,8 +34,10 @@ inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 inline int64_t blocks_of(const GemmJob& g) { return (int64_t)g.tiles_m * g.tiles_n * g.splits; }
 
+inline int tile_rows(int kind) { return kind == 2 ? 256 : kind == 1 ? 128 : 64; }
+
 inline void set_tiles(GemmJob& g, int kind, bool gate) {
-  const int bm = kind == 2 ? 256 : kind == 1 ? 128 : 64, bn = gate ? bm / 2 : bm;
+  const int bm = tile_rows(kind), bn = gate ? bm / 2 : bm;
   g.tiles_m = cdiv(g.M, bm);
   g.tiles_n = cdiv(g.N, bn);
 }
@@ -47,9 +50,17 @@ inline void set_tiles(GemmJob& g, int kind, bool gate) {
 struct TileCost {
   double step, full, end, fused;  // fused: the end with an epilogue of the block's elementwise steps
 };
-constexpr TileCost kTileCost[3] = {{0.2, 0.26, 0.8, 1.2}, {0.65, 0.55, 2.5, 3.2}, {1.25, 1.5, 9.0, 14.0}};
+// The last is the 64 x 64 tile with two LDS stages: up to five workgroups share a CU, whose loads run one step ahead. It is
+// faster where workgroups are many and their sums short (25,000 x 128 x 128 float32, forward 21.5 -> 20.1 us, dx and dW 27.0
+// -> 24.2; 8,192 x 512 x 512 bf16 forward 17.0 -> 14.6), slower where they are few and long (1 x 4,096 x 10,240 15 -> 31).
+constexpr int kKinds = 4;
+constexpr TileCost kTileCost[kKinds] = {{0.2, 0.26, 0.8, 1.2}, {0.65, 0.55, 2.5, 3.2}, {1.25, 1.5, 9.0, 14.0}, {0.47, 0.25, 0.9, 1.3}};
 // native float32, 32 k a step: bound by the matrix cores
-constexpr TileCost kNativeCost[2] = {{0.5, 0.56, 1.0, 2.2}, {2.05, 1.85, 5.0, 6.0}};
+constexpr TileCost kNativeCost[kKinds] = {{0.5, 0.56, 1.0, 2.2}, {2.05, 1.85, 5.0, 6.0}, {}, {0.6, 0.48, 0.6, 1.6}};
+constexpr int kShare[kKinds] = {2, 2, 1, 5};  // workgroups that a CU runs at once
+// What the first load and the epilogue (plain, of a dense layer) take when nothing hides them: rounds of workgroups with short
+// sums are bound by that (8,192 x 64 x 512 bf16 forward, tiles of 64, 128 and 64 with two stages: 14.5, 13.7, 10.5 us).
+constexpr double kLatency[kKinds][2] = {{2.0, 4.5}, {4.0, 9.0}, {10.0, 18.0}, {2.0, 4.5}};
 
 enum Form { FORM_16, FORM_NATIVE, FORM_PLANES, FORM_8 };
 
@@ -60,9 +71,10 @@ inline int steps_of(int k, Form form) {
 }
 
 // Tile size and splits of the K loops (plain outputs only) of one launch: those of the least time by the costs above, a
-// split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them.
+// split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them. `short_tiles`: the
+// 64 x 64 tile with two stages is one of the choices.
 template <class Job>
-int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, bool gate, double* time_us) {
+int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, bool gate, bool short_tiles, double* time_us) {
   const int cus = device_cu_count();
   for (int q = 0; q < count; ++q) {
     const int k = jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k;
@@ -70,7 +82,8 @@ int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, b
   }
   int best_kind = 0, best_splits[2] = {1, 1};
   double best = 1e30;
-  for (int kind = 0; kind < (form == FORM_NATIVE ? 2 : 3); ++kind) {
+  for (int kind = 0; kind < (short_tiles ? 4 : 3); ++kind) {
+    if (form == FORM_NATIVE && kind == 2) continue;
     const TileCost& c = form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
     double chain = 0;  // the longest sum that may be split
     for (int q = 0; q < count; ++q)
@@ -100,7 +113,7 @@ int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, b
         load += n * (steps[q] * c.full + end) / cus;
       }
       // the longest workgroup, which shares its CU with another one where the device is full (not the largest tile)
-      const double shared = (kind < 2 ? 2 : 1) * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
+      const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
       double longest = 0;
       for (int q = 0; q < count; ++q)
         if (steps[q] * pace + ends[q] > longest) longest = steps[q] * pace + ends[q];
@@ -108,6 +121,14 @@ int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, b
       const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
       if (blocks > cus) load *= form == FORM_NATIVE && blocks <= 2 * cus ? rounds : 0.5 + 0.5 * rounds;
       double time = load > longest ? load : longest;
+      if (short_tiles && blocks > 0) {
+        double alone = 0;
+        for (int q = 0; q < count; ++q)
+          if (jobs[q]->M > 0)
+            alone += (double)jobs[q]->tiles_m * jobs[q]->tiles_n * splits[q] * (steps[q] * c.step + kLatency[kind][!can_split[q]]);
+        alone *= (double)((blocks + cus * kShare[kind] - 1) / (cus * kShare[kind])) / blocks;
+        if (alone > time) time = alone;
+      }
       if (sums > 0) time += sums + 3.5;
       if (time < best) {
         best = time;
