@@ -1,5 +1,5 @@
 """Network layers: radial basis/cutoff, interaction, product, gates, norms, readout; node-wise embedding, feed-forward
-block and dropout (their functions: ``flashcart_amd.nn.functional``)."""
+block, dropout, row norm and dense layers (their functions: ``flashcart_amd.nn.functional``)."""
 
 from flashcart_amd.nn.radial import BesselBasis, ChebyshevBasis, PolynomialCutoff
 from flashcart_amd.nn.layers import (
@@ -13,10 +13,17 @@ from flashcart_amd.nn.layers import (
     ScaleShiftEnergyLayer,
 )
 from flashcart_amd.nn.node_layers import (
+    DenseLayer,
+    ElementDenseLayer,
+    ElementRows,
     EmbeddingLayer,
     GatedFeedForwardLayer,
     NodeNetwork,
+    NormNodeNetwork,
+    QuantizedDenseLayer,
+    QuantizedNodeNetwork,
     ResidualDropoutLayer,
+    RowNormLayer,
 )
 
 __all__ = [
@@ -31,8 +38,15 @@ __all__ = [
     "RescaledSiLULayer",
     "RMSLayerNorm",
     "ScaleShiftEnergyLayer",
+    "DenseLayer",
+    "ElementDenseLayer",
+    "ElementRows",
     "EmbeddingLayer",
     "GatedFeedForwardLayer",
     "NodeNetwork",
+    "NormNodeNetwork",
+    "QuantizedDenseLayer",
+    "QuantizedNodeNetwork",
     "ResidualDropoutLayer",
+    "RowNormLayer",
 ]

@@ -250,3 +250,26 @@ def test_oracle_against_torch():
     v = torch.randn(50, 300, generator=g) * torch.exp(3 * torch.randn(50, 300, generator=g))
     q, scale = O.e4m3_rows(v.double())
     assert torch.equal(q, (v.double() / scale[:, None]).float().to(F8).double())
+
+
+def test_rows_by_element():
+    """Sorted and put back, on the CPU; gradients go the way back; ids outside are in no group."""
+    from flashcart_amd.nn import ElementRows
+    ids = torch.tensor([[2, 0, 1], [-1, 0, 5], [2, 2, 0]])
+    rows = ElementRows(ids, 3)
+    x = torch.randn(3, 3, 4, requires_grad=True)
+    s = rows.sort(x)
+    assert rows.offsets.tolist() == [1, 4, 5, 8]
+    assert torch.equal(ids.reshape(-1)[rows.order], torch.tensor([-1, 0, 0, 0, 1, 2, 2, 2, 5]))
+    assert torch.equal(rows.unsort(s).view_as(x), x)
+    g = torch.randn(9, 4)
+    (gx,) = torch.autograd.grad(s, x, g)
+    assert torch.equal(gx.view(9, 4)[rows.order], g)
+    assert torch.autograd.gradgradcheck(lambda t: rows.sort(t) ** 3, torch.randn(3, 3, 2, dtype=torch.float64, requires_grad=True))
+
+
+def test_layers_refuse_other_activations():
+    from flashcart_amd.nn import DenseLayer, ElementDenseLayer
+    for make in (lambda: DenseLayer(4, 4, "relu"), lambda: ElementDenseLayer(2, 4, 4, "relu")):
+        with pytest.raises(ValueError, match="activation must be None or one of"):
+            make()
