@@ -144,62 +144,67 @@ inline int plan_groups(DenseJob* rows, DenseJob* sums, const Dense& f) {
   const int cus = device_cu_count();
   const double groups = (double)(f.d.groups < f.n ? f.d.groups : f.n), each = f.n / groups;
   const int per = f.form == FORM_NATIVE ? 32 : f.form == FORM_8 ? 128 : 64, planes = f.form == FORM_PLANES ? 6 : 1;
-  int best_kind = 0;
-  int64_t best_unit = 0;
-  double best = 1e30;
   if (rows) rows->steps = steps_of(rows->A.k > rows->B.k ? rows->A.k : rows->B.k, f.form);
-  for (int kind = 0; kind < kKinds; ++kind) {
-    if (f.form == FORM_NATIVE && kind == 2) continue;
-    const TileCost& c = f.form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
-    const int bm = tile_rows(kind);
-    double row_blocks = 0, row_load = 0, row_chain = 0, row_alone = 0;
-    if (rows) {
-      row_blocks = (f.n / (double)bm + 0.5 * groups) * cdiv(rows->N, bm);
-      row_chain = rows->steps;
-      row_load = row_blocks * (rows->steps * c.full + c.fused);
-      row_alone = row_blocks * (rows->steps * c.step + kLatency[kind][!sums]);
-    }
-    for (int64_t unit = (f.n + per - 1) / per * per;;) {
-      double blocks = row_blocks, load = row_load, chain = row_chain, alone = row_alone, extra = 0;
-      if (sums) {
-        const double tiles = (double)cdiv(sums->M, bm) * cdiv(sums->N, bm);
-        const double parts = each > unit ? f.n / (double)unit + 0.5 * groups : groups;
-        const double steps = planes * (each > unit ? (double)unit : each) / per;
-        // (the groups are not even: the longest sum of an undivided group is taken as twice the mean)
-        const double longest = planes * (double)(unit < 2 * each ? unit : 2 * each) / per;
-        blocks += parts * tiles;
-        load += parts * tiles * (steps * c.full + c.end) + (f.d.groups - groups) * tiles * c.end;
-        alone += parts * tiles * (steps * c.step + kLatency[kind][0]);
-        if (longest > chain) chain = longest;
-        if (each * 2 > unit) extra = 8e-6 / 3 * (2.0 * f.n / unit) * sums->M * sums->N + 3.5;
+  const PlanKey key{{cus, -1, (int)f.form, (int)f.n, f.d.groups, rows ? rows->N : 0, rows ? rows->steps : 0, sums ? sums->M : 0,
+                     sums ? sums->N : 0}};
+  const PlanChoice choice = remembered(key, [&]() {
+    int best_kind = 0;
+    int64_t best_unit = 0;
+    double best = 1e30;
+    for (int kind = 0; kind < kKinds; ++kind) {
+      if (f.form == FORM_NATIVE && kind == 2) continue;
+      const TileCost& c = f.form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
+      const int bm = tile_rows(kind);
+      double row_blocks = 0, row_load = 0, row_chain = 0, row_alone = 0;
+      if (rows) {
+        row_blocks = (f.n / (double)bm + 0.5 * groups) * cdiv(rows->N, bm);
+        row_chain = rows->steps;
+        row_load = row_blocks * (rows->steps * c.full + c.fused);
+        row_alone = row_blocks * (rows->steps * c.step + kLatency[kind][!sums]);
       }
-      const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
-      const double longest = chain * pace + c.fused;
-      load /= cus;
-      if (blocks > cus) load *= 0.5 + 0.5 * (double)(int64_t)((blocks + cus - 1) / cus) * cus / blocks;
-      double time = load > longest ? load : longest;
-      const double rounds = (double)(int64_t)(blocks / (cus * kShare[kind]) + 1) / blocks;
-      if (alone * rounds > time) time = alone * rounds;
-      time += extra;
-      if (time < best) {
-        best = time;
-        best_kind = kind;
-        best_unit = unit;
+      for (int64_t unit = (f.n + per - 1) / per * per;;) {
+        double blocks = row_blocks, load = row_load, chain = row_chain, alone = row_alone, extra = 0;
+        if (sums) {
+          const double tiles = (double)cdiv(sums->M, bm) * cdiv(sums->N, bm);
+          const double parts = each > unit ? f.n / (double)unit + 0.5 * groups : groups;
+          const double steps = planes * (each > unit ? (double)unit : each) / per;
+          // (the groups are not even: the longest sum of an undivided group is taken as twice the mean)
+          const double longest = planes * (double)(unit < 2 * each ? unit : 2 * each) / per;
+          blocks += parts * tiles;
+          load += parts * tiles * (steps * c.full + c.end) + (f.d.groups - groups) * tiles * c.end;
+          alone += parts * tiles * (steps * c.step + kLatency[kind][0]);
+          if (longest > chain) chain = longest;
+          if (each * 2 > unit) extra = 8e-6 / 3 * (2.0 * f.n / unit) * sums->M * sums->N + 3.5;
+        }
+        const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
+        const double longest = chain * pace + c.fused;
+        load /= cus;
+        if (blocks > cus) load *= 0.5 + 0.5 * (double)(int64_t)((blocks + cus - 1) / cus) * cus / blocks;
+        double time = load > longest ? load : longest;
+        const double rounds = (double)(int64_t)(blocks / (cus * kShare[kind]) + 1) / blocks;
+        if (alone * rounds > time) time = alone * rounds;
+        time += extra;
+        if (time < best) {
+          best = time;
+          best_kind = kind;
+          best_unit = unit;
+        }
+        if (!sums || unit <= 4 * per) break;
+        unit = (unit / 2 + per - 1) / per * per;
       }
-      if (!sums || unit <= 4 * per) break;
-      unit = (unit / 2 + per - 1) / per * per;
     }
-  }
+    return PlanChoice{best_kind, {best_unit, 0}, best};
+  });
   if (rows) {
-    set_tiles(*rows, best_kind, false);
+    set_tiles(*rows, choice.kind, false);
     rows->splits = 1;
   }
   if (sums) {
-    set_tiles(*sums, best_kind, false);
+    set_tiles(*sums, choice.kind, false);
     sums->splits = 1;
-    sums->unit = (int32_t)best_unit;
+    sums->unit = (int32_t)choice.split[0];
   }
-  return best_kind;
+  return choice.kind;
 }
 // Workgroups that any offsets can need.
 inline int64_t group_blocks(const DenseJob& g, int bm) {

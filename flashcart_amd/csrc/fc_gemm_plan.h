@@ -70,6 +70,32 @@ inline int steps_of(int k, Form form) {
   return (form == FORM_PLANES ? 6 : 1) * cdiv(k, per);
 }
 
+// The answers to the last questions, by sizes alone: a layer asks the same ones call after call, twice in each (for the
+// workspace's size, and for the launch), and an answer takes 1 to 3 us of the host's time.
+struct PlanKey {
+  int32_t v[12];
+};
+struct PlanChoice {
+  int kind;
+  int64_t split[2];
+  double time;
+};
+template <class F>
+PlanChoice remembered(const PlanKey& key, F&& choose) {
+  constexpr int SLOTS = 64;
+  struct Slot {
+    PlanKey key;
+    PlanChoice choice;
+    bool used;
+  };
+  static thread_local Slot slots[SLOTS];
+  uint32_t h = 2166136261u;
+  for (int32_t v : key.v) h = (h ^ (uint32_t)v) * 16777619u;
+  Slot& s = slots[(h ^ h >> 15) % SLOTS];
+  if (!s.used || memcmp(&s.key, &key, sizeof(key)) != 0) s = Slot{key, choose(), true};
+  return s.choice;
+}
+
 // Tile size and splits of the K loops (plain outputs only) of one launch: those of the least time by the costs above, a
 // split K loop paying for its partial sums, written and read at 3 TB/s, and for the launch that adds them. `short_tiles`: the
 // 64 x 64 tile with two stages is one of the choices.
@@ -80,70 +106,79 @@ int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, b
     const int k = jobs[q]->A.k > jobs[q]->B.k ? jobs[q]->A.k : jobs[q]->B.k;
     jobs[q]->steps = steps_of(k, form);
   }
-  int best_kind = 0, best_splits[2] = {1, 1};
-  double best = 1e30;
-  for (int kind = 0; kind < (short_tiles ? 4 : 3); ++kind) {
-    if (form == FORM_NATIVE && kind == 2) continue;
-    const TileCost& c = form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
-    double chain = 0;  // the longest sum that may be split
-    for (int q = 0; q < count; ++q)
-      if (jobs[q]->M > 0 && can_split[q] && jobs[q]->steps * c.step > chain) chain = jobs[q]->steps * c.step;
-    double most = chain + 1;  // of a workgroup's steps
-    do {
-      double load = 0, sums = 0, steps[2] = {0, 0}, ends[2] = {0, 0};
-      int64_t blocks = 0;
-      int splits[2] = {1, 1};
-      for (int q = 0; q < count; ++q) {
-        GemmJob& g = *jobs[q];
-        if (g.M == 0) continue;
-        set_tiles(g, kind, gate);
-        double end = (can_split[q] ? c.end : c.fused) * (form == FORM_PLANES ? 1.5 : 1);
-        if (can_split[q] && g.steps * c.step > most) {
-          splits[q] = (int)(g.steps * c.step / most) + 1;
-          if (splits[q] > g.steps / 4) splits[q] = g.steps / 4 > 1 ? g.steps / 4 : 1;
-        }
-        if (splits[q] > 1) {
-          end *= 1.5;
-          sums += 8e-6 / 3 * splits[q] * g.M * g.N;
-        }
-        const int64_t n = (int64_t)g.tiles_m * g.tiles_n * splits[q];
-        steps[q] = (double)g.steps / splits[q];
-        ends[q] = end;
-        blocks += n;
-        load += n * (steps[q] * c.full + end) / cus;
-      }
-      // the longest workgroup, which shares its CU with another one where the device is full (not the largest tile)
-      const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
-      double longest = 0;
-      for (int q = 0; q < count; ++q)
-        if (steps[q] * pace + ends[q] > longest) longest = steps[q] * pace + ends[q];
-      // whole rounds of workgroups where they are few and the matrix cores bound them, something between otherwise
-      const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
-      if (blocks > cus) load *= form == FORM_NATIVE && blocks <= 2 * cus ? rounds : 0.5 + 0.5 * rounds;
-      double time = load > longest ? load : longest;
-      if (short_tiles && blocks > 0) {
-        double alone = 0;
-        for (int q = 0; q < count; ++q)
-          if (jobs[q]->M > 0)
-            alone += (double)jobs[q]->tiles_m * jobs[q]->tiles_n * splits[q] * (steps[q] * c.step + kLatency[kind][!can_split[q]]);
-        alone *= (double)((blocks + cus * kShare[kind] - 1) / (cus * kShare[kind])) / blocks;
-        if (alone > time) time = alone;
-      }
-      if (sums > 0) time += sums + 3.5;
-      if (time < best) {
-        best = time;
-        best_kind = kind;
-        for (int q = 0; q < count; ++q) best_splits[q] = splits[q];
-      }
-      most /= 2;
-    } while (most > 2);
-  }
+  PlanKey key{{cus, count, (int)form, gate, short_tiles}};
   for (int q = 0; q < count; ++q) {
-    set_tiles(*jobs[q], best_kind, gate);
-    jobs[q]->splits = best_splits[q];
+    key.v[5 + 3 * q] = jobs[q]->M;
+    key.v[6 + 3 * q] = jobs[q]->N;
+    key.v[7 + 3 * q] = 2 * jobs[q]->steps + can_split[q];
   }
-  *time_us = best;
-  return best_kind;
+  const PlanChoice choice = remembered(key, [&]() {
+    int best_kind = 0, best_splits[2] = {1, 1};
+    double best = 1e30;
+    for (int kind = 0; kind < (short_tiles ? 4 : 3); ++kind) {
+      if (form == FORM_NATIVE && kind == 2) continue;
+      const TileCost& c = form == FORM_NATIVE ? kNativeCost[kind] : kTileCost[kind];
+      double chain = 0;  // the longest sum that may be split
+      for (int q = 0; q < count; ++q)
+        if (jobs[q]->M > 0 && can_split[q] && jobs[q]->steps * c.step > chain) chain = jobs[q]->steps * c.step;
+      double most = chain + 1;  // of a workgroup's steps
+      do {
+        double load = 0, sums = 0, steps[2] = {0, 0}, ends[2] = {0, 0};
+        int64_t blocks = 0;
+        int splits[2] = {1, 1};
+        for (int q = 0; q < count; ++q) {
+          GemmJob& g = *jobs[q];
+          if (g.M == 0) continue;
+          set_tiles(g, kind, gate);
+          double end = (can_split[q] ? c.end : c.fused) * (form == FORM_PLANES ? 1.5 : 1);
+          if (can_split[q] && g.steps * c.step > most) {
+            splits[q] = (int)(g.steps * c.step / most) + 1;
+            if (splits[q] > g.steps / 4) splits[q] = g.steps / 4 > 1 ? g.steps / 4 : 1;
+          }
+          if (splits[q] > 1) {
+            end *= 1.5;
+            sums += 8e-6 / 3 * splits[q] * g.M * g.N;
+          }
+          const int64_t n = (int64_t)g.tiles_m * g.tiles_n * splits[q];
+          steps[q] = (double)g.steps / splits[q];
+          ends[q] = end;
+          blocks += n;
+          load += n * (steps[q] * c.full + end) / cus;
+        }
+        // the longest workgroup, which shares its CU with another one where the device is full (not the largest tile)
+        const double shared = kShare[kind] * c.full, pace = blocks > cus && shared > c.step ? shared : c.step;
+        double longest = 0;
+        for (int q = 0; q < count; ++q)
+          if (steps[q] * pace + ends[q] > longest) longest = steps[q] * pace + ends[q];
+        // whole rounds of workgroups where they are few and the matrix cores bound them, something between otherwise
+        const double rounds = blocks > 0 ? (double)((blocks + cus - 1) / cus) * cus / blocks : 1;
+        if (blocks > cus) load *= form == FORM_NATIVE && blocks <= 2 * cus ? rounds : 0.5 + 0.5 * rounds;
+        double time = load > longest ? load : longest;
+        if (short_tiles && blocks > 0) {
+          double alone = 0;
+          for (int q = 0; q < count; ++q)
+            if (jobs[q]->M > 0)
+              alone += (double)jobs[q]->tiles_m * jobs[q]->tiles_n * splits[q] * (steps[q] * c.step + kLatency[kind][!can_split[q]]);
+          alone *= (double)((blocks + cus * kShare[kind] - 1) / (cus * kShare[kind])) / blocks;
+          if (alone > time) time = alone;
+        }
+        if (sums > 0) time += sums + 3.5;
+        if (time < best) {
+          best = time;
+          best_kind = kind;
+          for (int q = 0; q < count; ++q) best_splits[q] = splits[q];
+        }
+        most /= 2;
+      } while (most > 2);
+    }
+    return PlanChoice{best_kind, {best_splits[0], best_splits[1]}, best};
+  });
+  for (int q = 0; q < count; ++q) {
+    set_tiles(*jobs[q], choice.kind, gate);
+    jobs[q]->splits = (int)choice.split[q];
+  }
+  *time_us = choice.time;
+  return choice.kind;
 }
 inline int64_t partial_bytes(const GemmJob& g) { return g.splits > 1 ? 4ll * g.splits * g.M * g.N : 0; }
 

@@ -16,7 +16,20 @@ const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nu
 Tensor take_optional(const char* name, const optional<Tensor>& t, at::ScalarType type, const Tensor& first) {
   return t && t->defined() ? take(name, *t, type, first) : Tensor();
 }
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::empty(sizes, like.options().dtype(type));
+}
 Tensor none_like(const Tensor& t) { return at::empty({0}, t.options()); }
+struct Workspace {
+  Tensor memory;
+  void* at = nullptr;
+  Workspace(const Tensor& like, int64_t size, const char* what) {
+    if (size < 0) check(-size, what);
+    if (size == 0) return;
+    memory = fresh({size}, at::kByte, like);
+    at = memory.mutable_data_ptr();
+  }
+};
 
 // ---- root-mean-square norm with the residual's addition ----
 
@@ -49,7 +62,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_add(const Tensor& x, const optional<
   const c10::DeviceGuard guard(r.x.device());
   Tensor y = at::empty(r.x.sizes(), r.x.options());
   Tensor total = r.residual.defined() ? at::empty(r.x.sizes(), r.x.options()) : none_like(r.x);
-  Tensor rstd = at::empty({save ? r.n : 0}, r.x.options().dtype(at::kFloat));
+  Tensor rstd = fresh({save ? r.n : 0}, at::kFloat, r.x);
   check(api.row_norm_fwd(r.code, r.n, r.width, r.x.const_data_ptr(), data(r.residual), data(r.weight), (float)eps,
                          r.residual.defined() ? total.mutable_data_ptr() : nullptr, y.mutable_data_ptr(),
                          save ? rstd.mutable_data_ptr<float>() : nullptr, stream_of(r.x)),
@@ -73,10 +86,10 @@ std::tuple<Tensor, Tensor> rms_norm_add_bwd(const Tensor& grad_, const optional<
                            : at::empty({r.width}, r.x.options());
   if (r.n == 0) return {dx, dw};
   const int64_t size = api.row_norm_bwd_workspace(r.code, r.n, r.width, need_weight);
-  Tensor ws = bytes(r.x, size, "fc_row_norm_bwd_workspace");
+  const Workspace ws(r.x, size, "fc_row_norm_bwd_workspace");
   check(api.row_norm_bwd(r.code, r.n, r.width, grad.const_data_ptr(), data(r.residual), r.x.const_data_ptr(),
                          data(r.weight), rstd.const_data_ptr<float>(), need_x ? dx.mutable_data_ptr() : nullptr,
-                         need_weight ? dw.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), size, stream_of(r.x)),
+                         need_weight ? dw.mutable_data_ptr() : nullptr, ws.at, size, stream_of(r.x)),
         "fc_row_norm_bwd");
   return {dx, dw};
 }
@@ -165,8 +178,8 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_add_quantized(const Tensor& x, const
   const c10::DeviceGuard guard(r.x.device());
   auto shape = r.x.sizes().vec();
   shape.pop_back();
-  Tensor q = at::empty(r.x.sizes(), r.x.options().dtype(at::kFloat8_e4m3fn));
-  Tensor scale = at::empty(shape, r.x.options().dtype(at::kFloat));
+  Tensor q = fresh(r.x.sizes(), at::kFloat8_e4m3fn, r.x);
+  Tensor scale = fresh(shape, at::kFloat, r.x);
   Tensor total = r.residual.defined() ? at::empty(r.x.sizes(), r.x.options()) : none_like(r.x);
   check(api.row_norm_quantize(r.code, 1, r.n, r.width, r.x.const_data_ptr(), data(r.residual), data(r.weight), (float)eps,
                               r.residual.defined() ? total.mutable_data_ptr() : nullptr, q.mutable_data_ptr(),
@@ -186,8 +199,8 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   const c10::DeviceGuard guard(r.x.device());
   auto shape = r.x.sizes().vec();
   shape.pop_back();
-  Tensor q = at::empty(r.x.sizes(), r.x.options().dtype(at::kFloat8_e4m3fn));
-  Tensor scale = at::empty(shape, r.x.options().dtype(at::kFloat));
+  Tensor q = fresh(r.x.sizes(), at::kFloat8_e4m3fn, r.x);
+  Tensor scale = fresh(shape, at::kFloat, r.x);
   check(api.row_norm_quantize(r.code, 0, r.n, r.width, r.x.const_data_ptr(), nullptr, nullptr, 0.f, nullptr,
                               q.mutable_data_ptr(), scale.mutable_data_ptr<float>(), stream_of(r.x)),
         "fc_row_norm_quantize");
@@ -272,11 +285,13 @@ std::tuple<Tensor, Tensor> node_dense(const Tensor& x_, const Tensor& weight_, c
   const int64_t n = x.numel() / d.in;
   d.aligned = aligned({&x, &weight});
   const int64_t size = api.node_dense_fwd_workspace(&d, n);
-  Tensor y = at::empty(shape, x.options()), ws = bytes(x, size, "fc_node_dense_fwd_workspace");
-  Tensor saved = bytes(x, save ? api.node_dense_saved(&d, n) : 0, "fc_node_dense_saved");
+  const int64_t kept = save ? api.node_dense_saved(&d, n) : 0;
+  if (kept < 0) check(-kept, "fc_node_dense_saved");
+  const Workspace ws(x, size, "fc_node_dense_fwd_workspace");
+  Tensor y = at::empty(shape, x.options()), saved = fresh({kept}, at::kByte, x);
   check(api.node_dense_fwd(&d, n, x.const_data_ptr(), weight.const_data_ptr(), data(bias), data(residual),
                            (const int64_t*)data(offsets), y.mutable_data_ptr(),
-                           saved.numel() ? saved.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), size, stream_of(x)),
+                           kept ? saved.mutable_data_ptr() : nullptr, ws.at, size, stream_of(x)),
         "fc_node_dense_fwd");
   return {y, saved};
 }
@@ -309,11 +324,11 @@ std::tuple<Tensor, Tensor, Tensor> node_dense_bwd(const Tensor& grad_, const Ten
   Tensor gb = result(groups ? at::IntArrayRef({d.groups, d.out}) : at::IntArrayRef({d.out}), need_bias);
   if (n > 0) {
     const int64_t size = api.node_dense_bwd_workspace(&d, n, need_x, need_weight, need_bias);
-    Tensor ws = bytes(x, size, "fc_node_dense_bwd_workspace");
+    const Workspace ws(x, size, "fc_node_dense_bwd_workspace");
     check(api.node_dense_bwd(&d, n, grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(),
                              kept ? saved.const_data_ptr() : nullptr, (const int64_t*)data(offsets),
                              need_x ? gx.mutable_data_ptr() : nullptr, need_weight ? gw.mutable_data_ptr() : nullptr,
-                             need_bias ? gb.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), size, stream_of(x)),
+                             need_bias ? gb.mutable_data_ptr() : nullptr, ws.at, size, stream_of(x)),
           "fc_node_dense_bwd");
   }
   return {gx, gw, gb};
@@ -414,10 +429,11 @@ Tensor quantized_dense(const Tensor& x_, const Tensor& x_scale_, const Tensor& w
   const int64_t n = x.numel() / d.in;
   d.aligned = aligned({&x, &weight});
   const int64_t size = api.quantized_dense_workspace(&d, n);
-  Tensor y = at::empty(shape, x.options().dtype(dtype)), ws = bytes(x, size, "fc_quantized_dense_workspace");
+  const Workspace ws(x, size, "fc_quantized_dense_workspace");
+  Tensor y = fresh(shape, dtype, x);
   check(api.quantized_dense(&d, n, x.const_data_ptr(), x_scale.const_data_ptr<float>(), weight.const_data_ptr(),
                             weight_scale.const_data_ptr<float>(), data(bias), data(residual), y.mutable_data_ptr(),
-                            ws.mutable_data_ptr(), size, stream_of(x)),
+                            ws.at, size, stream_of(x)),
         "fc_quantized_dense");
   return y;
 }
