@@ -76,6 +76,7 @@ struct DenseJob : GemmJob {
   float act_scale;
   const int64_t* offsets;        // (groups + 1)
   int32_t groups;
+  int32_t halves;                // tiles at the end that are taken as two halves of their columns
   int32_t unit;                  // > 0: sums over a group's rows, in parts of so many
   int64_t rows, b_stride, out_stride;  // rows of the call; elements from one group's B, and output, to the next one's
 

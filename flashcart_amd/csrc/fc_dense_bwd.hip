@@ -1,5 +1,7 @@
 // Dense layers backward (fc_dense.h): dz and the bias' gradient in one pass over the incoming gradient, then the products
 // for dx and dW in one launch, the one with the longer sums first.
+#include <algorithm>
+
 #include "fc_dense_plan.h"
 
 namespace fc {
@@ -270,7 +272,9 @@ static int launch_products(const DenseBwd& p, hipStream_t s) {
   const int64_t blocks2 = g2.M == 0 ? 0 : GROUPS ? group_blocks(g2, bm) : blocks_of(g2), blocks = blocks1 + blocks2;
   if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
   const dim3 grid((unsigned)blocks);
-  const int steps1 = g1.M == 0 ? 0 : GROUPS ? g1.unit / 64 : g1.steps / g1.splits;
+  // (with groups: of one of twice the mean size)
+  const int64_t most = GROUPS && g1.M > 0 ? std::min<int64_t>(g1.unit, 2 * g1.rows / g1.groups) : 0;
+  const int steps1 = g1.M == 0 ? 0 : GROUPS ? (int)most / 64 : g1.steps / g1.splits;
   const bool swapped = blocks2 > 0 && (blocks1 == 0 || g2.steps / g2.splits > steps1);
   const int front = (int)(swapped ? blocks2 : blocks1);
   if constexpr (!std::is_same_v<MT, float>) {

@@ -154,8 +154,8 @@ struct Loader {
           if (second) first += up;
         }
         base[j] = o.p + ES * first * o.ld;
-        row = min(row, o.rows - 1 - r0);
-        off[j] = (uint32_t)row * (uint32_t)(o.ld * ES) + 16 * ((lane & 7) ^ (lane >> 3));
+        // (rows past the last are zeros that no memory is read for: a tile of few rows costs their bytes alone)
+        off[j] = row < o.rows - r0 ? (uint32_t)row * (uint32_t)(o.ld * ES) + 16 * ((lane & 7) ^ (lane >> 3)) : kOutOfRange;
         kl[0] = CE * ((lane & 7) ^ (lane >> 3));
       } else {
         constexpr int CPR = R / CE, CPP = ES == 4 ? 4 : 2;  // chunks of a row, and of what is permuted as one
@@ -426,9 +426,15 @@ struct FfnTile {
   template <class Job>
   __device__ static __forceinline__ void run(const Job& g, int block, lds_char* lds0, lds_char* lds1, lds_char* lds2,
                                          lds_char* lds3) {
+    run(g, block, g.tiles_m * g.tiles_n, lds0, lds1, lds2, lds3);
+  }
+
+  // The first `tiles` tiles of the job.
+  template <class Job>
+  __device__ static __forceinline__ void run(const Job& g, int block, int tiles, lds_char* lds0, lds_char* lds1,
+                                         lds_char* lds2, lds_char* lds3) {
     // block -> split, tile. Consecutive blocks go to the 8 XCDs in turn: each XCD takes a run of tiles, in groups of 8
     // tile rows, whose operands its L2 then serves.
-    const int tiles = g.tiles_m * g.tiles_n;
     int split = 0, tile = block;
     if (g.splits > 1) {
       split = block / tiles;
@@ -520,12 +526,13 @@ struct FfnTile {
       // everyone has read in one phase is loaded again from the next phase on, for the step after next: a load has four
       // turns (32 products each) to arrive. It is waited for, by all waves, one turn before it is read. (16,384 x 5,632 by
       // 2,048 columns: 306 us, 1,235 TFLOP/s; with four phases of 16 products 334, without turns 1,377.)
+      constexpr int LOADS = la.SEGS + lb.SEGS, ALL_B = (1 << lb.SEGS) - 1, HALF_B = (1 << lb.SEGS / 2) - 1;
       constexpr int MH = ATR ? T::MF : T::MF / 2, KH = ATR ? 1 : 2;
       constexpr std::integral_constant<int, ATR ? 3 : 5> a1{};
       constexpr std::integral_constant<int, ATR ? 12 : 10> a2{};
-      constexpr std::integral_constant<int, ATR ? 3 : 15> b1{};
-      constexpr std::integral_constant<int, ATR ? 12 : 0> b2{};
-      static_assert(T::MF == 8 && T::NF == 4, "segments of the halves");
+      constexpr std::integral_constant<int, ATR ? HALF_B : ALL_B> b1{};
+      constexpr std::integral_constant<int, ATR ? ALL_B - HALF_B : 0> b2{};
+      static_assert(T::MF == 8 && (T::NF == 4 || T::NF == 2), "segments of the halves");
       static_assert(!ATR || BTR, "halves of k are separate segments in the (K, rows) form alone");
       s16x8 a[KH][MH], c[KH][T::NF];
       Cursor first = cursor_at(s0), second = first;  // of the segments that phase 1 reads, and phase 2
@@ -534,9 +541,9 @@ struct FfnTile {
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
       };
-      // 8 loads are younger than the oldest that the next turn reads
+      // the loads of a step are younger than the oldest that the next turn reads
       auto read_done = [&]() {
-        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
         turn();
         __builtin_amdgcn_s_setprio(1);
       };
@@ -581,7 +588,7 @@ struct FfnTile {
       fetch(first, lds0, a1, b1);
       fetch(second, lds0, a2, b2);
       fetch(first, lds1, a1, b1);
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
       turn();
       if (wave >= 4) turn();
 #pragma unroll 1
@@ -657,7 +664,7 @@ struct FfnTile {
           constexpr int PRODUCTS = (EIGHT ? 1 : 2) * T::MF * T::NF * (std::is_same_v<MT, float> ? 4 : 1);
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / 8, 0);  // matrix
+            if constexpr (PRODUCTS >= 8) __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / 8, 0);  // matrix
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);             // LDS reads
             __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);             // loads
           }

@@ -7,8 +7,10 @@ namespace fc {
 
 // (native float32 has no 256 x 256 tile: planes take over before it would fill the device)
 using TileL = Tile<256, 256, 2, 4, 2>;
+using TileH = Tile<256, 128, 2, 4, 2>;  // half a TileL, in its LDS (of the dense layers alone)
 using TileM = Tile<128, 128, 2, 2, 2>;
 using TileS = Tile<64, 64, 2, 2, 4>;
+using TileR = Tile<32, 64, 2, 2, 4>;  // (of groups of few rows alone)
 using TileX = Tile<64, 64, 2, 2, 2>;  // (of the dense layers alone)
 
 inline int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
@@ -34,7 +36,7 @@ inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 inline int64_t blocks_of(const GemmJob& g) { return (int64_t)g.tiles_m * g.tiles_n * g.splits; }
 
-inline int tile_rows(int kind) { return kind == 2 ? 256 : kind == 1 ? 128 : 64; }
+inline int tile_rows(int kind) { return kind == 2 ? 256 : kind == 1 ? 128 : kind == 4 ? 32 : 64; }
 
 inline void set_tiles(GemmJob& g, int kind, bool gate) {
   const int bm = tile_rows(kind), bn = gate ? bm / 2 : bm;
