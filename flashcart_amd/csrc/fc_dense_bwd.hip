@@ -82,42 +82,62 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   if (c < a.op) a.sums[(int64_t)chunk * a.op + c] = s;
 }
 
-// The bias' gradient: 32 columns of a group, 32 lanes each; the chunks of a group are added in a fixed order.
-template <class T>
-__global__ void __launch_bounds__(1024) dense_db_kernel(DzArgs a, void* out, int64_t chunks) {
-  __shared__ float part[32][33];
-  const int blocks = (a.out + 31) / 32, e = blockIdx.x / blocks, cl = threadIdx.x % 32, grp = threadIdx.x / 32;
-  const int c = (blockIdx.x - e * blocks) * 32 + cl;
-  int64_t c0 = 0, c1 = chunks;
+// The bias' gradient, from the sums of 32 rows each: a workgroup of NT threads takes 32 columns of a group, whose chunks it
+// adds in a fixed order.
+struct DbArgs {
+  const float* sums;  // (chunks, op)
+  void* out;          // (groups, out), or null
+  int64_t chunks, rows;
+  const int64_t* offsets;
+  int32_t groups, n_out, op;
+};
+template <class T, int NT>
+__device__ __forceinline__ void db_block(const DbArgs& a, int block, float (&part)[NT / 32][33]) {
+  const int blocks = (a.n_out + 31) / 32, e = block / blocks, cl = threadIdx.x % 32, grp = threadIdx.x / 32;
+  const int c = (block - e * blocks) * 32 + cl;
+  int64_t c0 = 0, c1 = a.chunks;
   if (a.offsets) {
     const GroupUnit u = find_unit<true>(a.offsets, a.groups, a.rows, kDzRows, 0, e, false);
     c0 = u.before;
     c1 = c0 + (u.rows + kDzRows - 1) / kDzRows;
   }
   float s = 0.f;
-  if (c < a.out) {
+  if (c < a.n_out) {
 #pragma unroll 8
-    for (int64_t k = c0 + grp; k < c1; k += 32) s += a.sums[k * a.op + c];
+    for (int64_t k = c0 + grp; k < c1; k += NT / 32) s += a.sums[k * a.op + c];
   }
   part[grp][cl] = s;
   __syncthreads();
-  if (grp > 0 || c >= a.out) return;
+  if (grp > 0 || c >= a.n_out) return;
 #pragma unroll
-  for (int k = 1; k < 32; ++k) s += part[k][cl];
-  ((T*)out)[(int64_t)e * a.out + c] = from_f32<T>(s);
+  for (int k = 1; k < NT / 32; ++k) s += part[k][cl];
+  ((T*)a.out)[(int64_t)e * a.n_out + c] = from_f32<T>(s);
+}
+// (where neither dx nor dW is asked for; with them it is part of their launch)
+template <class T>
+__global__ void __launch_bounds__(1024) dense_db_kernel(DbArgs a) {
+  __shared__ float part[32][33];
+  db_block<T, 1024>(a, blockIdx.x, part);
 }
 
-// ---- the products: g1 forms dW (sums over rows), g2 dx. The first `front` workgroups take the one with the longer sums ----
+// ---- the products: g1 forms dW (sums over rows), g2 dx. The first `front` workgroups take the one with the longer sums; the
+// workgroups from `products` on the bias' gradient ----
 template <class T, class MT, bool F32, bool GROUPS>
-__global__ void __launch_bounds__(T::NT, 2) dense_bwd_kernel(DenseJob g1, DenseJob g2, int front, bool swapped) {
+__global__ void __launch_bounds__(T::NT, 2) dense_bwd_kernel(DenseJob g1, DenseJob g2, DbArgs db, int front, int products,
+                                                                bool swapped) {
   __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
   __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
   lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
   lds_char* const l3 = (lds_char*)lds3;
+  if ((int)blockIdx.x >= products) {
+    static_assert(T::STAGE >= T::NT / 32 * 33 * 4, "sums in a stage");
+    db_block<std::conditional_t<F32, float, MT>, T::NT>(db, blockIdx.x - products, *(float (*)[T::NT / 32][33])lds0);
+    return;
+  }
   const bool in_front = (int)blockIdx.x < front;
-  const int block = in_front ? blockIdx.x : blockIdx.x - front, blocks = in_front ? front : gridDim.x - front;
+  const int block = in_front ? blockIdx.x : blockIdx.x - front, blocks = in_front ? front : products - front;
   if (in_front != swapped) {
     if constexpr (GROUPS) GroupTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, blocks, l0, l1, l2, l3);
     else FfnTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, l0, l1, l2, l3);
@@ -265,13 +285,15 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
 }
 
 template <class MT, bool F32, bool GROUPS>
-static int launch_products(const DenseBwd& p, hipStream_t s) {
+static int launch_products(const DenseBwd& p, const DbArgs& db, hipStream_t s) {
   const DenseJob &g1 = p.dw, &g2 = p.dx;
   const int bm = tile_rows(p.kind);
   const int64_t blocks1 = g1.M == 0 ? 0 : GROUPS ? group_blocks(g1, bm) : blocks_of(g1);
   const int64_t blocks2 = g2.M == 0 ? 0 : GROUPS ? group_blocks(g2, bm) : blocks_of(g2), blocks = blocks1 + blocks2;
-  if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks);
+  const int64_t db_blocks = db.out ? (int64_t)(GROUPS ? db.groups : 1) * cdiv(db.n_out, 32) : 0;
+  if (!grid_fits(blocks + db_blocks, 512)) return FC_ERR_SHAPE;
+  const dim3 grid((unsigned)(blocks + db_blocks));
+  const int products = (int)blocks;
   // (with groups: of one of twice the mean size)
   const int64_t most = GROUPS && g1.M > 0 ? std::min<int64_t>(g1.unit, 2 * g1.rows / g1.groups) : 0;
   const int steps1 = g1.M == 0 ? 0 : GROUPS ? (int)most / 64 : g1.steps / g1.splits;
@@ -279,14 +301,18 @@ static int launch_products(const DenseBwd& p, hipStream_t s) {
   const int front = (int)(swapped ? blocks2 : blocks1);
   if constexpr (!std::is_same_v<MT, float>) {
     if (p.kind == 2)
-      hipLaunchKernelGGL((dense_bwd_kernel<TileL, MT, F32, GROUPS>), grid, dim3(TileL::NT), 0, s, g1, g2, front, swapped);
+      hipLaunchKernelGGL((dense_bwd_kernel<TileL, MT, F32, GROUPS>), grid, dim3(TileL::NT), 0, s, g1, g2, db, front,
+                       products, swapped);
   }
   if (p.kind == 1)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, front, swapped);
+    hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, db, front,
+                       products, swapped);
   else if (p.kind == 3)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileX, MT, F32, GROUPS>), grid, dim3(TileX::NT), 0, s, g1, g2, front, swapped);
+    hipLaunchKernelGGL((dense_bwd_kernel<TileX, MT, F32, GROUPS>), grid, dim3(TileX::NT), 0, s, g1, g2, db, front,
+                       products, swapped);
   else if (p.kind == 0)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, front, swapped);
+    hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, db, front,
+                       products, swapped);
   FC_LAUNCH_CHECK();
   // the sums of split sums
   BwdSums a{};
@@ -355,13 +381,14 @@ extern "C" int fc_node_dense_bwd(const fc_dense_desc* d, int64_t n, const void* 
       hipLaunchKernelGGL((dense_dz_kernel<T, MT>), dim3((unsigned)blocks), dim3(256), 0, s, p.dz);
       FC_LAUNCH_CHECK();
     }
-    if (gb) {
+    const DbArgs db{p.dz.sums, gb, p.chunks, f.n, p.dz.offsets, f.d.groups, (int32_t)f.out, (int32_t)f.op};
+    if (!gx && !gw) {
       const int64_t blocks = (int64_t)(f.d.groups > 0 ? f.d.groups : 1) * cdiv(f.out, 32);
       if (!grid_fits(blocks, 1024)) return FC_ERR_SHAPE;
-      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, p.dz, gb, p.chunks);
+      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, db);
       FC_LAUNCH_CHECK();
+      return FC_OK;
     }
-    if (!gx && !gw) return FC_OK;
-    return d->groups > 0 ? launch_products<MT, F32, true>(p, s) : launch_products<MT, F32, false>(p, s);
+    return d->groups > 0 ? launch_products<MT, F32, true>(p, db, s) : launch_products<MT, F32, false>(p, db, s);
   });
 }

@@ -290,6 +290,7 @@ struct RowNormBwd {
   const float* rstd;
   void* dx;     // or null
   float* sums;  // (blocks, width), or null
+  void* dw;     // one workgroup writes it itself
   int64_t n, width;
 };
 
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(256) row_norm_bwd_kernel(RowNormBwd g) {
   }
   if (!g.sums) return;
   float* const out = g.sums + (int64_t)blockIdx.x * g.width;
+  const bool alone = gridDim.x == 1;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int64_t c = ((int64_t)k * L + lane) * V;
@@ -370,8 +372,11 @@ __global__ void __launch_bounds__(256) row_norm_bwd_kernel(RowNormBwd g) {
         for (int i = 0; i < V; ++i) dw[k][i] += part[(q * L + lane) * V + i];
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < g.width) out[c + i] = dw[k][i];
+    for (int i = 0; i < V; ++i) {
+      if (c + i >= g.width) continue;
+      if (alone) ((T*)g.dw)[c + i] = from_f32<T>(dw[k][i]);
+      else out[c + i] = dw[k][i];
+    }
   }
 }
 
@@ -533,12 +538,12 @@ extern "C" int fc_row_norm_bwd(int32_t dtype, int64_t n, int64_t width, const vo
   hipStream_t s = (hipStream_t)stream;
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const RowNormBwd g{grad, grad_total, total, weight, rstd, grad_x, grad_weight ? (float*)ws : nullptr, n, width};
+    const RowNormBwd g{grad, grad_total, total, weight, rstd, grad_x, grad_weight ? (float*)ws : nullptr, grad_weight, n, width};
     int64_t blocks = 0;
     const bool fits = with_row<kChunk<T>, 4>(width, 2, [&](auto l, auto k, auto even) {
       constexpr int L = decltype(l)::value, K = decltype(k)::value;
       blocks = (n + 256 / L - 1) / (256 / L);
-      if (grad_weight) blocks = bwd_blocks(blocks);
+      if (grad_weight) blocks = blocks <= 4 ? 1 : bwd_blocks(blocks);  // (few rows: no second launch)
       else if (blocks > kLaunchBlocks) blocks = kLaunchBlocks;
       hipLaunchKernelGGL((row_norm_bwd_kernel<T, L, K, decltype(even)::value>), dim3((unsigned)blocks), dim3(256), 0, s, g);
     });
@@ -547,7 +552,7 @@ extern "C" int fc_row_norm_bwd(int32_t dtype, int64_t n, int64_t width, const vo
       hipLaunchKernelGGL((row_norm_wide_bwd_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, g);
     }
     FC_LAUNCH_CHECK();
-    if (!grad_weight) return FC_OK;
+    if (!grad_weight || (fits && blocks == 1)) return FC_OK;
     hipLaunchKernelGGL((row_norm_dw_kernel<T>), dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, s, (const float*)ws,
                        blocks, width, (T*)grad_weight);
     FC_LAUNCH_CHECK();
