@@ -55,6 +55,15 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
   memcpy(p, &x, sizeof(x));
 }
 
+// 16 bytes of 16-bit elements, stored for a reader that comes much later.
+template <class T>
+__device__ __forceinline__ void stream_pack(T* p, const Pack<T, 8>& x) {
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+  words w;
+  memcpy(&w, &x, 16);
+  __builtin_nontemporal_store(w, (words*)p);
+}
+
 inline bool node_dtype_ok(int32_t dtype) { return dtype == FC_F32 || dtype == FC_BF16 || dtype == FC_F16; }
 inline int64_t node_dtype_size(int32_t dtype) { return dtype == FC_F32 ? 4 : 2; }
 
