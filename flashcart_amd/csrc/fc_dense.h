@@ -131,7 +131,7 @@ struct DenseJob : GemmJob {
         if (inside && row + p * step < g.M) next[p] = part(g, res + p * step * g.ld_out);
       }
     }
-    // y of those rows from x = s x W^T; the cursor goes on to the next turn, 16 rows further
+    // y of those rows from their sums, scaled by s; the cursor goes on to the next turn, 16 rows further
     template <int PASSES>
     __device__ __forceinline__ void finish(const DenseJob& g, bool inside, int64_t row, int step,
                                            float (&x)[PASSES][V]) {
@@ -210,8 +210,8 @@ struct DenseJob : GemmJob {
   };
 };
 
-// Where unit `t` of the groups' rows is, or (BY_GROUP) group `t`'s first: of the units of `size` rows (an empty group has `least` of them), counted group by
-// group. Offsets are taken into [0, n] and as their running maximum, so that the groups' rows are apart whatever they hold.
+// Where unit `t` of the groups' rows is, or (BY_GROUP) group `t`'s first: of the units of `size` rows (an empty group has
+// `least` of them), counted group by group. Offsets are taken into [0, n] and as their running maximum, so that the groups' rows are apart whatever they hold.
 struct GroupUnit {
   int group, index;   // -1: there are fewer units than that; index within the group
   int64_t row, rows;  // the group's first row and its rows

@@ -1,5 +1,11 @@
 // Dense layers forward (fc_dense.h), in three types, with one weight or one for each group of rows, and in 8 bits:
-//   y = residual + c act(s (x_scale x) (w_scale W)^T + b)  with e4m3 x and W, a float32 scale for each of their rows, and y in 16 bits.
+//   y = residual + c act(s (x_scale x) (w_scale W)^T + b)
+// with e4m3 x and W, a float32 scale for each of their rows, and y in 16 bits.
+//
+// Bound by the matrix cores and the stores of y and act'(z) where n is large (16,384 x 2,048 x 5,632 bf16 371 us, 1,020
+// TFLOP/s; 8,192 x 4,096 x 5,120 in 8 bits 161-174 us, 1,970-2,130 TFLOP/s; 16,384 rows over 32 experts of 2,048 x 2,816
+// 257 us), by the weights' bytes where it is small (1 x 4,096 x 10,240 bf16 15 us, 5.6 TB/s; 64 rows over 64 experts of
+// 2,048 x 1,024 41 us, 4.1 TB/s).
 #include "fc_dense_few.h"
 #include "fc_dense_plan.h"
 

@@ -56,7 +56,8 @@ struct TileCost {
 // faster where workgroups are many and their sums short (25,000 x 128 x 128 float32, forward 21.5 -> 20.1 us, dx and dW 27.0
 // -> 24.2; 8,192 x 512 x 512 bf16 forward 17.0 -> 14.6), slower where they are few and long (1 x 4,096 x 10,240 15 -> 31).
 constexpr int kKinds = 4;
-constexpr TileCost kTileCost[kKinds] = {{0.2, 0.26, 0.8, 1.2}, {0.65, 0.55, 2.5, 3.2}, {1.25, 1.5, 9.0, 14.0}, {0.47, 0.25, 0.9, 1.3}};
+constexpr TileCost kTileCost[kKinds] = {{0.2, 0.26, 0.8, 1.2}, {0.65, 0.55, 2.5, 3.2}, {1.25, 1.5, 9.0, 14.0},
+                                        {0.47, 0.25, 0.9, 1.3}};
 // native float32, 32 k a step: bound by the matrix cores
 constexpr TileCost kNativeCost[kKinds] = {{0.5, 0.56, 1.0, 2.2}, {2.05, 1.85, 5.0, 6.0}, {}, {0.6, 0.48, 0.6, 1.6}};
 constexpr int kShare[kKinds] = {2, 2, 1, 5};  // workgroups that a CU runs at once
@@ -160,7 +161,8 @@ int plan_launch(Job* const* jobs, const bool* can_split, int count, Form form, b
           double alone = 0;
           for (int q = 0; q < count; ++q)
             if (jobs[q]->M > 0)
-              alone += (double)jobs[q]->tiles_m * jobs[q]->tiles_n * splits[q] * (steps[q] * c.step + kLatency[kind][!can_split[q]]);
+              alone += (double)jobs[q]->tiles_m * jobs[q]->tiles_n * splits[q] *
+                       (steps[q] * c.step + kLatency[kind][!can_split[q]]);
           alone *= (double)((blocks + cus * kShare[kind] - 1) / (cus * kShare[kind])) / blocks;
           if (alone > time) time = alone;
         }
