@@ -88,7 +88,7 @@ struct DenseJob : GemmJob {
     const OT* res;
     int64_t factor_at;
     float bias[V], col_scale[V];
-    float lin, one, act_scale;  // silu, sigmoid: act(z) = s(z) (lin z + one), s the logistic function; times act_scale
+    float lin, act_scale;  // lin: 1, of the logistic function s 0; act(z) is s z or s, times act_scale
     int col_at;
     bool whole;
     Pack<OT, V> next[2];
@@ -100,7 +100,6 @@ struct DenseJob : GemmJob {
       col_at = col;
       whole = col + V <= g.n_out;
       lin = g.act == 1 ? 0.f : 1.f;
-      one = 1.f - lin;
       act_scale = g.act_scale;
       Pack<OT, V> b{};
       Pack<float, V> c{};
@@ -168,7 +167,8 @@ struct DenseJob : GemmJob {
         } else {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float z = x[p][v], s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), q = fmaf(lin, z, one);
+            // (chosen, not multiplied: an infinite z has a logistic function)
+            const float z = x[p][v], s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), q = g.act == 1 ? 1.f : z;
             d[v] = s * fmaf(q, 1.f - s, lin);
             x[p][v] = act_scale * (s * q);
           }
