@@ -15,10 +15,10 @@ namespace fc {
 
 enum { ACT_NONE = 3 };
 
-// act'(z) as it is kept for the backward pass: in float32; in float16 beside bfloat16 operands (its rounding is an eighth of
-// theirs); beside float16 ones with 24 bits, (upper 16, next 8) in two arrays.
-template <class OT>
-constexpr int kFactorBytes = std::is_same_v<OT, float> ? 4 : std::is_same_v<OT, bf16_t> ? 2 : 3;
+// act'(z) as it is kept for the backward pass: in float32; beside bfloat16 operands 2^15 act'(z) in float16, which has
+// |act'| <= 1.13 inside its range and 11 significant bits (a rounding of an eighth of the operands') down to 2^-29, fewer
+// below, none below 2^-40; beside float16 ones with 24 bits, (upper 16, next 8) in two arrays.
+constexpr float kFactorScale = 0x1p15f;
 
 template <class OT, int V>
 __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t count, const float (&d)[V]) {
@@ -27,7 +27,7 @@ __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t cou
   } else if constexpr (std::is_same_v<OT, bf16_t>) {
     uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) w[i] = pack2<f16_t>(d[2 * i], d[2 * i + 1]);
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2<f16_t>(kFactorScale * d[2 * i], kFactorScale * d[2 * i + 1]);
     put_words<V>(factor + 2 * at, w);
   } else {
     uint32_t hi[V / 2], lo[V / 4];
@@ -53,7 +53,7 @@ __device__ __forceinline__ void get_factor(const char* factor, int64_t at, int64
   } else if constexpr (std::is_same_v<OT, bf16_t>) {
     const Pack<f16_t, 8> p = *(const Pack<f16_t, 8>*)__builtin_assume_aligned(factor + 2 * at, 16);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] = to_f32(p.v[i]);
+    for (int i = 0; i < 8; ++i) d[i] = to_f32(p.v[i]) * (1.f / kFactorScale);
   } else {
     const uint4 h = *(const uint4*)(factor + 2 * at);
     const uint2 l = *(const uint2*)(factor + 2 * count + at);

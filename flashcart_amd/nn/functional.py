@@ -151,8 +151,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
     Sums are float32, and bias, activation and residual are applied before the one rounding of the output. For bfloat16
     and float16 the gradient of the activation's argument is rounded to that type in the backward pass, being an operand of
     the matrix instructions (gradients of x and weight are 1.4 times as far from exact ones as one rounding); the
-    activation's derivative is kept for it with 11 significant bits beside bfloat16, 16 beside float16, in 2 and 3 bytes an
-    output (float32: all, in 4). float32 products
+    activation's derivative is kept for it with 11 significant bits beside bfloat16 (fewer for a derivative below 2^-29, none
+    below 2^-40), 16 beside float16, in 2 and 3 bytes an output (float32: all, in 4). float32 products
     keep float32 accuracy, as in ``gated_feed_forward``; so does the activation. There are no second derivatives.
     """
     return _node_ops.ops().node_dense.default(x, weight, bias, residual, None, _activation(act), float(act_scale),

@@ -543,7 +543,7 @@ int fc_ffn_bwd(const fc_ffn_desc* desc, int64_t n, const void* grad, const void*
  * (groups, out), no residual; row r has weight e where offsets[e] <= r < offsets[e + 1]; offsets: groups + 1 int64 on the
  * device, taken into [0, n] and as their running maximum; rows of no group give zeros. In 16-bit types the gradient of
  * act's argument is rounded to the type between the products, and act's derivative is kept with 11 significant bits beside
- * bfloat16, 16 beside float16.
+ * bfloat16 (fewer below 2^-29, none below 2^-40), 16 beside float16.
  * `aligned`: x, W and grad are aligned to 16 bytes (otherwise they are copied). in and out are at most 2^20, n below 2^27,
  * groups at most 2^16 with (groups + 1) out below 2^30. */
 typedef struct fc_dense_desc {

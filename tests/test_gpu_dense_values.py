@@ -1,4 +1,4 @@
-"""Dense layers where their values are hard to hold: infinite arguments of every activation."""
+"""Dense layers where their values are hard to hold: infinite arguments of every activation, derivatives that vanish."""
 
 import math
 
@@ -77,3 +77,38 @@ def test_sums_that_leave_the_range(dtype):
     grad = torch.ones(n, out, device=DEV, dtype=dtype)
     got = _run(x, w, None, None, "sigmoid", 1.0, s, grad)
     assert not got["y"][:, ::2].any() and bool((got["y"][:, 1::2] == 1).all()) and not got["dw"].any()
+
+
+# activation and the range of its argument
+RANGES = [("silu", -40.0, 40.0), ("sigmoid", -40.0, 0.5)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,low,high", RANGES)
+@pytest.mark.parametrize("n", [1, 70, 300])
+def test_derivatives_that_vanish(n, act, low, high, dtype):
+    """act'(z) through the bias' gradient of one row, relative to itself: one rounding of the type (eps / 2), the kept
+    derivative's (2^-11 beside bfloat16, with float16's smallest half step 2^-25 after a factor of 2^15, so 2^-40; 2^-16 beside
+    float16), and what float32 makes of the formula: 8 roundings of its terms, and an exponential whose argument, rounded, is off
+    by 2^-24 of itself."""
+    z = torch.linspace(low, high, 1000, device=DEV).to(dtype)
+    x, w = torch.zeros(n, 8, device=DEV, dtype=dtype), torch.randn(1000, 8, device=DEV).to(dtype)
+    grad = torch.zeros(n, 1000, device=DEV, dtype=dtype)
+    grad[n // 2] = 1
+    got = _run(x, w, z, None, act, 1.0, 1.0, grad)
+    v = z.double()
+    s = torch.sigmoid(v)
+    t = torch.sigmoid(-v)  # 1 - s
+    if act == "sigmoid":
+        want = s * t
+        terms = want * (1 + v.abs())
+    else:
+        want = s * (1 + v * t)
+        terms = s * (1 + v.abs() * t) * (1 + v.abs())
+    u = torch.finfo(dtype).eps / 2
+    kept, least = {torch.float32: (0.0, 0.0), torch.bfloat16: (2.0 ** -11, 2.0 ** -40),
+                   torch.float16: (2.0 ** -16, 0.0)}[dtype]
+    bound = (u + kept + u * kept) * want.abs() + least + 8 * 2.0 ** -24 * terms
+    bound = bound + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    off = (got["db"].double() - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), float(z[(off / bound).argmax()]))
