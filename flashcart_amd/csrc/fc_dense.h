@@ -18,7 +18,10 @@ enum { ACT_NONE = 3 };
 // act'(z) as it is kept for the backward pass: in float32; beside bfloat16 operands 2^15 act'(z) in float16, which has
 // |act'| <= 1.13 inside its range and 11 significant bits (a rounding of an eighth of the operands') down to 2^-29, fewer
 // below, none below 2^-40; beside float16 ones with 24 bits, (upper 16, next 8) in two arrays.
-constexpr float kFactorScale = 0x1p15f;
+template <class OT>
+constexpr float kFactorScale = std::is_same_v<OT, bf16_t> ? 0x1p15f : 1.f;
+
+// d: act'(z) times that scale.
 
 template <class OT, int V>
 __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t count, const float (&d)[V]) {
@@ -27,7 +30,7 @@ __device__ __forceinline__ void put_factor(char* factor, int64_t at, int64_t cou
   } else if constexpr (std::is_same_v<OT, bf16_t>) {
     uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) w[i] = pack2<f16_t>(kFactorScale * d[2 * i], kFactorScale * d[2 * i + 1]);
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2<f16_t>(d[2 * i], d[2 * i + 1]);
     put_words<V>(factor + 2 * at, w);
   } else {
     uint32_t hi[V / 2], lo[V / 4];
@@ -53,7 +56,7 @@ __device__ __forceinline__ void get_factor(const char* factor, int64_t at, int64
   } else if constexpr (std::is_same_v<OT, bf16_t>) {
     const Pack<f16_t, 8> p = *(const Pack<f16_t, 8>*)__builtin_assume_aligned(factor + 2 * at, 16);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] = to_f32(p.v[i]) * (1.f / kFactorScale);
+    for (int i = 0; i < 8; ++i) d[i] = to_f32(p.v[i]);
   } else {
     const uint4 h = *(const uint4*)(factor + 2 * at);
     const uint2 l = *(const uint2*)(factor + 2 * count + at);
@@ -88,7 +91,7 @@ struct DenseJob : GemmJob {
     const OT* res;
     int64_t factor_at;
     float bias[V], col_scale[V];
-    float lin, act_scale;  // lin: 1, of the logistic function s 0; act(z) is s z or s, times act_scale
+    float act_scale;
     int col_at;
     bool whole;
     Pack<OT, V> next[2];
@@ -99,7 +102,6 @@ struct DenseJob : GemmJob {
       factor_at = g.factor_at + row * g.N + col;
       col_at = col;
       whole = col + V <= g.n_out;
-      lin = g.act == 1 ? 0.f : 1.f;
       act_scale = g.act_scale;
       Pack<OT, V> b{};
       Pack<float, V> c{};
@@ -135,6 +137,8 @@ struct DenseJob : GemmJob {
     __device__ __forceinline__ void finish(const DenseJob& g, bool inside, int64_t row, int step,
                                            float (&x)[PASSES][V]) {
       static_assert(PASSES <= 2, "residuals ahead");
+      constexpr float KEEP = kFactorScale<OT>;
+      const bool keep = !EIGHT && g.factor != nullptr;
       Pack<OT, V> r[PASSES];
       const bool with_res = g.residual != nullptr;
       if (with_res) {
@@ -162,16 +166,39 @@ struct DenseJob : GemmJob {
           for (int v = 0; v < V; ++v) {
             float f;
             ffn_act(2, x[p][v], f, d[v]);
+            d[v] *= KEEP;
             x[p][v] = act_scale * f;
           }
         } else {
+          // y = s z, or the logistic function s = 1 / (1 + e) itself (also of an infinite z), and act' = y (1 - s) + s, or
+          // y (1 - s). 1 - s = s e keeps its bits where s is near one; where e is infinite, s and y are zero, and the smaller of
+          // NaN and one is one.
+          float s[V], e[V];
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            // (chosen, not multiplied: an infinite z has a logistic function)
-            const float z = x[p][v], s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), q = g.act == 1 ? 1.f : z;
-            d[v] = s * fmaf(q, 1.f - s, lin);
-            x[p][v] = act_scale * (s * q);
+            e[v] = __expf(-x[p][v]);
+            s[v] = __builtin_amdgcn_rcpf(1.f + e[v]);
           }
+          if (g.act == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[p][v] = s[v];
+          } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[p][v] *= s[v];
+          }
+          if (keep) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              s[v] *= KEEP;
+              d[v] = x[p][v] * fminf(s[v] * e[v], KEEP);
+            }
+            if (g.act != 1) {
+#pragma unroll
+              for (int v = 0; v < V; ++v) d[v] += s[v];
+            }
+          }
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[p][v] *= act_scale;
         }
         if (with_res) {
 #pragma unroll
@@ -201,7 +228,7 @@ struct DenseJob : GemmJob {
             if (col_at + v < g.n_out) to[v] = from_f32<OT>(x[p][v]);
         }
         if constexpr (!EIGHT) {
-          if (g.factor) put_factor<OT, V>(g.factor, factor_at + (int64_t)p * step * g.N, g.factor_count, d);
+          if (keep) put_factor<OT, V>(g.factor, factor_at + (int64_t)p * step * g.N, g.factor_count, d);
         }
       }
       out += 16 * g.ld_out;

@@ -18,7 +18,7 @@ struct DzArgs {
   int64_t plane;
   float* sums;              // (chunks, op), or null
   int32_t out, op, col_blocks;
-  float act_scale;
+  float act_scale;          // over the scale that act'(z) is kept with
   const int64_t* offsets;   // or null
   int32_t groups;
   int64_t rows;
@@ -64,9 +64,8 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = to_f32(v[k].v[i]);
+        x[i] = to_f32(v[k].v[i]) * a.act_scale;
         if (a.factor) x[i] = col + i < a.out ? x[i] * d[k][i] : 0.f;
-        x[i] *= a.act_scale;
         sum[i] += x[i];
       }
       if (a.dz) put<MT, F32, 8>(a.dz, r * a.op + col, a.plane, x);
@@ -249,7 +248,7 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
   a.out = (int32_t)f.out;
   a.op = (int32_t)f.op;
   a.col_blocks = cdiv(f.op, kDzCols);
-  a.act_scale = f.d.act_scale;
+  a.act_scale = f.d.act_scale / (factor && f.d.dtype == FC_BF16 ? kFactorScale<bf16_t> : 1.f);
   a.rows = f.n;
   if (nx) {
     DenseJob& g = p.dx;
