@@ -80,7 +80,7 @@ def test_sums_that_leave_the_range(dtype):
 
 
 # activation and the range of its argument
-RANGES = [("silu", -40.0, 40.0), ("sigmoid", -40.0, 40.0)]
+RANGES = [("silu", -40.0, 40.0), ("sigmoid", -40.0, 40.0), ("gelu", -14.0, 14.0)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -90,7 +90,9 @@ def test_derivatives_that_vanish(n, act, low, high, dtype):
     """act'(z) through the bias' gradient of one row, relative to itself: one rounding of the type (eps / 2), the kept
     derivative's (2^-11 beside bfloat16, with float16's smallest half step 2^-25 after a factor of 2^15, so 2^-40; 2^-16 beside
     float16), and what float32 makes of the formula: 8 roundings of its terms, and an exponential whose argument, rounded, is off
-    by 2^-24 of itself."""
+    by 2^-24 of itself. exp(-z^2 / 2) is below float32's smallest normal number 2^-126 from |z| = 13.22 on, where the
+    exponential instruction gives zero: an error of that, times R + |z| pdf(0) <= 0.5 + 14 x 0.4 < 2^3, in gelu's."""
+    print(f"derivatives n={n} {act} {dtype}", flush=True)
     z = torch.linspace(low, high, 1000, device=DEV).to(dtype)
     x, w = torch.zeros(n, 8, device=DEV, dtype=dtype), torch.randn(1000, 8, device=DEV).to(dtype)
     grad = torch.zeros(n, 1000, device=DEV, dtype=dtype)
@@ -99,7 +101,11 @@ def test_derivatives_that_vanish(n, act, low, high, dtype):
     v = z.double()
     s = torch.sigmoid(v)
     t = torch.sigmoid(-v)  # 1 - s
-    if act == "sigmoid":
+    if act == "gelu":
+        cdf, pdf = 0.5 * torch.erfc(-v / math.sqrt(2)), torch.exp(-0.5 * v * v) / math.sqrt(2 * math.pi)
+        want = cdf + v * pdf
+        terms = (cdf + v.abs() * pdf) * (1 + v * v)
+    elif act == "sigmoid":
         want = s * t
         terms = want * (1 + v.abs())
     else:
@@ -109,6 +115,20 @@ def test_derivatives_that_vanish(n, act, low, high, dtype):
     kept, least = {torch.float32: (0.0, 0.0), torch.bfloat16: (2.0 ** -11, 2.0 ** -40),
                    torch.float16: (2.0 ** -16, 0.0)}[dtype]
     bound = (u + kept + u * kept) * want.abs() + least + 8 * 2.0 ** -24 * terms
-    bound = bound + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    bound = bound + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -123 if act == "gelu" else 2.0 ** -134)
     off = (got["db"].double() - want).abs()
     assert bool((off <= bound).all()), (float((off / bound).max()), float(z[(off / bound).argmax()]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 70, 300])
+def test_tails_of_gelu(n, dtype):
+    """y relative to itself: one rounding of the type, 8 of float32, and those of the exponential's argument."""
+    z = torch.linspace(-13, 13, 1000, device=DEV).to(dtype)
+    x, w = torch.zeros(n, 8, device=DEV, dtype=dtype), torch.randn(1000, 8, device=DEV).to(dtype)
+    v = z.double()
+    want = 0.5 * v * torch.erfc(-v / math.sqrt(2))
+    bound = (torch.finfo(dtype).eps / 2 + 8 * 2.0 ** -24 * (1 + v * v)) * want.abs()
+    bound = bound + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    off = (_F().dense(x, w, z, "gelu").double() - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), float(z[(off / bound).amax(0).argmax()]))
