@@ -3,7 +3,9 @@
 // y being the norm of the total as it is stored, so that the backward pass, which reads the stored total, differentiates what
 // was computed. With xhat = r total and g the gradient of y
 //   dx = g_total + r (w g - xhat mean(w g xhat)),  dw = sum over the rows of g xhat.
-// In 8 bits y is written as round(y / s) in e4m3 with s = max(|y|, 2^-100) / 448 for each row.
+// In 8 bits y is written as round(y / s) in e4m3 with s = max(|y|, 2^-100) / 448 for each row. r has no part in the quotient
+// y / s = 448 t w / max|t w|, in which 16-bit values often lie on a midpoint of two e4m3 numbers (1 in 8,000): it is formed from
+// the products without r, rounded once, so that these go to the even number as they should.
 //
 // Bound by memory: every tensor is read or written once. A row is held in registers by a group of 16, 64 or 256 lanes, 16
 // bytes a lane and load; squares, means and dw are summed in float32. dw: a workgroup adds up the rows it takes, in
@@ -117,27 +119,47 @@ __device__ __forceinline__ float over_row(float v, float* lds) {
   return v;
 }
 
-__device__ __forceinline__ float row_scale(float most) { return fmaxf(most, 0x1p-100f) / 448.f; }
-
-// e4m3 numbers of 4 values, to nearest even; beyond 448 the largest number, NaN stays.
-__device__ __forceinline__ uint32_t pack_e4m3(const float (&x)[4], float inv) {
-  float v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = x[i] * inv;
-    v[i] = v[i] > 448.f ? 448.f : v[i] < -448.f ? -448.f : v[i];
-  }
-  int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], u, true);
+// r = power * rest with power of two `power`, rest in [1, 2): values times `power` have no rounding that others had not. (0,
+// infinity and NaN are their own power.)
+__device__ __forceinline__ float power_of(float r, float& rest) {
+  const uint32_t u = __float_as_uint(r);
+  rest = __uint_as_float((u & 0x007fffffu) | 0x3f800000u);
+  return r == r ? __uint_as_float(u & 0x7f800000u) : r;
 }
-template <int V>
-__device__ __forceinline__ Pack<uint8_t, V> to_e4m3(const float (&x)[V], float inv) {
+
+// How a row goes to 8 bits whose largest |x| is `most`, its values being rest x: scale = max(rest most, 2^-100) / 448, and
+// rest x / scale = x num / den, with num / den = 448 / most unless the least scale or an infinity stands in its place. No
+// quotient is above 448; with an infinite scale the finite ones are zero and the others NaN.
+struct RowEight {
+  float scale, num, den, inv;
+  __device__ __forceinline__ RowEight(float most, float rest) {
+    const float top = rest * most;
+    scale = fmaxf(top, 0x1p-100f) / 448.f;
+    const bool finite = top < __builtin_inff(), plain = top >= 0x1p-100f && finite;
+    num = plain ? 0.875f : rest;  // (448 / 2^9)
+    den = plain ? 0x1p-9f * most : finite ? scale : 1.f;
+    inv = finite ? 1.f / den : 0.f;
+  }
+  // The quotient, rounded once: an estimate, and what is left of it. LONG: with what x num loses, which has no more than 24
+  // bits for bfloat16 products and for 16-bit values alone (and float32's is rounded, as its products are).
+  template <bool LONG>
+  __device__ __forceinline__ float of(float x) const {
+    const float n = x * num, q = n * inv;
+    float left = fmaf(-q, den, n);
+    if constexpr (LONG) left += fmaf(x, num, -n);
+    return fmaf(left, inv, q);
+  }
+};
+
+// e4m3 numbers of V values of a row, to nearest even.
+template <bool LONG, int V>
+__device__ __forceinline__ Pack<uint8_t, V> to_e4m3(const float (&x)[V], const RowEight& e) {
   Pack<uint8_t, V> p;
   uint32_t w[V / 4];
 #pragma unroll
   for (int i = 0; i < V; i += 4) {
-    const float q[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
-    w[i / 4] = pack_e4m3(q, inv);
+    const int u = __builtin_amdgcn_cvt_pk_fp8_f32(e.of<LONG>(x[i]), e.of<LONG>(x[i + 1]), 0, false);
+    w[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e.of<LONG>(x[i + 2]), e.of<LONG>(x[i + 3]), u, true);
   }
   memcpy(&p, w, V);
   return p;
@@ -181,9 +203,11 @@ __global__ void __launch_bounds__(256) row_norm_fwd_kernel(RowNorm g) {
 #pragma unroll
     for (int i = 0; i < V; ++i) sum = fmaf(t[k][i], t[k][i], sum);
   }
+  float rest = 1.f;
   if constexpr (MODE != ROW_EIGHT) {
-    const float r = 1.f / sqrtf(over_row<L, 256, false>(sum, lds) / (float)g.width + g.eps);
+    float r = 1.f / sqrtf(over_row<L, 256, false>(sum, lds) / (float)g.width + g.eps);
     if (g.rstd && on && lane == 0) g.rstd[row] = r;
+    if constexpr (MODE == NORM_EIGHT) r = power_of(r, rest);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int64_t c = ((int64_t)k * L + lane) * V;
@@ -211,12 +235,12 @@ __global__ void __launch_bounds__(256) row_norm_fwd_kernel(RowNorm g) {
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(t[k][i]));
-    const float scale = row_scale(over_row<L, 256, true>(most, lds)), inv = 1.f / scale;
-    if (on && lane == 0) g.scale[row] = scale;
+    const RowEight eight(over_row<L, 256, true>(most, lds), rest);
+    if (on && lane == 0) g.scale[row] = eight.scale;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int64_t c = ((int64_t)k * L + lane) * V;
-      const Pack<uint8_t, V> o = to_e4m3<V>(t[k], inv);
+      const Pack<uint8_t, V> o = to_e4m3<std::is_same_v<T, f16_t> && MODE == NORM_EIGHT>(t[k], eight);
       if (on && c < g.width) store_chunk<uint8_t, V, EVEN>((uint8_t*)g.y + at, c, g.width, &o);
     }
   }
@@ -230,7 +254,7 @@ __global__ void __launch_bounds__(1024) row_norm_wide_kernel(RowNorm g) {
   const int64_t row = g.first + blockIdx.x, at = row * g.width;
   const T* const x = (const T*)g.x + at;
   const T* const t = g.residual ? (const T*)g.total + at : x;
-  float r = 1.f;
+  float r = 1.f, rest = 1.f;
   if (MODE != ROW_EIGHT) {
     float sum = 0.f;
     for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
@@ -250,6 +274,7 @@ __global__ void __launch_bounds__(1024) row_norm_wide_kernel(RowNorm g) {
     }
     r = 1.f / sqrtf(over_row<NT, NT, false>(sum, lds) / (float)g.width + g.eps);
     if (g.rstd && threadIdx.x == 0) g.rstd[row] = r;
+    if constexpr (MODE == NORM_EIGHT) r = power_of(r, rest);
   }
   // (a thread reads back the elements that it wrote)
   auto values = [&](int64_t c, float (&v)[V]) {
@@ -274,12 +299,12 @@ __global__ void __launch_bounds__(1024) row_norm_wide_kernel(RowNorm g) {
 #pragma unroll
       for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(v[i]));
     }
-    const float scale = row_scale(over_row<NT, NT, true>(most, lds)), inv = 1.f / scale;
-    if (threadIdx.x == 0) g.scale[row] = scale;
+    const RowEight eight(over_row<NT, NT, true>(most, lds), rest);
+    if (threadIdx.x == 0) g.scale[row] = eight.scale;
     for (int64_t c = (int64_t)threadIdx.x * V; c < g.width; c += NT * V) {
       float v[V];
       values(c, v);
-      const Pack<uint8_t, V> o = to_e4m3<V>(v, inv);
+      const Pack<uint8_t, V> o = to_e4m3<std::is_same_v<T, f16_t> && MODE == NORM_EIGHT>(v, eight);
       store_chunk<uint8_t, V, false>((uint8_t*)g.y + at, c, g.width, &o);
     }
   }

@@ -122,8 +122,9 @@ def rms_norm_add_quantized(x: torch.Tensor, residual: Optional[torch.Tensor] = N
                            eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``rms_norm_add`` with its norm in 8 bits, for inference: (q, scale, total), the norm being ``q * scale[..., None]``.
 
-    q is float8_e4m3fn, ``round(y / scale)`` of the unrounded norm y; scale (float32) is ``max(|y|, 2^-100) / 448`` over the
-    row. A row with an infinity has an infinite scale, and NaN for its values. There are no gradients: arguments that
+    scale (float32) is ``max(|y|, 2^-100) / 448`` over the row, y being the unrounded norm. q is float8_e4m3fn, the number
+    nearest to ``448 y / max(|y|, 2^-100)`` (for 16-bit types exactly, ties going to the even number; for float32 up to
+    the rounding of y). A row with an infinity has an infinite scale, and NaN for its values. There are no gradients: arguments that
     require them are refused where autograd records.
     """
     q, scale, total = _node_ops.ops().rms_norm_add_quantized.default(x, residual, weight, float(eps))

@@ -580,7 +580,8 @@ int fc_quantized_dense(const fc_dense_desc* desc, int64_t n, const void* x, cons
  * is at most 2^20, n below 2^31. */
 int fc_row_norm_fwd(int32_t dtype, int64_t n, int64_t width, const void* x, const void* residual, const void* weight,
                     float eps, void* total, void* y, float* rstd, void* stream);
-/* The same with y in e4m3 and a scale for each row, max(largest |y|, 2^-100) / 448: q = round(y / scale). norm = 0: y is
+/* The same with y in e4m3 and a scale for each row, max(largest |y|, 2^-100) / 448: q = round(y / scale), the
+ * quotient formed from y and the unrounded scale. norm = 0: y is
  * the row of x itself (no residual, weight, total or eps). */
 int fc_row_norm_quantize(int32_t dtype, int32_t norm, int64_t n, int64_t width, const void* x, const void* residual,
                          const void* weight, float eps, void* total, void* q, float* scale, void* stream);
