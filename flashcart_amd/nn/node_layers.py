@@ -236,7 +236,7 @@ class NormNodeNetwork(nn.Module):
         for norm, expand, contract in zip(self.norms[1:], self.expand, self.contract):
             hidden = expand(y, rows) if self.per_element else expand(y)
             y, total = norm(contract(hidden), total)
-        return rows.unsort(y).view(*ids.shape, -1) if self.per_element else y
+        return rows.unsort(y).view(*ids.shape, y.shape[-1]) if self.per_element else y
 
 
 class QuantizedNodeNetwork(nn.Module):
