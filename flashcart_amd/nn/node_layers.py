@@ -137,9 +137,24 @@ class DenseLayer(nn.Module):
         return functional.dense(x, self.weight, self.bias, self.activation, self.act_scale, self.scale, residual)
 
 
-class QuantizedDenseLayer(nn.Module):
+class _FixedTypes(nn.Module):
+    """A module whose buffers keep their types: ``.half()``, ``.to(dtype)`` and the like, also of a module that holds it, move it
+    between devices alone."""
+
+    def _apply(self, fn, recurse=True):
+        kept = dict(self.named_buffers(recurse=False))
+        super()._apply(fn, recurse)
+        for name, before in kept.items():
+            after = getattr(self, name)
+            if after.dtype != before.dtype:
+                setattr(self, name, before.to(after.device))
+        return self
+
+
+class QuantizedDenseLayer(_FixedTypes):
     """A ``DenseLayer`` on the GPU in 8 bits, for inference (``functional.quantized_dense``): its weight as float8_e4m3fn with a
-    scale for each row, laid out here once, bias and output in ``dtype``. Arguments that ask for gradients are refused."""
+    scale for each row, laid out here once, bias and output in ``dtype``. Arguments that ask for gradients are refused. The types
+    stay as they are laid out here under ``.half()``, ``.to(dtype)`` and the like."""
 
     def __init__(self, layer: DenseLayer, dtype: torch.dtype = torch.bfloat16):
         super().__init__()
@@ -239,9 +254,10 @@ class NormNodeNetwork(nn.Module):
         return rows.unsort(y).view(*ids.shape, y.shape[-1]) if self.per_element else y
 
 
-class QuantizedNodeNetwork(nn.Module):
+class QuantizedNodeNetwork(_FixedTypes):
     """A ``NormNodeNetwork`` on the GPU (not ``per_element``) for inference in 8 bits: the norms write what the expanding layers
-    read, activations are quantized row by row between the layers, sums of blocks are in ``dtype``."""
+    read, activations are quantized row by row between the layers, sums of blocks are in ``dtype``. The types stay so under
+    ``.half()``, ``.to(dtype)`` and the like."""
 
     def __init__(self, network: NormNodeNetwork, dtype: torch.dtype = torch.bfloat16):
         super().__init__()
