@@ -102,6 +102,7 @@ struct DenseJob : GemmJob {
   int32_t halves;                // tiles at the end that are taken as two halves of their columns
   int32_t unit;                  // > 0: sums over a group's rows, in parts of so many
   int64_t rows, b_stride, out_stride;  // rows of the call; elements from one group's B, and output, to the next one's
+  int32_t first, blocks;         // first workgroup of this launch, workgroups of all
 
   // V columns from `col` on of the rows that a lane finishes one after the other:
   // where it is, what its columns have in common in all rows, and the residuals of its next rows, loaded ahead.

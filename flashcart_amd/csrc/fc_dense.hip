@@ -19,11 +19,12 @@ __global__ void __launch_bounds__(T::NT, 2) dense_fwd_kernel(DenseJob g) {
   __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
   lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
   lds_char* const l3 = (lds_char*)lds3;
+  const int block = g.first + blockIdx.x;
   if constexpr (GROUPS) {
-    GroupTile<T, MT, F32, false, false, EPI_DENSE, OT>::run(g, blockIdx.x, gridDim.x, l0, l1, l2, l3);
+    GroupTile<T, MT, F32, false, false, EPI_DENSE, OT>::run(g, block, g.blocks, l0, l1, l2, l3);
     return;
   }
-  const int block = blockIdx.x, whole = g.tiles_m * g.tiles_n - g.halves;
+  const int whole = g.tiles_m * g.tiles_n - g.halves;
   if constexpr (!GROUPS && T::BN == 256) {
     if (g.splits == 1 && block >= whole) {  // (tiles in the order of FfnTile::run)
       const int tile = whole + (block - whole) / 2, group = tile / (8 * g.tiles_n), in = tile - group * 8 * g.tiles_n;
@@ -40,12 +41,12 @@ __global__ void __launch_bounds__(T::NT, 2) dense_fwd_kernel(DenseJob g) {
 // A workgroup forms 256 / groups times 4 outputs: the lanes of an output add every groups-th part, their sums are added in
 // order.
 template <class MT, bool F32, class OT>
-__global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups) {
+__global__ void __launch_bounds__(256) dense_sum_kernel(DenseJob g, int groups, int64_t first) {
   constexpr int ES = std::is_same_v<MT, float> ? 4 : 2;
   constexpr bool EIGHT = std::is_same_v<MT, e4m3_t>;
   __shared__ f32x4v part[256];
   const int per = 256 / groups, grp = threadIdx.x / per;
-  const int64_t chunks = g.N / 4, t = (int64_t)blockIdx.x * per + threadIdx.x % per;
+  const int64_t chunks = g.N / 4, t = (first + blockIdx.x) * per + threadIdx.x % per;
   const bool ok = t < g.M * chunks;
   const int64_t row = ok ? t / chunks : 0;
   const int col = ok ? (int)(t - row * chunks) * 4 : 0;
@@ -155,41 +156,35 @@ static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const vo
 }
 
 template <class MT, bool F32, class OT, bool GROUPS>
-static int launch_tiles(const DenseJob& g, int kind, hipStream_t s) {
-  const int bm = tile_rows(kind);
-  const int64_t blocks = GROUPS ? group_blocks(g, bm) : blocks_of(g) + g.halves;
-  if (!grid_fits(blocks, 512)) return FC_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks);
-  if constexpr (!std::is_same_v<MT, float>) {
-    if (kind == 2) {
-      hipLaunchKernelGGL((dense_fwd_kernel<TileL, MT, F32, OT, GROUPS>), grid, dim3(TileL::NT), 0, s, g);
-      FC_LAUNCH_CHECK();
-      return FC_OK;
+static int launch_tiles(DenseJob g, int kind, hipStream_t s) {
+  const int64_t blocks = GROUPS ? group_blocks(g, tile_rows(kind)) : blocks_of(g) + g.halves;
+  if (blocks > INT32_MAX) return FC_ERR_SHAPE;
+  g.blocks = (int32_t)blocks;
+  return in_launches(blocks, [&](int64_t first, unsigned count) {
+    const dim3 grid(count);
+    g.first = (int32_t)first;
+    if constexpr (!std::is_same_v<MT, float>) {
+      if (kind == 2) hipLaunchKernelGGL((dense_fwd_kernel<TileL, MT, F32, OT, GROUPS>), grid, dim3(TileL::NT), 0, s, g);
     }
-  }
-  if constexpr (GROUPS) {
-    if (kind == 4) {
-      hipLaunchKernelGGL((dense_fwd_kernel<TileR, MT, F32, OT, GROUPS>), grid, dim3(TileR::NT), 0, s, g);
-      FC_LAUNCH_CHECK();
-      return FC_OK;
+    if constexpr (GROUPS) {
+      if (kind == 4) hipLaunchKernelGGL((dense_fwd_kernel<TileR, MT, F32, OT, GROUPS>), grid, dim3(TileR::NT), 0, s, g);
     }
-  }
-  if (kind == 3) hipLaunchKernelGGL((dense_fwd_kernel<TileX, MT, F32, OT, GROUPS>), grid, dim3(TileX::NT), 0, s, g);
-  else if (kind == 1) hipLaunchKernelGGL((dense_fwd_kernel<TileM, MT, F32, OT, GROUPS>), grid, dim3(TileM::NT), 0, s, g);
-  else hipLaunchKernelGGL((dense_fwd_kernel<TileS, MT, F32, OT, GROUPS>), grid, dim3(TileS::NT), 0, s, g);
-  FC_LAUNCH_CHECK();
-  return FC_OK;
+    if (kind == 3) hipLaunchKernelGGL((dense_fwd_kernel<TileX, MT, F32, OT, GROUPS>), grid, dim3(TileX::NT), 0, s, g);
+    else if (kind == 1) hipLaunchKernelGGL((dense_fwd_kernel<TileM, MT, F32, OT, GROUPS>), grid, dim3(TileM::NT), 0, s, g);
+    else if (kind == 0) hipLaunchKernelGGL((dense_fwd_kernel<TileS, MT, F32, OT, GROUPS>), grid, dim3(TileS::NT), 0, s, g);
+  });
 }
 
 template <class MT, class OT, bool GROUPS>
-static int launch_few(const DenseJob& g, hipStream_t s) {
+static int launch_few(DenseJob g, hipStream_t s) {
   const int64_t blocks = (int64_t)(GROUPS ? g.groups : 1) * cdiv(g.n_out, 16);
-  if (!grid_fits(blocks, 64 * kFewWaves)) return FC_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
-  if (GROUPS || g.M <= 16) hipLaunchKernelGGL((dense_few_kernel<MT, OT, 1, GROUPS>), grid, block, 0, s, g);
-  else hipLaunchKernelGGL((dense_few_kernel<MT, OT, 2, GROUPS>), grid, block, 0, s, g);
-  FC_LAUNCH_CHECK();
-  return FC_OK;
+  g.blocks = (int32_t)blocks;  // (below 2^27)
+  return in_launches(blocks, [&](int64_t first, unsigned count) {
+    const dim3 grid(count), block(64 * kFewWaves);
+    g.first = (int32_t)first;
+    if (GROUPS || g.M <= 16) hipLaunchKernelGGL((dense_few_kernel<MT, OT, 1, GROUPS>), grid, block, 0, s, g);
+    else hipLaunchKernelGGL((dense_few_kernel<MT, OT, 2, GROUPS>), grid, block, 0, s, g);
+  });
 }
 
 template <class MT, bool F32, class OT>
@@ -210,11 +205,9 @@ static int launch_dense(const DenseFwd& p, hipStream_t s) {
   if (r != FC_OK || g.splits == 1) return r;
   int groups = 1;
   while (groups < 16 && groups * 4 <= g.splits) groups *= 2;
-  const int64_t blocks = cdiv((int64_t)g.M * (g.N / 4), 256 / groups);
-  if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
-  hipLaunchKernelGGL((dense_sum_kernel<MT, F32, OT>), dim3((unsigned)blocks), dim3(256), 0, s, g, groups);
-  FC_LAUNCH_CHECK();
-  return FC_OK;
+  return in_launches(cdiv((int64_t)g.M * (g.N / 4), 256 / groups), [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL((dense_sum_kernel<MT, F32, OT>), dim3(blocks), dim3(256), 0, s, g, groups, first);
+  });
 }
 
 }  // namespace fc

@@ -22,6 +22,7 @@ struct DzArgs {
   const int64_t* offsets;   // or null
   int32_t groups;
   int64_t rows;
+  int64_t first;            // workgroup of this launch
 };
 
 // A workgroup takes 32 rows (of one group) by 256 columns, a thread 8 columns of every 8th row, all loaded before the first is
@@ -31,7 +32,7 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   constexpr bool F32 = std::is_same_v<T, float>;
   constexpr int N = kDzRows / 8;
   __shared__ float part[8][kDzCols + 8];
-  const int chunk = blockIdx.x / a.col_blocks, cb = blockIdx.x - chunk * a.col_blocks;
+  const int id = (int)(a.first + blockIdx.x), chunk = id / a.col_blocks, cb = id - chunk * a.col_blocks;
   int64_t r0 = (int64_t)chunk * kDzRows, r1 = min(r0 + kDzRows, a.rows);
   if (a.offsets) {
     const GroupUnit u = find_unit(a.offsets, a.groups, a.rows, kDzRows, 0, chunk, false);
@@ -115,29 +116,30 @@ __device__ __forceinline__ void db_block(const DbArgs& a, int block, float (&par
 }
 // (where neither dx nor dW is asked for; with them it is part of their launch)
 template <class T>
-__global__ void __launch_bounds__(1024) dense_db_kernel(DbArgs a) {
+__global__ void __launch_bounds__(1024) dense_db_kernel(DbArgs a, int first) {
   __shared__ float part[32][33];
-  db_block<T, 1024>(a, blockIdx.x, part);
+  db_block<T, 1024>(a, first + blockIdx.x, part);
 }
 
 // ---- the products: g1 forms dW (sums over rows), g2 dx. The first `front` workgroups take the one with the longer sums; the
 // workgroups from `products` on the bias' gradient ----
 template <class T, class MT, bool F32, bool GROUPS>
 __global__ void __launch_bounds__(T::NT, 2) dense_bwd_kernel(DenseJob g1, DenseJob g2, DbArgs db, int front, int products,
-                                                                bool swapped) {
+                                                                bool swapped, int first) {
   __shared__ __attribute__((aligned(1024))) char lds0[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds1[T::STAGE];
   __shared__ __attribute__((aligned(1024))) char lds2[T::STAGES > 2 ? T::STAGE : 1];
   __shared__ __attribute__((aligned(1024))) char lds3[T::STAGES > 2 ? T::STAGE : 1];
   lds_char *const l0 = (lds_char*)lds0, *const l1 = (lds_char*)lds1, *const l2 = (lds_char*)lds2;
   lds_char* const l3 = (lds_char*)lds3;
-  if ((int)blockIdx.x >= products) {
+  const int id = first + blockIdx.x;
+  if (id >= products) {
     static_assert(T::STAGE >= T::NT / 32 * 33 * 4, "sums in a stage");
-    db_block<std::conditional_t<F32, float, MT>, T::NT>(db, blockIdx.x - products, *(float (*)[T::NT / 32][33])lds0);
+    db_block<std::conditional_t<F32, float, MT>, T::NT>(db, id - products, *(float (*)[T::NT / 32][33])lds0);
     return;
   }
-  const bool in_front = (int)blockIdx.x < front;
-  const int block = in_front ? blockIdx.x : blockIdx.x - front, blocks = in_front ? front : products - front;
+  const bool in_front = id < front;
+  const int block = in_front ? id : id - front, blocks = in_front ? front : products - front;
   if (in_front != swapped) {
     if constexpr (GROUPS) GroupTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, blocks, l0, l1, l2, l3);
     else FfnTile<T, MT, F32, true, true, EPI_OUT>::run(g1, block, l0, l1, l2, l3);
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(T::NT, 2) dense_bwd_kernel(DenseJob g1, DenseJ
 struct BwdSums {
   DenseJob job[2];
   int64_t base;      // first workgroup of the second
+  int64_t first;     // workgroup of this launch
   int32_t lanes[2];  // that share the parts of an output
 };
 template <class MT, bool F32, bool GROUPS>
@@ -158,11 +161,12 @@ __global__ void __launch_bounds__(256) dense_bwd_sum_kernel(BwdSums a) {
   using OT = std::conditional_t<F32, float, MT>;
   constexpr int ES = std::is_same_v<MT, float> ? 4 : 2;
   __shared__ f32x4v part[256];
-  const bool dx = !GROUPS && blockIdx.x >= a.base;
+  const int64_t id = a.first + blockIdx.x;
+  const bool dx = !GROUPS && id >= a.base;
   DenseJob g = a.job[dx];
   const int lanes = a.lanes[dx], per = 256 / lanes, grp = threadIdx.x / per;
   const int64_t chunks = g.N / 4;
-  int64_t block = dx ? blockIdx.x - a.base : blockIdx.x;
+  int64_t block = dx ? id - a.base : id;
   if constexpr (GROUPS) {
     const int64_t each = (g.M * chunks + per - 1) / per;
     const int e = (int)(block / each);
@@ -291,29 +295,31 @@ static int launch_products(const DenseBwd& p, const DbArgs& db, hipStream_t s) {
   const int64_t blocks1 = g1.M == 0 ? 0 : GROUPS ? group_blocks(g1, bm) : blocks_of(g1);
   const int64_t blocks2 = g2.M == 0 ? 0 : GROUPS ? group_blocks(g2, bm) : blocks_of(g2), blocks = blocks1 + blocks2;
   const int64_t db_blocks = db.out ? (int64_t)(GROUPS ? db.groups : 1) * cdiv(db.n_out, 32) : 0;
-  if (!grid_fits(blocks + db_blocks, 512)) return FC_ERR_SHAPE;
-  const dim3 grid((unsigned)(blocks + db_blocks));
+  if (blocks + db_blocks > INT32_MAX) return FC_ERR_SHAPE;
   const int products = (int)blocks;
   // (with groups: of one of twice the mean size)
   const int64_t most = GROUPS && g1.M > 0 ? std::min<int64_t>(g1.unit, 2 * g1.rows / g1.groups) : 0;
   const int steps1 = g1.M == 0 ? 0 : GROUPS ? (int)most / 64 : g1.steps / g1.splits;
   const bool swapped = blocks2 > 0 && (blocks1 == 0 || g2.steps / g2.splits > steps1);
   const int front = (int)(swapped ? blocks2 : blocks1);
-  if constexpr (!std::is_same_v<MT, float>) {
-    if (p.kind == 2)
-      hipLaunchKernelGGL((dense_bwd_kernel<TileL, MT, F32, GROUPS>), grid, dim3(TileL::NT), 0, s, g1, g2, db, front,
-                       products, swapped);
-  }
-  if (p.kind == 1)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, db, front,
-                       products, swapped);
-  else if (p.kind == 3)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileX, MT, F32, GROUPS>), grid, dim3(TileX::NT), 0, s, g1, g2, db, front,
-                       products, swapped);
-  else if (p.kind == 0)
-    hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, db, front,
-                       products, swapped);
-  FC_LAUNCH_CHECK();
+  const int st = in_launches(blocks + db_blocks, [&](int64_t first, unsigned count) {
+    const dim3 grid(count);
+    if constexpr (!std::is_same_v<MT, float>) {
+      if (p.kind == 2)
+        hipLaunchKernelGGL((dense_bwd_kernel<TileL, MT, F32, GROUPS>), grid, dim3(TileL::NT), 0, s, g1, g2, db, front,
+                           products, swapped, (int)first);
+    }
+    if (p.kind == 1)
+      hipLaunchKernelGGL((dense_bwd_kernel<TileM, MT, F32, GROUPS>), grid, dim3(TileM::NT), 0, s, g1, g2, db, front,
+                         products, swapped, (int)first);
+    else if (p.kind == 3)
+      hipLaunchKernelGGL((dense_bwd_kernel<TileX, MT, F32, GROUPS>), grid, dim3(TileX::NT), 0, s, g1, g2, db, front,
+                         products, swapped, (int)first);
+    else if (p.kind == 0)
+      hipLaunchKernelGGL((dense_bwd_kernel<TileS, MT, F32, GROUPS>), grid, dim3(TileS::NT), 0, s, g1, g2, db, front,
+                         products, swapped, (int)first);
+  });
+  if (st != FC_OK) return st;
   // the sums of split sums
   BwdSums a{};
   int64_t sum_blocks = 0;
@@ -332,11 +338,10 @@ static int launch_products(const DenseBwd& p, const DbArgs& db, hipStream_t s) {
     a.base = sum_blocks;
     if (g2.M > 0 && g2.splits > 1) add(1, g2, g2.splits, 1);
   }
-  if (sum_blocks == 0) return FC_OK;
-  if (!grid_fits(sum_blocks, 256)) return FC_ERR_SHAPE;
-  hipLaunchKernelGGL((dense_bwd_sum_kernel<MT, F32, GROUPS>), dim3((unsigned)sum_blocks), dim3(256), 0, s, a);
-  FC_LAUNCH_CHECK();
-  return FC_OK;
+  return in_launches(sum_blocks, [&](int64_t first, unsigned count) {
+    a.first = first;
+    hipLaunchKernelGGL((dense_bwd_sum_kernel<MT, F32, GROUPS>), dim3(count), dim3(256), 0, s, a);
+  });
 }
 
 }  // namespace fc
@@ -377,17 +382,20 @@ extern "C" int fc_node_dense_bwd(const fc_dense_desc* d, int64_t n, const void* 
     using T = std::conditional_t<F32, float, MT>;
     if (p.run_dz) {
       const int64_t blocks = p.chunks * p.dz.col_blocks;
-      if (!grid_fits(blocks, 256)) return FC_ERR_SHAPE;
-      hipLaunchKernelGGL((dense_dz_kernel<T, MT>), dim3((unsigned)blocks), dim3(256), 0, s, p.dz);
-      FC_LAUNCH_CHECK();
+      if (blocks > INT32_MAX) return FC_ERR_SHAPE;
+      DzArgs a = p.dz;
+      const int r = in_launches(blocks, [&](int64_t first, unsigned count) {
+        a.first = first;
+        hipLaunchKernelGGL((dense_dz_kernel<T, MT>), dim3(count), dim3(256), 0, s, a);
+      });
+      if (r != FC_OK) return r;
     }
     const DbArgs db{p.dz.sums, gb, p.chunks, f.n, p.dz.offsets, f.d.groups, (int32_t)f.out, (int32_t)f.op};
     if (!gx && !gw) {
       const int64_t blocks = (int64_t)(f.d.groups > 0 ? f.d.groups : 1) * cdiv(f.out, 32);
-      if (!grid_fits(blocks, 1024)) return FC_ERR_SHAPE;
-      hipLaunchKernelGGL((dense_db_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, db);
-      FC_LAUNCH_CHECK();
-      return FC_OK;
+      return in_launches(blocks, [&](int64_t first, unsigned count) {
+        hipLaunchKernelGGL((dense_db_kernel<T>), dim3(count), dim3(1024), 0, s, db, (int)first);
+      });
     }
     return d->groups > 0 ? launch_products<MT, F32, true>(p, db, s) : launch_products<MT, F32, false>(p, db, s);
   });

@@ -42,14 +42,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) dense_few_kernel(DenseJob g) {
   __shared__ f32x4v part[kFewWaves][ROWS][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4, col_blocks = (g.n_out + 15) / 16;
-  const int n0 = (GROUPS ? blockIdx.x % col_blocks : blockIdx.x) * 16;
+  const int id = g.first + blockIdx.x, n0 = (GROUPS ? id % col_blocks : id) * 16;
   const char *xs = g.A.p, *ws = g.B.p;
   int rows = g.M;
   if constexpr (GROUPS) {
-    const int e = blockIdx.x / col_blocks;
+    const int e = id / col_blocks;
     const GroupUnit u = find_unit<true>(g.offsets, g.groups, g.rows, 1, 0, e, true);
     // rows of no group
-    for (int64_t k = blockIdx.x; k < g.rows - (u.end - u.begin); k += gridDim.x) {
+    for (int64_t k = id; k < g.rows - (u.end - u.begin); k += g.blocks) {
       OT* const out = (OT*)g.out + (k < u.begin ? k : k + (u.end - u.begin)) * g.ld_out;
       for (int c = threadIdx.x; c < g.n_out; c += 64 * kFewWaves) out[c] = from_f32<OT>(0.f);
     }
