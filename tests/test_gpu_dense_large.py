@@ -72,3 +72,40 @@ def test_many_rows():
             sums += gf.double().t() @ xf.double()
             bias += gf.double().sum(0)
     assert torch.equal(dw, sums.bfloat16()) and torch.equal(db, bias.bfloat16())
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 1 << 20, 1 << 20, (1 << 20) + 40, 1 << 22]])
+@pytest.mark.parametrize("alone", [False, True])
+def test_bias_gradient_of_many_rows(offsets, alone):
+    """A float32 sum of n equal numbers whose additions are no longer chain than 4 + 8 + 64 + 512 + 32 is off by at most
+    2^-24 of it for each. (Other numbers in the last rows, so that a part taken twice or left out shows.)"""
+    n, out = 1 << 22, 8
+    g = torch.full((n, out), 0.1, device=DEV)
+    g[-5000:] = torch.arange(out, device=DEV) + 1.0
+    g[(1 << 20) - 70:1 << 20] = 3.0
+    x = torch.ones(n, 8, device=DEV, requires_grad=not alone)
+    w = torch.ones(*(() if offsets is None else (4,)), out, 8, device=DEV)
+    b = torch.zeros(w.shape[:-1], device=DEV, requires_grad=True)
+    y = _F().dense(x, w, b) if offsets is None else _F().grouped_dense(x, w, torch.tensor(offsets, device=DEV), b)
+    db = torch.autograd.grad(y, b if alone else (b, x), g)[0]
+    if offsets is None:
+        want = g.double().sum(0)
+    else:
+        want = torch.stack([g[p:q].double().sum(0) for p, q in zip(offsets, offsets[1:])])
+    off = (db.double() - want).abs()
+    assert bool((off <= 620 * 2.0 ** -24 * want).all()), float((off / want.clamp_min(1e-30)).max())
+
+
+@pytest.mark.parametrize("groups", [3, 1000])
+def test_bias_gradients_of_many_rows_in_groups(groups):
+    """Uneven groups, each sum exact: more than one level of sums, in groups of none, one and many of their parts."""
+    n, out = (1 << 21) + 333, 264
+    gen = torch.Generator().manual_seed(groups)
+    ends = torch.randint(0, n + 1, (groups - 1,), generator=gen).sort().values
+    offsets = torch.cat([torch.tensor([5]), ends.clamp(min=5), torch.tensor([n - 9])]).clamp(max=n - 9).to(DEV)
+    x = torch.zeros(n, 8, device=DEV)
+    b = torch.zeros(groups, out, device=DEV, requires_grad=True)
+    g = _small_integers(n, out).float()
+    (db,) = torch.autograd.grad(_F().grouped_dense(x, torch.zeros(groups, out, 8, device=DEV), offsets, b), b, g)
+    sums = torch.cat([torch.zeros(1, out, device=DEV, dtype=torch.float64), g.double().cumsum(0)])
+    assert torch.equal(db.double(), sums[offsets[1:]] - sums[offsets[:-1]])
