@@ -169,6 +169,7 @@ _SIGNATURES = {
     "fc_node_dense_fwd": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 8 + [c_i64, c_vp]),
     "fc_node_dense_bwd_workspace": (c_i64, [ctypes.POINTER(DenseDesc), c_i64, c_i32, c_i32, c_i32]),
     "fc_node_dense_bwd": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 9 + [c_i64, c_vp]),
+    "fc_node_dense_tile": (c_i32, [ctypes.POINTER(DenseDesc), c_i64, c_i32, ctypes.POINTER(c_i32)]),
     "fc_quantized_dense_workspace": (c_i64, [ctypes.POINTER(DenseDesc), c_i64]),
     "fc_quantized_dense": (c_int, [ctypes.POINTER(DenseDesc), c_i64] + [c_vp] * 8 + [c_i64, c_vp]),
     "fc_row_norm_fwd": (c_int, [c_i32, c_i64, c_i64, c_vp, c_vp, c_vp, c_f32, c_vp, c_vp, c_vp, c_vp]),

@@ -256,6 +256,21 @@ static int eight_check(const fc_dense_desc* d, int64_t n) {
   return st != FC_OK ? st : d->groups != 0 || d->dtype == FC_F32 ? FC_ERR_BAD_DESC : FC_OK;
 }
 
+extern "C" int32_t fc_node_dense_tile(const fc_dense_desc* d, int64_t n, int32_t pass, int32_t* halves) {
+  const int st = pass == 1 ? eight_check(d, n) : dense_check(d, n);
+  if (st != FC_OK) return -st;
+  if (pass < 0 || pass > 2) return -FC_ERR_BAD_DESC;
+  if (n == 0) return -FC_ERR_SHAPE;
+  if (halves) *halves = 0;
+  fc_dense_desc desc = *d;
+  desc.aligned = 1;
+  if (pass == 2) return dense_bwd_tile(desc, n);
+  Dense f(desc, n, nullptr, pass == 1);
+  const DenseFwd p = plan_dense(f, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+  if (halves && !p.few) *halves = p.job.halves;
+  return p.few ? 0 : tile_rows(p.kind);
+}
+
 extern "C" int64_t fc_quantized_dense_workspace(const fc_dense_desc* d, int64_t n) {
   const int st = eight_check(d, n);
   if (st != FC_OK) return -st;

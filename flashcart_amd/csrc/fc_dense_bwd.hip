@@ -336,6 +336,11 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
   return p;
 }
 
+int dense_bwd_tile(const fc_dense_desc& d, int64_t n) {
+  Dense f(d, n, nullptr);
+  return tile_rows(plan_dense_bwd(f, nullptr, nullptr, nullptr, nullptr, nullptr, 7, nullptr, nullptr).kind);
+}
+
 template <class MT, bool F32, bool GROUPS>
 static int launch_products(const DenseBwd& p, const DbArgs& db, hipStream_t s) {
   const DenseJob &g1 = p.dw, &g2 = p.dx;

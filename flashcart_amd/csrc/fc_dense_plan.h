@@ -212,6 +212,8 @@ inline int64_t group_blocks(const DenseJob& g, int bm) {
   if (g.unit > 0) return (g.rows / g.unit + g.groups) * g.tiles_m * g.tiles_n;
   return (g.rows / bm + g.groups) * g.tiles_n;
 }
+// Edge of the tiles of a backward pass with all gradients.
+int dense_bwd_tile(const fc_dense_desc& d, int64_t n);
 // Partial sums of groups of more than one unit: at most 2 rows / unit of them.
 inline int64_t group_partial_bytes(const DenseJob& g) { return 4 * (2 * g.rows / g.unit) * g.M * g.N; }
 

@@ -566,7 +566,12 @@ int fc_node_dense_bwd(const fc_dense_desc* desc, int64_t n, const void* grad, co
                       const void* saved, const int64_t* offsets, void* grad_x, void* grad_weight, void* grad_bias,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The same without groups on e4m3 operands (OCP, 448 the largest) x and W with a float32 scale for each of their rows,
+/* The edge of the output tiles (256, 128, 64 or 32) that the products of a call with these sizes and aligned operands take, 0 for
+ * the kernel of few rows, negative for a status; pass: 0 forward, 1 fc_quantized_dense, 2 backward with all gradients. halves
+ * receives the number of tiles that a forward pass takes as two halves. For tests and profiles. */
+int32_t fc_node_dense_tile(const fc_dense_desc* desc, int64_t n, int32_t pass, int32_t* halves);
+
+/* Dense layers without groups on e4m3 operands (OCP, 448 the largest) x and W with a float32 scale for each of their rows,
  * the values being x[r, :] x_scale[r] and W[c, :] weight_scale[c]; bias, residual and y of desc's type, one of 16 bits: the
  * 8-bit matrix instructions add with about 16. */
 int64_t fc_quantized_dense_workspace(const fc_dense_desc* desc, int64_t n);
