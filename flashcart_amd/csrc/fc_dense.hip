@@ -91,13 +91,21 @@ struct DenseFwd {
 // 1,031 -> 4,096 8.0 / 15.8; 16 rows 4,097 -> 4,096 29 / 28; 32 rows 1,024 -> 4,096 6.1 / 6.8, 2,048 -> 1,024 8.6 / 8.9.
 // float32, one row 2,048 -> 8,192 15 / 28, 4,096 -> 10,240 52 / 59, 4,096 -> 64 11.5 / 8.8; 32 rows 4,097 -> 4,096 29 / 53.
 // Groups: 16 of 2,048 -> 1,024 with 64 rows 20 / 14, 64 of 1,031 -> 512 with 32 rows 24 / 39 and with 512 41 / 47,
-// 8 of 4,099 -> 1,000 with 128 rows 66 / 41.
+// 8 of 4,099 -> 1,000 with 128 rows 66 / 41. (All with the weight in the last-level cache, from the call before.)
+// 8 bits, weights from memory: one row 1,024 -> 10,240 5.6 / 6.5, 4,096 -> 4,096 6.8 / 12, 4,096 -> 10,240 13 / 16; 16 rows
+// 2,048 -> 8,192 7.4 / 8.5, 4,096 -> 10,240 15 / 14, 8,192 -> 8,192 19 / 21; 32 rows 4,096 -> 4,096 9.4 / 12.5, 1,024 -> 10,240
+// 9.1 / 6.7, 8,192 -> 1,024 14 / 11. Rows that are copied for tiles: 16 rows 4,097 -> 4,096 19 / 22, 8,195 -> 4,096 28 / 31,
+// 4,097 -> 10,240 46 / 33; 32 rows 2,055 -> 4,096 13.5 / 17, 4,097 -> 4,096 28 / 23.
 static bool few_rows(const Dense& f) {
   if (f.form == FORM_PLANES) return false;
   const bool direct = f.direct(f.in, f.ip);
   if (f.d.groups > 0) return !direct && f.n <= 8 * (int64_t)f.d.groups;
   if (f.n > kFewRows) return false;
   const int64_t blocks = (f.n + 15) / 16, k = blocks * f.in;
+  if (f.form == FORM_8) {
+    if (direct) return blocks == 1 || (f.in <= 4096 && f.out <= 4096);
+    return f.in * f.out <= (blocks == 1 ? 5 << 23 : 1 << 24);
+  }
   if (f.form == FORM_NATIVE) return k <= (direct ? 2048 : 16384) || (blocks == 1 && f.out >= 4096);
   return direct ? k <= 2048 && k * f.out <= 1 << 23 : k <= 4096;
 }
