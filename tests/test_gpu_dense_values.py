@@ -132,3 +132,17 @@ def test_tails_of_gelu(n, dtype):
     bound = bound + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
     off = (_F().dense(x, w, z, "gelu").double() - want).abs()
     assert bool((off <= bound).all()), (float((off / bound).max()), float(z[(off / bound).amax(0).argmax()]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_large_gradients(dtype):
+    """Gradients near the largest number of the type, whose product with the activation's factor alone would leave it: silu'(0) =
+    1/2, so the bias' gradient is exactly 5/6 of it."""
+    n, out = 40, 72
+    x, w, z = (torch.zeros(*s, device=DEV, dtype=dtype) for s in ((n, 8), (out, 8), (out,)))
+    grad = torch.zeros(n, out, device=DEV, dtype=dtype)
+    grad[17] = 1.5 * 2.0 ** 127
+    got = _run(x, w, z, None, "silu", 5 / 3, 1.0, grad)
+    want = grad[17].double() * float(torch.tensor(5 / 3, dtype=torch.float32)) / 2
+    off = (got["db"].double() - want).abs()
+    assert bool((off <= (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * want).all())
