@@ -213,11 +213,14 @@ struct DenseJob : GemmJob {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
               s[v] *= KEEP;
-              d[v] = x[p][v] * fminf(s[v] * e[v], KEEP);
+              e[v] = fminf(s[v] * e[v], KEEP);
             }
-            if (g.act != 1) {
+            if (g.act == 1) {
 #pragma unroll
-              for (int v = 0; v < V; ++v) d[v] += s[v];
+              for (int v = 0; v < V; ++v) d[v] = x[p][v] * e[v];
+            } else {
+#pragma unroll
+              for (int v = 0; v < V; ++v) d[v] = fmaf(x[p][v], e[v], s[v]);
             }
           }
 #pragma unroll
