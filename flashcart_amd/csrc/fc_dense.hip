@@ -2,10 +2,11 @@
 //   y = residual + c act(s (x_scale x) (w_scale W)^T + b)
 // with e4m3 x and W, a float32 scale for each of their rows, and y in 16 bits.
 //
-// Bound by the matrix cores and the stores of y and act'(z) where n is large (16,384 x 2,048 x 5,632 bf16 371 us, 1,020
-// TFLOP/s; 8,192 x 4,096 x 5,120 in 8 bits 161-174 us, 1,970-2,130 TFLOP/s; 16,384 rows over 32 experts of 2,048 x 2,816
-// 257 us), by the weights' bytes where it is small (1 x 4,096 x 10,240 bf16 15 us, 5.6 TB/s; 64 rows over 64 experts of
-// 2,048 x 1,024 41 us, 4.1 TB/s).
+// Bound by the matrix cores and the stores of y and act'(z) where n is large (16,384 x 2,048 x 5,632 bf16 372 us, 1,020
+// TFLOP/s; 8,192 x 4,096 x 5,120 in 8 bits 159-173 us, 1,990-2,160 TFLOP/s; 16,384 rows over 32 experts of 2,048 x 2,816
+// 254 us), by the weights' bytes where it is small (1 x 4,096 x 10,240 bf16 15 us, 5.6 TB/s; 64 rows over 64 experts of
+// 2,048 x 1,024 41 us, 4.1 TB/s: repeated calls, whose weights the last-level cache holds in whole or in part; from memory the first
+// takes 24 us, 3.5 TB/s).
 #include "fc_dense_few.h"
 #include "fc_dense_plan.h"
 

@@ -1,6 +1,6 @@
 // Dense layers backward (fc_dense.h): dz and the bias' gradient in one pass over the incoming gradient, then the products
-// for dx and dW in one launch, the one with the longer sums first. 16,384 x 2,048 x 5,632 bf16: dz 101 us (5.5 TB/s, bound by
-// memory), products 658 us (1,149 TFLOP/s, the matrix cores busy 62%).
+// for dx and dW in one launch, the one with the longer sums first. 16,384 x 2,048 x 5,632 bf16: dz 100 us (5.5 TB/s, bound by
+// memory), products 645-661 us (1,149-1,170 TFLOP/s, the matrix cores busy 62%).
 #include <algorithm>
 
 #include "fc_dense_plan.h"

@@ -11,7 +11,7 @@
 // bytes a lane and load; squares, means and dw are summed in float32. dw: a workgroup adds up the rows it takes, in
 // registers, and a second launch adds the workgroups' sums: a fixed order. Rows too wide for that (above 16,384 16-bit or
 // 8,192 float32 elements; half as many backward) are read again instead. 16,384 x 4,096 bf16 with a residual: forward 86 us
-// (6.2 TB/s), backward 115 + 5 (4.7 TB/s); 8,192 x 5,120 to 8 bits 56 us (5.2 TB/s); 25,000 x 128 float32 10 and 12 + 4 us;
+// (6.2 TB/s), backward 115 + 5 (4.7 TB/s); 8,192 x 5,120 to 8 bits 52 us (5.6 TB/s), its rows alone 20; 25,000 x 128 float32 10 and 12 + 4 us;
 // one row of 4,096 3 us.
 #include "fc_node.h"
 

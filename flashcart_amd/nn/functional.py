@@ -111,7 +111,7 @@ def rms_norm_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
 
     The norm is that of the total as it is returned, rounded to the tensors' type. Both outputs have gradients; the
     weight's adds its rows in float32 in an order that the sizes fix. There are no second derivatives. A row of zeros with
-    ``eps=0`` gives NaN.
+    ``eps=0`` gives NaN. Squares are summed in float32: a row whose sum leaves it gives zeros.
     """
     y, total, _ = _node_ops.ops().rms_norm_add.default(x, residual, weight, float(eps), _wants_grad(x, residual, weight))
     return y, x if residual is None else total
@@ -124,7 +124,8 @@ def rms_norm_add_quantized(x: torch.Tensor, residual: Optional[torch.Tensor] = N
 
     scale (float32) is ``max(|y|, 2^-100) / 448`` over the row, y being the unrounded norm. q is float8_e4m3fn, the number
     nearest to ``448 y / max(|y|, 2^-100)`` (for 16-bit types exactly, ties going to the even number; for float32 up to
-    the rounding of y). A row with an infinity has an infinite scale, and NaN for its values. There are no gradients: arguments that
+    the rounding of y). A row with an infinity has an infinite square sum: NaN at the infinity, a norm of zero elsewhere and the
+    least scale; with an infinity in the weight the scale is infinite, finite values give zero and infinite ones NaN. There are no gradients: arguments that
     require them are refused where autograd records.
     """
     q, scale, total = _node_ops.ops().rms_norm_add_quantized.default(x, residual, weight, float(eps))
@@ -133,7 +134,8 @@ def rms_norm_add_quantized(x: torch.Tensor, residual: Optional[torch.Tensor] = N
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) of the rows of x (..., width), as ``rms_norm_add_quantized`` gives them for its norm: the operands of
-    ``quantized_dense``. A weight is laid out so once."""
+    ``quantized_dense``. A weight is laid out so once. A row with an infinity has an infinite scale, zeros, and NaN at the
+    infinity."""
     return _node_ops.ops().quantize_rows.default(x)
 
 
@@ -151,7 +153,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = 
 
     Sums are float32, and bias, activation and residual are applied before the one rounding of the output. For bfloat16
     and float16 the gradient of the activation's argument is rounded to that type in the backward pass, being an operand of
-    the matrix instructions (gradients of x and weight are 1.4 times as far from exact ones as one rounding); the
+    the matrix instructions (gradients of x and weight are 1.4 times as far from exact ones as one rounding; in float16 it is zero
+    below 2^-25, as any float16 gradient is: scale the loss); the
     activation's derivative is kept for it with 11 significant bits beside bfloat16 (fewer for a derivative below 2^-29, none
     below 2^-40), 16 beside float16, in 2 and 3 bytes an output (float32: all, in 4). float32 products
     keep float32 accuracy, as in ``gated_feed_forward``; so does the activation. There are no second derivatives.
