@@ -6,7 +6,8 @@
 // exact sum's: gradients of x and W are 1.4 times as far off as a rounding).
 //
 // Groups: the rows offsets[e] .. offsets[e + 1] - 1 have weight e. The offsets stay on the device: a workgroup finds its
-// group and tile from them, the grid is the most that any offsets can need.
+// group and tile from them, or of many groups from a table that a launch before it makes of them; the grid is the most that any
+// offsets can need.
 #pragma once
 
 #include "fc_gemm_plan.h"
@@ -88,6 +89,14 @@ __device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
   if constexpr (EXACT) cdf = z > -1.f ? 0.5f * (1.f + erff(z * 0.70710678118654752f)) : cdf;
 }
 
+// What find_unit finds by scanning all offsets, made once for the whole call where groups are many: then the scan would take
+// longer than the work (find_unit reads 64 offsets at a time, every workgroup all of them).
+struct UnitTable {
+  const int32_t* ends;    // (groups + 1): the first row of each group, and the end of the last; null: there is no table
+  const int32_t* before;  // (groups + 1): units of the groups before each, of all
+  const int32_t* slots;   // (groups): the same, of those that have more than one
+};
+
 // One product of a dense layer. For groups the pointers are those of the whole call, and a workgroup shifts them.
 struct DenseJob : GemmJob {
   const void* bias;              // (groups, n_out), or null
@@ -98,6 +107,7 @@ struct DenseJob : GemmJob {
   int32_t act;
   float act_scale;
   const int64_t* offsets;        // (groups + 1)
+  UnitTable table;               // of the units that this product's tiles take
   int32_t groups;
   int32_t halves;                // tiles at the end that are taken as two halves of their columns
   int32_t unit;                  // > 0: sums over a group's rows, in parts of so many
@@ -274,9 +284,34 @@ struct GroupUnit {
   int64_t begin, end; // rows of all groups
 };
 template <bool BY_GROUP = false>
-__device__ __forceinline__ GroupUnit find_unit(const int64_t* offsets, int groups, int64_t n, int size, int least, int t,
-                                               bool want_total) {
+__device__ __forceinline__ GroupUnit find_unit(const int64_t* offsets, const UnitTable& table, int groups, int64_t n, int size,
+                                               int least, int t, bool want_total) {
   const int lane = threadIdx.x & 63;
+  if (table.ends) {
+    GroupUnit u{-1, 0, 0, 0, 0, 0, 0, table.ends[0], table.ends[groups]};
+    int e = t;
+    if constexpr (!BY_GROUP) {
+      u.total = table.before[groups];
+      if (t < 0 || t >= u.total) return u;
+      // the last group with no more units before it than t, in steps of 64
+      e = 0;
+      for (int span = groups; span > 1;) {
+        const int step = (span + 63) / 64, at = lane * step;
+        const uint64_t hit = __ballot(at < span && table.before[e + (at < span ? at : 0)] <= t);
+        const int k = (__popcll(hit) - 1) * step;
+        e += k;
+        span = min(step, span - k);
+      }
+    }
+    u.group = __builtin_amdgcn_readfirstlane(e);
+    u.before = table.before ? table.before[u.group] : 0;
+    u.index = BY_GROUP ? 0 : t - u.before;
+    const int row = __builtin_amdgcn_readfirstlane(table.ends[u.group]);
+    u.row = row;
+    u.rows = __builtin_amdgcn_readfirstlane(table.ends[u.group + 1]) - row;
+    u.slot = table.slots ? table.slots[u.group] : 0;
+    return u;
+  }
   auto clamped = [&](int64_t v) { return v < 0 ? 0 : v > n ? n : v; };
   GroupUnit u{-1, 0, 0, 0, 0, 0, 0, 0, 0};
   int64_t last = clamped(offsets[0]);
@@ -348,7 +383,7 @@ struct GroupTile {
     DenseJob g = arg;
     const int size = SUMS ? g.unit : T::BM, least = SUMS ? 1 : 0, per = SUMS ? g.tiles_m * g.tiles_n : g.tiles_n;
     // block -> tile as without groups: a run of tiles for each XCD
-    const GroupUnit all = find_unit(g.offsets, g.groups, g.rows, size, least, -1, true);
+    const GroupUnit all = find_unit(g.offsets, g.table, g.groups, g.rows, size, least, -1, true);
     const int total = all.total * per;
     if constexpr (!SUMS) {  // rows of no group
       for (int64_t r = block; r < g.rows - (all.end - all.begin); r += blocks) {
@@ -362,7 +397,7 @@ struct GroupTile {
       const int each = total / 8, rest = total % 8, x = tile % 8;
       tile = x * each + min(x, rest) + tile / 8;
     }
-    const GroupUnit u = find_unit(g.offsets, g.groups, g.rows, size, least, tile / per, false);
+    const GroupUnit u = find_unit(g.offsets, g.table, g.groups, g.rows, size, least, tile / per, false);
     int tiles_m = g.tiles_m, in;
     if constexpr (SUMS) {
       const int64_t row = u.row + (int64_t)u.index * g.unit, left = u.rows - (int64_t)u.index * g.unit;

@@ -135,12 +135,14 @@ static DenseFwd plan_dense(Dense& f, const void* x, const void* weight, const vo
   g.factor_count = f.n * f.op;
   if (f.d.groups > 0) {
     f.grouped(g, offsets, f.out * (p.few ? f.in : f.ip), 0);
+    if (p.few) g.table = f.units(0, 0);
     if (p.few) return p;
     p.kind = plan_groups(&g, nullptr, f);
     // Few rows a group: tiles of 32 rows, three of which a CU runs at once (64 experts of 2,048 -> 1,024, 64 and 1,024 rows,
     // bf16 45.6 -> 41.3 and 62 -> 56 us, 256 rows float32 146 -> 100; 8 experts of 4,096 -> 4,096, 64 rows, bf16 54 -> 58).
     const bool native = f.form == FORM_NATIVE;
     if (p.kind == 0 && f.n <= (native ? 64 : 16) * (int64_t)f.d.groups && (native || f.d.groups >= 16)) p.kind = 4;
+    g.table = f.units(tile_rows(p.kind), 0);
     return p;
   }
   if (p.few) return p;
@@ -251,7 +253,8 @@ extern "C" int fc_node_dense_fwd(const fc_dense_desc* d, int64_t n, const void* 
   if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
   if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  st = f.run_pad(s);
+  st = f.run_units(offsets, s);
+  if (st == FC_OK) st = f.run_pad(s);
   if (st != FC_OK) return st;
   return with_operand_form(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);

@@ -20,6 +20,7 @@ struct DzArgs {
   int32_t out, op, col_blocks;
   float act_scale;          // over the scale that act'(z) is kept with
   const int64_t* offsets;   // or null
+  UnitTable table;
   int32_t groups;
   int64_t rows;
   int64_t first;            // workgroup of this launch
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DzArgs a) {
   const int id = (int)(a.first + blockIdx.x), chunk = id / a.col_blocks, cb = id - chunk * a.col_blocks;
   int64_t r0 = (int64_t)chunk * kDzRows, r1 = min(r0 + kDzRows, a.rows);
   if (a.offsets) {
-    const GroupUnit u = find_unit(a.offsets, a.groups, a.rows, kDzRows, 0, chunk, false);
+    const GroupUnit u = find_unit(a.offsets, a.table, a.groups, a.rows, kDzRows, 0, chunk, false);
     if (u.group < 0) return;
     r0 = u.row + (int64_t)u.index * kDzRows;
     r1 = min(r0 + kDzRows, u.row + u.rows);
@@ -96,6 +97,7 @@ struct FoldArgs {
   float* out;
   int64_t chunks, rows, first;
   const int64_t* offsets;
+  UnitTable from, to;  // of the units that are added, and of those that they become
   int32_t groups, op, col_blocks, size;
 };
 __global__ void __launch_bounds__(256) dense_fold_kernel(FoldArgs a) {
@@ -103,9 +105,9 @@ __global__ void __launch_bounds__(256) dense_fold_kernel(FoldArgs a) {
   const int c = (id - unit * a.col_blocks) * 256 + threadIdx.x;
   int64_t c0 = (int64_t)unit * kFold, end = a.chunks;
   if (a.offsets) {
-    const GroupUnit u = find_unit(a.offsets, a.groups, a.rows, a.size * kFold, 0, unit, false);
+    const GroupUnit u = find_unit(a.offsets, a.to, a.groups, a.rows, a.size * kFold, 0, unit, false);
     if (u.group < 0) return;
-    const int before = find_unit<true>(a.offsets, a.groups, a.rows, a.size, 0, u.group, false).before;
+    const int before = find_unit<true>(a.offsets, a.from, a.groups, a.rows, a.size, 0, u.group, false).before;
     c0 = before + (int64_t)u.index * kFold;
     end = before + (u.rows + a.size - 1) / a.size;
   }
@@ -124,6 +126,7 @@ struct DbArgs {
   void* out;          // (groups, out), or null
   int64_t chunks, rows;
   const int64_t* offsets;
+  UnitTable table;
   int32_t groups, n_out, op, size;
 };
 template <class T, int NT>
@@ -132,7 +135,7 @@ __device__ __forceinline__ void db_block(const DbArgs& a, int block, float (&par
   const int c = (block - e * blocks) * 32 + cl;
   int64_t c0 = 0, c1 = a.chunks;
   if (a.offsets) {
-    const GroupUnit u = find_unit<true>(a.offsets, a.groups, a.rows, a.size, 0, e, false);
+    const GroupUnit u = find_unit<true>(a.offsets, a.table, a.groups, a.rows, a.size, 0, e, false);
     c0 = u.before;
     c1 = c0 + (u.rows + a.size - 1) / a.size;
   }
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(256) dense_bwd_sum_kernel(BwdSums a) {
     const int64_t each = (g.M * chunks + per - 1) / per;
     const int e = (int)(block / each);
     block -= e * each;
-    const GroupUnit u = find_unit<true>(g.offsets, g.groups, g.rows, g.unit, 1, e, false);
+    const GroupUnit u = find_unit<true>(g.offsets, g.table, g.groups, g.rows, g.unit, 1, e, false);
     if (u.rows <= g.unit) return;
     g.splits = (int)((u.rows + g.unit - 1) / g.unit);
     g.partial += (int64_t)u.slot * g.M * g.N;
@@ -281,6 +284,7 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
     if (groups) {
       a.offsets = (const int64_t*)offsets;
       a.groups = f.d.groups;
+      a.table = f.units(kDzRows, 0);
     }
   }
   a.grad = grad;
@@ -291,17 +295,19 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
   a.col_blocks = cdiv(f.op, kDzCols);
   if (nb) {
     DbArgs& b = p.db;
-    b = DbArgs{a.sums, nullptr, p.chunks, f.n, a.offsets, f.d.groups, (int32_t)f.out, (int32_t)f.op, kDzRows};
+    b = DbArgs{a.sums, nullptr, p.chunks, f.n, a.offsets, a.table, f.d.groups, (int32_t)f.out, (int32_t)f.op, kDzRows};
     // A chain of up to 256 additions for each of 8 lanes is left; two folds are enough for 2^27 rows. Backward without and with a
     // fold, us: 40,000 x 128 x 128 bf16 58 / 61, 60,000 x 64 x 1,024 bf16 125 / 123, 80,000 x 512 x 128 bf16 74 / 69, 131,072 x
     // 128 x 128 float32 140 / 129.
     for (; f.n > 2048 * (int64_t)b.size; ++p.folds) {
       const int64_t chunks = groups ? f.n / (b.size * kFold) + f.d.groups : (b.chunks + kFold - 1) / kFold;
       float* const out = (float*)f.take(4 * chunks * f.op);
-      p.fold[p.folds] = FoldArgs{b.sums, out, b.chunks, f.n, 0, a.offsets, f.d.groups, (int32_t)f.op, a.col_blocks, b.size};
+      const UnitTable to = groups ? f.units(b.size * kFold, 0) : UnitTable{};
+      p.fold[p.folds] = FoldArgs{b.sums, out, b.chunks, f.n, 0, a.offsets, b.table, to, f.d.groups, (int32_t)f.op, a.col_blocks, b.size};
       b.sums = out;
       b.chunks = chunks;
       b.size *= kFold;
+      b.table = to;
     }
   }
   a.act_scale = f.d.act_scale / (factor && f.d.dtype == FC_BF16 ? kFactorScale<bf16_t> : 1.f);
@@ -329,6 +335,8 @@ static DenseBwd plan_dense_bwd(Dense& f, const void* grad, const void* x, const 
   if (!nx && !nw) return p;
   if (groups) {
     p.kind = plan_groups(nx ? &p.dx : nullptr, nw ? &p.dw : nullptr, f);
+    if (nx) p.dx.table = f.units(tile_rows(p.kind), 0);
+    if (nw) p.dw.table = f.units(p.dw.unit, 1);
     if (nw && p.dw.unit < f.n) p.dw.partial = (float*)f.take(group_partial_bytes(p.dw));
     return p;
   }
@@ -433,7 +441,8 @@ extern "C" int fc_node_dense_bwd(const fc_dense_desc* d, int64_t n, const void* 
   if (f.at > 0 && (!ws || ws_bytes < f.at)) return FC_ERR_WORKSPACE;
   if (!aligned16(saved) || !aligned16(ws)) return FC_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  st = f.run_pad(s);
+  st = f.run_units((const int64_t*)offsets, s);
+  if (st == FC_OK) st = f.run_pad(s);
   if (st != FC_OK) return st;
   return with_operand_form(d->dtype, f.form, [&](auto m, auto is32) -> int {
     using MT = decltype(m);

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) dense_few_kernel(DenseJob g) {
   int rows = g.M;
   if constexpr (GROUPS) {
     const int e = id / col_blocks;
-    const GroupUnit u = find_unit<true>(g.offsets, g.groups, g.rows, 1, 0, e, true);
+    const GroupUnit u = find_unit<true>(g.offsets, g.table, g.groups, g.rows, 1, 0, e, true);
     // rows of no group
     for (int64_t k = id; k < g.rows - (u.end - u.begin); k += g.blocks) {
       OT* const out = (OT*)g.out + (k < u.begin ? k : k + (u.end - u.begin)) * g.ld_out;

@@ -43,6 +43,79 @@ __global__ void __launch_bounds__(256) dense_pad_kernel(PadArgs a) {
   }
 }
 
+// ---- tables of units (UnitTable) ----
+struct UnitsArgs {
+  const int64_t* offsets;
+  int32_t* ends;
+  int64_t rows;
+  int32_t groups, count;
+  struct {
+    int32_t size, least;  // size 0: the ends alone
+    int32_t *before, *slots;
+  } table[5];
+};
+
+// v of the lanes and waves before this thread's, by f; `none` for the first.
+template <class F>
+__device__ __forceinline__ int before_thread(int v, int none, int* lds, F&& f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int w = __shfl_up(v, o, 64);
+    if (lane >= o) v = f(v, w);
+  }
+  __syncthreads();  // (the last call's values have been read)
+  if (lane == 63) lds[wave] = v;
+  __syncthreads();
+  int all = none;
+  for (int k = 0; k < waves; ++k)
+    if (k < wave) all = f(all, lds[k]);
+  const int up = __shfl_up(v, 1, 64);
+  return lane > 0 ? f(all, up) : all;
+}
+
+// A workgroup a table. A thread takes a run of groups; the largest offset, and the units, of the runs before it come by a scan.
+static __global__ void __launch_bounds__(1024) dense_units_kernel(UnitsArgs a) {
+  __shared__ int lds[16];
+  const int each = (a.groups + 1023) / 1024, e0 = min((int)threadIdx.x * each, a.groups), e1 = min(e0 + each, a.groups);
+  const int n = (int)a.rows;
+  auto offset = [&](int e) {
+    const int64_t v = a.offsets[e];
+    return v < 0 ? 0 : v > n ? n : (int)v;
+  };
+  auto larger = [](int u, int v) { return u > v ? u : v; };
+  auto sum = [](int u, int v) { return u + v; };
+  const int start = offset(0);
+  int most = start;
+  for (int e = e0; e < e1; ++e) most = larger(most, offset(e + 1));
+  const int first = before_thread(most, start, lds, larger);  // where group e0 begins
+  const auto& t = a.table[blockIdx.x];
+  const int least = t.least, size = t.size;
+  auto units = [&](int rows) { return larger(least, (rows + size - 1) / size); };
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) a.ends[0] = start;
+    for (int e = e0, at = first; e < e1; ++e) a.ends[e + 1] = at = larger(at, offset(e + 1));
+  }
+  if (size == 0) return;
+  int count = 0, several = 0;
+  for (int e = e0, at = first; e < e1; ++e) {
+    const int end = larger(at, offset(e + 1)), c = units(end - at);
+    count += c;
+    several += c > 1 ? c : 0;
+    at = end;
+  }
+  int before = before_thread(count, 0, lds, sum), slot = before_thread(several, 0, lds, sum);
+  for (int e = e0, at = first; e < e1; ++e) {
+    const int end = larger(at, offset(e + 1)), c = units(end - at);
+    t.before[e] = before;
+    t.slots[e] = slot;
+    before += c;
+    slot += c > 1 ? c : 0;
+    at = end;
+  }
+  if (e0 < e1 && e1 == a.groups) t.before[a.groups] = before;
+}
+
 // f(type of the operands in memory, is the operator's type float32)
 template <class F>
 int with_operand_form(int32_t dtype, Form form, F&& f) {
@@ -127,6 +200,36 @@ struct Dense {
   }
   int64_t factor_bytes() const {
     return d.act == ACT_NONE ? 0 : (d.dtype == FC_F32 ? 4 : d.dtype == FC_BF16 ? 2 : 3) * n * op;
+  }
+  // Whether the units of groups stand in a table: of more than 64 groups, which a scan takes in one step, where the weights are
+  // many workgroups' work, and of more than 256. us, scan / table, forward and backward: 100 groups of 64 x 64, 16,384 rows 9 and
+  // 51 / 13 and 53; 100 of 1,024 x 1,024, 512 rows 41 and 182 / 39 and 145, 200 102 and 423 / 90 and 271; 320 of 256 x 256, 16,384
+  // rows 30 and 75 / 21 and 54; 4,096 of 64 x 64 522 and 1,700 / 34 and 91; 65,536 78,000 and 336,000 / 370 and 1,060.
+  bool tabled() const { return d.groups > 256 || (d.groups > 64 && d.groups * in * out >= 1 << 26); }
+  UnitsArgs unit_tables{};
+  UnitTable units(int size, int least) {
+    if (!tabled()) return UnitTable{};
+    UnitsArgs& a = unit_tables;
+    if (a.count == 0) a.ends = (int32_t*)take(4 * ((int64_t)d.groups + 1));
+    auto& t = a.table[a.count++];
+    t.size = size;
+    t.least = least;
+    t.before = t.slots = nullptr;
+    if (size > 0) {
+      t.before = (int32_t*)take(4 * ((int64_t)d.groups + 1));
+      t.slots = (int32_t*)take(4 * (int64_t)d.groups);
+    }
+    return UnitTable{a.ends, t.before, t.slots};
+  }
+  int run_units(const int64_t* offsets, hipStream_t s) {
+    UnitsArgs& a = unit_tables;
+    if (a.count == 0) return FC_OK;
+    a.offsets = offsets;
+    a.rows = n;
+    a.groups = d.groups;
+    hipLaunchKernelGGL(dense_units_kernel, dim3(a.count), dim3(1024), 0, s, a);
+    FC_LAUNCH_CHECK();
+    return FC_OK;
   }
   void grouped(DenseJob& g, const void* offsets, int64_t b_stride, int64_t out_stride) const {
     g.offsets = (const int64_t*)offsets;
